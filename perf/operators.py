@@ -495,8 +495,8 @@ def _exact_append(st):
             b = min(page, a + length - pos)
             for x, pool, scale in ((st["xk"], "k", "ks"), (st["xv"], "v", "vs")):
                 x = x[row:row + b - a].double().permute(1, 0, 2)                      # [kv, tokens, dim]
-                s = torch.pow(2.0, torch.ceil(torch.log2(x.abs().amax((1, 2)).clamp(min=1e-300) / E4M3_MAX)))
-                s = s.clamp(min=2.0 ** MIN_EXP)
+                e = torch.ceil(torch.log2(x.abs().amax((1, 2)).clamp(min=1e-300) / E4M3_MAX)).clamp(min=MIN_EXP)
+                s = torch.ldexp(torch.ones_like(e), e.int())       # pow(2, e) is off by an ulp on some devices
                 if a:
                     was = got[scale][lay, p].double()
                     s = torch.maximum(s, was)
