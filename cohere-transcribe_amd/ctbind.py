@@ -193,10 +193,38 @@ ABI_SIGS = {
     "backend_sdp_attn_batch_decode_ca": ([_P, _P, _P, _P, _I, _I, _P], None),
 }
 assert len(ABI_SIGS) == 40
-# This backend's addition to the ABI (include/backend.h, after the 40).
+# This backend's additions to the ABI (include/backend.h, after the 40).
+_L = C.c_long
 ABI_EXT_SIGS = {
     "backend_rel_pos_mhsa_noalloc": ([_P, _P, _I, _P], None),
+    "backend_kv8_floats": ([_P], _Z),
+    "backend_kv8_plan_ints": ([_P], _Z),
+    "backend_kv8_bind": ([_P, _P], None),
+    "backend_kv8_reserve": ([_P, _P], None),
+    "backend_kv8_append": ([_P, _I, _P, _P, _L, _I, _P, _I], None),
+    "backend_kv8_attn_work": ([_P, _P], _Z),
+    "backend_kv8_attn": ([_P, _I, _P], None),
+    "backend_kv8_fork": ([_P, _P, _P, _I], None),
+    "backend_kv8_free": ([_P, _P, _I], None),
+    "backend_kv8_trim": ([_P, _I, _I], None),
+    "backend_kv8_compact": ([_P], None),
+    "backend_kv8_status": ([_P], _I),
+    "backend_stream": ([], _P),
 }
+KV8_NO_PAGES, KV8_NO_ROOM, KV8_BAD_ARG = 1, 2, 4
+
+
+class BackendKv8(C.Structure):
+    """A paged 8-bit key/value cache (include/backend.h); pass C.byref(cache)."""
+    _fields_ = ([(n, _I) for n in ("layers", "pages", "page_tokens", "kv_heads", "head_dim", "seqs", "table_w")]
+                + [(n, _P) for n in ("k", "v", "kscale", "vscale", "table", "len", "refs", "rows", "plan")])
+
+
+class BackendKv8Attn(C.Structure):
+    """An attention call over such a cache; pass C.byref(call)."""
+    _fields_ = [("out", _P), ("q", _P), ("ld_out", _L), ("ld_q", _L), ("bf16", _I), ("heads", _I), ("scale", _F),
+                ("causal", _I), ("window", _I), ("sinks", _I), ("rows", _P), ("n_rows", _I), ("max_rows", _I),
+                ("max_len", _I), ("work", _P)]
 
 
 def bind_abi(lib):

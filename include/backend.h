@@ -148,6 +148,141 @@ void backend_sdp_attn_batch_decode_ca(float *out, const float *Q,
  * race.  Same results, bit for bit, as backend_rel_pos_mhsa. */
 void backend_rel_pos_mhsa_noalloc(float *x, const float *pos_emb, int T, const ELayer *L);
 
+/* ---- Paged key/value cache in 8 bits ------------------------------------ *
+ * The batched decode step above keeps K and V as fp32 rows of MAX_SEQ tokens
+ * per item.  The calls below keep them as e4m3 codes (a quarter of the bytes)
+ * in pages that sequences take as they grow, share and give back: long texts,
+ * grouped heads, beams, streams with a window.  They have no counterpart in
+ * the reference.
+ *
+ * A page holds page_tokens consecutive tokens of one sequence, in every
+ * layer, K and V.  Its codes have one scale for each layer and kv head, a
+ * power of two: value = code * scale, and dividing by the scale is exact, so
+ * a value is rounded once.  The cache holds finite values and NaN: what lies
+ * beyond 448 scales, infinities included, is stored as +-448 scales.
+ *
+ * Conventions beside those at the head of this file:
+ *  - Every pointer in the structs and every int array argument is DEVICE
+ *    memory, and the calls read nothing back: they are asynchronous on the
+ *    calling thread's stream, allocate nothing and can be captured in a graph
+ *    (backend_kv8_status and the size functions apart).
+ *  - Calls on one cache are ordered by the stream they run on; two threads
+ *    that share a cache order their calls themselves, and graphs that were
+ *    captured over one cache, or one work buffer, do not run at the same time.
+ *  - Sizes and pointers that the host sees are checked (errors print and
+ *    exit).  Contents of device arrays are checked by the kernels: page ids
+ *    outside the pool, rows outside [0, n_rows) and sequence numbers outside
+ *    the table are not followed, as each call says. */
+typedef struct {
+    int layers;          /* layers the pools hold, >= 1                       */
+    int pages;           /* pages of each layer's pools, >= 1                 */
+    int page_tokens;     /* tokens of a page: 16, 32, 64 or 128               */
+    int kv_heads;        /* heads of K and V, 1..256                          */
+    int head_dim;        /* 64 or 128                                         */
+    int seqs;            /* sequences, rows of the table: 1..256              */
+    int table_w;         /* page ids of a table row;
+                            table_w * page_tokens <= 2^24                     */
+    /* pools [layers][pages][kv_heads][page_tokens][head_dim] of codes
+     * (16-byte aligned) and [layers][pages][kv_heads] of scales */
+    uint8_t *k, *v;
+    float   *kscale, *vscale;
+    int *table;          /* [seqs][table_w] page ids; -1: none                */
+    int *len;            /* [seqs] tokens held                                */
+    int *refs;           /* [pages] table entries that hold the page; 0: free */
+    int *rows;           /* [seqs + 1] rows of the step, written by
+                            backend_kv8_reserve (may be NULL without it)      */
+    int *plan;           /* scratch of the page calls and the status word:
+                            backend_kv8_plan_ints ints, zeroed once           */
+} BackendKv8;
+
+/* Floats the cache's arrays take together; ints of its plan. */
+size_t backend_kv8_floats(const BackendKv8 *c);
+size_t backend_kv8_plan_ints(const BackendKv8 *c);
+/* Points the arrays into mem (device memory of backend_kv8_floats floats,
+ * 16-byte aligned, as backend_arena_alloc gives it) and empties the cache:
+ * no pages taken, lengths 0, status 0. */
+void backend_kv8_bind(BackendKv8 *c, float *mem);
+/* Opens a step: sequence s gets add[s] (>= 0) more tokens.  Writes
+ * rows[0..seqs], the prefix sums of add; takes the pages the new tokens need,
+ * in the order of sequences, lowest free page first; adds add[s] to len[s].
+ * If the pool or a table row has no room, or an add[s] is negative, nothing
+ * is taken: rows become all 0, so that the appends and attention of the
+ * step do nothing, and the status tells it (KV8_NO_PAGES, KV8_NO_ROOM,
+ * KV8_BAD_ARG). */
+void backend_kv8_reserve(const BackendKv8 *c, const int *add);
+/* Rounds a layer's new K and V rows into their pages.  Sequence s has the
+ * rows rows[s] .. rows[s + 1] - 1 (in all at most n_rows); they are the last
+ * ones of its len[s] tokens.  A row is kv_heads * head_dim values (fp32, or
+ * bf16 if bf16 != 0), ld values after the one before it.  The scale of a
+ * page is the smallest 2^e >= 2^-100 that holds its largest finite value
+ * within 448 scales.  Where a page held tokens already its scale never gets
+ * smaller; where it has to grow, those tokens' codes are rounded again (exact
+ * but for the smallest values).  Tokens behind the last one are left as they
+ * are.  A row whose page is not in the pool, or shared (refs above 1), is
+ * skipped; sequences whose rows lie outside [0, n_rows) are skipped. */
+void backend_kv8_append(const BackendKv8 *c, int layer, const void *k, const void *v, long ld, int bf16,
+                        const int *rows, int n_rows);
+typedef struct {
+    void *out;           /* [n_rows] rows of heads * head_dim, ld_out apart   */
+    const void *q;       /* the same, ld_q apart                              */
+    long ld_out, ld_q;   /* in values                                         */
+    int bf16;            /* q and out: 0 fp32, 1 bf16                         */
+    int heads;           /* query heads, a multiple of kv_heads: head h reads
+                            kv head h / (heads / kv_heads)                    */
+    float scale;         /* of the scores; 1 / sqrt(head_dim) for this model  */
+    int causal;          /* 1: a sequence's rows are its last tokens and see
+                            the tokens up to their own; 0: they see all       */
+    int window;          /* causal only: a row at position p sees p - window
+                            + 1 .. p; 0: no limit                             */
+    int sinks;           /* with a window: tokens 0 .. sinks - 1 stay visible */
+    const int *rows;     /* [seqs + 1] as in backend_kv8_append               */
+    int n_rows;          /* rows of q and out; n_rows * heads <= 2^27         */
+    int max_rows;        /* no sequence has more rows than this; the rows of
+                            one that has more may be left as they are         */
+    int max_len;         /* no sequence holds more tokens than this; those
+                            past it are not seen; 0: table_w * page_tokens    */
+    float *work;         /* backend_kv8_attn_work floats, 16-byte aligned     */
+} BackendKv8Attn;
+/* Floats of work an attention call takes (0: none, work may be NULL).  It
+ * depends on the sizes alone, not on the pointers. */
+size_t backend_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a);
+/* Softmax attention of the rows over a layer's pages: o = sum_j p_j v_j,
+ * p = softmax_j(scale * q . k_j) over the tokens the row sees.  A row that
+ * sees none gets zeros; tokens on a page that is not in the pool are not
+ * seen; what a masked token holds, NaN included, has no effect.  Rows of out
+ * that belong to no sequence are left as they are.  Scores, softmax and sums
+ * are fp32; fp32 rows keep fp32 accuracy, bf16 rows enter the products as
+ * they are. */
+void backend_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a);
+/* Sequences dst[i] become copies of src[i], all n (<= seqs) at once, from
+ * what the cache held before the call (beam search: src = each beam's
+ * parent).  Full pages are shared; a partly filled last page is copied, in
+ * every layer, to the lowest free page, in the order of i.  dst[i]'s earlier
+ * pages are given back.  A pair with dst == src changes nothing.  Pages given
+ * back by this call are not taken by it, so it needs as many free pages as
+ * there are partly filled pages to copy.  If there are fewer, or a sequence
+ * number is out of range, or a dst appears twice, nothing changes and the
+ * status tells it (KV8_NO_PAGES, KV8_BAD_ARG). */
+void backend_kv8_fork(const BackendKv8 *c, const int *dst, const int *src, int n);
+/* Gives back the pages of n (<= seqs) sequences and empties them.  Numbers
+ * out of range change nothing and set KV8_BAD_ARG; one that appears twice is
+ * freed once. */
+void backend_kv8_free(const BackendKv8 *c, const int *seqs, int n);
+/* Gives back the pages that a causal row with this window (>= 1) and sinks
+ * at position len[s] or later does not see; their table entries become -1. */
+void backend_kv8_trim(const BackendKv8 *c, int window, int sinks);
+/* Moves the pages in use to the front: with m pages in use, those at m and
+ * above go, in ascending order, to the free ones below m. */
+void backend_kv8_compact(const BackendKv8 *c);
+/* Waits for the stream; returns the flags since the last call and clears
+ * them. */
+#define KV8_NO_PAGES 1
+#define KV8_NO_ROOM  2
+#define KV8_BAD_ARG  4
+int  backend_kv8_status(const BackendKv8 *c);
+/* The calling thread's stream (hipStream_t), to order other work with. */
+void *backend_stream(void);
+
 #ifdef __cplusplus
 }
 #endif

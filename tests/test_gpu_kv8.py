@@ -1,0 +1,592 @@
+"""The paged 8-bit key/value cache on the device against its 64-bit model
+(kv8_ref.py) — needs an MI355X.
+
+Appends and page calls must give the model's codes, scales and tables
+exactly; attention must be within kv8_ref.tolerance of the 64-bit result.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import ctbind as cb
+import kv8_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def values(rng, *shape):
+    """Normal values whose size differs from row to row, representable in bf16."""
+    x = rng.standard_normal(shape) * np.exp(rng.standard_normal(shape[:-1] + (1,)))
+    return ref.bf16_value(ref.bf16_bits(x.astype(np.float32)))
+
+
+def check_rows(got, want, vmax, smax, bf16, what):
+    """Rows of no sequence untouched (55), the others within the tolerance, NaN where the model has NaN."""
+    none = np.isnan(want).all(axis=(1, 2)) & (vmax == 0).all(axis=(1, 2))
+    assert np.all(got[none] == 55.0), what
+    w, g = want[~none], got[~none].astype(np.float64)
+    assert np.array_equal(np.isnan(w), np.isnan(g)), what
+    t = ref.tolerance(w, vmax[~none], smax[~none], bf16, w.shape[2])
+    with np.errstate(invalid="ignore"):
+        d = np.abs(g - w)
+    bad = ~(d <= t) & ~np.isnan(w)
+    assert not bad.any(), (what, float(np.nanmax(d / np.maximum(t, 1e-300))), np.argwhere(bad)[:4])
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("P,D,kv,bf16", [(16, 64, 1, False), (32, 64, 3, True), (64, 128, 2, False),
+                                         (128, 128, 1, True), (16, 128, 8, True), (128, 64, 2, False)])
+def test_append(hip, P, D, kv, bf16):
+    """Prompts over several pages, then tokens one by one and a few at a time,
+    in the second of two layers; the other layer and what lies behind a
+    sequence's last token stay as they were."""
+    print(f"case: append P={P} D={D} kv={kv} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(P + D + kv)
+    d = ref.Dev(hip, 2, 40, P, kv, D, 5, 6)
+    d.model.k[:] = rng.integers(0, 256, d.model.k.shape)
+    d.model.v[:] = rng.integers(0, 256, d.model.v.shape)
+    d.model.ks[:] = 2.0 ** rng.integers(-8, 3, d.model.ks.shape)
+    d.push()
+    for add in ([P, 1, 0, 2 * P + 3, P - 1], [1, 1, 1, 1, 1], [0, P, 0, 1, 2], [1, 0, 3, P + 1, 1], [1, 1, 1, 1, 1]):
+        d.reserve(add)
+        n = sum(add)
+        k, v = values(rng, n, kv, D), values(rng, n, kv, D)
+        d.append(1, k, v, bf16)
+        d.check(add)
+
+
+def test_append_growing_scale_and_special_values(hip):
+    """Later tokens larger than a page's scale holds (its codes are rounded
+    again), smaller ones, zeros, values at 448 scales, subnormals, the largest
+    floats, infinities (held at 448 scales) and NaN."""
+    print("case: append special values", flush=True)
+    D, kv = 64, 2
+    d = ref.Dev(hip, 1, 8, 16, kv, D, 3, 3)
+    rng = np.random.default_rng(4)
+    sizes = [1.0, 2.0 ** -120, 3.0, 2.0 ** 9, 448.0, 449.0, 1e-44, 0.0, 3e38, 1.0, 2.0 ** 20]
+    for i, size in enumerate(sizes):
+        d.reserve([1, 2 if i < 5 else 0, 0])
+        n = 3 if i < 5 else 1
+        k = (np.clip(rng.standard_normal((n, kv, D)), -1, 1) * size).astype(np.float32)
+        v = (np.sign(k) * size).astype(np.float32)
+        if i in (2, 6):
+            k[0, 0, :6] = [np.inf, -np.inf, np.nan, -0.0, size, -size]
+            v[0, 1, 5] = np.nan
+        d.append(0, k, v)
+        d.check((i, size))
+
+
+def test_append_rounds_every_tie_to_even(hip):
+    """All midpoints between neighbouring codes, and their neighbours in fp32."""
+    print("case: append ties", flush=True)
+    d = ref.Dev(hip, 1, 8, 32, 1, 128, 1, 4)
+    mid = ref._MID.astype(np.float32)
+    x = np.concatenate([mid, np.nextafter(mid, np.float32(1e9)), np.nextafter(mid, np.float32(0)), ref._POS])
+    x = np.concatenate([x, -x]).astype(np.float32)
+    n = -(-x.size // 127)
+    k = np.zeros((n, 1, 128), np.float32)
+    k[:, 0, 0] = 448.0                       # the scale is 1 on every page
+    k[:, 0, 1:].reshape(-1)[:] = 0
+    k[:, 0, 1:] = np.pad(x, (0, n * 127 - x.size)).reshape(n, 127)
+    d.reserve([n])
+    d.append(0, k, k * np.float32(2.0 ** -30))
+    d.check()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("pad,off", [(0, 1), (1, 0), (8, 0), (512, 8), (3, 5)])
+def test_append_strided_rows(hip, bf16, pad, off):
+    """Rows apart, as a fused projection leaves them, and off 16 bytes."""
+    print(f"case: append pad={pad} off={off} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(9)
+    d = ref.Dev(hip, 1, 8, 32, 2, 64, 2, 3)
+    d.reserve([37, 5])
+    d.append(0, values(rng, 42, 2, 64), values(rng, 42, 2, 64), bf16, pad=pad, off=off)
+    d.check()
+
+
+def test_append_skips_what_it_must_not_write(hip):
+    """Pages outside the pool or shared, rows outside [0, n_rows), rows before
+    the first token, lengths past the table row."""
+    print("case: append bad pages and rows", flush=True)
+    rng = np.random.default_rng(10)
+    d = ref.Dev(hip, 1, 12, 16, 1, 64, 8, 2)
+    m = d.model
+    m.table[:] = [[0, 1], [2, 12], [-1, 3], [4, -7], [5, 6], [7, 8], [9, 10], [11, 2 ** 31 - 1]]
+    m.refs[:12] = 1
+    m.refs[6] = 2
+    m.len[:] = [20, 32, 32, 20, 24, 3, 50, 20]
+    d.push()
+    rows = [0, 20, 52, 84, 104, 128, 136, 146, 150]      # sequence 5 has 8 rows for 3 tokens, 6 passes its table row
+    n = 148                                              # the last sequence's rows pass the end
+    d.append(0, values(rng, n, 1, 64), values(rng, n, 1, 64), rows=rows)
+    d.check()
+    d.append(0, values(rng, n, 1, 64), values(rng, n, 1, 64), rows=[-3, 20, 10, 10, 200, 3, 2 ** 31 - 1, -2 ** 31, 5])
+    d.check()
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+def filled(hip, rng, P, kv, D, lens, layers=1, spare=3, extra=1 << 22):
+    """A cache whose sequences hold lens tokens on shuffled pages; every other
+    byte of the pools, behind the last tokens too, is a NaN code or large."""
+    held = [-(-n // P) for n in lens]
+    width, pages = max(max(held), 1) + 1, max(sum(held), 1) + spare
+    d = ref.Dev(hip, layers, pages, P, kv, D, len(lens), width, extra)
+    m = d.model
+    m.k[:] = rng.choice(np.array([0x7F, 0xFF, 0x7E, 0xFE], np.uint8), m.k.shape)
+    m.v[:] = rng.choice(np.array([0x7F, 0xFF, 0x7E, 0xFE], np.uint8), m.v.shape)
+    m.ks[:] = 2.0 ** 5
+    m.vs[:] = 2.0 ** 5
+    order = list(rng.permutation(pages)[:sum(held)])
+    for s, n in enumerate(lens):
+        m.len[s] = n
+        for j in range(held[s]):
+            p = int(order.pop())
+            m.table[s, j] = p
+            m.refs[p] = 1
+            t = min(P, n - j * P)
+            e = rng.integers(-9, -5, (2, layers, kv))
+            m.k[:, p, :, :t] = ref.to_codes(rng.standard_normal((layers, kv, t, D)) / 2.0 ** e[0][..., None, None])
+            m.v[:, p, :, :t] = ref.to_codes(rng.standard_normal((layers, kv, t, D)) / 2.0 ** e[1][..., None, None])
+            m.ks[:, p], m.vs[:, p] = 2.0 ** e[0], 2.0 ** e[1]
+    d.push()
+    return d
+
+
+def starts(n):
+    return np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+
+
+def run_attn(hip, rng, P, kv, group, D, lens, n, what, layer=0, layers=1, bf16=False, behind=0, **kw):
+    d = filled(hip, rng, P, kv, D, lens, layers, extra=1 << 24)
+    rows = starts(n)
+    total = int(rows[-1]) + behind
+    q = values(rng, total, kv * group, D)
+    got = d.attn(layer, q, kv * group, bf16=bf16, rows=rows, **kw)
+    args = {k: kw[k] for k in ("causal", "window", "sinks") if k in kw}
+    want = d.model.attend(layer, q, kv * group, kw.get("scale") or D ** -0.5, args.get("causal", True),
+                          args.get("window", 0), args.get("sinks", 0), rows, total, kw.get("max_len"))
+    check_rows(got, *want, bf16, what)
+    return d, q, got
+
+
+SHAPES = [  # P, kv, group, D
+    (16, 1, 1, 64), (64, 2, 1, 128), (32, 1, 4, 128), (128, 3, 3, 64), (16, 2, 8, 128), (64, 1, 16, 64), (32, 2, 5, 64)]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("P,kv,group,D", SHAPES)
+def test_decode(hip, P, kv, group, D, bf16):
+    """One token of each sequence: lengths 1 to several chunks, around every
+    tile and page edge; a sequence without a row; rows behind the last one."""
+    print(f"case: decode P={P} kv={kv} group={group} D={D} bf16={bf16}", flush=True)
+    lens = [1, 2, 15, 16, 17, 31, 32, 33, 40, 63, 64, 65, 127, 129, 257, 511, 513, 1030]
+    n = [1] * len(lens)
+    n[8] = 0
+    run_attn(hip, np.random.default_rng(P + kv + group), P, kv, group, D, lens, n, "decode", layer=1, layers=2,
+             bf16=bf16, behind=2)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("P,kv,group,D", SHAPES)
+def test_several_rows(hip, P, kv, group, D, bf16):
+    """A few new tokens on held ones, whole prompts, and none, together."""
+    print(f"case: rows P={P} kv={kv} group={group} D={D} bf16={bf16}", flush=True)
+    lens = [3, 70, 33, 300, 5, 64]
+    n = [3, 7, 33, 40, 0, 64]
+    run_attn(hip, np.random.default_rng(P + kv + group), P, kv, group, D, lens, n, "rows", bf16=bf16, behind=3)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (5, 3), (16, 4), (33, 64), (100, 33), (64, 500), (2000, 4),
+                                          (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_window(hip, window, sinks, bf16):
+    """Windows and first tokens around the tile and page edges, single rows and prompts."""
+    print(f"case: window={window} sinks={sinks} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(window % 1000 + sinks % 1000)
+    run_attn(hip, rng, 16, 2, 3, 64, [1, 40, 129, 300, 700], [1, 1, 1, 1, 1], "one row", window=window, sinks=sinks, bf16=bf16)
+    run_attn(hip, rng, 32, 1, 2, 128, [1, 90, 200, 333], [1, 90, 30, 130], "prompt", window=window, sinks=sinks, bf16=bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_not_causal(hip, bf16):
+    """Every row sees all tokens: encoder frames; a sequence of none gives zeros."""
+    print(f"case: not causal bf16={bf16}", flush=True)
+    rng = np.random.default_rng(3)
+    _, _, got = run_attn(hip, rng, 32, 2, 1, 128, [376, 0, 1, 33], [1, 1, 1, 1], "one", causal=False, bf16=bf16)
+    assert np.all(got[1] == 0.0)
+    _, _, got = run_attn(hip, rng, 64, 1, 4, 64, [100, 0, 1, 700], [9, 3, 2, 40], "more", causal=False, bf16=bf16)
+    assert np.all(got[9:12] == 0.0)
+
+
+def test_max_len_hides_what_is_past_it(hip):
+    print("case: max_len", flush=True)
+    rng = np.random.default_rng(5)
+    run_attn(hip, rng, 32, 1, 2, 64, [100, 40, 700], [1, 1, 1], "cut", causal=False, max_len=64)
+    run_attn(hip, rng, 32, 1, 2, 64, [100, 40, 700], [1, 1, 1], "cut at an odd length", causal=False, max_len=83)
+
+
+@pytest.mark.parametrize("pad,off", [(1, 1), (8, 0), (64, 8), (0, 3)])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_strided_rows(hip, pad, off, bf16):
+    print(f"case: strides pad={pad} off={off} bf16={bf16}", flush=True)
+    run_attn(hip, np.random.default_rng(6), 32, 2, 2, 64, [40, 100], [1, 1], "one", pad=pad, off=off, bf16=bf16)
+    run_attn(hip, np.random.default_rng(6), 32, 2, 2, 64, [40, 100], [40, 30], "more", pad=pad, off=off, bf16=bf16)
+
+
+@pytest.mark.parametrize("n", [[1, 1, 1, 1], [30, 20, 64, 90]])
+def test_pages_that_are_not_there(hip, n):
+    """Table entries -1 or outside the pool hide their tokens; a row that sees
+    none of its tokens gets zeros."""
+    print(f"case: missing pages n={n}", flush=True)
+    rng = np.random.default_rng(7)
+    d = filled(hip, rng, 16, 1, 64, [30, 50, 64, 200])
+    m = d.model
+    m.table[0] = -1
+    m.table[1, 2] = m.dims[1]
+    m.table[2, :] = [2 ** 31 - 1, m.table[2, 1], -5, -2 ** 31] + [-1] * (m.dims[6] - 4)
+    m.table[3, [0, 5, 12]] = -1
+    d.push()
+    rows = starts(n)
+    q = values(rng, int(rows[-1]), 2, 64)
+    got = d.attn(0, q, 2, rows=rows)
+    check_rows(got, *m.attend(0, q, 2, 0.125, True, 0, 0, rows, len(q)), False, "missing")
+    assert np.all(got[:n[0]] == 0.0)
+
+
+def test_bad_rows_and_lengths(hip):
+    """Rows outside [0, n_rows), lengths below the rows or past the table: what
+    is not followed is left, the other sequences are right."""
+    print("case: bad rows", flush=True)
+    rng = np.random.default_rng(8)
+    for max_rows in (1, 40):
+        d = filled(hip, rng, 16, 1, 64, [30, 50, 20, 16, 48], extra=1 << 23)
+        m = d.model
+        m.len[:] = [30, 2 ** 31 - 1, -4, 0, 48]
+        d.push()
+        rows = np.array([0, 1, 2, 3, 4, 5], np.int32)
+        q = values(rng, 5, 1, 64)
+        got = d.attn(0, q, 1, rows=rows, max_rows=max_rows, causal=False)
+        check_rows(got, *m.attend(0, q, 1, 0.125, False, 0, 0, rows, 5), False, "lengths")
+        rows = np.array([-1, 3, 2, 6, 4, 5], np.int32)
+        m.len[:] = [30, 50, 20, 16, 48]
+        d.push()
+        got = d.attn(0, q, 1, rows=rows, max_rows=max_rows)
+        check_rows(got, *m.attend(0, q, 1, 0.125, True, 0, 0, rows, 5), False, "rows")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_values_that_are_not_finite(hip, bf16):
+    """NaN in a token reaches the rows that see it and no other, in V only its
+    dim; a query row with an infinity or NaN is NaN alone."""
+    print(f"case: NaN bf16={bf16}", flush=True)
+    rng = np.random.default_rng(12)
+    d = filled(hip, rng, 32, 1, 64, [100, 90, 80, 70])
+    m = d.model
+    m.v[0, m.table[0, 2], 0, 20, 7] = 0x7F          # token 84: rows 84.. see it
+    m.v[0, m.table[0, 0], 0, 3, 9] = 0xFF           # token 3: with the window, the sinks do not reach it
+    m.k[0, m.table[1, 2], 0, 16, 0] = 0x7F          # token 80
+    d.push()
+    n = [30, 20, 5, 1]
+    rows = starts(n)
+    q = values(rng, int(rows[-1]), 3, 64)
+    q[52, 1, 5] = np.inf
+    q[53, 0, 63] = np.nan
+    q[54, 2, 0] = -np.inf
+    for window, sinks in ((0, 0), (40, 2), (40, 5)):
+        got = d.attn(0, q, 3, rows=rows, bf16=bf16, window=window, sinks=sinks)
+        want = m.attend(0, q, 3, 0.125, True, window, sinks, rows, len(q))
+        check_rows(got, *want, bf16, (window, sinks))
+        assert np.isnan(got[14:30, :, 7]).all() and np.isfinite(got[:14, :, 7]).all()
+    m.v[0, m.table[3, 1], 0, 5, 2] = 0x7F
+    d.push()
+    got = d.attn(0, q[:4], 3, rows=[0, 1, 2, 3, 4], bf16=bf16)
+    check_rows(got, *m.attend(0, q[:4], 3, 0.125, True, 0, 0, [0, 1, 2, 3, 4], 4), bf16, "one row")
+
+
+def test_scales_far_apart(hip):
+    """Pages whose scales differ by up to 2^24, large and small scores, query
+    rows of every size."""
+    print("case: scales", flush=True)
+    rng = np.random.default_rng(13)
+    for size in (1e-30, 1e-3, 1.0, 1e4):
+        d = filled(hip, rng, 16, 1, 64, [200, 64])
+        m = d.model
+        m.vs[:] = 2.0 ** rng.integers(-20, 5, m.vs.shape)
+        d.push()
+        q = (values(rng, 33, 2, 64) * np.float32(size)).astype(np.float32)
+        for rows in (np.array([0, 1, 2], np.int32), np.array([0, 20, 33], np.int32)):
+            got = d.attn(0, q, 2, rows=rows, scale=0.125 / size)
+            check_rows(got, *m.attend(0, q, 2, 0.125 / size, True, 0, 0, rows, 33), False, size)
+
+
+def test_a_sequence_alone_and_in_a_batch_gives_the_same_bits(hip):
+    """Single-token rows: the same sequences, in other company and on other pages."""
+    print("case: batch invariance", flush=True)
+    rng = np.random.default_rng(14)
+    lens = [700, 33, 1030, 5]
+    d = filled(hip, rng, 32, 2, 128, lens, spare=8)
+    q = values(rng, 4, 4, 128)
+    both = d.attn(0, q, 4, rows=[0, 1, 2, 3, 4])
+    for s in range(4):
+        rows = [0] * (s + 1) + [1] * (4 - s)
+        alone = d.attn(0, q[s:s + 1], 4, rows=rows)
+        assert np.array_equal(alone[0].view(np.uint32), both[s].view(np.uint32)), s
+    d.hip.backend_kv8_compact(d.h)
+    d.model.compact()
+    d.check("compacted")
+    moved = d.attn(0, q, 4, rows=[0, 1, 2, 3, 4])
+    assert np.array_equal(moved.view(np.uint32), both.view(np.uint32))
+
+
+def test_pool_past_32_bit_offsets(hip):
+    """A layer's pool of more than 4 GiB: appended, attended, forked and
+    compacted at its far end."""
+    print("case: large pool", flush=True)
+    rng = np.random.default_rng(15)
+    P, kv, D = 128, 8, 128
+    pages = 33000                                     # 4.33 GB of K
+    c = cb.BackendKv8(layers=1, pages=pages, page_tokens=P, kv_heads=kv, head_dim=D, seqs=2, table_w=3)
+    h = C.byref(c)
+    n = hip.backend_kv8_floats(h)
+    base = hip.backend_arena_alloc(n + (1 << 22))
+    hip.backend_kv8_bind(h, base)
+    d = ref.Dev.__new__(ref.Dev)
+    d.hip, d.c, d.h, d.at, d.end = hip, c, h, base + (n + 63) // 64 * 256, base + (n + (1 << 22)) * 4
+    # the far pages of a small model stand for the last ones of the pool
+    d.model = m = ref.Cache(1, 8, P, kv, D, 2, 3)
+    shift = pages - 8
+    refs = np.ones(pages, np.int32)
+    refs[[1, pages - 5, pages - 1]] = 0               # one near page and two far ones are free
+    table = np.array([[pages - 8, pages - 3, -1], [pages - 2, -1, -1]], np.int32)
+    for ptr, x in ((c.refs, refs), (c.table, table), (c.len, np.array([140, 9], np.int32))):
+        d.write(ptr, x)
+    m.table[:] = np.where(table >= 0, table - shift, -1)
+    m.refs[:] = 1
+    m.len[:] = [140, 9]
+    k, v = values(rng, 149, kv, D), values(rng, 149, kv, D)
+    d.append(0, k, v, rows=[0, 140, 149])
+    q = values(rng, 2, 8, D)
+    got = d.attn(0, q, 8, rows=[0, 1, 2])
+    want = m.attend(0, q, 8, D ** -0.5, True, 0, 0, [0, 1, 2], 2)
+    check_rows(got, *want, False, "far pages")
+    # sequence 1 becomes a copy of sequence 0: its partly filled page goes to page 1
+    hip.backend_kv8_fork(h, d.ints([1]), d.ints([0]), 1)
+    t = d.get(c.table, (2, 3), np.int32)
+    assert t.tolist() == [[pages - 8, pages - 3, -1], [pages - 8, 1, -1]]
+    again = d.attn(0, q[[0, 0]], 8, rows=[0, 1, 2])
+    assert np.array_equal(again[1].view(np.uint32), got[0].view(np.uint32))
+    # three pages are free now (pages - 5, pages - 2, pages - 1): page pages - 3 moves to pages - 5
+    hip.backend_kv8_compact(h)
+    r = d.get(c.refs, (pages,), np.int32)
+    assert r[:pages - 3].all() and not r[pages - 3:].any()
+    assert d.get(c.table, (2, 3), np.int32).tolist() == [[pages - 8, pages - 5, -1], [pages - 8, 1, -1]]
+    third = d.attn(0, q[[0, 0]], 8, rows=[0, 1, 2])
+    assert np.array_equal(third.view(np.uint32), again.view(np.uint32))
+    assert hip.backend_kv8_status(h) == 0
+
+
+# ---------------------------------------------------------------------------
+# pages
+# ---------------------------------------------------------------------------
+def test_reserve(hip):
+    """Pages in order, all or nothing, and what a refused step does."""
+    print("case: reserve", flush=True)
+    d = ref.Dev(hip, 1, 11, 16, 1, 64, 4, 5)
+    for add in ([1, 16, 0, 17], [15, 1, 0, 0], [1, 0, 16, 0], [0, 0, 0, 0], [0, 0, 64, 64], [200, 0, 0, 0], [0, -1, 0, 0],
+                [2 ** 31 - 1, 0, 0, 0], [-2 ** 31, -1, 5, 5], [0, 14, 16, 0], [1, 1, 1, 1]):
+        d.reserve(add)
+        d.check(add)
+    d.model.rows[:] = d.get(d.c.rows, (5,), np.int32)
+    x = np.ones((4, 1, 64), np.float32)
+    d.reserve([70, 70, 0, 0])                        # no room in the rows: the step does nothing
+    before = d.state()
+    d.append(0, x, x)
+    assert np.all(d.attn(0, values(np.random.default_rng(0), 4, 1, 64), 1, max_rows=4) == 55.0)
+    after = d.state()
+    assert all(np.array_equal(before[k], after[k]) for k in before)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_page_calls_together(hip, seed):
+    """Random reserve, append, fork, free, trim and compact calls against the
+    model, with pools that run out, swaps, chains, repeated and bad numbers."""
+    rng = np.random.default_rng(seed)
+    P = [16, 32, 64, 128, 16, 32][seed]
+    pages, seqs, width, kv, layers = int(rng.integers(20, 70)), int(rng.integers(2, 9)), 9, 2, 2
+    print(f"case: pages seed={seed} P={P} pages={pages} seqs={seqs}", flush=True)
+    d = ref.Dev(hip, layers, pages, P, kv, 64, seqs, width, extra=1 << 23)
+    for step in range(40):
+        do = rng.choice(["add", "add", "add", "fork", "fork", "free", "trim", "compact"])
+        if do == "add":
+            add = [int(rng.choice([0, 1, 1, P // 3, P + 1, 3 * P])) for _ in range(seqs)]
+            d.reserve(add)
+            n = int(d.model.rows[-1])
+            if n:
+                for lay in range(layers):
+                    d.append(lay, values(rng, n, kv, 64), values(rng, n, kv, 64))
+        elif do == "fork":
+            n = int(rng.integers(1, seqs + 1))
+            dst = [int(x) for x in rng.permutation(seqs)[:n]]
+            src = [int(x) for x in rng.integers(0, seqs, n)]
+            if rng.random() < 0.1:
+                src[0] = int(rng.choice([-1, seqs, 2 ** 31 - 1]))
+            if n > 1 and rng.random() < 0.1:
+                dst[1] = dst[0]
+            d.hip.backend_kv8_fork(d.h, d.ints(dst), d.ints(src), n)
+            d.model.fork(dst, src)
+        elif do == "free":
+            which = [int(x) for x in rng.integers(0, seqs, int(rng.integers(1, 3)))]
+            if rng.random() < 0.2:
+                which[0] = int(rng.choice([-1, seqs]))
+            d.hip.backend_kv8_free(d.h, d.ints(which), len(which[:seqs]))
+            d.model.free(which[:seqs])
+        elif do == "trim":
+            window, sinks = int(rng.integers(1, 4 * P)), int(rng.integers(0, P + 2))
+            d.hip.backend_kv8_trim(d.h, window, sinks)
+            d.model.trim(window, sinks)
+        else:
+            d.hip.backend_kv8_compact(d.h)
+            d.model.compact()
+        assert all(d.model.refs[p] == np.sum(d.model.table == p) for p in range(pages))
+        d.check((step, do))
+
+
+def test_many_pages_and_long_rows(hip):
+    """Tables wider than a workgroup and pools larger than one: more pages than
+    the planning workgroup has threads."""
+    print("case: many pages", flush=True)
+    rng = np.random.default_rng(20)
+    d = ref.Dev(hip, 1, 5000, 16, 1, 64, 6, 1200, extra=1 << 24)
+    m = d.model
+    d.reserve([16 * 900, 16 * 300 + 5, 0, 7, 16 * 1100, 0])
+    d.check_book("reserve")
+    dst, src = [2, 0, 3], [0, 1, 4]
+    d.hip.backend_kv8_fork(d.h, d.ints(dst), d.ints(src), 3)
+    m.fork(dst, src)
+    d.check_book("fork")
+    d.hip.backend_kv8_trim(d.h, 1000, 100)
+    m.trim(1000, 100)
+    d.check_book("trim")
+    m.k[:] = rng.integers(0, 127, m.k.shape)
+    m.vs[:] = rng.random(m.vs.shape)
+    d.push()
+    d.hip.backend_kv8_compact(d.h)
+    m.compact()
+    d.check("compact")
+    d.hip.backend_kv8_free(d.h, d.ints([0, 2, 4]), 3)
+    m.free([0, 2, 4])
+    d.check_book("free")
+
+
+def test_plan_and_empty_calls(hip):
+    """Calls with nothing to do: no rows, no pairs, an empty cache."""
+    print("case: empty calls", flush=True)
+    d = ref.Dev(hip, 1, 4, 16, 1, 64, 2, 2)
+    x = np.zeros((0, 1, 64), np.float32)
+    d.hip.backend_kv8_fork(d.h, None, None, 0)
+    d.hip.backend_kv8_free(d.h, None, 0)
+    d.hip.backend_kv8_trim(d.h, 1, 0)
+    d.hip.backend_kv8_compact(d.h)
+    d.reserve([0, 0])
+    d.hip.backend_kv8_append(d.h, 0, None, None, 64, 0, d.c.rows, 0)
+    d.hip.backend_kv8_free(d.h, d.ints([1, 1]), 2)
+    dst = [0, 1]
+    d.hip.backend_kv8_fork(d.h, d.ints(dst), d.ints([1, 0]), 2)
+    d.check()
+    assert x.size == 0
+
+
+# ---------------------------------------------------------------------------
+# together, as a program uses them
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("bf16", [False, True])
+def test_beam_search_run(hip, bf16):
+    """A clip's prompt, then beams that fork at every step: each layer's new
+    rows appended and attended, the window's old pages given back, the pool
+    compacted on the way; every step's rows within the tolerance and the state
+    the model's."""
+    print(f"case: beam run bf16={bf16}", flush=True)
+    rng = np.random.default_rng(30)
+    layers, kv, group, D, P, beams = 2, 2, 2, 64, 16, 4
+    d = ref.Dev(hip, layers, 48, P, kv, D, beams, 8, extra=1 << 24)
+    window, sinks = 40, 3
+
+    def layer_step(n):
+        for lay in range(layers):
+            d.append(lay, values(rng, n, kv, D), values(rng, n, kv, D), bf16)
+            q = values(rng, n, kv * group, D)
+            got = d.attn(lay, q, kv * group, bf16=bf16, window=window, sinks=sinks)
+            check_rows(got, *d.model.attend(lay, q, kv * group, D ** -0.5, True, window, sinks, d.model.rows, n), bf16, lay)
+
+    d.reserve([23, 0, 0, 0])
+    layer_step(23)
+    dst, src = [1, 2, 3], [0, 0, 0]
+    d.hip.backend_kv8_fork(d.h, d.ints(dst), d.ints(src), 3)
+    d.model.fork(dst, src)
+    for step in range(30):
+        d.reserve([1] * beams)
+        layer_step(beams)
+        parents = [int(x) for x in rng.integers(0, beams, beams)]
+        d.hip.backend_kv8_fork(d.h, d.ints(range(beams)), d.ints(parents), beams)
+        d.model.fork(list(range(beams)), parents)
+        if step % 7 == 6:
+            d.hip.backend_kv8_trim(d.h, window, sinks)
+            d.model.trim(window, sinks)
+            d.hip.backend_kv8_compact(d.h)
+            d.model.compact()
+        d.check(step)
+
+
+def test_captured_step(hip):
+    """A step (reserve, append, attention in two layers) captured once and
+    replayed as the texts grow, with eager work and waits in between: the bits
+    of the same steps run eagerly."""
+    print("case: captured step", flush=True)
+    layers, kv, D, P, seqs = 2, 2, 64, 16, 3
+
+    def program(graph):
+        d = ref.Dev(hip, layers, 40, P, kv, D, seqs, 10, extra=1 << 22)
+        r = np.random.default_rng(32)
+        d.reserve([20, 1, 40])
+        for lay in range(layers):
+            d.append(lay, values(r, 61, kv, D), values(r, 61, kv, D))
+        add, x = d.ints([1] * seqs), d.put(np.zeros((3, seqs, kv * D), np.float32))
+        out = d.put(np.zeros((layers, seqs, kv * D), np.float32))
+        step = seqs * kv * D * 4
+        calls = []
+        for lay in range(layers):
+            a = cb.BackendKv8Attn(out=out + lay * step, q=x, ld_out=kv * D, ld_q=kv * D, heads=kv, scale=0.125, causal=1,
+                                  rows=d.c.rows, n_rows=seqs, max_rows=1)
+            a.work = d.take(hip.backend_kv8_attn_work(d.h, C.byref(a)) * 4 + 16)
+            calls.append(a)
+
+        def region():
+            hip.backend_kv8_reserve(d.h, add)
+            for lay in range(layers):
+                hip.backend_kv8_append(d.h, lay, x + step, x + 2 * step, kv * D, 0, d.c.rows, seqs)
+                hip.backend_kv8_attn(d.h, lay, C.byref(calls[lay]))
+
+        got = []
+        for i in range(25):
+            d.write(x, values(r, 3, seqs, kv * D))
+            if not graph:
+                region()
+            elif not hip.backend_graph_replay(9, 1, 1, seqs):
+                hip.backend_graph_begin_capture(9)
+                region()
+                hip.backend_graph_end_capture(9, 1, 1, seqs)
+            got.append(d.get(out, (layers, seqs, kv * D), np.float32))
+            if i % 5 == 2:
+                hip.backend_add_inplace(d.put(np.ones(64, np.float32)), d.put(np.ones(64, np.float32)), 64)
+        return np.stack(got), d.state()
+
+    (a, sa), (b, sb) = program(False), program(True)
+    assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+    assert all(np.array_equal(sa[k], sb[k]) for k in sa)
+    assert np.isfinite(a).all()

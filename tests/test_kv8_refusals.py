@@ -1,0 +1,126 @@
+"""Refusals of the paged 8-bit cache's calls, and its 64-bit model (no GPU
+needed: the checks run before any device work)."""
+import ctypes as C
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+import ctbind as cb
+import kv8_ref as ref
+
+GOOD = dict(layers=2, pages=8, page_tokens=16, kv_heads=2, head_dim=64, seqs=3, table_w=4)
+PTRS = dict(k=4096, v=8192, kscale=4096, vscale=4096, table=4096, len=4096, refs=4096, rows=4096, plan=4096)
+CALL = dict(out=4096, q=4096, ld_out=128, ld_q=128, heads=2, scale=0.125, causal=1, rows=4096, n_rows=4, max_rows=2,
+            work=4096)
+
+
+def program(call, cache=None, attn=None):
+    c = {**GOOD, **PTRS, **(cache or {})}
+    a = {**CALL, **(attn or {})}
+    return (f"import sys; sys.path.insert(0, {cb.PKG_DIR!r}); import ctypes as C, ctbind as cb; L = cb.hip(); "
+            f"c = cb.BackendKv8(**{c!r}); h = C.byref(c); nan = float('nan'); a = cb.BackendKv8Attn(**{a!r}); p = C.byref(a); {call}; print('returned')")
+
+
+APPEND = "L.backend_kv8_append(h, 0, 4096, 4096, 128, 0, 4096, 4)"
+ATTN = "L.backend_kv8_attn(h, 0, p)"
+CASES = {
+    "no_cache": ("L.backend_kv8_compact(None)", {}, {}, "no cache"),
+    "layers": (APPEND, dict(layers=0), {}, "layers outside"),
+    "pages": (APPEND, dict(pages=0), {}, "pages outside"),
+    "pages_many": ("L.backend_kv8_floats(h)", dict(pages=(1 << 24) + 1), {}, "pages outside"),
+    "page_tokens": ("L.backend_kv8_plan_ints(h)", dict(page_tokens=48), {}, "page_tokens is not"),
+    "head_dim": (ATTN, dict(head_dim=160), {}, "head_dim is not"),
+    "kv_heads": (ATTN, dict(kv_heads=257), {}, "kv_heads outside"),
+    "seqs": (APPEND, dict(seqs=257), {}, "seqs outside"),
+    "table_w": (APPEND, dict(table_w=0), {}, "table_w outside"),
+    "table_w_long": (APPEND, dict(table_w=(1 << 20) + 1), {}, "table_w outside"),
+    "null_pool": (APPEND, dict(v=0), {}, "a pointer of the cache is NULL"),
+    "null_plan": ("L.backend_kv8_trim(h, 1, 0)", dict(plan=0), {}, "a pointer of the cache is NULL"),
+    "pool_alignment": (APPEND, dict(k=4104), {}, "not 16-byte aligned"),
+    "bind_null": ("L.backend_kv8_bind(h, None)", {}, {}, "memory is NULL"),
+    "bind_alignment": ("L.backend_kv8_bind(h, 4100)", {}, {}, "not 16-byte aligned"),
+    "reserve_null": ("L.backend_kv8_reserve(h, None)", {}, {}, "add or the cache's rows"),
+    "reserve_rows": ("L.backend_kv8_reserve(h, 4096)", dict(rows=0), {}, "add or the cache's rows"),
+    "append_layer": ("L.backend_kv8_append(h, 2, 4096, 4096, 128, 0, 4096, 4)", {}, {}, "layer outside"),
+    "append_layer_negative": ("L.backend_kv8_append(h, -1, 4096, 4096, 128, 0, 4096, 4)", {}, {}, "layer outside"),
+    "append_rows_null": ("L.backend_kv8_append(h, 0, 4096, 4096, 128, 0, None, 4)", {}, {}, "rows are NULL"),
+    "append_rows_negative": ("L.backend_kv8_append(h, 0, 4096, 4096, 128, 0, 4096, -1)", {}, {}, "n_rows outside"),
+    "append_rows_many": ("L.backend_kv8_append(h, 0, 4096, 4096, 128, 0, 4096, (1 << 24) + 1)", {}, {}, "n_rows outside"),
+    "append_null": ("L.backend_kv8_append(h, 0, 4096, None, 128, 0, 4096, 4)", {}, {}, "k or v is NULL"),
+    "append_alignment": ("L.backend_kv8_append(h, 0, 4098, 4096, 128, 0, 4096, 4)", {}, {}, "not aligned"),
+    "append_alignment_bf16": ("L.backend_kv8_append(h, 0, 4097, 4096, 128, 1, 4096, 4)", {}, {}, "not aligned"),
+    "append_ld": ("L.backend_kv8_append(h, 0, 4096, 4096, 127, 0, 4096, 4)", {}, {}, "ld below"),
+    "attn_null_call": ("L.backend_kv8_attn(h, 0, None)", {}, {}, "no arguments"),
+    "attn_heads": (ATTN, {}, dict(heads=3), "heads is not a multiple"),
+    "attn_heads_none": (ATTN, {}, dict(heads=0), "heads is not a multiple"),
+    "attn_rows_many": ("L.backend_kv8_attn_work(h, p)", {}, dict(n_rows=1 << 24, heads=16), "n_rows * heads above"),
+    "attn_rows_negative": (ATTN, {}, dict(n_rows=-1), "n_rows outside"),
+    "attn_max_rows": (ATTN, {}, dict(max_rows=0), "max_rows < 1"),
+    "attn_max_len": (ATTN, {}, dict(max_len=-1), "max_len < 0"),
+    "attn_window": (ATTN, {}, dict(window=-1), "window or sinks < 0"),
+    "attn_sinks": (ATTN, {}, dict(sinks=-1), "window or sinks < 0"),
+    "attn_window_causal": (ATTN, {}, dict(window=4, causal=0), "a window needs causal rows"),
+    "attn_scale_zero": (ATTN, {}, dict(scale=0.0), "scale is not positive"),
+    "attn_scale_nan": (ATTN, {}, dict(scale=float("nan")), "scale is not positive"),
+    "attn_rows_null": (ATTN, {}, dict(rows=0), "rows are NULL"),
+    "attn_q": (ATTN, {}, dict(q=0), "q or out is NULL"),
+    "attn_out_alignment": (ATTN, {}, dict(out=4098), "not aligned"),
+    "attn_ld": (ATTN, {}, dict(ld_q=127), "ld_q or ld_out below"),
+    "attn_layer": ("L.backend_kv8_attn(h, 5, p)", {}, {}, "layer outside"),
+    "attn_work": (ATTN, dict(table_w=4096), dict(work=0), "work is NULL"),
+    "attn_work_alignment": (ATTN, dict(table_w=4096), dict(work=4100), "work is NULL or not 16-byte"),
+    "fork_n": ("L.backend_kv8_fork(h, 4096, 4096, 4)", {}, {}, "n outside"),
+    "fork_null": ("L.backend_kv8_fork(h, 4096, None, 2)", {}, {}, "dst or src is NULL"),
+    "free_n": ("L.backend_kv8_free(h, 4096, -1)", {}, {}, "n outside"),
+    "free_null": ("L.backend_kv8_free(h, None, 1)", {}, {}, "seqs is NULL"),
+    "trim_window": ("L.backend_kv8_trim(h, 0, 0)", {}, {}, "window < 1"),
+    "trim_sinks": ("L.backend_kv8_trim(h, 4, -1)", {}, {}, "window < 1 or sinks < 0"),
+    "before_init": (APPEND, {}, {}, "has not called backend_init"),
+    "before_init_attn": (ATTN, {}, {}, "has not called backend_init"),
+    "stream_before_init": ("L.backend_stream()", {}, {}, "has not called backend_init"),
+}
+
+
+@pytest.mark.parametrize("case", sorted(CASES))
+def test_refused_before_device_work(case):
+    call, cache, attn, msg = CASES[case]
+    r = subprocess.run([sys.executable, "-c", program(call, cache, attn)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 1, (r.returncode, r.stdout, r.stderr)
+    assert msg in r.stderr, r.stderr
+    assert "returned" not in r.stdout
+
+
+def test_sizes():
+    """The arena's share covers the arrays; more rows, tokens or heads never take less work."""
+    L = cb.hip()
+    c = cb.BackendKv8(**GOOD)
+    h = C.byref(c)
+    pool = 2 * 8 * 2 * 16 * 64
+    least = 2 * pool // 4 + 2 * (2 * 8 * 2) + 3 * 4 + 3 + 8 + 4 + L.backend_kv8_plan_ints(h)
+    assert least <= L.backend_kv8_floats(h) <= least + 4 * 9
+    big = cb.BackendKv8(**{**GOOD, "pages": 1 << 24, "page_tokens": 128, "head_dim": 128, "kv_heads": 8})
+    assert L.backend_kv8_floats(C.byref(big)) > 2 * (1 << 24) * 2 * 8 * 128 * 128 // 4       # past 32 bits
+    c.table_w = 4096
+    work = []
+    for n, heads in ((1, 2), (3, 2), (3, 8), (40, 8), (400, 8)):
+        a = cb.BackendKv8Attn(**{**CALL, "n_rows": n, "max_rows": n, "heads": heads, "ld_q": 512, "ld_out": 512})
+        work.append(L.backend_kv8_attn_work(h, C.byref(a)))
+    assert work[0] > 0
+    # one chunk needs none, whatever the pointers
+    short = cb.BackendKv8Attn(**{**CALL, "max_len": 40})
+    assert L.backend_kv8_attn_work(h, C.byref(short)) == 0
+
+
+def test_model_rounding():
+    """The model's rounding against the definition: every code is its own
+    nearest, midpoints go to the even code, values past the largest are held."""
+    fine = np.array([c for c in range(256) if c & 0x7F != 0x7F], np.uint8)
+    assert np.array_equal(ref.to_codes(ref.E4M3[fine]), fine)
+    mid = ref.to_codes(ref._MID)
+    assert np.all(mid % 2 == 0)
+    below, above = np.nextafter(ref._MID, 0), np.nextafter(ref._MID, 1e9)
+    assert np.array_equal(ref.to_codes(below), np.arange(126)) and np.array_equal(ref.to_codes(above), np.arange(1, 127))
+    assert ref.to_codes([449, np.inf, -np.inf, np.nan, -0.0]).tolist() == [0x7E, 0x7E, 0xFE, 0x7F, 0x80]
+    assert ref.need_exp([448.0]) == 0 and ref.need_exp([448.1, np.inf]) == 1 and ref.need_exp([0.0]) == -100
