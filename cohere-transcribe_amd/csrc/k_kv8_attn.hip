@@ -6,7 +6,8 @@
 //                 % 16, g = lane / 16, holds query c's scores of keys 4g..4g+3
 //                 of each half;
 //   P             online softmax in base 2; the four lanes of a query share
-//                 one running maximum;
+//                 one running maximum, which follows the scores only when
+//                 they pass it by 2^8 (most steps then rescale nothing);
 //   O^T += V^T P^T  the same lane's eight p are one B operand if the product's
 //                 k index runs over keys {4g..4g+3, 16+4g..16+4g+3}, so P
 //                 never leaves its lane; V's rows are loaded to match, 8 dims
@@ -16,8 +17,8 @@
 // are those of the codes.  Scales are powers of two and never touch a code:
 // the key scale multiplies the score; the value scale is an offset of the
 // softmax exponent, relative to a running reference exponent (eref) of the
-// sums: p' = 2^(s - m + 14 + e - eref) enters the product, O counts in units
-// of 2^(eref - 14).  Query rows are brought to a largest value in [2^12, 2^13)
+// sums: p' = 2^(s - m + 6 + e - eref) <= 2^14 enters the product, O counts in
+// units of 2^(eref - 6).  Query rows are brought to a largest value in [2^12, 2^13)
 // by a power of two.  fp32 rows enter as the sum of two f16 (22 bits and
 // more), and so do their p; bf16 rows are one f16 each, exactly, and so p.
 #include "ct_dev.h"
@@ -27,11 +28,15 @@
 namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int NT = 256, NW = NT / CT_WAVE;   // threads, wavefronts of a workgroup
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int P_EXP = 14;                    // p' is at most 2^14
+constexpr int P_EXP = 6;                     // p' is at most 2^(P_EXP + SLACK), within f16
+constexpr int SLACK = 8;                     // how far scores may pass the running maximum, in bits
 
 struct Args {
     const uint8_t *k, *v;        // the layer's pools
@@ -43,8 +48,10 @@ struct Args {
     long ld_q, ld_out;
     int group, causal, window, sinks, n_rows, cap;   // cap: tokens looked at
     float scale2;                // scale * log2(e)
+    int vec;                     // q rows are 16-byte aligned
     int one_tile;                // every sequence's rows fit one tile: tile = sequence
     int chunk, nchunk;           // 32-key steps of a chunk, chunks of the grid
+    int tile_rows;               // packed rows of a tile: 16 or rows_of(bf16)
     int rpt;                     // rows of a tile kept in the partial results
     float *part;                 // partial O [tile][kv][chunk][rpt][D], then (m, l) pairs
     float2 *stat;
@@ -162,12 +169,241 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7
 // V as D / 16 dims of keys 4g + j (j < 4) and 16 + 4g + j - 4.
 template <int D>
 struct Raw {
-    uint4 k[2][D / 64];
+    u32x4 k[2][D / 64];
     uint32_t v[8][D / 64];
 };
 
+// The query row at element `off`, as this lane's dims of a B operand.
 template <int D, bool BF16>
-__global__ __launch_bounds__(NT) void attn_kernel(Args a) {
+__device__ __forceinline__ void fetch_query(const Args &a, long off, int g, float (&x)[D / 32][8]) {
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+        const long d = off + 64 * (i >> 1) + 16 * g + 8 * (i & 1);
+        if (BF16) {
+            const uint16_t *q = reinterpret_cast<const uint16_t *>(a.q) + d;
+            u16x8 y;
+            if (a.vec) y = *reinterpret_cast<const u16x8 *>(q);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = q[j];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[i][j] = bf2f(y[j]);
+        } else {
+            const float *q = reinterpret_cast<const float *>(a.q) + d;
+            if (a.vec) {
+                const f32x4 y = reinterpret_cast<const f32x4 *>(q)[0], z = reinterpret_cast<const f32x4 *>(q)[1];
+#pragma unroll
+                for (int j = 0; j < 4; j++) { x[i][j] = y[j]; x[i][4 + j] = z[j]; }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[i][j] = q[j];
+            }
+        }
+    }
+}
+
+// Brings the row to a largest value in [2^12, 2^13) and splits it into f16
+// terms; returns the factor of its scores: what the power of two and the
+// softmax scale leave.  A row with a value that is not finite is all NaN.
+template <int D, bool BF16>
+__device__ __forceinline__ float split_query(const Args &a, bool have, const float (&x)[D / 32][8],
+                                             f16x8 (&qf)[BF16 ? 1 : 2][D / 32]) {
+    constexpr int KS = D / 32, NB = BF16 ? 1 : 2;
+    // the largest magnitude as an integer: infinities and NaN are the largest
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < KS; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[i][j]) & 0x7fffffffu);
+    if (!have) top = 0;
+    auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+    top = max(r[0], r[1]);
+    r = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+    top = max(r[0], r[1]);
+    const bool fine = top < 0x7f800000u;
+    // exponent of the row's largest value (zero and subnormal rows: 2^-126)
+    const int e = fine ? max((int)(top >> 23), 1) - 127 : 0;
+    const int up = 12 - e;                   // in [-115, 138]: two factors
+    const float f0 = pow2i(up >> 1), f1 = pow2i(up - (up >> 1));
+#pragma unroll
+    for (int i = 0; i < KS; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float y = !have ? 0.0f : fine ? x[i][j] * f0 * f1 : __uint_as_float(0x7fc00000u);
+            qf[0][i][j] = (_Float16)y;
+            if (NB > 1) qf[NB - 1][i][j] = (_Float16)(y - (float)qf[0][i][j]);
+        }
+    return a.scale2 * pow2i((-up) >> 1) * pow2i(-up - ((-up) >> 1));
+}
+
+// What the queries of a step's U 16-key halves share: the exponent offset of
+// p' and what undoes it in l.
+template <int U>
+struct Halves {
+    float adj[U], undo[U];
+    __device__ __forceinline__ void set(int u, int ev, bool in, int eref) {
+        const int x = max(in ? P_EXP + ev - eref : P_EXP, -40);
+        adj[u] = (float)x;
+        undo[u] = pow2i(-x);
+    }
+};
+
+// p' of one query over U halves: 2^(s f - m + adj).
+template <int U, int NB>
+__device__ __forceinline__ void powers(const f32x4 (&s)[U], const float (&f)[U], const Halves<U> &hv, float m,
+                                       float (&sum)[U], f16x8 (&pf)[U / 2][NB]) {
+    const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const float ms = mu - hv.adj[u];
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], f[u], -ms));
+            pf[u >> 1][0][4 * (u & 1) + j] = (_Float16)p[j];
+            if (NB > 1) pf[u >> 1][NB - 1][4 * (u & 1) + j] = (_Float16)(p[j] - (float)pf[u >> 1][0][4 * (u & 1) + j]);
+        }
+        if (NB > 1) {
+            sum[u] = (p[0] + p[1]) + (p[2] + p[3]);
+        } else {
+            // the weights as the product takes them, two at a time
+            const f16x8 &q = pf[u >> 1][0];
+            const int j = 4 * (u & 1);
+            const f16x2 a = {q[j], q[j + 1]}, b = {q[j + 2], q[j + 3]}, one = {1, 1};
+            sum[u] = __builtin_amdgcn_fdot2(a, one, __builtin_amdgcn_fdot2(b, one, 0.0f, false), false);
+        }
+    }
+}
+
+// One query's online softmax over U halves: scores s (-inf: not seen) times
+// f, in base 2; p' as B operands.  The maximum is found only when it has to
+// be: p' are computed with the one so far, and if one of them (in any lane)
+// passes 2^(P_EXP + SLACK) the maximum moves and they are computed again.
+// Returns the factor of the sums so far, which is 1 unless `moved`, the same
+// in the whole wavefront.
+template <int U, int NB>
+__device__ __forceinline__ float weigh(const f32x4 (&s)[U], const float (&f)[U], const Halves<U> &hv, float &m, float &l,
+                                       bool &moved, f16x8 (&pf)[U / 2][NB]) {
+    float sum[U];
+    moved = __any(m == -INFINITY);
+    if (!moved) {
+        powers<U, NB>(s, f, hv, m, sum, pf);
+        // f16 bits as integers: p' >= 0, and infinities and NaN are the largest
+        u16x2 top = {0, 0};
+#pragma unroll
+        for (int y = 0; y < U / 2; y++) {
+            const auto q = __builtin_bit_cast(u16x8, pf[y][0]);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) top = __builtin_elementwise_max(top, (u16x2){q[j], q[j + 1]});
+        }
+        moved = __any(max(top[0], top[1]) > (15 + P_EXP + SLACK) << 10);
+    }
+    float al = 1.0f;
+    if (__builtin_expect(moved, 0)) {
+        float mt = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            mt = fmaxf(mt, f[u] * fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
+        const float mn = fmaxf(m, fmax_q(mt));
+        al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= al;
+        powers<U, NB>(s, f, hv, m, sum, pf);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) l = __builtin_fmaf(sum[u], hv.undo[u], l);
+    return al;
+}
+
+// -inf * 0 is NaN: where scores are masked their factors are kept from
+// underflowing (scores below 2^-70 are 0 to the softmax).
+__device__ __forceinline__ float above0(float f) { return f < 0x1p-100f ? 0x1p-100f : f; }
+
+// The keys a query sees: [0, first) and [lo, lo + n).
+struct Sight {
+    unsigned first, n;
+    int lo;
+    __device__ __forceinline__ void set(const Args &a, int pos, int len, bool have) {
+        const int end = have ? max(min(a.causal ? pos + 1 : len, a.cap), 0) : 0;
+        lo = a.window ? pos - a.window + 1 : 0;
+        first = a.window ? min(a.sinks, end) : end;
+        n = a.window ? max(end - lo, 0) : 0;
+    }
+    __device__ __forceinline__ bool sees(int key) const { return (unsigned)key < first || (unsigned)(key - lo) < n; }
+};
+
+// The reference exponent follows the value scales (e1: the largest of this
+// step), but not more than 60 below the largest one met; returns the factor
+// that brings the sums to it.
+__device__ __forceinline__ float follow(int e1, int emax, int &eref) {
+    const int to = max(e1, emax - 60), by = max(min(eref - to, 126), -126);
+    eref = to;
+    return pow2i(by);
+}
+
+// V's A operands of four dims, code(j) their codes of the lane's key j: pairs
+// of keys side by side.
+template <int D, class Code>
+__device__ __forceinline__ void operand_v(Code code, f16x8 (&vf)[4]) {
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int y = 0; y < 4; y++) {
+        lo[y] = __builtin_amdgcn_perm(code(2 * y + 1), code(2 * y), 0x05010400u);
+        hi[y] = __builtin_amdgcn_perm(code(2 * y + 1), code(2 * y), 0x07030602u);
+    }
+#pragma unroll
+    for (int b = 0; b < 4; b++)
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+            const f16x2 z = cvt2(b < 2 ? lo[y] : hi[y], b & 1);
+            vf[b][2 * y] = z[0];
+            vf[b][2 * y + 1] = z[1];
+        }
+}
+
+// The NaN codes among a step's values, which the products took as zeros: they
+// reach the rows that see their token, and they alone (0 * NaN is NaN, so a
+// product over a masked one would spread it).  Rare, so the codes are read
+// again: kept in registers they cost the common path 40 of them.
+template <int D, int NQ>
+__device__ __forceinline__ void spread_nan(const Args &a, const Tile &t, int h, int key, int c, int g,
+                                           const Sight (&see)[NQ], f32x4 (&o)[NQ][D / 16]) {
+    f16x8 one[NQ];
+    uint32_t nan[8][D / 64];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int kk = key + 16 * (j >> 2) + 4 * g + (j & 3);
+        const bool held = kk < min(t.len, a.cap);
+        const int p = a.table[(long)t.seq * a.table_w + (held ? kk >> a.lp : 0)];
+        const bool in = held && (unsigned)p < (unsigned)a.pages;
+        const long base = ((((long)(in ? p : 0) * a.kv + h) << a.lp) + (in ? kk & ((1 << a.lp) - 1) : 0)) * D + c * (D / 16);
+#pragma unroll
+        for (int x = 0; x < D / 64; x++)
+            nan[j][x] = in ? nan_bytes(*reinterpret_cast<const uint32_t *>(a.v + base + 4 * x)) : 0;
+#pragma unroll
+        for (int n = 0; n < NQ; n++)
+            one[n][j] = in && see[n].sees(kk) ? (_Float16)1.0f : (_Float16)0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) {
+        f16x8 hit;
+#pragma unroll
+        for (int j = 0; j < 8; j++) hit[j] = (nan[j][i >> 2] >> (8 * (i & 3) + 7)) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const f32x4 x = mfma_f16(hit, one[n], (f32x4){0, 0, 0, 0});
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (x[j] > 0.0f) o[n][i][j] = __uint_as_float(0x7fc00000u);
+        }
+    }
+}
+
+// w with its NaN codes as zeros.
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~((nan_bytes(w) >> 7) * 0xffu); }
+
+template <int D, bool BF16>
+__global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
     constexpr int KS = D / 32;            // k steps of the score product
     constexpr int DI = D / 16;            // 16-dim tiles of O; dims of V a lane loads
     constexpr int NB = BF16 ? 1 : 2;      // f16 terms of a query value and of p
@@ -178,243 +414,161 @@ __global__ __launch_bounds__(NT) void attn_kernel(Args a) {
     // heads vary fastest: workgroup i runs on XCD i % 8, so with 8 kv heads the
     // tiles of one head share an L2
     const int h = blockIdx.x % a.kv, id = blockIdx.x / a.kv, ch = blockIdx.y;
+    const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
+    // this wavefront's steps: first, first + NW, ...; lane i keeps the page and
+    // the scales of 16-key half i (-1: not in the pool).  Where a step's keys do
+    // not depend on the lengths, its page is read along with them.
+    const int first = ch * a.chunk + w;
+    const bool ahead = a.one_tile && !a.window;
+    int key_i = 32 * (first + NW * (lane >> 1)) + 16 * (lane & 1), pg = -1;
+    if (ahead && (lane >> 1) * NW < a.chunk && key_i < a.cap) pg = a.table[(long)id * a.table_w + (key_i >> a.lp)];
     Tile t;
     if (!find_tile(a, id, 16, sh, t)) return;
     const int chunks = (t.steps + a.chunk - 1) / a.chunk;
     if (ch >= max(chunks, 1)) return;
-    const int lane = threadIdx.x % CT_WAVE, w = threadIdx.x / CT_WAVE, c = lane & 15, g = lane >> 4;
+    const int last = min(t.steps, (ch + 1) * a.chunk);
 
-    // this lane's query row, normalised and split
+    // this lane's query row: asked for first, used after the keys are asked for
     const int R = t.row + c;
     const bool have = R < t.n * a.group;
     const int qi = have ? R / a.group : 0, qh = have ? R % a.group : 0;
-    const int pos = t.pos0 + qi;
-    f16x8 qf[NB][KS];
-    float qs;
-    {
-        const long off = (long)(t.r0 + qi) * a.ld_q + (long)(h * a.group + qh) * D;
-        float x[KS][8];
-        float amax = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < KS; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const long d = off + 64 * (i >> 1) + 16 * g + 8 * (i & 1) + j;
-                const float u = BF16 ? bf2f(reinterpret_cast<const uint16_t *>(a.q)[d])
-                                     : reinterpret_cast<const float *>(a.q)[d];
-                x[i][j] = have ? u : 0.0f;
-                amax = fmaxf(amax, fabsf(x[i][j]));
-                bad |= !(fabsf(x[i][j]) < INFINITY);
-            }
-        amax = fmax_q(bad ? INFINITY : amax);
-        // exponent of the row's largest value (zero and subnormal rows: 2^-126)
-        const int e = amax < INFINITY ? max((int)(__float_as_uint(amax) >> 23), 1) - 127 : 0;
-        // a row that is not finite has no scores
-        qs = amax < INFINITY ? 1.0f : __uint_as_float(0x7fc00000u);
-        const int up = 12 - e;               // in [-115, 138]: two factors
-        const float f0 = pow2i(up >> 1), f1 = pow2i(up - (up >> 1));
-        qs = qs * a.scale2 * pow2i((-up) >> 1) * pow2i(-up - ((-up) >> 1));
-#pragma unroll
-        for (int i = 0; i < KS; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float y = x[i][j] * f0 * f1;
-                qf[0][i][j] = (_Float16)y;
-                if (NB > 1) qf[NB - 1][i][j] = (_Float16)(y - (float)qf[0][i][j]);
-            }
-    }
-    // keys this lane's query sees: [wlo, kend) and [0, sink_end)
-    const int kend = have ? min(a.causal ? pos + 1 : t.len, a.cap) : 0;
-    const int wlo = a.window ? pos - a.window + 1 : 0;
-    const int hard = min(t.len, a.cap);      // tokens at and past it hold anything
-
-    // this wavefront's steps: first, first + NW, ...; lane i keeps the page and
-    // the scales of 16-key half i (-1: not in the pool)
-    const int first = ch * a.chunk + w, last = min(t.steps, (ch + 1) * a.chunk);
-    int pg = -1;
-    float pks = 0.0f, pvs = 0.0f;
     {
         const int st = first + NW * (lane >> 1);
-        if (st < last) {
-            const int key = step_key(t, st) + 16 * (lane & 1);
-            if (key < t.end) pg = a.table[(long)t.seq * a.table_w + (key >> a.lp)];
-            if ((unsigned)pg >= (unsigned)a.pages) pg = -1;
-            if (pg >= 0) {
-                pks = a.ks[(long)pg * a.kv + h];
-                pvs = a.vs[(long)pg * a.kv + h];
-            }
-        }
+        key_i = step_key(t, st) + 16 * (lane & 1);
+        const bool mine = st < last && key_i < t.end;
+        if (!ahead && mine) pg = a.table[(long)t.seq * a.table_w + (key_i >> a.lp)];
+        if (!mine || (unsigned)pg >= (unsigned)a.pages) pg = -1;
     }
+    float x[KS][8];
+    fetch_query<D, BF16>(a, (long)(t.r0 + qi) * a.ld_q + (long)(h * a.group + qh) * D, g, x);
+
     const int P = 1 << a.lp;
+    const unsigned koff = c * D + 16 * g, voff = 4 * g * D + c * DI;
     auto load = [&](int st, int i, Raw<D> &r) {          // step st, this wavefront's i-th
+        unsigned ka = koff, va = voff;
+        asm volatile("" : "+v"(ka), "+v"(va));   // 32-bit offsets beside a scalar base, not a 64-bit sum a load
         const int key = step_key(t, st);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int p = max(__builtin_amdgcn_readlane(pg, 2 * i + u), 0);   // any page if there is none
             const long base = ((((long)p * a.kv + h) << a.lp) + ((key + 16 * u) & (P - 1))) * D;
-            const uint8_t *kp = a.k + base + c * D + 16 * g, *vp = a.v + base + 4 * g * D + c * DI;
+            const uint8_t *kp = a.k + base, *vp = a.v + base;
+            // non-temporal: a step's codes are read once (7.1 against 6.3 TB/s
+            // in a plain read of 4 GiB)
 #pragma unroll
-            for (int x = 0; x < D / 64; x++) r.k[u][x] = *reinterpret_cast<const uint4 *>(kp + 64 * x);
+            for (int y = 0; y < D / 64; y++)
+                r.k[u][y] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kp + ka + 64 * y));
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (D == 128) {
-                    const uint2 y = *reinterpret_cast<const uint2 *>(vp + j * D);
-                    r.v[4 * u + j][0] = y.x;
-                    r.v[4 * u + j][D / 64 - 1] = y.y;
+                    const u32x2 y = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vp + va + j * D));
+                    r.v[4 * u + j][0] = y[0];
+                    r.v[4 * u + j][D / 64 - 1] = y[1];
                 } else {
-                    r.v[4 * u + j][0] = *reinterpret_cast<const uint32_t *>(vp + j * D);
+                    r.v[4 * u + j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(vp + va + j * D));
                 }
             }
         }
     };
+    Raw<D> ra, rb;
+    if (first < last) load(first, 0, ra);
+    float pks = 0.0f, pvs = 0.0f;
+    if (pg >= 0) {
+        pks = a.ks[(long)pg * a.kv + h];
+        pvs = a.vs[(long)pg * a.kv + h];
+    }
+    f16x8 qf[NB][KS];
+    const float qs = split_query<D, BF16>(a, have, x, qf);
+    Sight see[1];
+    see[0].set(a, t.pos0 + qi, t.len, have);
+    const int hard = min(t.len, a.cap);      // tokens at and past it hold anything
 
-    f32x4 o[DI];
+    f32x4 o[1][DI];
 #pragma unroll
-    for (int i = 0; i < DI; i++) o[i] = (f32x4){0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;
+    for (int i = 0; i < DI; i++) o[0][i] = (f32x4){0, 0, 0, 0};
+    float m = have ? -INFINITY : 0.0f, l = 0.0f;         // lanes without a row never move the maximum
     int eref = KV8_MIN_EXP, emax = KV8_MIN_EXP;
 
     auto use = [&](int st, int i, Raw<D> &r) {
         const int key = step_key(t, st);
-        float s[2][4];
+        f32x4 s[2];
+        float f[2];
         int ev[2];
         bool in[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             in[u] = __builtin_amdgcn_readlane(pg, 2 * i + u) >= 0;
-            const float ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pks), 2 * i + u));
+            f[u] = qs * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pks), 2 * i + u));
             ev[u] = max((int)(__builtin_amdgcn_readlane(__float_as_uint(pvs), 2 * i + u) >> 23 & 255) - 127, KV8_MIN_EXP);
-            f32x4 acc = {0, 0, 0, 0};
+            s[u] = (f32x4){0, 0, 0, 0};
 #pragma unroll
-            for (int x = 0; x < D / 64; x++) {
-                const f16x8 k0 = cvt8(r.k[u][x].x, r.k[u][x].y), k1 = cvt8(r.k[u][x].z, r.k[u][x].w);
+            for (int y = 0; y < D / 64; y++) {
+                const f16x8 k0 = cvt8(r.k[u][y][0], r.k[u][y][1]), k1 = cvt8(r.k[u][y][2], r.k[u][y][3]);
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
-                    acc = mfma_f16(k0, qf[b][2 * x], acc);
-                    acc = mfma_f16(k1, qf[b][2 * x + 1], acc);
+                    s[u] = mfma_f16(k0, qf[b][2 * y], s[u]);
+                    s[u] = mfma_f16(k1, qf[b][2 * y + 1], s[u]);
                 }
             }
-            const float f = qs * ks;
-#pragma unroll
-            for (int j = 0; j < 4; j++) s[u][j] = acc[j] * f;
         }
         const bool whole = key >= t.full_lo && key + 32 <= t.full_hi && in[0] && in[1];   // sink steps lie below full_lo
-        uint32_t bad = 0;
-        uint32_t vis = 0xff;                 // bit 4u + j: this lane's query sees key 16u + 4g + j
-        if (!whole) {
-            vis = 0;
+        bool nan = false;
+        if (__builtin_expect(!whole, 0)) {
+            uint32_t bad = 0;
+            f[0] = above0(f[0]);
+            f[1] = above0(f[1]);
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int kk = key + 16 * u + 4 * g + j;
-                    const bool see = in[u] && kk < kend && (kk >= wlo || kk < a.sinks);
-                    if (see) vis |= 1u << (4 * u + j);
-                    else s[u][j] = -INFINITY;
+                    if (!(in[u] && see[0].sees(kk))) s[u][j] = -INFINITY;
                     // a token nobody sees may hold anything: 0 * NaN is NaN
                     const bool any = in[u] && kk < hard;
 #pragma unroll
-                    for (int x = 0; x < D / 64; x++) {
-                        if (!any) r.v[4 * u + j][x] = 0;
-                        bad |= nan_bytes(r.v[4 * u + j][x]);
+                    for (int y = 0; y < D / 64; y++) {
+                        if (!any) r.v[4 * u + j][y] = 0;
+                        bad |= nan_bytes(r.v[4 * u + j][y]);
                     }
                 }
-        }
-        float mt = s[0][0];
+            nan = __any(bad != 0);
+            if (nan) {
 #pragma unroll
-        for (int j = 1; j < 8; j++) mt = fmaxf(mt, s[j >> 2][j & 3]);
-        mt = fmax_q(mt);
-        // reference exponent of the sums: follows the value scales, but not
-        // more than 60 below the largest one met
+                for (int j = 0; j < 8; j++)
+#pragma unroll
+                    for (int y = 0; y < D / 64; y++) r.v[j][y] = without_nan(r.v[j][y]);
+            }
+        }
         const int e1 = max(in[0] ? ev[0] : KV8_MIN_EXP, in[1] ? ev[1] : KV8_MIN_EXP);
         emax = max(emax, e1);
-        if (e1 > eref || e1 < eref - 8) {
-            const int to = max(e1, emax - 60);
-            const int by = max(min(eref - to, 126), -126);
-            eref = to;
-            const float f = pow2i(by);
+        if (__builtin_expect(e1 > eref || e1 < eref - 8, 0)) {
+            const float by = follow(e1, emax, eref);
 #pragma unroll
-            for (int i2 = 0; i2 < DI; i2++) o[i2] *= f;
+            for (int y = 0; y < DI; y++) o[0][y] *= by;
         }
-        if (__any(mt > m)) {
-            const float mn = fmaxf(m, mt);
-            const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= al;
+        Halves<2> hv;
+        hv.set(0, ev[0], in[0], eref);
+        hv.set(1, ev[1], in[1], eref);
+        f16x8 pf[1][NB];
+        bool moved;
+        const float al = weigh<2, NB>(s, f, hv, m, l, moved, pf);
+        if (moved) {
 #pragma unroll
-            for (int i2 = 0; i2 < DI; i2++) o[i2] *= al;
-        }
-        const float mu = m == -INFINITY ? 0.0f : m;
-        f16x8 pf[NB];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int adj = max(in[u] ? P_EXP + ev[u] - eref : P_EXP, -40);
-            const float ms = mu - (float)adj;
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float p = __builtin_amdgcn_exp2f(s[u][j] - ms);
-                sum += p;
-                pf[0][4 * u + j] = (_Float16)p;
-                if (NB > 1) pf[NB - 1][4 * u + j] = (_Float16)(p - (float)pf[0][4 * u + j]);
-            }
-            l += sum * pow2i(-adj);
-        }
-        if (__any(bad)) {
-            // a NaN among values that some row sees and another does not: it
-            // reaches the rows that see it, and they alone
-            f16x8 one;
-#pragma unroll
-            for (int j = 0; j < 8; j++) one[j] = (vis >> j) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
-#pragma unroll
-            for (int x = 0; x < D / 64; x++)
-#pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    f16x8 hit;
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        hit[j] = (nan_bytes(r.v[j][x]) >> (8 * b + 7)) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
-                    const f32x4 n = mfma_f16(hit, one, (f32x4){0, 0, 0, 0});
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (n[j] > 0.0f) o[4 * x + b][j] = __uint_as_float(0x7fc00000u);
-                }
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-#pragma unroll
-                for (int x = 0; x < D / 64; x++) {
-                    const uint32_t z = nan_bytes(r.v[j][x]);
-                    r.v[j][x] &= ~((z >> 7) * 0xffu);
-                }
+            for (int y = 0; y < DI; y++) o[0][y] *= al;
         }
 #pragma unroll
-        for (int x = 0; x < D / 64; x++) {
-            // pairs of keys side by side: byte b of keys 2y, 2y + 1
-            uint32_t lo[4], hi[4];
+        for (int y = 0; y < D / 64; y++) {
+            f16x8 vf[4];
+            operand_v<D>([&](int j) { return r.v[j][y]; }, vf);
 #pragma unroll
-            for (int y = 0; y < 4; y++) {
-                lo[y] = __builtin_amdgcn_perm(r.v[2 * y + 1][x], r.v[2 * y][x], 0x05010400u);
-                hi[y] = __builtin_amdgcn_perm(r.v[2 * y + 1][x], r.v[2 * y][x], 0x07030602u);
-            }
+            for (int b = 0; b < 4; b++)
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                f16x8 vf;
-#pragma unroll
-                for (int y = 0; y < 4; y++) {
-                    const f16x2 z = cvt2(b < 2 ? lo[y] : hi[y], b & 1);
-                    vf[2 * y] = z[0];
-                    vf[2 * y + 1] = z[1];
-                }
-#pragma unroll
-                for (int n = 0; n < NB; n++) o[4 * x + b] = mfma_f16(vf, pf[n], o[4 * x + b]);
-            }
+                for (int n = 0; n < NB; n++) o[0][4 * y + b] = mfma_f16(vf[b], pf[0][n], o[0][4 * y + b]);
         }
+        if (__builtin_expect(nan, 0)) spread_nan<D, 1>(a, t, h, key, c, g, see, o);
     };
 
     // two steps in flight
-    Raw<D> ra, rb;
-    if (first < last) load(first, 0, ra);
     for (int st = first, i = 0; st < last; st += 2 * NW, i += 2) {
         if (st + NW < last) load(st + NW, i + 1, rb);
         use(st, i, ra);
@@ -431,7 +585,7 @@ __global__ __launch_bounds__(NT) void attn_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < DI; i++) so[w][c][(4 * g + j) * DI + i] = o[i][j] * unit;
+            for (int i = 0; i < DI; i++) so[w][c][(4 * g + j) * DI + i] = o[0][i][j] * unit;
     }
     __syncthreads();
     const int nr = min(16, t.n * a.group - t.row);
@@ -462,63 +616,396 @@ __global__ __launch_bounds__(NT) void attn_kernel(Args a) {
     }
 }
 
-// Joins a tile's chunks, in their order: a wavefront a row.
+// Many rows of a sequence: a workgroup holds 128 packed rows, 32 a wavefront
+// (fp32: 64 and 16, whose two f16 terms make as many products of each operand
+// read from LDS), and takes 64 keys at a time.  Each wavefront fetches and
+// converts a quarter of them (K or V of one 32-key step) and leaves them in
+// LDS as the products' A operands, lane by lane, so that every LDS access is
+// a run of 1 KB; all four then read the whole 64 keys.  Two LDS buffers: the
+// next keys' codes are in flight while this step's products run, and one
+// barrier a step keeps them apart.
+constexpr int rows_of(bool bf16) { return bf16 ? 128 : 64; }
+
 template <int D, bool BF16>
-__global__ __launch_bounds__(NT) void join_kernel(Args a) {
+__global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
+    constexpr int KS = D / 32, DI = D / 16, NB = BF16 ? 1 : 2;
+    constexpr int ROWS = rows_of(BF16), WR = ROWS / NW, NQ = WR / 16;
+    constexpr int UNIT = D * 32;               // halves of a 32-key step's K or V
+    static_assert(2 * KS == DI, "K and V take the same number of operands");
     __shared__ int sh[NW + 2];
+    __shared__ __align__(16) _Float16 lds[2][4][UNIT];   // buffer; K, K, V, V of the two steps
+    __shared__ float sscale[2][4];             // key scales of the four 16-key halves
+    __shared__ int sexp[2][4];                 // exponents of the value scales; NONE: not in the pool
+    __shared__ int snan[2][2];                 // the V of a step holds a NaN
+    constexpr int NONE = 1 << 20;
+
+    const int h = blockIdx.x % a.kv, id = gridDim.x / a.kv - 1 - blockIdx.x / a.kv, ch = blockIdx.y;
+    Tile t;
+    if (!find_tile(a, id, ROWS, sh, t)) return;
+    const int chunks = (t.steps + a.chunk - 1) / a.chunk;
+    if (ch >= max(chunks, 1)) return;
+    const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
+    const int all = t.n * a.group, hard = min(t.len, a.cap);
+
+    // this wavefront's rows
+    f16x8 qf[NQ][NB][KS];
+    float qs[NQ];
+    Sight see[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int R = t.row + WR * w + 16 * n + c;
+        const bool have = R < all;
+        const int qi = have ? R / a.group : 0, qh = have ? R % a.group : 0;
+        float x[KS][8];
+        fetch_query<D, BF16>(a, (long)(t.r0 + qi) * a.ld_q + (long)(h * a.group + qh) * D, g, x);
+        qs[n] = split_query<D, BF16>(a, have, x, qf[n]);
+        see[n].set(a, t.pos0 + qi, t.len, have);
+    }
+    const int wr0 = min(t.row + WR * w, all - 1), wr1 = min(t.row + WR * w + WR, all) - 1;
+    const bool idle = t.row + WR * w >= all;
+    const int p0 = t.pos0 + wr0 / a.group, p1 = t.pos0 + wr1 / a.group;
+    const int full_lo = a.window ? p1 - a.window + 1 : 0, full_hi = min(a.causal ? p0 + 1 : t.len, a.cap);
+    const int wend = idle ? 0 : min(a.causal ? p1 + 1 : t.len, a.cap);
+
+    // the unit this wavefront fetches: K (isv 0) or V of step 2 it + kb; lane i
+    // keeps the page and scale of half i & 1 of the step of iteration base + i / 2
+    const int kb = w & 1, isv = w >> 1;
+    const int s0 = ch * a.chunk, s1 = min(t.steps, s0 + a.chunk), iters = (s1 - s0 + 1) >> 1;
+    const int P = 1 << a.lp;
+    auto fetch_page = [&](int it0) {
+        const int st = s0 + 2 * (it0 + (lane >> 1)) + kb;
+        int p = -1;
+        if (st < s1) {
+            const int key = step_key(t, st) + 16 * (lane & 1);
+            if (key < t.end) p = a.table[(long)t.seq * a.table_w + (key >> a.lp)];
+        }
+        return (unsigned)p < (unsigned)a.pages ? p : -1;
+    };
+    auto fetch_scale = [&](int p) { return p >= 0 ? (isv ? a.vs : a.ks)[(long)p * a.kv + h] : 0.0f; };
+    int pg = fetch_page(0), pg2 = fetch_page(32);
+    float psc = fetch_scale(pg), psc2 = 0.0f;
+    const uint8_t *pool = isv ? a.v : a.k;
+    const unsigned off = isv ? 4 * g * D + c * DI : c * D + 16 * g;
+
+    uint32_t raw[D / 8];                         // the unit's codes: 8 D / 64 dwords of K or V
+    int rp[2];
+    float rs[2];
+    auto fetch = [&](int it) {
+        unsigned at = off;
+        asm volatile("" : "+v"(at));            // a 32-bit offset beside a scalar base, not a 64-bit sum a load
+        const int i = 2 * (it & 31), key = step_key(t, min(s0 + 2 * it + kb, s1 - 1));
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            rp[u] = __builtin_amdgcn_readlane(pg, i + u);
+            rs[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(psc), i + u));
+            const uint8_t *p = pool + ((((long)max(rp[u], 0) * a.kv + h) << a.lp) + ((key + 16 * u) & (P - 1))) * D;
+            uint32_t *to = raw + u * (D / 16);
+            if (!isv) {
+#pragma unroll
+                for (int x = 0; x < D / 64; x++) {
+                    const uint4 y = *reinterpret_cast<const uint4 *>(p + at + 64 * x);
+                    to[4 * x] = y.x; to[4 * x + 1] = y.y; to[4 * x + 2] = y.z; to[4 * x + 3] = y.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (D == 128) {
+                        const uint2 y = *reinterpret_cast<const uint2 *>(p + at + j * D);
+                        to[2 * j] = y.x;
+                        to[2 * j + 1] = y.y;
+                    } else {
+                        to[j] = *reinterpret_cast<const uint32_t *>(p + at + j * D);
+                    }
+                }
+            }
+        }
+        // pages and scales of the next 32 iterations, well before they are used
+        if ((it & 31) == 15) psc2 = fetch_scale(pg2);
+        if ((it & 31) == 31) {
+            pg = pg2;
+            psc = psc2;
+            pg2 = fetch_page(it + 33);
+        }
+    };
+    auto place = [&](int it) {                   // the fetched unit into buffer it & 1
+        const int b = it & 1;
+        f16x8 *to = reinterpret_cast<f16x8 *>(lds[b][2 * isv + kb]) + lane;
+        if (lane < 2) {
+            const int half = 2 * kb + lane;
+            const float sc = lane ? rs[1] : rs[0];
+            const int p = lane ? rp[1] : rp[0];
+            if (!isv) sscale[b][half] = sc;
+            else sexp[b][half] = p < 0 ? NONE : max((int)(__float_as_uint(sc) >> 23 & 255) - 127, KV8_MIN_EXP);
+        }
+        if (!isv) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int x = 0; x < D / 64; x++) {
+                    const uint32_t *y = raw + u * (D / 16) + 4 * x;
+                    to[(u * KS + 2 * x) * CT_WAVE] = cvt8(y[0], y[1]);
+                    to[(u * KS + 2 * x + 1) * CT_WAVE] = cvt8(y[2], y[3]);
+                }
+            return;
+        }
+        // a step that every row of the tile sees whole may spread its NaN; one
+        // that some row does not: tokens that are not there hold anything, and
+        // a NaN must not meet a masked row's zero
+        const int key = step_key(t, min(s0 + 2 * it + kb, s1 - 1));
+        bool nan = false;
+        if (__builtin_expect(!(rp[0] >= 0 && rp[1] >= 0 && key >= t.full_lo && key + 32 <= t.full_hi), 0)) {
+            uint32_t bad = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const bool in = rp[j >> 2] >= 0 && key + 4 * g + 16 * (j >> 2) + (j & 3) < hard;
+#pragma unroll
+                for (int x = 0; x < D / 64; x++) {
+                    uint32_t &y = raw[j * (D / 64) + x];
+                    y = in ? y : 0;
+                    bad |= nan_bytes(y);
+                }
+            }
+            nan = __any(bad != 0);
+            if (nan) {
+#pragma unroll
+                for (int x = 0; x < D / 8; x++) raw[x] = without_nan(raw[x]);
+            }
+        }
+        if (lane == 0) snan[b][kb] = nan;
+#pragma unroll
+        for (int x = 0; x < D / 64; x++) {
+            f16x8 vf[4];
+            operand_v<D>([&](int j) { return raw[j * (D / 64) + x]; }, vf);
+#pragma unroll
+            for (int i = 0; i < 4; i++) to[(4 * x + i) * CT_WAVE] = vf[i];
+        }
+    };
+
+    f32x4 o[NQ][DI];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        m[n] = t.row + WR * w + 16 * n + c < all ? -INFINITY : 0.0f;     // lanes without a row never move it
+        l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DI; i++) o[n][i] = (f32x4){0, 0, 0, 0};
+    }
+    int eref = KV8_MIN_EXP, emax = KV8_MIN_EXP;
+
+    if (iters > 0) {
+        fetch(0);
+        place(0);
+    }
+    for (int it = 0; it < iters; it++) {
+        __syncthreads();
+        const bool more = it + 1 < iters;
+        if (more) fetch(it + 1);
+        const int b = it & 1, k0 = step_key(t, s0 + 2 * it), k1 = step_key(t, min(s0 + 2 * it + 1, s1 - 1));
+        if (k0 < wend) {
+            const f16x8 *kl = reinterpret_cast<const f16x8 *>(lds[b][0]) + lane;
+            const f16x8 *vl = reinterpret_cast<const f16x8 *>(lds[b][2]) + lane;
+            f32x4 s[NQ][4];
+            int ev[4];
+            float f[NQ][4];
+            bool in[4], every = true;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float ks = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sscale[b][u])));
+                ev[u] = __builtin_amdgcn_readfirstlane(sexp[b][u]);
+                in[u] = ev[u] != NONE && (u < 2 || s0 + 2 * it + 1 < s1);
+                every = every && in[u];
+#pragma unroll
+                for (int n = 0; n < NQ; n++) {
+                    f[n][u] = qs[n] * ks;
+                    s[n][u] = (f32x4){0, 0, 0, 0};
+                }
+#pragma unroll
+                for (int x = 0; x < KS; x++) {
+                    const f16x8 kf = kl[((u >> 1) * DI + (u & 1) * KS + x) * CT_WAVE];
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+#pragma unroll
+                        for (int y = 0; y < NB; y++) s[n][u] = mfma_f16(kf, qf[n][y][x], s[n][u]);
+                }
+            }
+            const bool whole = every && k0 >= full_lo && k0 + 32 <= full_hi && k1 >= full_lo && k1 + 32 <= full_hi;
+            if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+                for (int n = 0; n < NQ; n++)
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        __builtin_amdgcn_sched_barrier(0);   // few comparisons' results at a time
+                        f[n][u] = above0(f[n][u]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int kk = (u < 2 ? k0 : k1) + 16 * (u & 1) + 4 * g + j;
+                            if (!(in[u] && see[n].sees(kk))) s[n][u][j] = -INFINITY;
+                        }
+                    }
+            }
+            const int e1 = max(max(in[0] ? ev[0] : KV8_MIN_EXP, in[1] ? ev[1] : KV8_MIN_EXP),
+                               max(in[2] ? ev[2] : KV8_MIN_EXP, in[3] ? ev[3] : KV8_MIN_EXP));
+            emax = max(emax, e1);
+            if (__builtin_expect(e1 > eref || e1 < eref - 8, 0)) {
+                const float by = follow(e1, emax, eref);
+#pragma unroll
+                for (int n = 0; n < NQ; n++)
+#pragma unroll
+                    for (int i = 0; i < DI; i++) o[n][i] *= by;
+            }
+            Halves<4> hv;
+#pragma unroll
+            for (int u = 0; u < 4; u++) hv.set(u, ev[u], in[u], eref);
+            f16x8 pf[NQ][2][NB];
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+                bool moved;
+                const float al = weigh<4, NB>(s[n], f[n], hv, m[n], l[n], moved, pf[n]);
+                if (moved) {
+#pragma unroll
+                    for (int i = 0; i < DI; i++) o[n][i] *= al;
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                if (y && s0 + 2 * it + 1 >= s1) break;
+#pragma unroll
+                for (int i = 0; i < DI; i++) {
+                    const f16x8 vf = vl[(y * DI + i) * CT_WAVE];
+#pragma unroll
+                    for (int n = 0; n < NQ; n++)
+#pragma unroll
+                        for (int z = 0; z < NB; z++) o[n][i] = mfma_f16(vf, pf[n][y][z], o[n][i]);
+                }
+            }
+#pragma unroll 1
+            for (int y = 0; y < 2; y++)
+                if (__builtin_expect(snan[b][y], 0) && s0 + 2 * it + y < s1) spread_nan<D, NQ>(a, t, h, y ? k1 : k0, c, g, see, o);
+        }
+        if (more) place(it + 1);
+    }
+
+    const float unit = pow2i(eref - P_EXP);
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const float den = sum_q(l[n]);
+        const int r = WR * w + 16 * n + c, R = t.row + r;
+        if (R >= all) continue;
+        if (chunks <= 1) {
+            const float f = den == 0.0f ? 0.0f : 1.0f / den;
+            const long off = (long)(t.r0 + R / a.group) * a.ld_out + (long)(h * a.group + R % a.group) * D;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < DI; i++) {
+                    const float y = den == 0.0f ? 0.0f : o[n][i][j] * unit * f;
+                    if (BF16) reinterpret_cast<uint16_t *>(a.out)[off + (4 * g + j) * DI + i] = f2bf(y);
+                    else reinterpret_cast<float *>(a.out)[off + (4 * g + j) * DI + i] = y;
+                }
+        } else {
+            const long at = (((long)id * a.kv + h) * a.nchunk + ch) * a.rpt + r;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < DI; i++) a.part[at * D + (4 * g + j) * DI + i] = o[n][i][j] * unit;
+            if (g == 0) a.stat[at] = make_float2(m[n], den);
+        }
+    }
+}
+
+// Joins a tile's chunks: WPR wavefronts a row (chunks w, w + WPR, ...), each
+// with four chunks' loads in flight, then their sums in order.
+template <int D, bool BF16, int WPR>
+__global__ __launch_bounds__(NT) void join_kernel(Args a) {
+    constexpr int DL = D / CT_WAVE, RPB = NW / WPR;       // dims of a lane, rows of a workgroup
+    __shared__ int sh[NW + 2];
+    __shared__ float so[NW][D], sl[NW];
     const int h = blockIdx.x % a.kv, id = blockIdx.x / a.kv;
     Tile t;
-    if (!find_tile(a, id, 16, sh, t)) return;
+    if (!find_tile(a, id, a.tile_rows, sh, t)) return;
     const int chunks = (t.steps + a.chunk - 1) / a.chunk;
     if (chunks <= 1) return;
-    const int lane = threadIdx.x % CT_WAVE, nr = min(16, t.n * a.group - t.row);
-    constexpr int DL = D / CT_WAVE;
-    for (int r = threadIdx.x / CT_WAVE; r < nr; r += NW) {
-        const long at = ((long)id * a.kv + h) * a.nchunk * a.rpt + r;
-        float M = -INFINITY;
-        for (int k = lane; k < chunks; k += CT_WAVE) M = fmaxf(M, a.stat[at + (long)k * a.rpt].x);
-        M = wave_max(M);
-        const float Mu = M == -INFINITY ? 0.0f : M;
-        float num[DL] = {}, den = 0.0f;
-        for (int k = 0; k < chunks; k++) {
-            const float2 st = a.stat[at + (long)k * a.rpt];
-            const float f = __builtin_amdgcn_exp2f(st.x - Mu);
-            den += f * st.y;
+    const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), part = w % WPR;
+    const int r = blockIdx.y * RPB + w / WPR, nr = min(a.tile_rows, t.n * a.group - t.row);
+    const bool have = r < nr;
+    const long at = ((long)id * a.kv + h) * a.nchunk * a.rpt + (have ? r : 0);
+    float M = -INFINITY;
+    for (int k = lane; k < chunks; k += CT_WAVE) M = fmaxf(M, a.stat[at + (long)k * a.rpt].x);
+    M = wave_max(M);
+    const float Mu = M == -INFINITY ? 0.0f : M;
+    float num[DL] = {}, den = 0.0f;
+    for (int k0 = part; k0 < chunks; k0 += 4 * WPR) {
+        float2 st[4];
+        float x[4][DL];
 #pragma unroll
-            for (int j = 0; j < DL; j++) num[j] += f * a.part[(at + (long)k * a.rpt) * D + lane * DL + j];
-        }
-        const int R = t.row + r;
-        const long off = (long)(t.r0 + R / a.group) * a.ld_out + (long)(h * a.group + R % a.group) * D + lane * DL;
+        for (int u = 0; u < 4; u++) {
+            const int k = min(k0 + u * WPR, chunks - 1);
+            st[u] = a.stat[at + (long)k * a.rpt];
 #pragma unroll
-        for (int j = 0; j < DL; j++) {
-            const float y = den == 0.0f ? 0.0f : num[j] / den;
-            if (BF16) reinterpret_cast<uint16_t *>(a.out)[off + j] = f2bf(y);
-            else reinterpret_cast<float *>(a.out)[off + j] = y;
+            for (int j = 0; j < DL; j++) x[u][j] = a.part[(at + (long)k * a.rpt) * D + lane * DL + j];
         }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (k0 + u * WPR >= chunks) break;
+            const float f = __builtin_amdgcn_exp2f(st[u].x - Mu);
+            den += f * st[u].y;
+#pragma unroll
+            for (int j = 0; j < DL; j++) num[j] += f * x[u][j];
+        }
+    }
+    if (WPR > 1) {
+#pragma unroll
+        for (int j = 0; j < DL; j++) so[w][lane * DL + j] = num[j];
+        if (lane == 0) sl[w] = den;
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int i = 1; i < WPR; i++) {
+            den += sl[w + i];
+#pragma unroll
+            for (int j = 0; j < DL; j++) num[j] += so[w + i][lane * DL + j];
+        }
+    }
+    if (!have) return;
+    const int R = t.row + r;
+    const long off = (long)(t.r0 + R / a.group) * a.ld_out + (long)(h * a.group + R % a.group) * D + lane * DL;
+#pragma unroll
+    for (int j = 0; j < DL; j++) {
+        const float y = den == 0.0f ? 0.0f : num[j] / den;
+        if (BF16) reinterpret_cast<uint16_t *>(a.out)[off + j] = f2bf(y);
+        else reinterpret_cast<float *>(a.out)[off + j] = y;
     }
 }
 
 // The launch's shape, from the sizes alone.
 struct Shape {
-    int one_tile, tiles, chunk, nchunk, rpt;
+    int tile_rows, one_tile, tiles, chunk, nchunk, rpt;
 };
 
 Shape shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
     Shape s;
     const int group = a->heads / c->kv_heads;
     const long rows = (long)(a->max_rows < a->n_rows ? a->max_rows : a->n_rows) * group;   // of a sequence
-    s.one_tile = rows <= 16;
-    s.tiles = s.one_tile ? c->seqs : (int)((long)a->n_rows * group / 16 + c->seqs);
-    s.rpt = rows < 16 ? (int)rows : 16;
+    s.tile_rows = rows > 32 ? rows_of(a->bf16) : 16;
+    s.one_tile = rows <= s.tile_rows;
+    s.tiles = s.one_tile ? c->seqs : (int)((long)a->n_rows * group / s.tile_rows + c->seqs);
+    s.rpt = rows < s.tile_rows ? (int)rows : s.tile_rows;
     long keys = (long)c->table_w * c->page_tokens;
     if (a->max_len > 0 && a->max_len < keys) keys = a->max_len;
     // the longest walk of a tile, in steps
     long steps = (keys + 31) / 32;
     if (a->window > 0) {
-        const long span = ((long)a->window + 16 + 62) / 32 + ((long)a->sinks + 31) / 32;
+        const long span = ((long)a->window + s.tile_rows + 62) / 32 + ((long)a->sinks + 31) / 32;
         if (span < steps) steps = span;
     }
-    s.chunk = (long)s.tiles * c->kv_heads >= 1024 ? 128 : 16;
+    if (s.tile_rows == 16) {
+        s.chunk = 16;
+    } else {
+        // two workgroups a CU; at least 512 keys each
+        const long want = (512 + (long)s.tiles * c->kv_heads - 1) / ((long)s.tiles * c->kv_heads);
+        s.chunk = (int)((steps + want - 1) / want);
+        s.chunk = s.chunk < 16 ? 16 : (s.chunk + 1) & ~1;
+    }
     s.nchunk = (int)((steps + s.chunk - 1) / s.chunk);
     if (s.nchunk < 1) s.nchunk = 1;
     return s;
@@ -551,16 +1038,24 @@ extern "C" void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Att
     const long cap = (long)c->table_w * c->page_tokens;
     a.cap = (int)(p->max_len > 0 && p->max_len < cap ? p->max_len : cap);
     a.scale2 = p->scale * LOG2E;
-    a.one_tile = sh.one_tile; a.chunk = sh.chunk; a.nchunk = sh.nchunk; a.rpt = sh.rpt;
+    a.vec = ((uintptr_t)p->q & 15) == 0 && p->ld_q % (p->bf16 ? 8 : 4) == 0;
+    a.tile_rows = sh.tile_rows; a.one_tile = sh.one_tile; a.chunk = sh.chunk; a.nchunk = sh.nchunk; a.rpt = sh.rpt;
     const size_t n = (size_t)sh.tiles * c->kv_heads * sh.nchunk * sh.rpt;
     a.part = p->work;
     a.stat = sh.nchunk > 1 ? reinterpret_cast<float2 *>(p->work + n * c->head_dim) : nullptr;
-    const dim3 grid((unsigned)(c->kv_heads * sh.tiles), sh.nchunk), join((unsigned)(c->kv_heads * sh.tiles));
+    const int wpr = sh.nchunk > 4 ? NW : 1;      // wavefronts that join a row
+    const dim3 grid((unsigned)(c->kv_heads * sh.tiles), sh.nchunk);
+    const dim3 join(grid.x, (unsigned)((sh.rpt * wpr + NW - 1) / NW));
 #define ATTN(D, B)                                                            \
     do {                                                                      \
-        hipLaunchKernelGGL((attn_kernel<D, B>), grid, dim3(NT), 0, s, a);     \
-        if (sh.nchunk > 1)                                                    \
-            hipLaunchKernelGGL((join_kernel<D, B>), join, dim3(NT), 0, s, a); \
+        if (sh.tile_rows == 16)                                               \
+            hipLaunchKernelGGL((attn_kernel<D, B>), grid, dim3(NT), 0, s, a); \
+        else                                                                  \
+            hipLaunchKernelGGL((rows_kernel<D, B>), grid, dim3(NT), 0, s, a); \
+        if (sh.nchunk > 1) {                                                  \
+            if (wpr == 1) hipLaunchKernelGGL((join_kernel<D, B, 1>), join, dim3(NT), 0, s, a);  \
+            else hipLaunchKernelGGL((join_kernel<D, B, NW>), join, dim3(NT), 0, s, a);          \
+        }                                                                     \
     } while (0)
     if (c->head_dim == 64) { if (p->bf16) ATTN(64, true); else ATTN(64, false); }
     else { if (p->bf16) ATTN(128, true); else ATTN(128, false); }
