@@ -93,28 +93,35 @@ __device__ __forceinline__ bool find_tile(const Args &a, int id, int rows_per_ti
     int tile = 0;
     if (a.one_tile) {
         t.seq = id;
+        t.r0 = a.rows[id];
+        t.n = a.rows[id + 1] - t.r0;
+        t.len = a.len[id];
+        if (t.r0 < 0 || t.n <= 0 || t.n > a.n_rows - t.r0) return false;
     } else {
-        int n = 0;
+        int n = 0, r0 = 0, rows = 0, len = 0;
         const int s = threadIdx.x;
         if (s < a.seqs) {
-            const int r0 = a.rows[s], r1 = a.rows[s + 1];
-            if (r0 >= 0 && r1 > r0 && r1 <= a.n_rows)
-                n = ((r1 - r0) * a.group + rows_per_tile - 1) / rows_per_tile;
+            r0 = a.rows[s];
+            rows = a.rows[s + 1] - r0;
+            len = a.len[s];
+            if (r0 >= 0 && rows > 0 && rows <= a.n_rows - r0) n = (rows * a.group + rows_per_tile - 1) / rows_per_tile;
         }
         int total;
         const int upto = scan256(n, sh, total);
         if (id >= total) return false;
-        if (id >= upto - n && id < upto) { sh[NW] = s; sh[NW + 1] = id - (upto - n); }
+        if (id >= upto - n && id < upto) {
+            sh[NW] = s; sh[NW + 1] = id - (upto - n); sh[NW + 2] = r0; sh[NW + 3] = rows; sh[NW + 4] = len;
+        }
         __syncthreads();
-        t.seq = sh[NW];
-        tile = sh[NW + 1];
+        t.seq = __builtin_amdgcn_readfirstlane(sh[NW]);
+        tile = __builtin_amdgcn_readfirstlane(sh[NW + 1]);
+        t.r0 = __builtin_amdgcn_readfirstlane(sh[NW + 2]);
+        t.n = __builtin_amdgcn_readfirstlane(sh[NW + 3]);
+        t.len = __builtin_amdgcn_readfirstlane(sh[NW + 4]);
     }
-    t.r0 = a.rows[t.seq];
-    t.n = a.rows[t.seq + 1] - t.r0;
-    if (t.r0 < 0 || t.n <= 0 || t.r0 + t.n > a.n_rows) return false;
     t.row = tile * rows_per_tile;
     if (t.row >= t.n * a.group || (a.one_tile && t.n * a.group > rows_per_tile)) return false;
-    t.len = max(a.len[t.seq], 0);
+    t.len = max(t.len, 0);
     t.pos0 = t.len - t.n;
     const int last = (min(t.row + rows_per_tile, t.n * a.group) - 1) / a.group;
     const int p0 = t.pos0 + t.row / a.group, p1 = t.pos0 + last;   // first and last row's positions
@@ -173,32 +180,48 @@ struct Raw {
     uint32_t v[8][D / 64];
 };
 
-// The query row at element `off`, as this lane's dims of a B operand.
-template <int D, bool BF16>
-__device__ __forceinline__ void fetch_query(const Args &a, long off, int g, float (&x)[D / 32][8]) {
+// The query row at element `off`: this lane's dims of each B operand, as
+// they lie in memory.
+template <bool BF16>
+struct QPiece;
+template <>
+struct QPiece<true> {
+    u16x8 v;
+    __device__ __forceinline__ float at(int j) const { return bf2f(v[j]); }
+};
+template <>
+struct QPiece<false> {
+    f32x4 v[2];
+    __device__ __forceinline__ float at(int j) const { return v[j >> 2][j & 3]; }
+};
+
+template <int D>
+__device__ __forceinline__ void fetch_query(const Args &a, long off, int g, QPiece<true> (&x)[D / 32]) {
+    const uint16_t *q = reinterpret_cast<const uint16_t *>(a.q) + off + 16 * g;
+    if (a.vec) {
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-        const long d = off + 64 * (i >> 1) + 16 * g + 8 * (i & 1);
-        if (BF16) {
-            const uint16_t *q = reinterpret_cast<const uint16_t *>(a.q) + d;
-            u16x8 y;
-            if (a.vec) y = *reinterpret_cast<const u16x8 *>(q);
-            else
+        for (int i = 0; i < D / 32; i++) x[i].v = *reinterpret_cast<const u16x8 *>(q + 64 * (i >> 1) + 8 * (i & 1));
+    } else {
 #pragma unroll
-                for (int j = 0; j < 8; j++) y[j] = q[j];
+        for (int i = 0; i < D / 32; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[i][j] = bf2f(y[j]);
-        } else {
-            const float *q = reinterpret_cast<const float *>(a.q) + d;
-            if (a.vec) {
-                const f32x4 y = reinterpret_cast<const f32x4 *>(q)[0], z = reinterpret_cast<const f32x4 *>(q)[1];
+            for (int j = 0; j < 8; j++) x[i].v[j] = q[64 * (i >> 1) + 8 * (i & 1) + j];
+    }
+}
+template <int D>
+__device__ __forceinline__ void fetch_query(const Args &a, long off, int g, QPiece<false> (&x)[D / 32]) {
+    const float *q = reinterpret_cast<const float *>(a.q) + off + 16 * g;
+    if (a.vec) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) { x[i][j] = y[j]; x[i][4 + j] = z[j]; }
-            } else {
+        for (int i = 0; i < D / 32; i++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[i][j] = q[j];
-            }
-        }
+            for (int j = 0; j < 2; j++)
+                x[i].v[j] = *reinterpret_cast<const f32x4 *>(q + 64 * (i >> 1) + 8 * (i & 1) + 4 * j);
+    } else {
+#pragma unroll
+        for (int i = 0; i < D / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[i].v[j >> 2][j & 3] = q[64 * (i >> 1) + 8 * (i & 1) + j];
     }
 }
 
@@ -206,7 +229,7 @@ __device__ __forceinline__ void fetch_query(const Args &a, long off, int g, floa
 // terms; returns the factor of its scores: what the power of two and the
 // softmax scale leave.  A row with a value that is not finite is all NaN.
 template <int D, bool BF16>
-__device__ __forceinline__ float split_query(const Args &a, bool have, const float (&x)[D / 32][8],
+__device__ __forceinline__ float split_query(const Args &a, bool have, const QPiece<BF16> (&x)[D / 32],
                                              f16x8 (&qf)[BF16 ? 1 : 2][D / 32]) {
     constexpr int KS = D / 32, NB = BF16 ? 1 : 2;
     // the largest magnitude as an integer: infinities and NaN are the largest
@@ -214,7 +237,7 @@ __device__ __forceinline__ float split_query(const Args &a, bool have, const flo
 #pragma unroll
     for (int i = 0; i < KS; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[i][j]) & 0x7fffffffu);
+        for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[i].at(j)) & 0x7fffffffu);
     if (!have) top = 0;
     auto r = __builtin_amdgcn_permlane32_swap(top, top, false, false);
     top = max(r[0], r[1]);
@@ -229,7 +252,7 @@ __device__ __forceinline__ float split_query(const Args &a, bool have, const flo
     for (int i = 0; i < KS; i++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float y = !have ? 0.0f : fine ? x[i][j] * f0 * f1 : __uint_as_float(0x7fc00000u);
+            const float y = !have ? 0.0f : fine ? x[i].at(j) * f0 * f1 : __uint_as_float(0x7fc00000u);
             qf[0][i][j] = (_Float16)y;
             if (NB > 1) qf[NB - 1][i][j] = (_Float16)(y - (float)qf[0][i][j]);
         }
@@ -407,7 +430,7 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
     constexpr int KS = D / 32;            // k steps of the score product
     constexpr int DI = D / 16;            // 16-dim tiles of O; dims of V a lane loads
     constexpr int NB = BF16 ? 1 : 2;      // f16 terms of a query value and of p
-    __shared__ int sh[NW + 2];
+    __shared__ int sh[NW + 5];
     __shared__ float so[NW][16][D];
     __shared__ float sm[NW][16], sl[NW][16];
 
@@ -439,8 +462,8 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
         if (!ahead && mine) pg = a.table[(long)t.seq * a.table_w + (key_i >> a.lp)];
         if (!mine || (unsigned)pg >= (unsigned)a.pages) pg = -1;
     }
-    float x[KS][8];
-    fetch_query<D, BF16>(a, (long)(t.r0 + qi) * a.ld_q + (long)(h * a.group + qh) * D, g, x);
+    QPiece<BF16> x[KS];
+    fetch_query<D>(a, (long)(t.r0 + qi) * a.ld_q + (long)(h * a.group + qh) * D, g, x);
 
     const int P = 1 << a.lp;
     const unsigned koff = c * D + 16 * g, voff = 4 * g * D + c * DI;
@@ -632,7 +655,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     constexpr int ROWS = rows_of(BF16), WR = ROWS / NW, NQ = WR / 16;
     constexpr int UNIT = D * 32;               // halves of a 32-key step's K or V
     static_assert(2 * KS == DI, "K and V take the same number of operands");
-    __shared__ int sh[NW + 2];
+    __shared__ int sh[NW + 5];
     __shared__ __align__(16) _Float16 lds[2][4][UNIT];   // buffer; K, K, V, V of the two steps
     __shared__ float sscale[2][4];             // key scales of the four 16-key halves
     __shared__ int sexp[2][4];                 // exponents of the value scales; NONE: not in the pool
@@ -647,20 +670,6 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
     const int all = t.n * a.group, hard = min(t.len, a.cap);
 
-    // this wavefront's rows
-    f16x8 qf[NQ][NB][KS];
-    float qs[NQ];
-    Sight see[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; n++) {
-        const int R = t.row + WR * w + 16 * n + c;
-        const bool have = R < all;
-        const int qi = have ? R / a.group : 0, qh = have ? R % a.group : 0;
-        float x[KS][8];
-        fetch_query<D, BF16>(a, (long)(t.r0 + qi) * a.ld_q + (long)(h * a.group + qh) * D, g, x);
-        qs[n] = split_query<D, BF16>(a, have, x, qf[n]);
-        see[n].set(a, t.pos0 + qi, t.len, have);
-    }
     const int wr0 = min(t.row + WR * w, all - 1), wr1 = min(t.row + WR * w + WR, all) - 1;
     const bool idle = t.row + WR * w >= all;
     const int p0 = t.pos0 + wr0 / a.group, p1 = t.pos0 + wr1 / a.group;
@@ -682,7 +691,14 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
         return (unsigned)p < (unsigned)a.pages ? p : -1;
     };
     auto fetch_scale = [&](int p) { return p >= 0 ? (isv ? a.vs : a.ks)[(long)p * a.kv + h] : 0.0f; };
+    // asked for together: the first pages, the query rows; then what they lead to
     int pg = fetch_page(0), pg2 = fetch_page(32);
+    QPiece<BF16> x[NQ][KS];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int R = min(t.row + WR * w + 16 * n + c, all - 1);
+        fetch_query<D>(a, (long)(t.r0 + R / a.group) * a.ld_q + (long)(h * a.group + R % a.group) * D, g, x[n]);
+    }
     float psc = fetch_scale(pg), psc2 = 0.0f;
     const uint8_t *pool = isv ? a.v : a.k;
     const unsigned off = isv ? 4 * g * D + c * DI : c * D + 16 * g;
@@ -703,16 +719,17 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
             if (!isv) {
 #pragma unroll
                 for (int x = 0; x < D / 64; x++) {
-                    const uint4 y = *reinterpret_cast<const uint4 *>(p + at + 64 * x);
-                    to[4 * x] = y.x; to[4 * x + 1] = y.y; to[4 * x + 2] = y.z; to[4 * x + 3] = y.w;
+                    const u32x4 y = *reinterpret_cast<const u32x4 *>(p + at + 64 * x);
+#pragma unroll
+                    for (int i2 = 0; i2 < 4; i2++) to[4 * x + i2] = y[i2];
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     if (D == 128) {
-                        const uint2 y = *reinterpret_cast<const uint2 *>(p + at + j * D);
-                        to[2 * j] = y.x;
-                        to[2 * j + 1] = y.y;
+                        const u32x2 y = *reinterpret_cast<const u32x2 *>(p + at + j * D);
+                        to[2 * j] = y[0];
+                        to[2 * j + 1] = y[1];
                     } else {
                         to[j] = *reinterpret_cast<const uint32_t *>(p + at + j * D);
                     }
@@ -781,6 +798,19 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
         }
     };
 
+    if (iters > 0) fetch(0);
+
+    // this wavefront's rows
+    f16x8 qf[NQ][NB][KS];
+    float qs[NQ];
+    Sight see[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int R = t.row + WR * w + 16 * n + c;
+        const bool have = R < all;
+        qs[n] = split_query<D, BF16>(a, have, x[n], qf[n]);
+        see[n].set(a, t.pos0 + (have ? R / a.group : 0), t.len, have);
+    }
     f32x4 o[NQ][DI];
     float m[NQ], l[NQ];
 #pragma unroll
@@ -792,10 +822,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     }
     int eref = KV8_MIN_EXP, emax = KV8_MIN_EXP;
 
-    if (iters > 0) {
-        fetch(0);
-        place(0);
-    }
+    if (iters > 0) place(0);
     for (int it = 0; it < iters; it++) {
         __syncthreads();
         const bool more = it + 1 < iters;
@@ -804,7 +831,15 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
         if (k0 < wend) {
             const f16x8 *kl = reinterpret_cast<const f16x8 *>(lds[b][0]) + lane;
             const f16x8 *vl = reinterpret_cast<const f16x8 *>(lds[b][2]) + lane;
+            // operands are read a group of four ahead of the products they feed
             f32x4 s[NQ][4];
+            f16x8 kf[2][4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                kf[0][u] = kl[((u >> 1) * DI + (u & 1) * KS) * CT_WAVE];
+#pragma unroll
+                for (int n = 0; n < NQ; n++) s[n][u] = (f32x4){0, 0, 0, 0};
+            }
             int ev[4];
             float f[NQ][4];
             bool in[4], every = true;
@@ -815,18 +850,23 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
                 in[u] = ev[u] != NONE && (u < 2 || s0 + 2 * it + 1 < s1);
                 every = every && in[u];
 #pragma unroll
-                for (int n = 0; n < NQ; n++) {
-                    f[n][u] = qs[n] * ks;
-                    s[n][u] = (f32x4){0, 0, 0, 0};
-                }
+                for (int n = 0; n < NQ; n++) f[n][u] = qs[n] * ks;
+            }
+            f16x8 vf[2][4];
 #pragma unroll
-                for (int x = 0; x < KS; x++) {
-                    const f16x8 kf = kl[((u >> 1) * DI + (u & 1) * KS + x) * CT_WAVE];
+            for (int x = 0; x < KS; x++) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    if (x + 1 < KS) kf[(x + 1) & 1][u] = kl[((u >> 1) * DI + (u & 1) * KS + x + 1) * CT_WAVE];
+                    else vf[0][u] = vl[u * CT_WAVE];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < 4; u++)
 #pragma unroll
                     for (int n = 0; n < NQ; n++)
 #pragma unroll
-                        for (int y = 0; y < NB; y++) s[n][u] = mfma_f16(kf, qf[n][y][x], s[n][u]);
-                }
+                        for (int y = 0; y < NB; y++) s[n][u] = mfma_f16(kf[x & 1][u], qf[n][y][x], s[n][u]);
             }
             const bool whole = every && k0 >= full_lo && k0 + 32 <= full_hi && k1 >= full_lo && k1 + 32 <= full_hi;
             if (__builtin_expect(!whole, 0)) {
@@ -866,17 +906,24 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
                     for (int i = 0; i < DI; i++) o[n][i] *= al;
                 }
             }
+            // group y of the V operands: four dim tiles of step y / (DI / 4); a
+            // second step that is not there has p' = 0 and holds finite values
+            constexpr int VG = DI / 2;
 #pragma unroll
-            for (int y = 0; y < 2; y++) {
-                if (y && s0 + 2 * it + 1 >= s1) break;
+            for (int y = 0; y < VG; y++) {
+                if (y + 1 < VG)
 #pragma unroll
-                for (int i = 0; i < DI; i++) {
-                    const f16x8 vf = vl[(y * DI + i) * CT_WAVE];
+                    for (int i = 0; i < 4; i++) vf[(y + 1) & 1][i] = vl[(4 * (y + 1) + i) * CT_WAVE];
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int n = 0; n < NQ; n++)
 #pragma unroll
-                        for (int z = 0; z < NB; z++) o[n][i] = mfma_f16(vf, pf[n][y][z], o[n][i]);
-                }
+                        for (int z = 0; z < NB; z++) {
+                            f32x4 &to = o[n][(4 * y + i) % DI];
+                            to = mfma_f16(vf[y & 1][i], pf[n][y / (DI / 4)][z], to);
+                        }
             }
 #pragma unroll 1
             for (int y = 0; y < 2; y++)
@@ -918,7 +965,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 template <int D, bool BF16, int WPR>
 __global__ __launch_bounds__(NT) void join_kernel(Args a) {
     constexpr int DL = D / CT_WAVE, RPB = NW / WPR;       // dims of a lane, rows of a workgroup
-    __shared__ int sh[NW + 2];
+    __shared__ int sh[NW + 5];
     __shared__ float so[NW][D], sl[NW];
     const int h = blockIdx.x % a.kv, id = blockIdx.x / a.kv;
     Tile t;
