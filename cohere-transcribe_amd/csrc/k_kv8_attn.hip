@@ -24,6 +24,7 @@
 #include "ct_dev.h"
 #include "ct_kv8.h"
 #include "k_kv8.h"
+#include <type_traits>
 
 namespace {
 
@@ -56,6 +57,14 @@ struct Args {
     float *part;                 // partial O [tile][kv][chunk][rpt][D], then (m, l) pairs
     float2 *stat;
 };
+
+// The kernel's arguments read again, past this point: what only its end
+// needs does not hold scalar registers through the loop.
+__device__ __forceinline__ const Args &args_again() {
+    auto p = (const __attribute__((address_space(4))) Args *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Args *)p;
+}
 
 // A tile's rows and the keys they see: 32-key steps 0 .. sink_steps - 1 hold
 // the first tokens, the rest start at lo (a multiple of 32).
@@ -259,30 +268,32 @@ __device__ __forceinline__ float split_query(const Args &a, bool have, const QPi
     return a.scale2 * pow2i((-up) >> 1) * pow2i(-up - ((-up) >> 1));
 }
 
-// What the queries of a step's U 16-key halves share: the exponent offset of
-// p' and what undoes it in l.
+// What the queries of a step's U 16-key halves share: the key scales, the
+// exponent offset of p' and what undoes it in l.  least: the smallest factor
+// of a score where some are masked, 0 elsewhere: -inf * 0 is NaN, and scores
+// that small are 0 to the softmax.
 template <int U>
 struct Halves {
-    float adj[U], undo[U];
-    __device__ __forceinline__ void set(int u, int ev, bool in, int eref) {
-        const int x = max(in ? P_EXP + ev - eref : P_EXP, -40);
+    float ks[U], adj[U], undo[U], least;
+    __device__ __forceinline__ void set(int u, int ev, int eref) {
+        const int x = max(P_EXP + ev - eref, -40);
         adj[u] = (float)x;
         undo[u] = pow2i(-x);
     }
 };
 
-// p' of one query over U halves: 2^(s f - m + adj).
+// p' of one query over U halves: 2^(s qs ks - m + adj).
 template <int U, int NB>
-__device__ __forceinline__ void powers(const f32x4 (&s)[U], const float (&f)[U], const Halves<U> &hv, float m,
+__device__ __forceinline__ void powers(const f32x4 (&s)[U], float qs, const Halves<U> &hv, float m,
                                        float (&sum)[U], f16x8 (&pf)[U / 2][NB]) {
     const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const float ms = mu - hv.adj[u];
+        const float ms = mu - hv.adj[u], f = fmaxf(qs * hv.ks[u], hv.least);
         float p[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], f[u], -ms));
+            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], f, -ms));
             pf[u >> 1][0][4 * (u & 1) + j] = (_Float16)p[j];
             if (NB > 1) pf[u >> 1][NB - 1][4 * (u & 1) + j] = (_Float16)(p[j] - (float)pf[u >> 1][0][4 * (u & 1) + j]);
         }
@@ -299,18 +310,18 @@ __device__ __forceinline__ void powers(const f32x4 (&s)[U], const float (&f)[U],
 }
 
 // One query's online softmax over U halves: scores s (-inf: not seen) times
-// f, in base 2; p' as B operands.  The maximum is found only when it has to
+// qs and the key scale, in base 2; p' as B operands.  The maximum is found only when it has to
 // be: p' are computed with the one so far, and if one of them (in any lane)
 // passes 2^(P_EXP + SLACK) the maximum moves and they are computed again.
 // Returns the factor of the sums so far, which is 1 unless `moved`, the same
 // in the whole wavefront.
 template <int U, int NB>
-__device__ __forceinline__ float weigh(const f32x4 (&s)[U], const float (&f)[U], const Halves<U> &hv, float &m, float &l,
+__device__ __forceinline__ float weigh(const f32x4 (&s)[U], float qs, const Halves<U> &hv, float &m, float &l,
                                        bool &moved, f16x8 (&pf)[U / 2][NB]) {
     float sum[U];
     moved = __any(m == -INFINITY);
     if (!moved) {
-        powers<U, NB>(s, f, hv, m, sum, pf);
+        powers<U, NB>(s, qs, hv, m, sum, pf);
         // f16 bits as integers: p' >= 0, and infinities and NaN are the largest
         u16x2 top = {0, 0};
 #pragma unroll
@@ -326,33 +337,40 @@ __device__ __forceinline__ float weigh(const f32x4 (&s)[U], const float (&f)[U],
         float mt = -INFINITY;
 #pragma unroll
         for (int u = 0; u < U; u++)
-            mt = fmaxf(mt, f[u] * fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
+            mt = fmaxf(mt, fmaxf(qs * hv.ks[u], hv.least) * fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
         const float mn = fmaxf(m, fmax_q(mt));
         al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= al;
-        powers<U, NB>(s, f, hv, m, sum, pf);
+        powers<U, NB>(s, qs, hv, m, sum, pf);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) l = __builtin_fmaf(sum[u], hv.undo[u], l);
     return al;
 }
 
-// -inf * 0 is NaN: where scores are masked their factors are kept from
-// underflowing (scores below 2^-70 are 0 to the softmax).
-__device__ __forceinline__ float above0(float f) { return f < 0x1p-100f ? 0x1p-100f : f; }
-
-// The keys a query sees: [0, first) and [lo, lo + n).
+// The keys the row at position pos of a sequence of len tokens sees: [0,
+// first) and [lo, lo + n).
 struct Sight {
-    unsigned first, n;
-    int lo;
-    __device__ __forceinline__ void set(const Args &a, int pos, int len, bool have) {
-        const int end = have ? max(min(a.causal ? pos + 1 : len, a.cap), 0) : 0;
+    int first, n, lo;
+    __device__ __forceinline__ Sight(const Args &a, int len, int pos) {
+        const int end = max(min(a.causal ? pos + 1 : len, a.cap), 0);
         lo = a.window ? pos - a.window + 1 : 0;
         first = a.window ? min(a.sinks, end) : end;
         n = a.window ? max(end - lo, 0) : 0;
     }
-    __device__ __forceinline__ bool sees(int key) const { return (unsigned)key < first || (unsigned)(key - lo) < n; }
+    // all ones if the query sees the key, else 0: no comparison, whose results
+    // for many keys at once would not fit the scalar registers
+    __device__ __forceinline__ uint32_t sees(const Args &a, int key) const {
+        const int before = (key - first) >> 31;
+        if (!a.window) return before;
+        return before | ~(((key - lo) | (lo + n - 1 - key)) >> 31);
+    }
+    // the score, or -inf
+    __device__ __forceinline__ float masked(const Args &a, int key, float s) const {
+        const uint32_t m = sees(a, key);
+        return __uint_as_float((__float_as_uint(s) & m) | (0xff800000u & ~m));
+    }
 };
 
 // The reference exponent follows the value scales (e1: the largest of this
@@ -386,11 +404,11 @@ __device__ __forceinline__ void operand_v(Code code, f16x8 (&vf)[4]) {
 
 // The NaN codes among a step's values, which the products took as zeros: they
 // reach the rows that see their token, and they alone (0 * NaN is NaN, so a
-// product over a masked one would spread it).  Rare, so the codes are read
-// again: kept in registers they cost the common path 40 of them.
+// product over a masked one would spread it).  Rare, so it is done after all
+// steps, from the codes read again: in the loop it cost 40 registers.
 template <int D, int NQ>
 __device__ __forceinline__ void spread_nan(const Args &a, const Tile &t, int h, int key, int c, int g,
-                                           const Sight (&see)[NQ], f32x4 (&o)[NQ][D / 16]) {
+                                           const int (&pos)[NQ], f32x4 (&o)[NQ][D / 16]) {
     f16x8 one[NQ];
     uint32_t nan[8][D / 64];
 #pragma unroll
@@ -405,7 +423,7 @@ __device__ __forceinline__ void spread_nan(const Args &a, const Tile &t, int h, 
             nan[j][x] = in ? nan_bytes(*reinterpret_cast<const uint32_t *>(a.v + base + 4 * x)) : 0;
 #pragma unroll
         for (int n = 0; n < NQ; n++)
-            one[n][j] = in && see[n].sees(kk) ? (_Float16)1.0f : (_Float16)0.0f;
+            one[n][j] = in && Sight(a, t.len, pos[n]).sees(a, kk) ? (_Float16)1.0f : (_Float16)0.0f;
     }
 #pragma unroll
     for (int i = 0; i < D / 16; i++) {
@@ -502,8 +520,7 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
     }
     f16x8 qf[NB][KS];
     const float qs = split_query<D, BF16>(a, have, x, qf);
-    Sight see[1];
-    see[0].set(a, t.pos0 + qi, t.len, have);
+    const int pos[1] = {t.pos0 + qi};
     const int hard = min(t.len, a.cap);      // tokens at and past it hold anything
 
     f32x4 o[1][DI];
@@ -511,17 +528,18 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
     for (int i = 0; i < DI; i++) o[0][i] = (f32x4){0, 0, 0, 0};
     float m = have ? -INFINITY : 0.0f, l = 0.0f;         // lanes without a row never move the maximum
     int eref = KV8_MIN_EXP, emax = KV8_MIN_EXP;
+    bool dirty = false;
 
     auto use = [&](int st, int i, Raw<D> &r) {
         const int key = step_key(t, st);
         f32x4 s[2];
-        float f[2];
+        Halves<2> hv;
         int ev[2];
         bool in[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             in[u] = __builtin_amdgcn_readlane(pg, 2 * i + u) >= 0;
-            f[u] = qs * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pks), 2 * i + u));
+            hv.ks[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pks), 2 * i + u));
             ev[u] = max((int)(__builtin_amdgcn_readlane(__float_as_uint(pvs), 2 * i + u) >> 23 & 255) - 127, KV8_MIN_EXP);
             s[u] = (f32x4){0, 0, 0, 0};
 #pragma unroll
@@ -535,17 +553,15 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
             }
         }
         const bool whole = key >= t.full_lo && key + 32 <= t.full_hi && in[0] && in[1];   // sink steps lie below full_lo
-        bool nan = false;
         if (__builtin_expect(!whole, 0)) {
             uint32_t bad = 0;
-            f[0] = above0(f[0]);
-            f[1] = above0(f[1]);
+            const Sight see(a, t.len, pos[0]);
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int kk = key + 16 * u + 4 * g + j;
-                    if (!(in[u] && see[0].sees(kk))) s[u][j] = -INFINITY;
+                    s[u][j] = in[u] ? see.masked(a, kk, s[u][j]) : -INFINITY;
                     // a token nobody sees may hold anything: 0 * NaN is NaN
                     const bool any = in[u] && kk < hard;
 #pragma unroll
@@ -554,27 +570,27 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
                         bad |= nan_bytes(r.v[4 * u + j][y]);
                     }
                 }
-            nan = __any(bad != 0);
-            if (nan) {
+            if (__builtin_expect(__any(bad != 0), 0)) {
+                dirty = true;
 #pragma unroll
                 for (int j = 0; j < 8; j++)
 #pragma unroll
                     for (int y = 0; y < D / 64; y++) r.v[j][y] = without_nan(r.v[j][y]);
             }
         }
-        const int e1 = max(in[0] ? ev[0] : KV8_MIN_EXP, in[1] ? ev[1] : KV8_MIN_EXP);
+        const int e1 = max(ev[0], ev[1]);        // pages that are not there have the least
         emax = max(emax, e1);
         if (__builtin_expect(e1 > eref || e1 < eref - 8, 0)) {
             const float by = follow(e1, emax, eref);
 #pragma unroll
             for (int y = 0; y < DI; y++) o[0][y] *= by;
         }
-        Halves<2> hv;
-        hv.set(0, ev[0], in[0], eref);
-        hv.set(1, ev[1], in[1], eref);
+        hv.least = whole ? 0.0f : 0x1p-100f;
+        hv.set(0, ev[0], eref);
+        hv.set(1, ev[1], eref);
         f16x8 pf[1][NB];
         bool moved;
-        const float al = weigh<2, NB>(s, f, hv, m, l, moved, pf);
+        const float al = weigh<2, NB>(s, qs, hv, m, l, moved, pf);
         if (moved) {
 #pragma unroll
             for (int y = 0; y < DI; y++) o[0][y] *= al;
@@ -588,7 +604,6 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
 #pragma unroll
                 for (int n = 0; n < NB; n++) o[0][4 * y + b] = mfma_f16(vf[b], pf[0][n], o[0][4 * y + b]);
         }
-        if (__builtin_expect(nan, 0)) spread_nan<D, 1>(a, t, h, key, c, g, see, o);
     };
 
     // two steps in flight
@@ -599,6 +614,8 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
         if (st + 2 * NW < last) load(st + 2 * NW, i + 2, ra);
         use(st + NW, i + 1, rb);
     }
+    if (__builtin_expect(dirty, 0))
+        for (int st = first; st < last; st += NW) spread_nan<D, 1>(a, t, h, step_key(t, st), c, g, pos, o);
 
     // the wavefronts' sums joined, in their order
     l = sum_q(l);
@@ -658,9 +675,9 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     __shared__ int sh[NW + 5];
     __shared__ __align__(16) _Float16 lds[2][4][UNIT];   // buffer; K, K, V, V of the two steps
     __shared__ float sscale[2][4];             // key scales of the four 16-key halves
-    __shared__ int sexp[2][4];                 // exponents of the value scales; NONE: not in the pool
-    __shared__ int snan[2][2];                 // the V of a step holds a NaN
-    constexpr int NONE = 1 << 20;
+    __shared__ int sexp[2][4];                 // exponents of the value scales
+    __shared__ int smiss[2][2];                // of each step: bit u: half u is not in the pool
+    __shared__ int snan;                       // the V of some step holds a NaN
 
     const int h = blockIdx.x % a.kv, id = gridDim.x / a.kv - 1 - blockIdx.x / a.kv, ch = blockIdx.y;
     Tile t;
@@ -703,20 +720,28 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     const uint8_t *pool = isv ? a.v : a.k;
     const unsigned off = isv ? 4 * g * D + c * DI : c * D + 16 * g;
 
-    uint32_t raw[D / 8];                         // the unit's codes: 8 D / 64 dwords of K or V
-    int rp[2];
-    float rs[2];
-    auto fetch = [&](int it) {
+    // the codes of a unit, asked for AHEAD iterations before they are converted,
+    // with their pages and scales; bf16 has no registers for a second one
+    constexpr int AHEAD = BF16 ? 1 : 2;
+    struct Unit {
+        uint32_t raw[D / 8];
+        int p0, p1;
+        float s0, s1;
+    };
+    auto fetch = [&](int it, Unit &r, auto is_v) __attribute__((always_inline)) {
+        constexpr bool V = decltype(is_v)::value;
         unsigned at = off;
         asm volatile("" : "+v"(at));            // a 32-bit offset beside a scalar base, not a 64-bit sum a load
         const int i = 2 * (it & 31), key = step_key(t, min(s0 + 2 * it + kb, s1 - 1));
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            rp[u] = __builtin_amdgcn_readlane(pg, i + u);
-            rs[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(psc), i + u));
-            const uint8_t *p = pool + ((((long)max(rp[u], 0) * a.kv + h) << a.lp) + ((key + 16 * u) & (P - 1))) * D;
-            uint32_t *to = raw + u * (D / 16);
-            if (!isv) {
+            const int page = __builtin_amdgcn_readlane(pg, i + u);
+            const float sc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(psc), i + u));
+            if (u) { r.p1 = page; r.s1 = sc; }
+            else { r.p0 = page; r.s0 = sc; }
+            const uint8_t *p = pool + ((((long)max(page, 0) * a.kv + h) << a.lp) + ((key + 16 * u) & (P - 1))) * D;
+            uint32_t *to = r.raw + u * (D / 16);
+            if constexpr (!V) {
 #pragma unroll
                 for (int x = 0; x < D / 64; x++) {
                     const u32x4 y = *reinterpret_cast<const u32x4 *>(p + at + 64 * x);
@@ -744,73 +769,77 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
             pg2 = fetch_page(it + 33);
         }
     };
-    auto place = [&](int it) {                   // the fetched unit into buffer it & 1
+    bool dirty = false;
+    auto place = [&](int it, Unit &r, auto is_v) __attribute__((always_inline)) {       // a fetched unit into buffer it & 1
+        constexpr bool V = decltype(is_v)::value;
         const int b = it & 1;
-        f16x8 *to = reinterpret_cast<f16x8 *>(lds[b][2 * isv + kb]) + lane;
+        f16x8 *to = reinterpret_cast<f16x8 *>(lds[b][2 * V + kb]) + lane;
         if (lane < 2) {
             const int half = 2 * kb + lane;
-            const float sc = lane ? rs[1] : rs[0];
-            const int p = lane ? rp[1] : rp[0];
-            if (!isv) sscale[b][half] = sc;
-            else sexp[b][half] = p < 0 ? NONE : max((int)(__float_as_uint(sc) >> 23 & 255) - 127, KV8_MIN_EXP);
+            const float sc = lane ? r.s1 : r.s0;
+            const int p = lane ? r.p1 : r.p0;
+            if (!V) sscale[b][half] = sc;
+            else sexp[b][half] = p < 0 ? KV8_MIN_EXP : max((int)(__float_as_uint(sc) >> 23 & 255) - 127, KV8_MIN_EXP);
+            if (V && lane == 0) smiss[b][kb] = (r.p0 < 0) | (r.p1 < 0) << 1;
         }
-        if (!isv) {
+        if constexpr (!V) {
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int x = 0; x < D / 64; x++) {
-                    const uint32_t *y = raw + u * (D / 16) + 4 * x;
+                    const uint32_t *y = r.raw + u * (D / 16) + 4 * x;
                     to[(u * KS + 2 * x) * CT_WAVE] = cvt8(y[0], y[1]);
                     to[(u * KS + 2 * x + 1) * CT_WAVE] = cvt8(y[2], y[3]);
                 }
-            return;
-        }
+        } else {
         // a step that every row of the tile sees whole may spread its NaN; one
         // that some row does not: tokens that are not there hold anything, and
         // a NaN must not meet a masked row's zero
         const int key = step_key(t, min(s0 + 2 * it + kb, s1 - 1));
-        bool nan = false;
-        if (__builtin_expect(!(rp[0] >= 0 && rp[1] >= 0 && key >= t.full_lo && key + 32 <= t.full_hi), 0)) {
+        if (__builtin_expect(!(r.p0 >= 0 && r.p1 >= 0 && key >= t.full_lo && key + 32 <= t.full_hi), 0)) {
             uint32_t bad = 0;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const bool in = rp[j >> 2] >= 0 && key + 4 * g + 16 * (j >> 2) + (j & 3) < hard;
+                // all ones where the token is there
+                const uint32_t in = (j < 4 ? r.p0 : r.p1) < 0 ? 0 : (key + 4 * g + 16 * (j >> 2) + (j & 3) - hard) >> 31;
 #pragma unroll
                 for (int x = 0; x < D / 64; x++) {
-                    uint32_t &y = raw[j * (D / 64) + x];
-                    y = in ? y : 0;
+                    uint32_t &y = r.raw[j * (D / 64) + x];
+                    y &= in;
                     bad |= nan_bytes(y);
                 }
             }
-            nan = __any(bad != 0);
-            if (nan) {
+            if (__builtin_expect(__any(bad != 0), 0)) {
+                dirty = true;
 #pragma unroll
-                for (int x = 0; x < D / 8; x++) raw[x] = without_nan(raw[x]);
+                for (int x = 0; x < D / 8; x++) r.raw[x] = without_nan(r.raw[x]);
             }
         }
-        if (lane == 0) snan[b][kb] = nan;
 #pragma unroll
         for (int x = 0; x < D / 64; x++) {
             f16x8 vf[4];
-            operand_v<D>([&](int j) { return raw[j * (D / 64) + x]; }, vf);
+            operand_v<D>([&](int j) { return r.raw[j * (D / 64) + x]; }, vf);
 #pragma unroll
             for (int i = 0; i < 4; i++) to[(4 * x + i) * CT_WAVE] = vf[i];
         }
+        }
     };
 
-    if (iters > 0) fetch(0);
 
     // this wavefront's rows
     f16x8 qf[NQ][NB][KS];
     float qs[NQ];
-    Sight see[NQ];
+    int pos[NQ];
+    auto split = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const int R = t.row + WR * w + 16 * n + c;
         const bool have = R < all;
         qs[n] = split_query<D, BF16>(a, have, x[n], qf[n]);
-        see[n].set(a, t.pos0 + (have ? R / a.group : 0), t.len, have);
+        pos[n] = t.pos0 + (have ? R / a.group : 0);
     }
+    };
+
     f32x4 o[NQ][DI];
     float m[NQ], l[NQ];
 #pragma unroll
@@ -822,11 +851,14 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     }
     int eref = KV8_MIN_EXP, emax = KV8_MIN_EXP;
 
-    if (iters > 0) place(0);
-    for (int it = 0; it < iters; it++) {
+    // iteration `it`: the unit asked for AHEAD iterations ago into the other
+    // buffer, the next one asked for, and this one's products.  One barrier:
+    // before it every wavefront has filled its part of this buffer and is done
+    // with the other.
+    auto step = [&](int it, Unit &r, auto is_v) __attribute__((always_inline)) {
         __syncthreads();
-        const bool more = it + 1 < iters;
-        if (more) fetch(it + 1);
+        if (it + 1 < iters) place(it + 1, r, is_v);
+        if (it + 1 + AHEAD < iters) fetch(it + 1 + AHEAD, r, is_v);
         const int b = it & 1, k0 = step_key(t, s0 + 2 * it), k1 = step_key(t, min(s0 + 2 * it + 1, s1 - 1));
         if (k0 < wend) {
             const f16x8 *kl = reinterpret_cast<const f16x8 *>(lds[b][0]) + lane;
@@ -841,16 +873,12 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
                 for (int n = 0; n < NQ; n++) s[n][u] = (f32x4){0, 0, 0, 0};
             }
             int ev[4];
-            float f[NQ][4];
-            bool in[4], every = true;
+            Halves<4> hv;
+            const int miss = __builtin_amdgcn_readfirstlane(smiss[b][0] | smiss[b][1] << 2);
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const float ks = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sscale[b][u])));
+                hv.ks[u] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sscale[b][u])));
                 ev[u] = __builtin_amdgcn_readfirstlane(sexp[b][u]);
-                in[u] = ev[u] != NONE && (u < 2 || s0 + 2 * it + 1 < s1);
-                every = every && in[u];
-#pragma unroll
-                for (int n = 0; n < NQ; n++) f[n][u] = qs[n] * ks;
             }
             f16x8 vf[2][4];
 #pragma unroll
@@ -858,7 +886,6 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     if (x + 1 < KS) kf[(x + 1) & 1][u] = kl[((u >> 1) * DI + (u & 1) * KS + x + 1) * CT_WAVE];
-                    else vf[0][u] = vl[u * CT_WAVE];
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -868,23 +895,23 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
                         for (int y = 0; y < NB; y++) s[n][u] = mfma_f16(kf[x & 1][u], qf[n][y][x], s[n][u]);
             }
-            const bool whole = every && k0 >= full_lo && k0 + 32 <= full_hi && k1 >= full_lo && k1 + 32 <= full_hi;
+#pragma unroll
+            for (int i = 0; i < 4; i++) vf[0][i] = vl[i * CT_WAVE];
+            const bool whole = !miss && k0 >= full_lo && k0 + 32 <= full_hi && k1 >= full_lo && k1 + 32 <= full_hi;
             if (__builtin_expect(!whole, 0)) {
 #pragma unroll
-                for (int n = 0; n < NQ; n++)
+                for (int n = 0; n < NQ; n++) {
+                    const Sight see(a, t.len, pos[n]);
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        __builtin_amdgcn_sched_barrier(0);   // few comparisons' results at a time
-                        f[n][u] = above0(f[n][u]);
+                    for (int u = 0; u < 4; u++)
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const int kk = (u < 2 ? k0 : k1) + 16 * (u & 1) + 4 * g + j;
-                            if (!(in[u] && see[n].sees(kk))) s[n][u][j] = -INFINITY;
+                            s[n][u][j] = miss >> u & 1 ? -INFINITY : see.masked(a, kk, s[n][u][j]);
                         }
-                    }
+                }
             }
-            const int e1 = max(max(in[0] ? ev[0] : KV8_MIN_EXP, in[1] ? ev[1] : KV8_MIN_EXP),
-                               max(in[2] ? ev[2] : KV8_MIN_EXP, in[3] ? ev[3] : KV8_MIN_EXP));
+            const int e1 = max(max(ev[0], ev[1]), max(ev[2], ev[3]));
             emax = max(emax, e1);
             if (__builtin_expect(e1 > eref || e1 < eref - 8, 0)) {
                 const float by = follow(e1, emax, eref);
@@ -893,14 +920,14 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
                     for (int i = 0; i < DI; i++) o[n][i] *= by;
             }
-            Halves<4> hv;
+            hv.least = whole ? 0.0f : 0x1p-100f;
 #pragma unroll
-            for (int u = 0; u < 4; u++) hv.set(u, ev[u], in[u], eref);
+            for (int u = 0; u < 4; u++) hv.set(u, ev[u], eref);
             f16x8 pf[NQ][2][NB];
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
                 bool moved;
-                const float al = weigh<4, NB>(s[n], f[n], hv, m[n], l[n], moved, pf[n]);
+                const float al = weigh<4, NB>(s[n], qs[n], hv, m[n], l[n], moved, pf[n]);
                 if (moved) {
 #pragma unroll
                     for (int i = 0; i < DI; i++) o[n][i] *= al;
@@ -925,12 +952,32 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
                             to = mfma_f16(vf[y & 1][i], pf[n][y / (DI / 4)][z], to);
                         }
             }
-#pragma unroll 1
-            for (int y = 0; y < 2; y++)
-                if (__builtin_expect(snan[b][y], 0) && s0 + 2 * it + y < s1) spread_nan<D, NQ>(a, t, h, y ? k1 : k0, c, g, see, o);
         }
-        if (more) place(it + 1);
-    }
+    };
+    // the loop twice: what a wavefront fetches and converts stays in registers
+    // of its own, whether K or V
+    auto walk = [&](auto is_v) __attribute__((always_inline)) {
+        Unit r[AHEAD];
+        if (iters > 0) fetch(0, r[0], is_v);
+        split();
+        if (iters > 0) place(0, r[0], is_v);
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (i + 1 < iters) fetch(i + 1, r[i], is_v);
+        for (int it = 0; it < iters; it += AHEAD)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                if (it + i < iters) step(it + i, r[i], is_v);
+    };
+    if (threadIdx.x == 0) snan = 0;              // the first step's barrier comes before the flag is set
+    if (isv) walk(std::true_type());
+    else walk(std::false_type());
+    if (dirty && lane == 0) snan = 1;
+    __syncthreads();
+    const Args &z = args_again();
+    if (__builtin_expect(snan, 0))
+        for (int st = s0; st < s1; st++) spread_nan<D, NQ>(z, t, h, step_key(t, st), c, g, pos, o);
+
 
     const float unit = pow2i(eref - P_EXP);
 #pragma unroll
@@ -940,22 +987,22 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
         if (R >= all) continue;
         if (chunks <= 1) {
             const float f = den == 0.0f ? 0.0f : 1.0f / den;
-            const long off = (long)(t.r0 + R / a.group) * a.ld_out + (long)(h * a.group + R % a.group) * D;
+            const long off = (long)(t.r0 + R / z.group) * z.ld_out + (long)(h * z.group + R % z.group) * D;
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int i = 0; i < DI; i++) {
                     const float y = den == 0.0f ? 0.0f : o[n][i][j] * unit * f;
-                    if (BF16) reinterpret_cast<uint16_t *>(a.out)[off + (4 * g + j) * DI + i] = f2bf(y);
-                    else reinterpret_cast<float *>(a.out)[off + (4 * g + j) * DI + i] = y;
+                    if (BF16) reinterpret_cast<uint16_t *>(z.out)[off + (4 * g + j) * DI + i] = f2bf(y);
+                    else reinterpret_cast<float *>(z.out)[off + (4 * g + j) * DI + i] = y;
                 }
         } else {
-            const long at = (((long)id * a.kv + h) * a.nchunk + ch) * a.rpt + r;
+            const long at = (((long)id * z.kv + h) * z.nchunk + ch) * z.rpt + r;
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
-                for (int i = 0; i < DI; i++) a.part[at * D + (4 * g + j) * DI + i] = o[n][i][j] * unit;
-            if (g == 0) a.stat[at] = make_float2(m[n], den);
+                for (int i = 0; i < DI; i++) z.part[at * D + (4 * g + j) * DI + i] = o[n][i][j] * unit;
+            if (g == 0) z.stat[at] = make_float2(m[n], den);
         }
     }
 }
