@@ -889,11 +889,11 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int u = 0; u < 4; u++)
+                for (int y = 0; y < NB; y++)
 #pragma unroll
-                    for (int n = 0; n < NQ; n++)
+                    for (int u = 0; u < 4; u++)
 #pragma unroll
-                        for (int y = 0; y < NB; y++) s[n][u] = mfma_f16(kf[x & 1][u], qf[n][y][x], s[n][u]);
+                        for (int n = 0; n < NQ; n++) s[n][u] = mfma_f16(kf[x & 1][u], qf[n][y][x], s[n][u]);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) vf[0][i] = vl[i * CT_WAVE];
@@ -943,11 +943,11 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
                     for (int i = 0; i < 4; i++) vf[(y + 1) & 1][i] = vl[(4 * (y + 1) + i) * CT_WAVE];
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int z = 0; z < NB; z++)
 #pragma unroll
-                    for (int n = 0; n < NQ; n++)
+                    for (int i = 0; i < 4; i++)
 #pragma unroll
-                        for (int z = 0; z < NB; z++) {
+                        for (int n = 0; n < NQ; n++) {
                             f32x4 &to = o[n][(4 * y + i) % DI];
                             to = mfma_f16(vf[y & 1][i], pf[n][y / (DI / 4)][z], to);
                         }
