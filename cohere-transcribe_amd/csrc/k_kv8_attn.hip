@@ -75,8 +75,9 @@ struct Tile {
     int full_lo, full_hi;        // steps at keys in [full_lo, full_hi) are seen whole by every row
 };
 
-// Inclusive prefix sum over the workgroup.
-__device__ __forceinline__ int scan256(int v, int *part, int &total) {
+// Inclusive prefix sum over the workgroup's W wavefronts.
+template <int W>
+__device__ __forceinline__ int block_sum(int v, int *part, int &total) {
     const int lane = threadIdx.x % CT_WAVE, w = threadIdx.x / CT_WAVE;
 #pragma unroll
     for (int o = 1; o < CT_WAVE; o <<= 1) {
@@ -88,7 +89,7 @@ __device__ __forceinline__ int scan256(int v, int *part, int &total) {
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int i = 0; i < NW; i++) {
+    for (int i = 0; i < W; i++) {
         if (i < w) before += part[i];
         total += part[i];
     }
@@ -98,6 +99,7 @@ __device__ __forceinline__ int scan256(int v, int *part, int &total) {
 
 // Finds tile `id` (rows_per_tile packed rows each); false if there is none.
 // Every thread of the workgroup calls it with the same id.
+template <int W>
 __device__ __forceinline__ bool find_tile(const Args &a, int id, int rows_per_tile, int *sh, Tile &t) {
     int tile = 0;
     if (a.one_tile) {
@@ -116,17 +118,17 @@ __device__ __forceinline__ bool find_tile(const Args &a, int id, int rows_per_ti
             if (r0 >= 0 && rows > 0 && rows <= a.n_rows - r0) n = (rows * a.group + rows_per_tile - 1) / rows_per_tile;
         }
         int total;
-        const int upto = scan256(n, sh, total);
+        const int upto = block_sum<W>(n, sh, total);
         if (id >= total) return false;
         if (id >= upto - n && id < upto) {
-            sh[NW] = s; sh[NW + 1] = id - (upto - n); sh[NW + 2] = r0; sh[NW + 3] = rows; sh[NW + 4] = len;
+            sh[W] = s; sh[W + 1] = id - (upto - n); sh[W + 2] = r0; sh[W + 3] = rows; sh[W + 4] = len;
         }
         __syncthreads();
-        t.seq = __builtin_amdgcn_readfirstlane(sh[NW]);
-        tile = __builtin_amdgcn_readfirstlane(sh[NW + 1]);
-        t.r0 = __builtin_amdgcn_readfirstlane(sh[NW + 2]);
-        t.n = __builtin_amdgcn_readfirstlane(sh[NW + 3]);
-        t.len = __builtin_amdgcn_readfirstlane(sh[NW + 4]);
+        t.seq = __builtin_amdgcn_readfirstlane(sh[W]);
+        tile = __builtin_amdgcn_readfirstlane(sh[W + 1]);
+        t.r0 = __builtin_amdgcn_readfirstlane(sh[W + 2]);
+        t.n = __builtin_amdgcn_readfirstlane(sh[W + 3]);
+        t.len = __builtin_amdgcn_readfirstlane(sh[W + 4]);
     }
     t.row = tile * rows_per_tile;
     if (t.row >= t.n * a.group || (a.one_tile && t.n * a.group > rows_per_tile)) return false;
@@ -180,6 +182,12 @@ __device__ __forceinline__ float pow2i(int e) {          // 2^e, e in [-126, 127
 
 // Bytes that are a NaN code (0x7f, 0xff) as 0x80 in their place.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+template <bool NONTEMPORAL, class T>
+__device__ __forceinline__ T ask(const T *p) {
+    if constexpr (NONTEMPORAL) return __builtin_nontemporal_load(p);
+    else return *p;
+}
 
 // The raw codes of one 32-key step: K as 16-byte pieces (half, 64-dim group),
 // V as D / 16 dims of keys 4g + j (j < 4) and 16 + 4g + j - 4.
@@ -443,28 +451,31 @@ __device__ __forceinline__ void spread_nan(const Args &a, const Tile &t, int h, 
 // w with its NaN codes as zeros.
 __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~((nan_bytes(w) >> 7) * 0xffu); }
 
-template <int D, bool BF16>
-__global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
+// ONCE: a sequence's rows are one tile, so its codes are read once.
+template <int D, bool BF16, int W, bool ONCE>
+__global__ __launch_bounds__(W * CT_WAVE, 2) void attn_kernel(Args a) {
     constexpr int KS = D / 32;            // k steps of the score product
     constexpr int DI = D / 16;            // 16-dim tiles of O; dims of V a lane loads
     constexpr int NB = BF16 ? 1 : 2;      // f16 terms of a query value and of p
-    __shared__ int sh[NW + 5];
-    __shared__ float so[NW][16][D];
-    __shared__ float sm[NW][16], sl[NW][16];
+    // the wavefronts' sums [W][rpt][D], maxima and l [W][16]: of the rows a tile
+    // has, mostly one
+    extern __shared__ float so[];
+    __shared__ int sh[W + 5];
+    __shared__ float sm[W][16], sl[W][16];
 
     // heads vary fastest: workgroup i runs on XCD i % 8, so with 8 kv heads the
     // tiles of one head share an L2
     const int h = blockIdx.x % a.kv, id = blockIdx.x / a.kv, ch = blockIdx.y;
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
-    // this wavefront's steps: first, first + NW, ...; lane i keeps the page and
+    // this wavefront's steps: first, first + W, ...; lane i keeps the page and
     // the scales of 16-key half i (-1: not in the pool).  Where a step's keys do
     // not depend on the lengths, its page is read along with them.
     const int first = ch * a.chunk + w;
     const bool ahead = a.one_tile && !a.window;
-    int key_i = 32 * (first + NW * (lane >> 1)) + 16 * (lane & 1), pg = -1;
-    if (ahead && (lane >> 1) * NW < a.chunk && key_i < a.cap) pg = a.table[(long)id * a.table_w + (key_i >> a.lp)];
+    int key_i = 32 * (first + W * (lane >> 1)) + 16 * (lane & 1), pg = -1;
+    if (ahead && (lane >> 1) * W < a.chunk && key_i < a.cap) pg = a.table[(long)id * a.table_w + (key_i >> a.lp)];
     Tile t;
-    if (!find_tile(a, id, 16, sh, t)) return;
+    if (!find_tile<W>(a, id, 16, sh, t)) return;
     const int chunks = (t.steps + a.chunk - 1) / a.chunk;
     if (ch >= max(chunks, 1)) return;
     const int last = min(t.steps, (ch + 1) * a.chunk);
@@ -474,7 +485,7 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
     const bool have = R < t.n * a.group;
     const int qi = have ? R / a.group : 0, qh = have ? R % a.group : 0;
     {
-        const int st = first + NW * (lane >> 1);
+        const int st = first + W * (lane >> 1);
         key_i = step_key(t, st) + 16 * (lane & 1);
         const bool mine = st < last && key_i < t.end;
         if (!ahead && mine) pg = a.table[(long)t.seq * a.table_w + (key_i >> a.lp)];
@@ -494,30 +505,30 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
             const int p = max(__builtin_amdgcn_readlane(pg, 2 * i + u), 0);   // any page if there is none
             const long base = ((((long)p * a.kv + h) << a.lp) + ((key + 16 * u) & (P - 1))) * D;
             const uint8_t *kp = a.k + base, *vp = a.v + base;
-            // non-temporal: a step's codes are read once (7.1 against 6.3 TB/s
-            // in a plain read of 4 GiB)
+            // non-temporal where codes are read once (7.1 against 6.3 TB/s in a
+            // plain read of 4 GiB); tiles of one sequence share them in L2
 #pragma unroll
             for (int y = 0; y < D / 64; y++)
-                r.k[u][y] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(kp + ka + 64 * y));
+                r.k[u][y] = ask<ONCE>(reinterpret_cast<const u32x4 *>(kp + ka + 64 * y));
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if (D == 128) {
-                    const u32x2 y = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(vp + va + j * D));
+                    const u32x2 y = ask<ONCE>(reinterpret_cast<const u32x2 *>(vp + va + j * D));
                     r.v[4 * u + j][0] = y[0];
                     r.v[4 * u + j][D / 64 - 1] = y[1];
                 } else {
-                    r.v[4 * u + j][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(vp + va + j * D));
+                    r.v[4 * u + j][0] = ask<ONCE>(reinterpret_cast<const uint32_t *>(vp + va + j * D));
                 }
             }
         }
     };
-    Raw<D> ra, rb;
-    if (first < last) load(first, 0, ra);
     float pks = 0.0f, pvs = 0.0f;
     if (pg >= 0) {
         pks = a.ks[(long)pg * a.kv + h];
         pvs = a.vs[(long)pg * a.kv + h];
     }
+    Raw<D> ra, rb;
+    if (first < last) load(first, 0, ra);
     f16x8 qf[NB][KS];
     const float qs = split_query<D, BF16>(a, have, x, qf);
     const int pos[1] = {t.pos0 + qi};
@@ -541,17 +552,23 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
             in[u] = __builtin_amdgcn_readlane(pg, 2 * i + u) >= 0;
             hv.ks[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pks), 2 * i + u));
             ev[u] = max((int)(__builtin_amdgcn_readlane(__float_as_uint(pvs), 2 * i + u) >> 23 & 255) - 127, KV8_MIN_EXP);
-            s[u] = (f32x4){0, 0, 0, 0};
-#pragma unroll
-            for (int y = 0; y < D / 64; y++) {
-                const f16x8 k0 = cvt8(r.k[u][y][0], r.k[u][y][1]), k1 = cvt8(r.k[u][y][2], r.k[u][y][3]);
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    s[u] = mfma_f16(k0, qf[b][2 * y], s[u]);
-                    s[u] = mfma_f16(k1, qf[b][2 * y + 1], s[u]);
-                }
-            }
         }
+        // a chain of products per half and query term, next to each other
+        f32x4 sb[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; b++) sb[b][0] = sb[b][1] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < KS; x++) {
+            f16x8 kf[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) kf[u] = cvt8(r.k[u][x >> 1][2 * (x & 1)], r.k[u][x >> 1][2 * (x & 1) + 1]);
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) sb[b][u] = mfma_f16(kf[u], qf[b][x], sb[b][u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) s[u] = NB > 1 ? sb[0][u] + sb[NB - 1][u] : sb[0][u];
         const bool whole = key >= t.full_lo && key + 32 <= t.full_hi && in[0] && in[1];   // sink steps lie below full_lo
         if (__builtin_expect(!whole, 0)) {
             uint32_t bad = 0;
@@ -600,22 +617,25 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
             f16x8 vf[4];
             operand_v<D>([&](int j) { return r.v[j][y]; }, vf);
 #pragma unroll
-            for (int b = 0; b < 4; b++)
+            for (int n = 0; n < NB; n++)
 #pragma unroll
-                for (int n = 0; n < NB; n++) o[0][4 * y + b] = mfma_f16(vf[b], pf[0][n], o[0][4 * y + b]);
+                for (int b = 0; b < 4; b++) o[0][4 * y + b] = mfma_f16(vf[b], pf[0][n], o[0][4 * y + b]);
         }
     };
 
+    // the scales are here before the loop: a wait for them inside it would be
+    // one for every load, the next step's too
+    asm volatile("" : "+v"(pks), "+v"(pvs));
     // two steps in flight
-    for (int st = first, i = 0; st < last; st += 2 * NW, i += 2) {
-        if (st + NW < last) load(st + NW, i + 1, rb);
+    for (int st = first, i = 0; st < last; st += 2 * W, i += 2) {
+        if (st + W < last) load(st + W, i + 1, rb);
         use(st, i, ra);
-        if (st + NW >= last) break;
-        if (st + 2 * NW < last) load(st + 2 * NW, i + 2, ra);
-        use(st + NW, i + 1, rb);
+        if (st + W >= last) break;
+        if (st + 2 * W < last) load(st + 2 * W, i + 2, ra);
+        use(st + W, i + 1, rb);
     }
     if (__builtin_expect(dirty, 0))
-        for (int st = first; st < last; st += NW) spread_nan<D, 1>(a, t, h, step_key(t, st), c, g, pos, o);
+        for (int st = first; st < last; st += W) spread_nan<D, 1>(a, t, h, step_key(t, st), c, g, pos, o);
 
     // the wavefronts' sums joined, in their order
     l = sum_q(l);
@@ -625,21 +645,21 @@ __global__ __launch_bounds__(NT, 2) void attn_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < DI; i++) so[w][c][(4 * g + j) * DI + i] = o[0][i][j] * unit;
+            for (int i = 0; i < DI; i++) so[(w * a.rpt + c) * D + (4 * g + j) * DI + i] = o[0][i][j] * unit;
     }
     __syncthreads();
     const int nr = min(16, t.n * a.group - t.row);
-    for (int x = threadIdx.x; x < nr * D; x += NT) {
+    for (int x = threadIdx.x; x < nr * D; x += W * CT_WAVE) {
         const int r = x / D, d = x % D;
         float M = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NW; i++) M = fmaxf(M, sm[i][r]);
+        for (int i = 0; i < W; i++) M = fmaxf(M, sm[i][r]);
         const float Mu = M == -INFINITY ? 0.0f : M;
         float num = 0.0f, den = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NW; i++) {
+        for (int i = 0; i < W; i++) {
             const float f = __builtin_amdgcn_exp2f(sm[i][r] - Mu);
-            num += f * so[i][r][d];
+            num += f * so[(i * a.rpt + r) * D + d];
             den += f * sl[i][r];
         }
         if (chunks <= 1) {
@@ -681,7 +701,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 
     const int h = blockIdx.x % a.kv, id = gridDim.x / a.kv - 1 - blockIdx.x / a.kv, ch = blockIdx.y;
     Tile t;
-    if (!find_tile(a, id, ROWS, sh, t)) return;
+    if (!find_tile<NW>(a, id, ROWS, sh, t)) return;
     const int chunks = (t.steps + a.chunk - 1) / a.chunk;
     if (ch >= max(chunks, 1)) return;
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
@@ -1016,7 +1036,7 @@ __global__ __launch_bounds__(NT) void join_kernel(Args a) {
     __shared__ float so[NW][D], sl[NW];
     const int h = blockIdx.x % a.kv, id = blockIdx.x / a.kv;
     Tile t;
-    if (!find_tile(a, id, a.tile_rows, sh, t)) return;
+    if (!find_tile<NW>(a, id, a.tile_rows, sh, t)) return;
     const int chunks = (t.steps + a.chunk - 1) / a.chunk;
     if (chunks <= 1) return;
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), part = w % WPR;
@@ -1073,14 +1093,19 @@ __global__ __launch_bounds__(NT) void join_kernel(Args a) {
 
 // The launch's shape, from the sizes alone.
 struct Shape {
-    int tile_rows, one_tile, tiles, chunk, nchunk, rpt;
+    int tile_rows, one_tile, tiles, waves, chunk, nchunk, rpt;
 };
 
 Shape shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
     Shape s;
     const int group = a->heads / c->kv_heads;
     const long rows = (long)(a->max_rows < a->n_rows ? a->max_rows : a->n_rows) * group;   // of a sequence
-    s.tile_rows = rows > 32 ? rows_of(a->bf16) : 16;
+    // Tiles of 16 rows while they leave CUs free, then the rows kernel's
+    // (bf16 1 x 500 rows, 256 units of 16: 12.7 us against 24.2; 32 x 32, 600
+    // units: 18.3 against 21.7; 4 x 500, 700 units: 27.3 against 24.5; fp32
+    // 8 x 300, 860 units: 30.5 against 16.2).
+    const long tiles16 = (long)a->n_rows * group / 16 + c->seqs;
+    s.tile_rows = rows > 16 && tiles16 * c->kv_heads > 640 ? rows_of(a->bf16) : 16;
     s.one_tile = rows <= s.tile_rows;
     s.tiles = s.one_tile ? c->seqs : (int)((long)a->n_rows * group / s.tile_rows + c->seqs);
     s.rpt = rows < s.tile_rows ? (int)rows : s.tile_rows;
@@ -1092,14 +1117,40 @@ Shape shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
         const long span = ((long)a->window + s.tile_rows + 62) / 32 + ((long)a->sinks + 31) / 32;
         if (span < steps) steps = span;
     }
+    const long units = (long)s.tiles * c->kv_heads;
+    s.waves = NW;
     if (s.tile_rows == 16) {
-        s.chunk = 16;
+        // A CU reads some 30 GB/s, so a few units have to be spread over many
+        // CUs, which costs a join (3.5 us).  One chunk up to 24 steps (8 units
+        // of 12 steps: 7.5 us, in two chunks 10.1), or up to 64 where there is
+        // a unit for every other CU (192 units of 36 steps: 9.7 us, in chunks
+        // of 16 13.2); else 512 chunks in all, of 8 to 128 steps (8 units of
+        // 125 steps: 10.6 us at 8, 24.8 at 64; 256 units of 938 steps: 325 us
+        // at 8, 245 at 64 and 128).
+        s.chunk = (int)steps;
+        if (steps > 24 && (steps > 64 || units < 128)) {
+            const long each = (units * steps + 511) / 512;
+            s.chunk = each < 8 ? 8 : each > 128 ? 128 : (int)each;
+        }
+        // 8 wavefronts a unit while that fills no CU twice (192 units of 36
+        // steps: 9.7 us against 12.4; 512 of 10: 13.4 against 10.2)
+        if (s.chunk >= steps && units <= 256) s.waves = 8;
+        if (!s.one_tile) {
+            // rows of one sequence share its codes in L2: fewer, longer chunks
+            // (fp32 3 x 201 rows, 248 units of 219 steps: 55 us in chunks of
+            // 128, 85 of 32; 4 x 100 rows over 63 steps: 23 us whole, 28 of 16)
+            const long each = (units * steps + 255) / 256;
+            s.waves = NW;
+            s.chunk = each < 64 ? 64 : each > 128 ? 128 : (int)each;
+        }
     } else {
-        // two workgroups a CU; at least 512 keys each
-        const long want = (512 + (long)s.tiles * c->kv_heads - 1) / ((long)s.tiles * c->kv_heads);
+        // a workgroup for each CU, of at least 512 keys (1 x 2000 rows, 32
+        // heads over 8, 504 units: 71 us whole, 100 in two chunks)
+        const long want = (256 + units - 1) / units;
         s.chunk = (int)((steps + want - 1) / want);
         s.chunk = s.chunk < 16 ? 16 : (s.chunk + 1) & ~1;
     }
+    if (s.chunk < 1) s.chunk = 1;
     s.nchunk = (int)((steps + s.chunk - 1) / s.chunk);
     if (s.nchunk < 1) s.nchunk = 1;
     return s;
@@ -1138,14 +1189,19 @@ extern "C" void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Att
     a.part = p->work;
     a.stat = sh.nchunk > 1 ? reinterpret_cast<float2 *>(p->work + n * c->head_dim) : nullptr;
     const int wpr = sh.nchunk > 4 ? NW : 1;      // wavefronts that join a row
+    const size_t lds = (size_t)sh.waves * sh.rpt * c->head_dim * sizeof(float);
     const dim3 grid((unsigned)(c->kv_heads * sh.tiles), sh.nchunk);
     const dim3 join(grid.x, (unsigned)((sh.rpt * wpr + NW - 1) / NW));
 #define ATTN(D, B)                                                            \
     do {                                                                      \
-        if (sh.tile_rows == 16)                                               \
-            hipLaunchKernelGGL((attn_kernel<D, B>), grid, dim3(NT), 0, s, a); \
-        else                                                                  \
+        if (sh.tile_rows > 16)                                                \
             hipLaunchKernelGGL((rows_kernel<D, B>), grid, dim3(NT), 0, s, a); \
+        else if (!sh.one_tile)                                                \
+            hipLaunchKernelGGL((attn_kernel<D, B, 4, false>), grid, dim3(4 * CT_WAVE), lds, s, a); \
+        else if (sh.waves == 4)                                               \
+            hipLaunchKernelGGL((attn_kernel<D, B, 4, true>), grid, dim3(4 * CT_WAVE), lds, s, a); \
+        else                                                                  \
+            hipLaunchKernelGGL((attn_kernel<D, B, 8, true>), grid, dim3(8 * CT_WAVE), lds, s, a); \
         if (sh.nchunk > 1) {                                                  \
             if (wpr == 1) hipLaunchKernelGGL((join_kernel<D, B, 1>), join, dim3(NT), 0, s, a);  \
             else hipLaunchKernelGGL((join_kernel<D, B, NW>), join, dim3(NT), 0, s, a);          \
