@@ -9,6 +9,7 @@
 
 #define CT_KV8_SEQS 256        /* sequences of a cache                       */
 #define CT_KV8_ROWS (1 << 24)  /* rows of a step                             */
+#define CT_KV8_ROW_HEADS (1L << 26)  /* appended rows * kv heads, and        */
 #define CT_KV8_HEAD_ROWS (1L << 27)  /* rows * query heads: with these the
                                   grids stay below 2^32 threads              */
 #define CT_KV8_KEYS (1 << 24)  /* tokens a table row may hold                */

@@ -43,31 +43,36 @@ __device__ __forceinline__ int block_scan(int v, int *part, int &total) {
 // Append
 // ---------------------------------------------------------------------------
 
-// 8 values of a row at p (element offset off), as floats.
+// 8 values of a row, as they lie in memory; read once, so non-temporally.
 template <bool BF16>
-__device__ __forceinline__ void load_row8(const void *p, long off, bool vec, float (&x)[8]) {
-    if (BF16) {
+struct Piece;
+template <>
+struct Piece<true> {
+    u16x8 v;
+    __device__ __forceinline__ void load(const void *p, long off, bool vec) {
         const uint16_t *q = reinterpret_cast<const uint16_t *>(p) + off;
-        if (vec) {
-            const u16x8 w = *reinterpret_cast<const u16x8 *>(q);
+        if (vec) v = __builtin_nontemporal_load(reinterpret_cast<const u16x8 *>(q));
+        else
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = bf2f(w[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = bf2f(q[i]);
-        }
-    } else {
+            for (int i = 0; i < 8; i++) v[i] = q[i];
+    }
+    __device__ __forceinline__ float at(int i) const { return bf2f(v[i]); }
+};
+template <>
+struct Piece<false> {
+    f32x4 v[2];
+    __device__ __forceinline__ void load(const void *p, long off, bool vec) {
         const float *q = reinterpret_cast<const float *>(p) + off;
         if (vec) {
-            const float4 a = reinterpret_cast<const float4 *>(q)[0], b = reinterpret_cast<const float4 *>(q)[1];
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+#pragma unroll
+            for (int i = 0; i < 2; i++) v[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(q) + i);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = q[i];
+            for (int i = 0; i < 8; i++) v[i >> 2][i & 3] = q[i];
         }
     }
-}
+    __device__ __forceinline__ float at(int i) const { return v[i >> 2][i & 3]; }
+};
 
 // Exponent of the smallest 2^e >= 2^-100 with amax <= 448 * 2^e; amax finite,
 // >= 0.  448 = 1.75 * 2^8.
@@ -83,10 +88,11 @@ __device__ __forceinline__ float clamp448(float x) {
     return x < -448.0f ? -448.0f : x;
 }
 
-__device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv) {
+template <bool BF16>
+__device__ __forceinline__ uint2 codes8(const Piece<BF16> &x, float inv) {
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = clamp448(x[i] * inv);
+    for (int i = 0; i < 8; i++) y[i] = clamp448(x.at(i) * inv);
     uint2 r;
     int a = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     r.x = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], a, true);
@@ -108,7 +114,9 @@ __device__ __forceinline__ uint32_t recode4(uint32_t c, float ratio) {
 // their rounding: each is read once and its code written once.
 // Pieces (pages touched) are numbered sequence by sequence; a workgroup finds
 // its own by a prefix sum over the sequences, so the grid follows n_rows and
-// not the longest sequence: at most n_rows / page_tokens + 2 * seqs.
+// not the longest sequence: at most n_rows, and n_rows / page_tokens + 2 *
+// seqs.  Heads vary fastest, then K and V: the workgroups of a piece, which
+// read parts of the same rows, run together.
 template <int D, bool BF16>
 __global__ __launch_bounds__(NT) void append_kernel(BackendKv8 c, int layer, const void *xk, const void *xv,
                                                     long ld, int vec, const int *rows, int n_rows, int lp) {
@@ -135,7 +143,7 @@ __global__ __launch_bounds__(NT) void append_kernel(BackendKv8 c, int layer, con
     }
     int total;
     const int upto = block_scan<NT>(n, part, total);
-    const int piece = blockIdx.x;
+    const int piece = blockIdx.x / (2 * c.kv_heads);
     if (piece >= total) return;           // the same for every thread
     if (piece >= upto - n && piece < upto) {
         const int p0 = ((a >> lp) + piece - (upto - n)) << lp;   // first token of the page
@@ -147,33 +155,39 @@ __global__ __launch_bounds__(NT) void append_kernel(BackendKv8 c, int layer, con
     }
     __syncthreads();
     const int row0 = own[0], pos0 = own[1], m = own[2] - pos0, tok0 = pos0 & (P - 1);
-    const int page = c.table[(long)own[3] * c.table_w + (pos0 >> lp)];
-    if ((unsigned)page >= (unsigned)c.pages || c.refs[page] > 1) return;
-    const int h = blockIdx.y;
-    const bool isv = blockIdx.z;
+    const bool isv = blockIdx.x / c.kv_heads & 1;
+    const int h = blockIdx.x % c.kv_heads;
     const void *x = isv ? xv : xk;
+    // the rows and the page are asked for together
+    const int tr = t / TPR, col = t % TPR * 8;
+    Piece<BF16> val[MAXP];
+#pragma unroll
+    for (int i = 0; i < MAXP; i++) {
+        const int r = i * RPP + tr;
+        if (r < m) val[i].load(x, (row0 + r) * ld + h * D + col, vec);
+    }
+    const int page = c.table[(long)own[3] * c.table_w + (pos0 >> lp)];
+    if ((unsigned)page >= (unsigned)c.pages) return;
     const long at = ((long)layer * c.pages + page) * c.kv_heads + h;
     uint8_t *codes = (isv ? c.v : c.k) + (at << lp) * D;
     float *scale = (isv ? c.vscale : c.kscale) + at;
+    const float was = tok0 ? *scale : 0.0f;      // read before any thread writes it
+    if (c.refs[page] > 1) return;                // the same for every thread
 
-    const int tr = t / TPR, col = t % TPR * 8;
-    float val[MAXP][8];
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < MAXP; i++) {
         const int r = i * RPP + tr;
         if (r < m) {
-            load_row8<BF16>(x, (row0 + r) * ld + h * D + col, vec, val[i]);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float u = fabsf(val[i][j]);
+                const float u = fabsf(val[i].at(j));
                 amax = u < INFINITY ? fmaxf(amax, u) : amax;     // finite values only
             }
         }
     }
     amax = wave_max(amax);
     if (t % CT_WAVE == 0) wmax[t / CT_WAVE] = amax;
-    const float was = tok0 ? *scale : 0.0f;      // read before any thread writes it
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NT / CT_WAVE; i++) amax = fmaxf(amax, wmax[i]);
@@ -213,21 +227,36 @@ __device__ __forceinline__ int *plan_from(const BackendKv8 &c) {
 }
 __device__ __forceinline__ int *plan_to(const BackendKv8 &c) { return plan_from(c) + max(c.pages, c.seqs); }
 
-// Calls take(rank, page) for the lowest `want` free pages, in ascending order
-// of page; returns the number of free pages.  One planning workgroup; each
-// thread owns a run of pages.  Nothing is taken if there are fewer.
-template <class Take>
-__device__ __forceinline__ int take_free(const BackendKv8 &c, int want, int *part, Take take) {
-    const int per = (c.pages + PNT - 1) / PNT, p0 = min((int)threadIdx.x * per, c.pages), p1 = min(p0 + per, c.pages);
-    int n = 0;
-    for (int p = p0; p < p1; p++) n += c.refs[p] == 0;
-    int total;
-    int r = block_scan<PNT>(n, part, total) - n;
-    if (total >= want)
-        for (int p = p0; p < p1 && r < want; p++)
-            if (c.refs[p] == 0) take(r++, p);
-    return total;
-}
+// A planning thread's run of pages and which of the first 64 of them are
+// free, asked for before the rest of the plan needs them.
+struct FreeRun {
+    int p0, p1, n;
+    uint64_t mask;
+    __device__ __forceinline__ FreeRun(const BackendKv8 &c) {
+        const int per = (c.pages + PNT - 1) / PNT;
+        p0 = min((int)threadIdx.x * per, c.pages);
+        p1 = min(p0 + per, c.pages);
+        n = 0;
+        mask = 0;
+        for (int p = p0; p < p1; p++) {
+            const bool f = c.refs[p] == 0;
+            n += f;
+            if (p - p0 < 64) mask |= (uint64_t)f << (p - p0);
+        }
+    }
+    // Calls take(rank, page) for the lowest `want` free pages, in ascending
+    // order of page; returns the number of free pages.  Nothing is taken if
+    // there are fewer.  All of the workgroup's threads call it.
+    template <class Take>
+    __device__ __forceinline__ int take(const BackendKv8 &c, int want, int *part, Take take) const {
+        int total;
+        int r = block_scan<PNT>(n, part, total) - n;
+        if (total >= want)
+            for (int p = p0; p < p1 && r < want; p++)
+                if (p - p0 < 64 ? mask >> (p - p0) & 1 : c.refs[p] == 0) take(r++, p);
+        return total;
+    }
+};
 
 __global__ __launch_bounds__(PNT) void reserve_kernel(BackendKv8 c, const int *add, int lp) {
     __shared__ int part[PNT / CT_WAVE];
@@ -235,6 +264,7 @@ __global__ __launch_bounds__(PNT) void reserve_kernel(BackendKv8 c, const int *a
     __shared__ int bad;
     const int t = threadIdx.x, P = 1 << lp;
     const long cap = (long)c.table_w << lp;
+    const FreeRun run(c);
     if (t == 0) bad = 0;
     __syncthreads();
     int n = 0, a = 0, len = 0, first = 0;
@@ -261,7 +291,7 @@ __global__ __launch_bounds__(PNT) void reserve_kernel(BackendKv8 c, const int *a
     int refuse = bad;
     rows = (int)min(((long)uhi << 8) + ulo, (long)CT_KV8_ROWS);
     if (!refuse && want > 0) {
-        const int have = take_free(c, want, part, [&](int r, int p) {
+        const int have = run.take(c, want, part, [&](int r, int p) {
             int lo = 0, up = c.seqs - 1;           // the last sequence with off <= r
             while (lo < up) {
                 const int mid = (lo + up + 1) >> 1;
@@ -285,15 +315,25 @@ __global__ __launch_bounds__(PNT) void reserve_kernel(BackendKv8 c, const int *a
     }
 }
 
-// Fork, first of three launches: checks the pairs and picks the pages that
-// partly filled last pages are copied to.  For pair i the plan gets the
+// Fork, first of two launches.  The workgroups past the first set the
+// sources' table rows aside.  The first checks the pairs and picks the pages
+// that partly filled last pages are copied to: for pair i the plan gets the
 // source sequence (-1: nothing to do), the table column of the copied page
 // (-1: none), its new page and the source's length; and the pages to copy.
-__global__ __launch_bounds__(PNT) void fork_plan_kernel(BackendKv8 c, const int *dst, const int *src, int n, int lp) {
+__global__ __launch_bounds__(PNT) void fork_plan_kernel(BackendKv8 c, const int *dst, const int *src, int n, int cols,
+                                                        int lp) {
+    if (blockIdx.x > 0) {
+        const int i = (blockIdx.x - 1) / cols, j = (blockIdx.x - 1) % cols * PNT + threadIdx.x;
+        const int s = src[i];
+        if ((unsigned)s < (unsigned)c.seqs && j < c.table_w)
+            plan_table(c)[(long)i * c.table_w + j] = c.table[(long)s * c.table_w + j];
+        return;
+    }
     __shared__ int part[PNT / CT_WAVE];
     __shared__ int seen[CT_KV8_SEQS], who[CT_KV8_SEQS], from[CT_KV8_SEQS];
     __shared__ int bad;
     const int t = threadIdx.x, P = 1 << lp;
+    const FreeRun run(c);
     if (t == 0) bad = 0;
     if (t < CT_KV8_SEQS) seen[t] = 0;
     __syncthreads();
@@ -320,7 +360,7 @@ __global__ __launch_bounds__(PNT) void fork_plan_kernel(BackendKv8 c, const int 
     int refuse = bad ? KV8_BAD_ARG : 0;
     int *pairs = plan_pairs(c);
     if (!refuse && want > 0) {
-        const int have = take_free(c, want, part, [&](int i, int p) {
+        const int have = run.take(c, want, part, [&](int i, int p) {
             pairs[4 * who[i] + 2] = p;
             c.refs[p] = 1;
             plan_from(c)[i] = from[i];
@@ -356,19 +396,19 @@ __device__ __forceinline__ void copy_pages(const BackendKv8 &c, int lp, int firs
         const int lay = (int)(pl % c.layers), r = (int)(pl / c.layers);
         const long a = (long)lay * c.pages + from[r], b = (long)lay * c.pages + to[r];
         uint8_t *pool = isv ? c.v : c.k;
-        const uint4 *p = reinterpret_cast<const uint4 *>(pool + a * bytes);
-        uint4 *q = reinterpret_cast<uint4 *>(pool + b * bytes);
+        const u32x4 *p = reinterpret_cast<const u32x4 *>(pool + a * bytes);
+        u32x4 *q = reinterpret_cast<u32x4 *>(pool + b * bytes);
         const int w0 = part << 10, w1 = (int)min((long)w0 + 1024, bytes >> 4);
-        uint4 x[4];
+        u32x4 x[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int w = w0 + j * NT + threadIdx.x;
-            if (w < w1) x[j] = p[w];
+            if (w < w1) x[j] = __builtin_nontemporal_load(p + w);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int w = w0 + j * NT + threadIdx.x;
-            if (w < w1) q[w] = x[j];
+            if (w < w1) __builtin_nontemporal_store(x[j], q + w);
         }
         if (part == 0 && (int)threadIdx.x < c.kv_heads) {
             float *sc = isv ? c.vscale : c.kscale;
@@ -377,9 +417,10 @@ __device__ __forceinline__ void copy_pages(const BackendKv8 &c, int lp, int firs
     }
 }
 
-// Fork, second launch: stages each pair's new table row and counts its pages;
-// the workgroups behind copy the partly filled pages.
-__global__ __launch_bounds__(NT) void fork_share_kernel(BackendKv8 c, int n, int cols, int lp) {
+// Fork, second launch: the rows set aside, with the copied pages in their
+// places, replace the old ones; pages gain and lose a holder.  The workgroups
+// behind copy the partly filled pages.
+__global__ __launch_bounds__(NT) void fork_swap_kernel(BackendKv8 c, const int *dst, int n, int cols, int lp) {
     const int books = n * cols;
     if ((int)blockIdx.x >= books) {
         copy_pages(c, lp, blockIdx.x - books, gridDim.x - books);
@@ -387,32 +428,21 @@ __global__ __launch_bounds__(NT) void fork_share_kernel(BackendKv8 c, int n, int
     }
     const int i = blockIdx.x / cols, j = blockIdx.x % cols * NT + threadIdx.x;
     const int *pair = plan_pairs(c) + 4 * i;
-    const int s = pair[0];
-    if (s < 0 || j >= c.table_w) return;
-    const int P = 1 << lp, used = (pair[3] + P - 1) >> lp;
-    int p = -1;
-    if (j < used) {
-        if (j == pair[1]) p = pair[2];             // counted when it was taken
-        else {
-            p = c.table[(long)s * c.table_w + j];
-            if ((unsigned)p < (unsigned)c.pages) atomicAdd(c.refs + p, 1);
-        }
-    }
-    plan_table(c)[(long)i * c.table_w + j] = p;
-}
-
-// Fork, third launch: the staged rows replace the old ones, whose pages are
-// given back.
-__global__ __launch_bounds__(NT) void fork_swap_kernel(BackendKv8 c, const int *dst, int cols) {
-    const int i = blockIdx.x / cols, j = blockIdx.x % cols * NT + threadIdx.x;
-    const int *pair = plan_pairs(c) + 4 * i;
     if (pair[0] < 0) return;
-    const int d = dst[i];
+    const int d = dst[i], used = (pair[3] + (1 << lp) - 1) >> lp;
     if (j == 0) c.len[d] = pair[3];
     if (j >= c.table_w) return;
     int *e = c.table + (long)d * c.table_w + j;
     const int old = *e;
-    *e = plan_table(c)[(long)i * c.table_w + j];
+    int p = -1;
+    if (j < used) {
+        if (j == pair[1]) p = pair[2];             // counted when it was taken
+        else {
+            p = plan_table(c)[(long)i * c.table_w + j];
+            if ((unsigned)p < (unsigned)c.pages) atomicAdd(c.refs + p, 1);
+        }
+    }
+    *e = p;
     if ((unsigned)old < (unsigned)c.pages) atomicSub(c.refs + old, 1);
 }
 
@@ -542,7 +572,8 @@ extern "C" void ctk_kv8_append(const BackendKv8 *c, int layer, const void *k, co
                                const int *rows, int n_rows, hipStream_t s) {
     const int lp = log2_of(c->page_tokens);
     const int vec = ((((uintptr_t)k | (uintptr_t)v) & 15) == 0 && ld % (bf16 ? 8 : 4) == 0);
-    const dim3 grid((unsigned)((n_rows >> lp) + 2 * c->seqs), c->kv_heads, 2);
+    const int most = (n_rows >> lp) + 2 * c->seqs, pieces = most < n_rows ? most : n_rows;
+    const dim3 grid((unsigned)pieces * 2 * c->kv_heads);
 #define APPEND(D, B) \
     hipLaunchKernelGGL((append_kernel<D, B>), grid, dim3(NT), 0, s, *c, layer, k, v, ld, vec, rows, n_rows, lp)
     if (c->head_dim == 64) { if (bf16) APPEND(64, true); else APPEND(64, false); }
@@ -552,9 +583,10 @@ extern "C" void ctk_kv8_append(const BackendKv8 *c, int layer, const void *k, co
 
 extern "C" void ctk_kv8_fork(const BackendKv8 *c, const int *dst, const int *src, int n, hipStream_t s) {
     const int lp = log2_of(c->page_tokens), cols = (c->table_w + NT - 1) / NT;
-    hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(PNT), 0, s, *c, dst, src, n, lp);
-    hipLaunchKernelGGL(fork_share_kernel, dim3((unsigned)(n * cols + copy_grid(c, n))), dim3(NT), 0, s, *c, n, cols, lp);
-    hipLaunchKernelGGL(fork_swap_kernel, dim3((unsigned)(n * cols)), dim3(NT), 0, s, *c, dst, cols);
+    const int wide = (c->table_w + PNT - 1) / PNT;
+    hipLaunchKernelGGL(fork_plan_kernel, dim3((unsigned)(1 + n * wide)), dim3(PNT), 0, s, *c, dst, src, n, wide, lp);
+    hipLaunchKernelGGL(fork_swap_kernel, dim3((unsigned)(n * cols + copy_grid(c, n))), dim3(NT), 0, s, *c, dst, n, cols,
+                       lp);
 }
 
 extern "C" void ctk_kv8_free(const BackendKv8 *c, const int *seqs, int n, hipStream_t s) {

@@ -107,6 +107,7 @@ void backend_kv8_append(const BackendKv8 *c, int layer, const void *k, const voi
     check_cache(c);
     check_layer(c, layer);
     check_rows(rows, n_rows);
+    if ((long)n_rows * c->kv_heads > CT_KV8_ROW_HEADS) CT_FATAL("kv8_append: n_rows * kv_heads above 2^26");
     if (n_rows == 0) return;
     const uintptr_t al = bf16 ? 1 : 3;
     if (!k || !v || ((uintptr_t)k & al) || ((uintptr_t)v & al)) CT_FATAL("kv8_append: k or v is NULL or not aligned");

@@ -211,7 +211,8 @@ void backend_kv8_bind(BackendKv8 *c, float *mem);
  * KV8_BAD_ARG). */
 void backend_kv8_reserve(const BackendKv8 *c, const int *add);
 /* Rounds a layer's new K and V rows into their pages.  Sequence s has the
- * rows rows[s] .. rows[s + 1] - 1 (in all at most n_rows); they are the last
+ * rows rows[s] .. rows[s + 1] - 1 (in all at most n_rows, n_rows * kv_heads
+ * <= 2^26); they are the last
  * ones of its len[s] tokens.  A row is kv_heads * head_dim values (fp32, or
  * bf16 if bf16 != 0), ld values after the one before it.  The scale of a
  * page is the smallest 2^e >= 2^-100 that holds its largest finite value

@@ -48,6 +48,7 @@ CASES = {
     "append_rows_null": ("L.backend_kv8_append(h, 0, 4096, 4096, 128, 0, None, 4)", {}, {}, "rows are NULL"),
     "append_rows_negative": ("L.backend_kv8_append(h, 0, 4096, 4096, 128, 0, 4096, -1)", {}, {}, "n_rows outside"),
     "append_rows_many": ("L.backend_kv8_append(h, 0, 4096, 4096, 128, 0, 4096, (1 << 24) + 1)", {}, {}, "n_rows outside"),
+    "append_rows_heads": ("L.backend_kv8_append(h, 0, 4096, 4096, 8192, 0, 4096, 1 << 20)", dict(kv_heads=128), {}, "n_rows * kv_heads above"),
     "append_null": ("L.backend_kv8_append(h, 0, 4096, None, 128, 0, 4096, 4)", {}, {}, "k or v is NULL"),
     "append_alignment": ("L.backend_kv8_append(h, 0, 4098, 4096, 128, 0, 4096, 4)", {}, {}, "not aligned"),
     "append_alignment_bf16": ("L.backend_kv8_append(h, 0, 4097, 4096, 128, 1, 4096, 4)", {}, {}, "not aligned"),
