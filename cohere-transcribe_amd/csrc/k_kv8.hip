@@ -43,7 +43,7 @@ __device__ __forceinline__ int block_scan(int v, int *part, int &total) {
 // Append
 // ---------------------------------------------------------------------------
 
-// 8 values of a row, as they lie in memory; read once, so non-temporally.
+// 8 values of a row, as they lie in memory.
 template <bool BF16>
 struct Piece;
 template <>
@@ -51,7 +51,7 @@ struct Piece<true> {
     u16x8 v;
     __device__ __forceinline__ void load(const void *p, long off, bool vec) {
         const uint16_t *q = reinterpret_cast<const uint16_t *>(p) + off;
-        if (vec) v = __builtin_nontemporal_load(reinterpret_cast<const u16x8 *>(q));
+        if (vec) v = *reinterpret_cast<const u16x8 *>(q);
         else
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = q[i];
@@ -65,7 +65,7 @@ struct Piece<false> {
         const float *q = reinterpret_cast<const float *>(p) + off;
         if (vec) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) v[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(q) + i);
+            for (int i = 0; i < 2; i++) v[i] = reinterpret_cast<const f32x4 *>(q)[i];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i >> 2][i & 3] = q[i];
