@@ -28,6 +28,7 @@
 
 namespace {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -288,7 +289,10 @@ struct Halves {
     }
 };
 
-// p' of one query over U halves: 2^(s qs ks - m + adj).
+// p' of one query over U halves, 2^(s qs ks - m + adj), as B operands, and
+// their sums.  The softmax is online, but its maximum is found only when it
+// has to be: p' are computed with the one so far, and again (settle) if that
+// was too_low for a lane of the wavefront.
 template <int U, int NB>
 __device__ __forceinline__ void powers(const f32x4 (&s)[U], float qs, const Halves<U> &hv, float m,
                                        float (&sum)[U], f16x8 (&pf)[U / 2][NB]) {
@@ -315,43 +319,35 @@ __device__ __forceinline__ void powers(const f32x4 (&s)[U], float qs, const Halv
     }
 }
 
-// One query's online softmax over U halves: scores s (-inf: not seen) times
-// qs and the key scale, in base 2; p' as B operands.  The maximum is found only when it has to
-// be: p' are computed with the one so far, and if one of them (in any lane)
-// passes 2^(P_EXP + SLACK) the maximum moves and they are computed again.
-// Returns the factor of the sums so far, which is 1 unless `moved`, the same
-// in the whole wavefront.
+// Whether a lane's p' of one query were computed with a maximum that is too
+// low: none yet, or one of them passes 2^(P_EXP + SLACK).
+template <int Y, int NB>
+__device__ __forceinline__ bool too_low(float m, const f16x8 (&pf)[Y][NB]) {
+    // f16 bits as integers: p' >= 0, and infinities and NaN are the largest
+    u16x2 top = {0, 0};
+#pragma unroll
+    for (int y = 0; y < Y; y++) {
+        const auto q = __builtin_bit_cast(u16x8, pf[y][0]);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) top = __builtin_elementwise_max(top, (u16x2){q[j], q[j + 1]});
+    }
+    return m == -INFINITY || max(top[0], top[1]) > (15 + P_EXP + SLACK) << 10;
+}
+
+// Moves a query's maximum to that of its scores s (-inf: not seen) and
+// computes its p' again; returns the factor of the sums so far.
 template <int U, int NB>
-__device__ __forceinline__ float weigh(const f32x4 (&s)[U], float qs, const Halves<U> &hv, float &m, float &l,
-                                       bool &moved, f16x8 (&pf)[U / 2][NB]) {
-    float sum[U];
-    moved = __any(m == -INFINITY);
-    if (!moved) {
-        powers<U, NB>(s, qs, hv, m, sum, pf);
-        // f16 bits as integers: p' >= 0, and infinities and NaN are the largest
-        u16x2 top = {0, 0};
+__device__ __forceinline__ float settle(const f32x4 (&s)[U], float qs, const Halves<U> &hv, float &m, float &l,
+                                        float (&sum)[U], f16x8 (&pf)[U / 2][NB]) {
+    float mt = -INFINITY;
 #pragma unroll
-        for (int y = 0; y < U / 2; y++) {
-            const auto q = __builtin_bit_cast(u16x8, pf[y][0]);
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) top = __builtin_elementwise_max(top, (u16x2){q[j], q[j + 1]});
-        }
-        moved = __any(max(top[0], top[1]) > (15 + P_EXP + SLACK) << 10);
-    }
-    float al = 1.0f;
-    if (__builtin_expect(moved, 0)) {
-        float mt = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            mt = fmaxf(mt, fmaxf(qs * hv.ks[u], hv.least) * fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
-        const float mn = fmaxf(m, fmax_q(mt));
-        al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= al;
-        powers<U, NB>(s, qs, hv, m, sum, pf);
-    }
-#pragma unroll
-    for (int u = 0; u < U; u++) l = __builtin_fmaf(sum[u], hv.undo[u], l);
+    for (int u = 0; u < U; u++)
+        mt = fmaxf(mt, fmaxf(qs * hv.ks[u], hv.least) * fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
+    const float mn = fmaxf(m, fmax_q(mt));
+    const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= al;
+    powers<U, NB>(s, qs, hv, m, sum, pf);
     return al;
 }
 
@@ -604,12 +600,15 @@ __global__ __launch_bounds__(W * CT_WAVE, 2) void attn_kernel(Args a) {
         hv.set(0, ev[0], eref);
         hv.set(1, ev[1], eref);
         f16x8 pf[1][NB];
-        bool moved;
-        const float al = weigh<2, NB>(s, qs, hv, m, l, moved, pf);
-        if (moved) {
+        float sum[2];
+        powers<2, NB>(s, qs, hv, m, sum, pf);
+        if (__builtin_expect(__any(too_low<1, NB>(m, pf)), 0)) {
+            const float al = settle<2, NB>(s, qs, hv, m, l, sum, pf);
 #pragma unroll
             for (int y = 0; y < DI; y++) o[0][y] *= al;
         }
+#pragma unroll
+        for (int u = 0; u < 2; u++) l = __builtin_fmaf(sum[u], hv.undo[u], l);
 #pragma unroll
         for (int y = 0; y < D / 64; y++) {
             f16x8 vf[4];
@@ -692,9 +691,12 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     static_assert(2 * KS == DI, "K and V take the same number of operands");
     __shared__ int sh[NW + 5];
     __shared__ __align__(16) _Float16 lds[2][4][UNIT];   // buffer; K, K, V, V of the two steps
-    __shared__ float sscale[2][4];             // key scales of the four 16-key halves
-    __shared__ int sexp[2][4];                 // exponents of the value scales
-    __shared__ int smiss[2][2];                // of each step: bit u: half u is not in the pool
+    // key scales and value scales' exponents (GONE: not in the pool) of each
+    // iteration's four 16-key halves; two batches of 32 iterations in turn
+    __shared__ __align__(16) float sscale[2][32][4];
+    __shared__ __align__(16) int sexp[2][32][4];
+    constexpr int GONE = KV8_MIN_EXP - 1;
+    __shared__ int spos[ROWS];                 // the rows' positions, for the steps that not all see
     __shared__ int snan;                       // the V of some step holds a NaN
 
     const int h = blockIdx.x % a.kv, id = gridDim.x / a.kv - 1 - blockIdx.x / a.kv, ch = blockIdx.y;
@@ -712,19 +714,21 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     const int wend = idle ? 0 : min(a.causal ? p1 + 1 : t.len, a.cap);
 
     // the unit this wavefront fetches: K (isv 0) or V of step 2 it + kb; lane i
-    // keeps the page and scale of half i & 1 of the step of iteration base + i / 2
+    // keeps the page and place of half i & 1 of the step of iteration base + i / 2
     const int kb = w & 1, isv = w >> 1;
     const int s0 = ch * a.chunk, s1 = min(t.steps, s0 + a.chunk), iters = (s1 - s0 + 1) >> 1;
     const int P = 1 << a.lp;
+    auto key_of = [&](int it0) {                 // first key of this lane's half
+        return step_key(t, min(s0 + 2 * (it0 + (lane >> 1)) + kb, s1 - 1)) + 16 * (lane & 1);
+    };
     auto fetch_page = [&](int it0) {
-        const int st = s0 + 2 * (it0 + (lane >> 1)) + kb;
+        const int st = s0 + 2 * (it0 + (lane >> 1)) + kb, key = key_of(it0);
         int p = -1;
-        if (st < s1) {
-            const int key = step_key(t, st) + 16 * (lane & 1);
-            if (key < t.end) p = a.table[(long)t.seq * a.table_w + (key >> a.lp)];
-        }
+        if (st < s1 && key < t.end) p = a.table[(long)t.seq * a.table_w + (key >> a.lp)];
         return (unsigned)p < (unsigned)a.pages ? p : -1;
     };
+    // where the half's codes start; page 0 for one that is not there
+    auto place_of = [&](int p, int it0) { return ((((long)max(p, 0) * a.kv + h) << a.lp) + (key_of(it0) & (P - 1))) * D; };
     auto fetch_scale = [&](int p) { return p >= 0 ? (isv ? a.vs : a.ks)[(long)p * a.kv + h] : 0.0f; };
     // asked for together: the first pages, the query rows; then what they lead to
     int pg = fetch_page(0), pg2 = fetch_page(32);
@@ -734,8 +738,15 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
         const int R = min(t.row + WR * w + 16 * n + c, all - 1);
         fetch_query<D>(a, (long)(t.r0 + R / a.group) * a.ld_q + (long)(h * a.group + R % a.group) * D, g, x[n]);
     }
-    float psc = fetch_scale(pg), psc2 = 0.0f;
+    float psc = fetch_scale(pg);
+    long at64 = place_of(pg, 0);
     const uint8_t *pool = isv ? a.v : a.k;
+    // the scales of the batch that starts at iteration it0, into LDS
+    auto put_scales = [&](int it0) {
+        const int bt = it0 >> 5 & 1, i = lane >> 1, half = 2 * kb + (lane & 1);
+        if (!isv) sscale[bt][i][half] = psc;
+        else sexp[bt][i][half] = pg < 0 ? GONE : max((int)(__float_as_uint(psc) >> 23 & 255) - 127, KV8_MIN_EXP);
+    };
     const unsigned off = isv ? 4 * g * D + c * DI : c * D + 16 * g;
 
     // the codes of a unit, asked for AHEAD iterations before they are converted,
@@ -744,20 +755,19 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     struct Unit {
         uint32_t raw[D / 8];
         int p0, p1;
-        float s0, s1;
     };
     auto fetch = [&](int it, Unit &r, auto is_v) __attribute__((always_inline)) {
         constexpr bool V = decltype(is_v)::value;
         unsigned at = off;
         asm volatile("" : "+v"(at));            // a 32-bit offset beside a scalar base, not a 64-bit sum a load
-        const int i = 2 * (it & 31), key = step_key(t, min(s0 + 2 * it + kb, s1 - 1));
+        const int i = 2 * (it & 31);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int page = __builtin_amdgcn_readlane(pg, i + u);
-            const float sc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(psc), i + u));
-            if (u) { r.p1 = page; r.s1 = sc; }
-            else { r.p0 = page; r.s0 = sc; }
-            const uint8_t *p = pool + ((((long)max(page, 0) * a.kv + h) << a.lp) + ((key + 16 * u) & (P - 1))) * D;
+            if (u) r.p1 = page;
+            else r.p0 = page;
+            const uint32_t lo = __builtin_amdgcn_readlane((int)at64, i + u), hi = __builtin_amdgcn_readlane((int)(at64 >> 32), i + u);
+            const uint8_t *p = pool + ((uint64_t)hi << 32 | lo);
             uint32_t *to = r.raw + u * (D / 16);
             if constexpr (!V) {
 #pragma unroll
@@ -780,10 +790,11 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
             }
         }
         // pages and scales of the next 32 iterations, well before they are used
-        if ((it & 31) == 15) psc2 = fetch_scale(pg2);
+        if ((it & 31) == 15) psc = fetch_scale(pg2);
         if ((it & 31) == 31) {
             pg = pg2;
-            psc = psc2;
+            at64 = place_of(pg, it + 1);
+            put_scales(it + 1);
             pg2 = fetch_page(it + 33);
         }
     };
@@ -792,14 +803,6 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
         constexpr bool V = decltype(is_v)::value;
         const int b = it & 1;
         f16x8 *to = reinterpret_cast<f16x8 *>(lds[b][2 * V + kb]) + lane;
-        if (lane < 2) {
-            const int half = 2 * kb + lane;
-            const float sc = lane ? r.s1 : r.s0;
-            const int p = lane ? r.p1 : r.p0;
-            if (!V) sscale[b][half] = sc;
-            else sexp[b][half] = p < 0 ? KV8_MIN_EXP : max((int)(__float_as_uint(sc) >> 23 & 255) - 127, KV8_MIN_EXP);
-            if (V && lane == 0) smiss[b][kb] = (r.p0 < 0) | (r.p1 < 0) << 1;
-        }
         if constexpr (!V) {
 #pragma unroll
             for (int u = 0; u < 2; u++)
@@ -847,14 +850,13 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     // this wavefront's rows
     f16x8 qf[NQ][NB][KS];
     float qs[NQ];
-    int pos[NQ];
     auto split = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const int R = t.row + WR * w + 16 * n + c;
         const bool have = R < all;
         qs[n] = split_query<D, BF16>(a, have, x[n], qf[n]);
-        pos[n] = t.pos0 + (have ? R / a.group : 0);
+        if (g == 0) spos[WR * w + 16 * n + c] = t.pos0 + (have ? R / a.group : 0);
     }
     };
 
@@ -881,55 +883,62 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
         if (k0 < wend) {
             const f16x8 *kl = reinterpret_cast<const f16x8 *>(lds[b][0]) + lane;
             const f16x8 *vl = reinterpret_cast<const f16x8 *>(lds[b][2]) + lane;
-            // operands are read a group of four ahead of the products they feed
+            // operands are read a group of KG ahead of the products they feed: of
+            // one 32-dim step, KG of the four halves
+            constexpr int KG = NQ == 2 ? 2 : 4;
             f32x4 s[NQ][4];
-            f16x8 kf[2][4];
+            f16x8 kf[2][KG];
+            auto read_k = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                kf[0][u] = kl[((u >> 1) * DI + (u & 1) * KS) * CT_WAVE];
+                for (int v = 0; v < KG; v++) {
+                    const int x = i / (4 / KG), u = i % (4 / KG) * KG + v;
+                    kf[i & 1][v] = kl[((u >> 1) * DI + (u & 1) * KS + x) * CT_WAVE];
+                }
+            };
+            read_k(0);
 #pragma unroll
-                for (int n = 0; n < NQ; n++) s[n][u] = (f32x4){0, 0, 0, 0};
-            }
+            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) s[n][u] = (f32x4){0, 0, 0, 0};
             int ev[4];
             Halves<4> hv;
-            const int miss = __builtin_amdgcn_readfirstlane(smiss[b][0] | smiss[b][1] << 2);
+            const f32x4 ks = *reinterpret_cast<const f32x4 *>(sscale[it >> 5 & 1][it & 31]);
+            const i32x4 ex = *reinterpret_cast<const i32x4 *>(sexp[it >> 5 & 1][it & 31]);
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                hv.ks[u] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sscale[b][u])));
-                ev[u] = __builtin_amdgcn_readfirstlane(sexp[b][u]);
+                hv.ks[u] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(ks[u])));
+                ev[u] = __builtin_amdgcn_readfirstlane(ex[u]);
             }
             f16x8 vf[2][4];
 #pragma unroll
-            for (int x = 0; x < KS; x++) {
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    if (x + 1 < KS) kf[(x + 1) & 1][u] = kl[((u >> 1) * DI + (u & 1) * KS + x + 1) * CT_WAVE];
-                }
+            for (int i = 0; i < KS * 4 / KG; i++) {
+                if (i + 1 < KS * 4 / KG) read_k(i + 1);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int y = 0; y < NB; y++)
 #pragma unroll
-                    for (int u = 0; u < 4; u++)
+                    for (int v = 0; v < KG; v++)
 #pragma unroll
-                        for (int n = 0; n < NQ; n++) s[n][u] = mfma_f16(kf[x & 1][u], qf[n][y][x], s[n][u]);
+                        for (int n = 0; n < NQ; n++) {
+                            f32x4 &to = s[n][i % (4 / KG) * KG + v];
+                            to = mfma_f16(kf[i & 1][v], qf[n][y][i / (4 / KG)], to);
+                        }
             }
-#pragma unroll
-            for (int i = 0; i < 4; i++) vf[0][i] = vl[i * CT_WAVE];
-            const bool whole = !miss && k0 >= full_lo && k0 + 32 <= full_hi && k1 >= full_lo && k1 + 32 <= full_hi;
+            const bool whole = min(min(ev[0], ev[1]), min(ev[2], ev[3])) > GONE && k0 >= full_lo && k0 + 32 <= full_hi && k1 >= full_lo && k1 + 32 <= full_hi;
             if (__builtin_expect(!whole, 0)) {
 #pragma unroll
                 for (int n = 0; n < NQ; n++) {
-                    const Sight see(a, t.len, pos[n]);
+                    const Sight see(a, t.len, spos[WR * w + 16 * n + c]);
 #pragma unroll
                     for (int u = 0; u < 4; u++)
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const int kk = (u < 2 ? k0 : k1) + 16 * (u & 1) + 4 * g + j;
-                            s[n][u][j] = miss >> u & 1 ? -INFINITY : see.masked(a, kk, s[n][u][j]);
+                            s[n][u][j] = ev[u] == GONE ? -INFINITY : see.masked(a, kk, s[n][u][j]);
                         }
                 }
             }
-            const int e1 = max(max(ev[0], ev[1]), max(ev[2], ev[3]));
+            const int e1 = max(max(max(ev[0], ev[1]), max(ev[2], ev[3])), KV8_MIN_EXP);
             emax = max(emax, e1);
             if (__builtin_expect(e1 > eref || e1 < eref - 8, 0)) {
                 const float by = follow(e1, emax, eref);
@@ -942,18 +951,23 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
             for (int u = 0; u < 4; u++) hv.set(u, ev[u], eref);
             f16x8 pf[NQ][2][NB];
+            float sum[NQ][4];
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
-                bool moved;
-                const float al = weigh<4, NB>(s[n], qs[n], hv, m[n], l[n], moved, pf[n]);
-                if (moved) {
+                powers<4, NB>(s[n], qs[n], hv, m[n], sum[n], pf[n]);
+                if (__builtin_expect(__any(too_low<2, NB>(m[n], pf[n])), 0)) {
+                    const float al = settle<4, NB>(s[n], qs[n], hv, m[n], l[n], sum[n], pf[n]);
 #pragma unroll
                     for (int i = 0; i < DI; i++) o[n][i] *= al;
                 }
+#pragma unroll
+                for (int u = 0; u < 4; u++) l[n] = __builtin_fmaf(sum[n][u], hv.undo[u], l[n]);
             }
             // group y of the V operands: four dim tiles of step y / (DI / 4); a
             // second step that is not there has p' = 0 and holds finite values
             constexpr int VG = DI / 2;
+#pragma unroll
+            for (int i = 0; i < 4; i++) vf[0][i] = vl[i * CT_WAVE];
 #pragma unroll
             for (int y = 0; y < VG; y++) {
                 if (y + 1 < VG)
@@ -978,6 +992,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
         Unit r[AHEAD];
         if (iters > 0) fetch(0, r[0], is_v);
         split();
+        put_scales(0);
         if (iters > 0) place(0, r[0], is_v);
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
@@ -993,6 +1008,9 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     if (dirty && lane == 0) snan = 1;
     __syncthreads();
     const Args &z = args_again();
+    int pos[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) pos[n] = spos[WR * w + 16 * n + c];
     if (__builtin_expect(snan, 0))
         for (int st = s0; st < s1; st++) spread_nan<D, NQ>(z, t, h, step_key(t, st), c, g, pos, o);
 
