@@ -37,6 +37,8 @@ void ctk_kv8_free(const BackendKv8 *c, const int *seqs, int n, hipStream_t s);
 void ctk_kv8_trim(const BackendKv8 *c, int window, int sinks, hipStream_t s);
 void ctk_kv8_compact(const BackendKv8 *c, hipStream_t s);
 size_t ctk_kv8_plan_ints(const BackendKv8 *c);
+/* floats a call of these sizes writes; floats for it and any smaller one */
+size_t ctk_kv8_attn_need(const BackendKv8 *c, const BackendKv8Attn *a);
 size_t ctk_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a);
 void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a, hipStream_t s);
 

@@ -1112,6 +1112,20 @@ struct Shape {
     int tile_rows, one_tile, tiles, waves, chunk, nchunk, rpt;
 };
 
+constexpr int SMALL_UNITS = 640;    // tiles of 16 rows * kv heads up to which they are taken
+
+// The longest walk of a tile of `tile_rows` rows, in steps.
+long walk_of(const BackendKv8 *c, const BackendKv8Attn *a, int tile_rows) {
+    long keys = (long)c->table_w * c->page_tokens;
+    if (a->max_len > 0 && a->max_len < keys) keys = a->max_len;
+    long steps = (keys + 31) / 32;
+    if (a->window > 0) {
+        const long span = ((long)a->window + tile_rows + 62) / 32 + ((long)a->sinks + 31) / 32;
+        if (span < steps) steps = span;
+    }
+    return steps;
+}
+
 Shape shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
     Shape s;
     const int group = a->heads / c->kv_heads;
@@ -1121,18 +1135,11 @@ Shape shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
     // units: 18.3 against 21.7; 4 x 500, 700 units: 27.3 against 24.5; fp32
     // 8 x 300, 860 units: 30.5 against 16.2).
     const long tiles16 = (long)a->n_rows * group / 16 + c->seqs;
-    s.tile_rows = rows > 16 && tiles16 * c->kv_heads > 640 ? rows_of(a->bf16) : 16;
+    s.tile_rows = rows > 16 && tiles16 * c->kv_heads > SMALL_UNITS ? rows_of(a->bf16) : 16;
     s.one_tile = rows <= s.tile_rows;
     s.tiles = s.one_tile ? c->seqs : (int)((long)a->n_rows * group / s.tile_rows + c->seqs);
     s.rpt = rows < s.tile_rows ? (int)rows : s.tile_rows;
-    long keys = (long)c->table_w * c->page_tokens;
-    if (a->max_len > 0 && a->max_len < keys) keys = a->max_len;
-    // the longest walk of a tile, in steps
-    long steps = (keys + 31) / 32;
-    if (a->window > 0) {
-        const long span = ((long)a->window + s.tile_rows + 62) / 32 + ((long)a->sinks + 31) / 32;
-        if (span < steps) steps = span;
-    }
+    const long steps = walk_of(c, a, s.tile_rows);
     const long units = (long)s.tiles * c->kv_heads;
     s.waves = NW;
     if (s.tile_rows == 16) {
@@ -1172,12 +1179,45 @@ Shape shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
     return s;
 }
 
-}  // namespace
-
-extern "C" size_t ctk_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a) {
-    const Shape s = shape_of(c, a);
+// Floats of the partial results of a shape: none for one chunk.
+size_t partials_of(const BackendKv8 *c, const Shape &s) {
     if (s.nchunk == 1) return 0;
     return (size_t)s.tiles * c->kv_heads * s.nchunk * s.rpt * (c->head_dim + 2);
+}
+
+}  // namespace
+
+extern "C" size_t ctk_kv8_attn_need(const BackendKv8 *c, const BackendKv8Attn *a) {
+    return partials_of(c, shape_of(c, a));
+}
+
+// An upper bound of ctk_kv8_attn_need over all calls with at most these rows
+// and tokens: the chunks of all units are at most the number aimed at, or one
+// for every 128 steps where that is more, and one a unit for rounding up.
+extern "C" size_t ctk_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a) {
+    const long group = a->heads / c->kv_heads, kv = c->kv_heads;
+    const long rows = (long)(a->max_rows < a->n_rows ? a->max_rows : a->n_rows) * group;
+    const int most_rows = rows_of(a->bf16);
+    const long steps = walk_of(c, a, most_rows), row = c->head_dim + 2;
+    const long all16 = (long)a->n_rows * group / 16 + c->seqs;
+    auto chunks = [&](long units, long aim) {
+        const long by128 = units * steps / 128;
+        return (by128 > aim ? by128 : aim) + units;
+    };
+    // a sequence's rows in one tile of 16
+    long most = chunks(c->seqs * kv, 512) * (rows < 16 ? rows : 16);
+    if (rows > 16) {
+        // in several, while there are few; then tiles of most_rows, split while
+        // there are fewer than 256
+        const long few = all16 * kv < SMALL_UNITS ? all16 * kv : SMALL_UNITS;
+        const long some = chunks(few, 256) * 16;
+        const long wide = ((long)a->n_rows * group / most_rows + c->seqs) * kv;
+        const long whole = all16 * kv > SMALL_UNITS ? (256 + 2 * (wide < 256 ? wide : 256)) * most_rows : 0;
+        most = some > most ? some : most;
+        most = whole > most ? whole : most;
+    }
+    // nothing is split where no tile walks further than one chunk's least
+    return steps <= 8 ? 0 : (size_t)(most * row);
 }
 
 extern "C" void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *p, hipStream_t s) {

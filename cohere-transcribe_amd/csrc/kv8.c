@@ -146,7 +146,7 @@ void backend_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a) {
         CT_FATAL("kv8_attn: q or out is NULL or not aligned");
     const long row = (long)a->heads * c->head_dim;
     if (a->ld_q < row || a->ld_out < row) CT_FATAL("kv8_attn: ld_q or ld_out below heads * head_dim");
-    if (ctk_kv8_attn_work(c, a) && (!a->work || ((uintptr_t)a->work & 15)))
+    if (ctk_kv8_attn_need(c, a) && (!a->work || ((uintptr_t)a->work & 15)))
         CT_FATAL("kv8_attn: work is NULL or not 16-byte aligned");
     require_init();
     ctk_kv8_attn(c, layer, a, ct_t.stream);

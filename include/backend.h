@@ -157,9 +157,10 @@ void backend_rel_pos_mhsa_noalloc(float *x, const float *pos_emb, int T, const E
  *
  * A page holds page_tokens consecutive tokens of one sequence, in every
  * layer, K and V.  Its codes have one scale for each layer and kv head, a
- * power of two: value = code * scale, and dividing by the scale is exact, so
- * a value is rounded once.  The cache holds finite values and NaN: what lies
- * beyond 448 scales, infinities included, is stored as +-448 scales.
+ * power of two (also where a caller fills the arrays itself): value = code *
+ * scale, and dividing by the scale is exact, so a value is rounded once.  The
+ * cache holds finite values and NaN: what lies beyond 448 scales, infinities
+ * included, is stored as +-448 scales.
  *
  * Conventions beside those at the head of this file:
  *  - Every pointer in the structs and every int array argument is DEVICE
@@ -244,8 +245,9 @@ typedef struct {
                             past it are not seen; 0: table_w * page_tokens    */
     float *work;         /* backend_kv8_attn_work floats, 16-byte aligned     */
 } BackendKv8Attn;
-/* Floats of work an attention call takes (0: none, work may be NULL).  It
- * depends on the sizes alone, not on the pointers. */
+/* Floats of work (0: none, work may be NULL) that are enough for this call
+ * and for any with the same cache, heads, window and sinks and no more n_rows,
+ * max_rows and max_len.  It depends on the sizes alone, not on the pointers. */
 size_t backend_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a);
 /* Softmax attention of the rows over a layer's pages: o = sum_j p_j v_j,
  * p = softmax_j(scale * q . k_j) over the tokens the row sees.  A row that

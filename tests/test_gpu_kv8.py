@@ -202,6 +202,112 @@ def test_several_rows(hip, P, kv, group, D, bf16):
     run_attn(hip, np.random.default_rng(P + kv + group), P, kv, group, D, lens, n, "rows", bf16=bf16, behind=3)
 
 
+WIDE = [  # P, kv, group, D: launches of so many rows that a workgroup takes 64 or 128
+    (16, 4, 8, 64), (64, 8, 4, 128), (128, 3, 16, 128), (32, 8, 5, 64)]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("P,kv,group,D", WIDE)
+def test_many_rows(hip, P, kv, group, D, bf16):
+    """Prompts, pieces over held tokens and single tokens in one launch, enough
+    of them for the tiles of many rows."""
+    print(f"case: many rows P={P} kv={kv} group={group} D={D} bf16={bf16}", flush=True)
+    total = 11000 // (kv * group) + 20
+    n = [total // 2, total // 3, 1, 0, 2, 17]
+    lens = [n[0], n[1] + 150, 90, 33, 2, 300]
+    run_attn(hip, np.random.default_rng(P + kv + group), P, kv, group, D, lens, n, "many rows", layer=1, layers=2, bf16=bf16,
+             behind=2, pad=0 if D == 64 else 3, off=0 if D == 64 else 5)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("kw", [dict(window=1), dict(window=50, sinks=3), dict(window=130, sinks=70), dict(causal=False),
+                                dict(causal=False, max_len=75), dict(window=2 ** 31 - 1, sinks=1)])
+def test_many_rows_masks(hip, kw, bf16):
+    print(f"case: many rows {kw} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(41)
+    run_attn(hip, rng, 16, 4, 8, 64, [160, 350, 1, 0], [160, 190, 1, 3], "masks", bf16=bf16, **kw)
+    run_attn(hip, rng, 64, 8, 4, 128, [200, 310], [200, 160], "masks", bf16=bf16, **kw)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_many_rows_over_a_long_text(hip, bf16):
+    """Few tiles over many tokens: the keys are split and joined."""
+    print(f"case: many rows, split bf16={bf16}", flush=True)
+    run_attn(hip, np.random.default_rng(42), 32, 2, 16, 64, [2600, 700], [330, 30], "split", bf16=bf16)
+    run_attn(hip, np.random.default_rng(43), 128, 1, 32, 128, [2111], [340], "split", bf16=bf16, window=1500, sinks=5)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_many_rows_bad_pages_and_values(hip, bf16):
+    """Missing pages, NaN in K, V and q, rows that see nothing, in the tiles of many rows."""
+    print(f"case: many rows, bad pages bf16={bf16}", flush=True)
+    rng = np.random.default_rng(44)
+    d = filled(hip, rng, 32, 4, 64, [230, 200, 90], extra=1 << 24)
+    m = d.model
+    m.table[0, [0, 4]] = [-1, 2 ** 31 - 1]
+    m.table[2] = -1
+    m.v[0, m.table[0, 5], 2, 20, 7] = 0x7F          # token 180 of sequence 0
+    m.v[0, m.table[1, 0], 1, 3, 9] = 0xFF           # token 3 of sequence 1
+    m.k[0, m.table[1, 3], 3, 16, 0] = 0x7F          # token 112
+    d.push()
+    n = [200, 160, 40]
+    q = values(rng, 400, 32, 64)
+    q[220, 3, 5], q[221, 30, 0] = np.inf, np.nan
+    for kw in (dict(), dict(window=45, sinks=2), dict(window=45, sinks=6)):
+        got = d.attn(0, q, 32, rows=starts(n), bf16=bf16, **kw)
+        want = m.attend(0, q, 32, 0.125, True, kw.get("window", 0), kw.get("sinks", 0), starts(n), 400)
+        check_rows(got, *want, bf16, kw)
+        assert np.all(got[360:] == 0.0)
+        if not kw:
+            assert np.isnan(got[150:200, 16:24, 7]).all() and np.isfinite(got[:149, :, 7]).all()
+
+
+def test_many_rows_scales_far_apart(hip):
+    print("case: many rows, scales", flush=True)
+    rng = np.random.default_rng(45)
+    d = filled(hip, rng, 16, 4, 64, [200, 150], extra=1 << 23)
+    d.model.vs[:] = 2.0 ** rng.integers(-20, 5, d.model.vs.shape)
+    d.model.ks[:] = 2.0 ** rng.integers(-10, -5, d.model.ks.shape)
+    d.push()
+    q = values(rng, 350, 32, 64)
+    rows = starts([200, 150])
+    got = d.attn(0, q, 32, rows=rows)
+    check_rows(got, *d.model.attend(0, q, 32, 0.125, True, 0, 0, rows, 350), False, "scales")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_sixteen_query_heads_of_128(hip, bf16):
+    """A tile full of one token's heads, by four and by eight wavefronts (64 KB of joined sums)."""
+    print(f"case: group 16 of 128 bf16={bf16}", flush=True)
+    rng = np.random.default_rng(46)
+    run_attn(hip, rng, 64, 1, 16, 128, [700, 1, 130], [1, 1, 1], "eight wavefronts", max_len=700, bf16=bf16)
+    run_attn(hip, rng, 64, 2, 16, 128, [40] * 140 + [700], [1] * 141, "four wavefronts", max_len=700, bf16=bf16)
+    run_attn(hip, rng, 64, 1, 32, 128, [700, 33], [1, 1], "two tiles", bf16=bf16)
+
+
+@pytest.mark.parametrize("n", [[1, 1, 1], [150, 180, 20]])
+def test_the_same_call_gives_the_same_bits(hip, n):
+    """Twice in a row, over one work buffer that the call before left full, and
+    with a larger one's work for a smaller call."""
+    print(f"case: same bits n={n}", flush=True)
+    rng = np.random.default_rng(47)
+    d = filled(hip, rng, 32, 4, 64, [900, 600, 1500], extra=1 << 24)
+    q = values(rng, sum(n), 32, 64)
+    rows, fl = d.ints(starts(n)), q.reshape(len(q), -1)
+    qp, outs = d.put(fl), []
+    big = cb.BackendKv8Attn(heads=32, scale=0.125, causal=1, n_rows=400, max_rows=400, max_len=1500)
+    work = d.put(np.full(hip.backend_kv8_attn_work(d.h, C.byref(big)) + 64, np.nan, np.float32))
+    for i in range(3):
+        op = d.put(np.zeros_like(fl))
+        a = cb.BackendKv8Attn(out=op, q=qp, ld_out=2048, ld_q=2048, heads=32, scale=0.125, causal=1, rows=rows, n_rows=len(q),
+                              max_rows=max(n), max_len=1500, work=work)
+        hip.backend_kv8_attn(d.h, 0, C.byref(a))
+        outs.append(d.get(op, fl.shape, np.float32))
+        assert np.array_equal(outs[0].view(np.uint32), outs[i].view(np.uint32)), i
+    want = d.model.attend(0, q, 32, 0.125, True, 0, 0, starts(n), len(q))
+    check_rows(outs[0].reshape(q.shape), *want, False, "larger work")
+
+
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (5, 3), (16, 4), (33, 64), (100, 33), (64, 500), (2000, 4),
                                           (2 ** 31 - 1, 2 ** 31 - 1)])
@@ -541,6 +647,64 @@ def test_beam_search_run(hip, bf16):
             d.hip.backend_kv8_compact(d.h)
             d.model.compact()
         d.check(step)
+
+
+def test_many_kv_heads(hip):
+    """256 kv heads: pages of 256 KB a layer, their scales copied with them."""
+    print("case: 256 kv heads", flush=True)
+    rng = np.random.default_rng(48)
+    d = ref.Dev(hip, 2, 8, 16, 256, 64, 3, 3, extra=1 << 23)
+    d.reserve([20, 3, 0])
+    for lay in (0, 1):
+        d.append(lay, values(rng, 23, 256, 64), values(rng, 23, 256, 64))
+    d.hip.backend_kv8_fork(d.h, d.ints([2, 1]), d.ints([0, 0]), 2)
+    d.model.fork([2, 1], [0, 0])
+    d.hip.backend_kv8_free(d.h, d.ints([0]), 1)
+    d.model.free([0])
+    d.hip.backend_kv8_compact(d.h)
+    d.model.compact()
+    d.check()
+    q = values(rng, 2, 256, 64)
+    got = d.attn(1, q, 256, rows=[0, 0, 1, 2])
+    check_rows(got, *d.model.attend(1, q, 256, 0.125, True, 0, 0, [0, 0, 1, 2], 2), False, "attention")
+
+
+def test_two_threads_with_a_cache_each(hip):
+    """Two threads, each with its own stream, arena and cache, at once: the
+    results each gets alone."""
+    print("case: two threads", flush=True)
+    import threading
+
+    def program(seed):
+        rng = np.random.default_rng(seed)
+        d = ref.Dev(hip, 1, 60, 16, 2, 64, 4, 12, extra=1 << 23)
+        got = []
+        for step in range(12):
+            add = [int(x) for x in rng.integers(0, 9, 4)]
+            d.reserve(add)
+            n = sum(add)
+            if n:
+                d.append(0, values(rng, n, 2, 64), values(rng, n, 2, 64))
+                got.append(d.attn(0, values(rng, n, 4, 64), 4))
+            d.hip.backend_kv8_fork(d.h, d.ints([3]), d.ints([int(rng.integers(3))]), 1)
+        return got, d.state()
+
+    alone = [program(50), program(51)]
+    both = [None, None]
+
+    def run(i):
+        hip.backend_init(0)
+        both[i] = program(50 + i)
+        hip.backend_thread_cleanup()
+
+    ts = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for x in ts:
+        x.start()
+    for x in ts:
+        x.join(60)
+    for (a, sa), (b, sb) in zip(alone, both):
+        assert len(a) == len(b) and all(np.array_equal(x.view(np.uint32), y.view(np.uint32)) for x, y in zip(a, b))
+        assert all(np.array_equal(sa[k], sb[k]) for k in sa)
 
 
 def test_captured_step(hip):

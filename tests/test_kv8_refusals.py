@@ -114,6 +114,37 @@ def test_sizes():
     assert L.backend_kv8_attn_work(h, C.byref(short)) == 0
 
 
+def test_work_is_enough_for_smaller_calls():
+    """Whatever a call with no more rows and tokens splits into, its partial
+    results fit the work of the larger one (the bound and the need are host
+    functions of the sizes)."""
+    L = cb.hip()
+    L.ctk_kv8_attn_need.argtypes, L.ctk_kv8_attn_need.restype = [C.c_void_p, C.c_void_p], C.c_size_t
+    rng = np.random.default_rng(3)
+
+    def log(a, b):
+        return int(round(float(np.exp(rng.uniform(np.log(a), np.log(b))))))
+
+    split = 0
+    for _ in range(4000):
+        kv, group = int(rng.choice([1, 2, 3, 8, 16, 256])), int(rng.choice([1, 2, 3, 5, 8, 16, 32]))
+        c = cb.BackendKv8(layers=1, pages=8, page_tokens=int(rng.choice([16, 32, 64, 128])), kv_heads=kv,
+                          head_dim=int(rng.choice([64, 128])), seqs=log(1, 256), table_w=log(1, 100000))
+        window = int(rng.choice([0, 0, 1])) * log(1, 100000)
+        fixed = dict(bf16=int(rng.integers(2)), heads=kv * group, scale=1.0, causal=1, window=window,
+                     sinks=log(1, 1000) if window else 0)
+        n = log(1, min(1 << 16, (1 << 27) // (kv * group)))
+        rows, most = log(1, n), int(rng.integers(2)) * log(1, 1 << 20)
+        work = L.backend_kv8_attn_work(C.byref(c), C.byref(cb.BackendKv8Attn(n_rows=n, max_rows=rows, max_len=most, **fixed)))
+        for k in range(4):
+            a = cb.BackendKv8Attn(n_rows=n if k == 0 else log(1, n), max_rows=rows if k == 0 else log(1, rows),
+                                  max_len=most if k == 0 else log(1, most) if most else int(k > 1) * log(1, 1 << 18), **fixed)
+            need = L.ctk_kv8_attn_need(C.byref(c), C.byref(a))
+            split += need > 0
+            assert need <= work, (kv, group, n, rows, most, a.n_rows, a.max_rows, a.max_len)
+    assert split > 1000
+
+
 def test_model_rounding():
     """The model's rounding against the definition: every code is its own
     nearest, midpoints go to the even code, values past the largest are held."""
