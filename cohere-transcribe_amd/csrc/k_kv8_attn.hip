@@ -445,6 +445,13 @@ __device__ __forceinline__ void spread_nan(const Args &a, const Tile &t, int h, 
 // w with its NaN codes as zeros.
 __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~((nan_bytes(w) >> 7) * 0xffu); }
 
+// Few rows of a sequence: W wavefronts share a tile's keys, step by step in
+// turn, each with two steps of codes in flight, and join their sums in LDS.
+// Bound by memory: 32 sequences of up to 30000 tokens, 32 heads over 8 of 128,
+// bf16 (1.35 GB of codes) take 244 us, 5.5 TB/s where a plain read reaches 6.3
+// to 7.1 and a copy 4.8; 64 of up to 1000 tokens, 8 heads, fp32 (88 MB) 22 us;
+// one of 376 tokens 7.3 us, of which 4.7 are an empty call's.  fp32
+// rows take two terms each, so twice the products.
 // ONCE: a sequence's rows are one tile, so its codes are read once.
 template <int D, bool BF16, int W, bool ONCE>
 __global__ __launch_bounds__(W * CT_WAVE, 2) void attn_kernel(Args a) {
@@ -681,6 +688,12 @@ __global__ __launch_bounds__(W * CT_WAVE, 2) void attn_kernel(Args a) {
 // a run of 1 KB; all four then read the whole 64 keys.  Two LDS buffers: the
 // next keys' codes are in flight while this step's products run, and one
 // barrier a step keeps them apart.
+// Bound by instructions: 6 prompts of up to 2500 tokens, 32 heads over 8 of
+// 128, bf16 (163 GFLOP) take 241 us, 677 TFLOP/s; the matrix units are busy
+// 30% of the time, and vector instructions issue in 59% of it, with the two
+// wavefronts a SIMD that the registers allow.  Measured slower, when this form
+// took 259 us: 8 wavefronts with 128 keys an iteration (273), the two 32-key
+// halves a stage apart so that weights and products interleave (266).
 constexpr int rows_of(bool bf16) { return bf16 ? 128 : 64; }
 
 template <int D, bool BF16>
@@ -1043,7 +1056,8 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     }
 }
 
-// Joins a tile's chunks: WPR wavefronts a row (chunks w, w + WPR, ...), each
+// Joins a tile's chunks, in an order that the lengths alone give (32 x 4 heads
+// over 8 chunks: 4 us): WPR wavefronts a row (chunks w, w + WPR, ...), each
 // with four chunks' loads in flight, then their sums in order.
 template <int D, bool BF16, int WPR>
 __global__ __launch_bounds__(NT) void join_kernel(Args a) {
@@ -1145,18 +1159,19 @@ Shape shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
     if (s.tile_rows == 16) {
         // A CU reads some 30 GB/s, so a few units have to be spread over many
         // CUs, which costs a join (3.5 us).  One chunk up to 24 steps (8 units
-        // of 12 steps: 7.5 us, in two chunks 10.1), or up to 64 where there is
-        // a unit for every other CU (192 units of 36 steps: 9.7 us, in chunks
+        // of 12 steps: 7.3 us, in two chunks 10.1), or up to 64 where there is
+        // a unit for every other CU (192 units of 36 steps: 9.2 us, in chunks
         // of 16 13.2); else 512 chunks in all, of 8 to 128 steps (8 units of
         // 125 steps: 10.6 us at 8, 24.8 at 64; 256 units of 938 steps: 325 us
-        // at 8, 245 at 64 and 128).
+        // at 8, 245 at 64 and 128).  seqs counts whether they have rows or not,
+        // so a row's bits do not depend on the other sequences.
         s.chunk = (int)steps;
         if (steps > 24 && (steps > 64 || units < 128)) {
             const long each = (units * steps + 511) / 512;
             s.chunk = each < 8 ? 8 : each > 128 ? 128 : (int)each;
         }
         // 8 wavefronts a unit while that fills no CU twice (192 units of 36
-        // steps: 9.7 us against 12.4; 512 of 10: 13.4 against 10.2)
+        // steps: 9.2 us against 12.4; 512 of 10: 13.4 against 10.2)
         if (s.chunk >= steps && units <= 256) s.waves = 8;
         if (!s.one_tile) {
             // rows of one sequence share its codes in L2: fewer, longer chunks
