@@ -130,7 +130,9 @@ __device__ __forceinline__ bool find_tile(const Args &a, int id, int rows_per_ti
         t.len = __builtin_amdgcn_readfirstlane(sh[W + 4]);
     }
     t.row = tile * rows_per_tile;
-    if (t.row >= t.n * a.group || (a.one_tile && t.n * a.group > rows_per_tile)) return false;
+    // one tile: the joined sums have room for rpt rows, so a sequence with more
+    // rows than max_rows is left out
+    if (t.row >= t.n * a.group || (a.one_tile && t.n * a.group > a.rpt)) return false;
     t.len = max(t.len, 0);
     t.pos0 = t.len - t.n;
     const int last = (min(t.row + rows_per_tile, t.n * a.group) - 1) / a.group;

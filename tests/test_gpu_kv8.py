@@ -386,6 +386,25 @@ def test_bad_rows_and_lengths(hip):
         check_rows(got, *m.attend(0, q, 1, 0.125, True, 0, 0, rows, 5), False, "rows")
 
 
+@pytest.mark.parametrize("kv,group,lens,n,max_rows", [
+    (1, 1, 40, [1, 4, 1, 3, 1], 1), (1, 1, 3000, [1, 4, 1, 3, 1], 1), (1, 4, 3000, [2, 4, 1, 3, 2], 2),
+    (8, 8, 1200, [6, 7, 6, 6, 8, 6, 6, 5] * 3, 6)])
+def test_more_rows_than_max_rows(hip, kv, group, lens, n, max_rows):
+    """Sequences with more rows than max_rows that would still fit a tile: their
+    rows are left as they are and the others are right, with the keys whole (40
+    tokens) and in chunks, in tiles of 16 rows and of many."""
+    print(f"case: rows past max_rows, kv {kv} group {group}, {lens} tokens", flush=True)
+    rng = np.random.default_rng(51)
+    d = filled(hip, rng, 64, kv, 64, [lens + 5 * i for i in range(len(n))], extra=1 << 24)
+    rows = starts(n)
+    q = values(rng, int(rows[-1]), kv * group, 64)
+    got = d.attn(0, q, kv * group, rows=rows, max_rows=max_rows)
+    want, vmax, smax = d.model.attend(0, q, kv * group, 0.125, True, 0, 0, rows, len(q))
+    over = np.repeat(np.asarray(n) > max_rows, n)
+    want[over], vmax[over] = np.nan, 0
+    check_rows(got, want, vmax, smax, False, max_rows)
+
+
 @pytest.mark.parametrize("bf16", [False, True])
 def test_values_that_are_not_finite(hip, bf16):
     """NaN in a token reaches the rows that see it and no other, in V only its
