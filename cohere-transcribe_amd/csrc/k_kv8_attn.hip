@@ -20,7 +20,8 @@
 // sums: p' = 2^(s - m + 6 + e - eref) <= 2^14 enters the product, O counts in
 // units of 2^(eref - 6).  Query rows are brought to a largest value in [2^12, 2^13)
 // by a power of two.  fp32 rows enter as the sum of two f16 (22 bits and
-// more), and so do their p; bf16 rows are one f16 each, exactly, and so p.
+// more), and so do their p; bf16 rows are one f16 each (exact down to 2^-26 of
+// the row's largest), and so p.
 #include "ct_dev.h"
 #include "ct_kv8.h"
 #include "k_kv8.h"

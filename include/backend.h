@@ -206,8 +206,8 @@ void backend_kv8_bind(BackendKv8 *c, float *mem);
 /* Opens a step: sequence s gets add[s] (>= 0) more tokens.  Writes
  * rows[0..seqs], the prefix sums of add; takes the pages the new tokens need,
  * in the order of sequences, lowest free page first; adds add[s] to len[s].
- * If the pool or a table row has no room, or an add[s] is negative, nothing
- * is taken: rows become all 0, so that the appends and attention of the
+ * If the pool or a table row has no room, an add[s] is negative or the step
+ * has more than 2^24 rows, nothing is taken: rows become all 0, so that the appends and attention of the
  * step do nothing, and the status tells it (KV8_NO_PAGES, KV8_NO_ROOM,
  * KV8_BAD_ARG). */
 void backend_kv8_reserve(const BackendKv8 *c, const int *add);
@@ -254,8 +254,8 @@ size_t backend_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a);
  * sees none gets zeros; tokens on a page that is not in the pool are not
  * seen; what a masked token holds, NaN included, has no effect.  Rows of out
  * that belong to no sequence are left as they are.  Scores, softmax and sums
- * are fp32; fp32 rows keep fp32 accuracy, bf16 rows enter the products as
- * they are. */
+ * are fp32; fp32 rows keep fp32 accuracy relative to the largest value the
+ * row sees, bf16 rows enter the products as they are. */
 void backend_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a);
 /* Sequences dst[i] become copies of src[i], all n (<= seqs) at once, from
  * what the cache held before the call (beam search: src = each beam's
