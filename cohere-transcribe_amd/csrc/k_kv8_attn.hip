@@ -451,13 +451,13 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~((nan_
 // Few rows of a sequence: W wavefronts share a tile's keys, step by step in
 // turn, each with two steps of codes in flight, and join their sums in LDS.
 // Bound by memory: 32 sequences of up to 30000 tokens, 32 heads over 8 of 128,
-// bf16 (1.35 GB of codes) take 244 us, 5.5 TB/s where a plain read reaches 6.3
+// bf16 (1.35 GB of codes) take 240 us, 5.6 TB/s where a plain read reaches 6.3
 // to 7.1 and a copy 4.8; 64 of up to 1000 tokens, 8 heads, fp32 (88 MB) 22 us;
 // one of 376 tokens 7.3 us, of which 4.7 are an empty call's.  fp32
 // rows take two terms each, so twice the products.
 // ONCE: a sequence's rows are one tile, so its codes are read once.
 template <int D, bool BF16, int W, bool ONCE>
-__global__ __launch_bounds__(W * CT_WAVE, 2) void attn_kernel(Args a) {
+__global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a) {
     constexpr int KS = D / 32;            // k steps of the score product
     constexpr int DI = D / 16;            // 16-dim tiles of O; dims of V a lane loads
     constexpr int NB = BF16 ? 1 : 2;      // f16 terms of a query value and of p
@@ -504,27 +504,33 @@ __global__ __launch_bounds__(W * CT_WAVE, 2) void attn_kernel(Args a) {
         unsigned ka = koff, va = voff;
         asm volatile("" : "+v"(ka), "+v"(va));   // 32-bit offsets beside a scalar base, not a 64-bit sum a load
         const int key = step_key(t, st);
+        long base[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int p = max(__builtin_amdgcn_readlane(pg, 2 * i + u), 0);   // any page if there is none
-            const long base = ((((long)p * a.kv + h) << a.lp) + ((key + 16 * u) & (P - 1))) * D;
-            const uint8_t *kp = a.k + base, *vp = a.v + base;
-            // non-temporal where codes are read once (7.1 against 6.3 TB/s in a
-            // plain read of 4 GiB); tiles of one sequence share them in L2
+            base[u] = ((((long)p * a.kv + h) << a.lp) + ((key + 16 * u) & (P - 1))) * D;
+        }
+        // non-temporal where codes are read once (7.1 against 6.3 TB/s in a
+        // plain read of 4 GiB); tiles of one sequence share them in L2.  K
+        // first, as it is used first (32 x 30000 tokens 244 -> 240 us)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int y = 0; y < D / 64; y++)
-                r.k[u][y] = ask<ONCE>(reinterpret_cast<const u32x4 *>(kp + ka + 64 * y));
+                r.k[u][y] = ask<ONCE>(reinterpret_cast<const u32x4 *>(a.k + base[u] + ka + 64 * y));
+#pragma unroll
+        for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
+                const uint8_t *vp = a.v + base[u] + va + j * D;
                 if (D == 128) {
-                    const u32x2 y = ask<ONCE>(reinterpret_cast<const u32x2 *>(vp + va + j * D));
+                    const u32x2 y = ask<ONCE>(reinterpret_cast<const u32x2 *>(vp));
                     r.v[4 * u + j][0] = y[0];
                     r.v[4 * u + j][D / 64 - 1] = y[1];
                 } else {
-                    r.v[4 * u + j][0] = ask<ONCE>(reinterpret_cast<const uint32_t *>(vp + va + j * D));
+                    r.v[4 * u + j][0] = ask<ONCE>(reinterpret_cast<const uint32_t *>(vp));
                 }
             }
-        }
     };
     float pks = 0.0f, pvs = 0.0f;
     if (pg >= 0) {
