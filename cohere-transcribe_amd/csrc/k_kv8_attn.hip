@@ -165,6 +165,16 @@ __device__ __forceinline__ float sum_q(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Two values as f16 terms: rounded, and what the rounding left, rounded; two
+// at a time, by one conversion and one mixed fma each (fp32 prompts of 2500
+// tokens 125 -> 120 us).
+__device__ __forceinline__ void two_terms(float a, float b, f16x2 &hi, f16x2 &lo) {
+    float minus = -1.0f;
+    asm("" : "+s"(minus));       // a known -1 makes a conversion and a subtraction of the mixed fma
+    hi = __builtin_convertvector((f32x2){a, b}, f16x2);
+    lo = __builtin_convertvector((f32x2){__builtin_fmaf((float)hi[0], minus, a), __builtin_fmaf((float)hi[1], minus, b)}, f16x2);
+}
+
 __device__ __forceinline__ f16x2 cvt2(uint32_t w, bool hi) {
     return hi ? __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))
               : __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
@@ -270,10 +280,17 @@ __device__ __forceinline__ float split_query(const Args &a, bool have, const QPi
 #pragma unroll
     for (int i = 0; i < KS; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float y = !have ? 0.0f : fine ? x[i].at(j) * f0 * f1 : __uint_as_float(0x7fc00000u);
-            qf[0][i][j] = (_Float16)y;
-            if (NB > 1) qf[NB - 1][i][j] = (_Float16)(y - (float)qf[0][i][j]);
+        for (int j = 0; j < 8; j += 2) {
+            float y[2];
+#pragma unroll
+            for (int n = 0; n < 2; n++) y[n] = !have ? 0.0f : fine ? x[i].at(j + n) * f0 * f1 : __uint_as_float(0x7fc00000u);
+            f16x2 hi, lo;
+            two_terms(y[0], y[1], hi, lo);
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                qf[0][i][j + n] = hi[n];
+                if (NB > 1) qf[NB - 1][i][j + n] = lo[n];
+            }
         }
     return a.scale2 * pow2i((-up) >> 1) * pow2i(-up - ((-up) >> 1));
 }
@@ -305,14 +322,22 @@ __device__ __forceinline__ void powers(const f32x4 (&s)[U], float qs, const Halv
         const float ms = mu - hv.adj[u], f = fmaxf(qs * hv.ks[u], hv.least);
         float p[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], f, -ms));
-            pf[u >> 1][0][4 * (u & 1) + j] = (_Float16)p[j];
-            if (NB > 1) pf[u >> 1][NB - 1][4 * (u & 1) + j] = (_Float16)(p[j] - (float)pf[u >> 1][0][4 * (u & 1) + j]);
-        }
+        for (int j = 0; j < 4; j++) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], f, -ms));
         if (NB > 1) {
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                f16x2 hi, lo;
+                two_terms(p[j], p[j + 1], hi, lo);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    pf[u >> 1][0][4 * (u & 1) + j + i] = hi[i];
+                    pf[u >> 1][NB - 1][4 * (u & 1) + j + i] = lo[i];
+                }
+            }
             sum[u] = (p[0] + p[1]) + (p[2] + p[3]);
         } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) pf[u >> 1][0][4 * (u & 1) + j] = (_Float16)p[j];
             // the weights as the product takes them, two at a time
             const f16x8 &q = pf[u >> 1][0];
             const int j = 4 * (u & 1);
@@ -698,7 +723,7 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
 // next keys' codes are in flight while this step's products run, and one
 // barrier a step keeps them apart.
 // Bound by instructions: 6 prompts of up to 2500 tokens, 32 heads over 8 of
-// 128, bf16 (163 GFLOP) take 241 us, 677 TFLOP/s; the matrix units are busy
+// 128, bf16 (163 GFLOP) take 238 us, 685 TFLOP/s; the matrix units are busy
 // 30% of the time, and vector instructions issue in 59% of it, with the two
 // wavefronts a SIMD that the registers allow.  Measured slower, when this form
 // took 259 us: 8 wavefronts with 128 keys an iteration (273), the two 32-key
