@@ -31,7 +31,6 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int NT = 256, NW = NT / CT_WAVE;   // threads, wavefronts of a workgroup
@@ -336,30 +335,27 @@ __device__ __forceinline__ void powers(const f32x4 (&s)[U], float qs, const Halv
             }
             sum[u] = (p[0] + p[1]) + (p[2] + p[3]);
         } else {
+            // the sum is of the weights as the product takes them, two at a time
+            const f16x2 a = __builtin_convertvector((f32x2){p[0], p[1]}, f16x2), b = __builtin_convertvector((f32x2){p[2], p[3]}, f16x2);
+            const f16x2 one = {1, 1};
 #pragma unroll
-            for (int j = 0; j < 4; j++) pf[u >> 1][0][4 * (u & 1) + j] = (_Float16)p[j];
-            // the weights as the product takes them, two at a time
-            const f16x8 &q = pf[u >> 1][0];
-            const int j = 4 * (u & 1);
-            const f16x2 a = {q[j], q[j + 1]}, b = {q[j + 2], q[j + 3]}, one = {1, 1};
+            for (int i = 0; i < 2; i++) {
+                pf[u >> 1][0][4 * (u & 1) + i] = a[i];
+                pf[u >> 1][0][4 * (u & 1) + 2 + i] = b[i];
+            }
             sum[u] = __builtin_amdgcn_fdot2(a, one, __builtin_amdgcn_fdot2(b, one, 0.0f, false), false);
         }
     }
 }
 
 // Whether a lane's p' of one query were computed with a maximum that is too
-// low: none yet, or one of them passes 2^(P_EXP + SLACK).
-template <int Y, int NB>
-__device__ __forceinline__ bool too_low(float m, const f16x8 (&pf)[Y][NB]) {
-    // f16 bits as integers: p' >= 0, and infinities and NaN are the largest
-    u16x2 top = {0, 0};
+// low: none yet, or four of them pass 2^(P_EXP + SLACK) together.
+template <int U>
+__device__ __forceinline__ bool too_low(float m, const float (&sum)[U]) {
+    float top = sum[0];
 #pragma unroll
-    for (int y = 0; y < Y; y++) {
-        const auto q = __builtin_bit_cast(u16x8, pf[y][0]);
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) top = __builtin_elementwise_max(top, (u16x2){q[j], q[j + 1]});
-    }
-    return m == -INFINITY || max(top[0], top[1]) > (15 + P_EXP + SLACK) << 10;
+    for (int u = 1; u < U; u++) top = fmaxf(top, sum[u]);
+    return m == -INFINITY || top > (float)(1 << (P_EXP + SLACK));    // a NaN needs no maximum
 }
 
 // Moves a query's maximum to that of its scores s (-inf: not seen) and
@@ -643,7 +639,7 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
         f16x8 pf[1][NB];
         float sum[2];
         powers<2, NB>(s, qs, hv, m, sum, pf);
-        if (__builtin_expect(__any(too_low<1, NB>(m, pf)), 0)) {
+        if (__builtin_expect(__any(too_low(m, sum)), 0)) {
             const float al = settle<2, NB>(s, qs, hv, m, l, sum, pf);
 #pragma unroll
             for (int y = 0; y < DI; y++) o[0][y] *= al;
@@ -723,8 +719,8 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
 // next keys' codes are in flight while this step's products run, and one
 // barrier a step keeps them apart.
 // Bound by instructions: 6 prompts of up to 2500 tokens, 32 heads over 8 of
-// 128, bf16 (163 GFLOP) take 238 us, 685 TFLOP/s; the matrix units are busy
-// 30% of the time, and vector instructions issue in 59% of it, with the two
+// 128, bf16 (163 GFLOP) take 228 us, 714 TFLOP/s; the matrix units are busy
+// 32% of the time, and vector instructions issue in 56% of it, with the two
 // wavefronts a SIMD that the registers allow.  Measured slower, when this form
 // took 259 us: 8 wavefronts with 128 keys an iteration (273), the two 32-key
 // halves a stage apart so that weights and products interleave (266).
@@ -1002,7 +998,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
             for (int n = 0; n < NQ; n++) {
                 powers<4, NB>(s[n], qs[n], hv, m[n], sum[n], pf[n]);
-                if (__builtin_expect(__any(too_low<2, NB>(m[n], pf[n])), 0)) {
+                if (__builtin_expect(__any(too_low(m[n], sum[n])), 0)) {
                     const float al = settle<4, NB>(s[n], qs[n], hv, m[n], l[n], sum[n], pf[n]);
 #pragma unroll
                     for (int i = 0; i < DI; i++) o[n][i] *= al;
