@@ -135,8 +135,13 @@ __device__ __forceinline__ bool find_tile(const Args &a, int id, int rows_per_ti
     if (t.row >= t.n * a.group || (a.one_tile && t.n * a.group > a.rpt)) return false;
     t.len = max(t.len, 0);
     t.pos0 = t.len - t.n;
-    const int last = (min(t.row + rows_per_tile, t.n * a.group) - 1) / a.group;
-    const int p0 = t.pos0 + t.row / a.group, p1 = t.pos0 + last;   // first and last row's positions
+    // divisions only where they are needed: each is 0.1 us of a short call
+    int first = t.row, last = min(t.row + rows_per_tile, t.n * a.group) - 1;
+    if (a.group > 1) {
+        first = a.one_tile ? 0 : first / a.group;
+        last = a.one_tile ? t.n - 1 : last / a.group;
+    }
+    const int p0 = t.pos0 + first, p1 = t.pos0 + last;             // first and last row's positions
     t.end = max(min(a.causal ? p1 + 1 : t.len, a.cap), 0);
     t.lo = a.window ? max(p0 - a.window + 1, 0) & ~31 : 0;
     t.sink_steps = a.window ? (min(a.sinks, t.lo) + 31) >> 5 : 0;
@@ -473,8 +478,8 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~((nan_
 // turn, each with two steps of codes in flight, and join their sums in LDS.
 // Bound by memory: 32 sequences of up to 30000 tokens, 32 heads over 8 of 128,
 // bf16 (1.35 GB of codes) take 240 us, 5.6 TB/s where a plain read reaches 6.3
-// to 7.1 and a copy 4.8; 64 of up to 1000 tokens, 8 heads, fp32 (88 MB) 22 us;
-// one of 376 tokens 7.3 us, of which 4.7 are an empty call's.  fp32
+// to 7.1 and a copy 4.8; 64 of up to 1000 tokens, 8 heads, fp32 (88 MB) 21.5 us;
+// one of 376 tokens 7.0 us, of which 4.7 are an empty call's.  fp32
 // rows take two terms each, so twice the products.
 // ONCE: a sequence's rows are one tile, so its codes are read once.
 template <int D, bool BF16, int W, bool ONCE>
@@ -490,7 +495,7 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
 
     // heads vary fastest: workgroup i runs on XCD i % 8, so with 8 kv heads the
     // tiles of one head share an L2
-    const int h = blockIdx.x % a.kv, id = blockIdx.x / a.kv, ch = blockIdx.y;
+    const int id = blockIdx.x / a.kv, h = blockIdx.x - id * a.kv, ch = blockIdx.y;
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
     // this wavefront's steps: first, first + W, ...; lane i keeps the page and
     // the scales of 16-key half i (-1: not in the pool).  Where a step's keys do
@@ -501,14 +506,14 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
     if (ahead && (lane >> 1) * W < a.chunk && key_i < a.cap) pg = a.table[(long)id * a.table_w + (key_i >> a.lp)];
     Tile t;
     if (!find_tile<W>(a, id, 16, sh, t)) return;
-    const int chunks = (t.steps + a.chunk - 1) / a.chunk;
+    const int chunks = a.nchunk > 1 ? (t.steps + a.chunk - 1) / a.chunk : 1;
     if (ch >= max(chunks, 1)) return;
     const int last = min(t.steps, (ch + 1) * a.chunk);
 
     // this lane's query row: asked for first, used after the keys are asked for
     const int R = t.row + c;
     const bool have = R < t.n * a.group;
-    const int qi = have ? R / a.group : 0, qh = have ? R % a.group : 0;
+    const int qi = have ? (a.group > 1 ? R / a.group : R) : 0, qh = have ? R - qi * a.group : 0;
     {
         const int st = first + W * (lane >> 1);
         key_i = step_key(t, st) + 16 * (lane & 1);
@@ -697,9 +702,9 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
             den += f * sl[i][r];
         }
         if (chunks <= 1) {
-            const int R2 = t.row + r;
+            const int R2 = t.row + r, i = a.group > 1 ? R2 / a.group : R2;
             const float y = den == 0.0f ? 0.0f : num / den;
-            const long off = (long)(t.r0 + R2 / a.group) * a.ld_out + (long)(h * a.group + R2 % a.group) * D + d;
+            const long off = (long)(t.r0 + i) * a.ld_out + (long)(h * a.group + R2 - i * a.group) * D + d;
             if (BF16) reinterpret_cast<uint16_t *>(a.out)[off] = f2bf(y);
             else reinterpret_cast<float *>(a.out)[off] = y;
         } else {
@@ -745,7 +750,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     const int h = blockIdx.x % a.kv, id = gridDim.x / a.kv - 1 - blockIdx.x / a.kv, ch = blockIdx.y;
     Tile t;
     if (!find_tile<NW>(a, id, ROWS, sh, t)) return;
-    const int chunks = (t.steps + a.chunk - 1) / a.chunk;
+    const int chunks = a.nchunk > 1 ? (t.steps + a.chunk - 1) / a.chunk : 1;
     if (ch >= max(chunks, 1)) return;
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
     const int all = t.n * a.group, hard = min(t.len, a.cap);
@@ -1189,7 +1194,7 @@ Shape shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
     if (s.tile_rows == 16) {
         // A CU reads some 30 GB/s, so a few units have to be spread over many
         // CUs, which costs a join (3.5 us).  One chunk up to 24 steps (8 units
-        // of 12 steps: 7.3 us, in two chunks 10.1), or up to 64 where there is
+        // of 12 steps: 7.0 us, in two chunks 10.1), or up to 64 where there is
         // a unit for every other CU (192 units of 36 steps: 9.2 us, in chunks
         // of 16 13.2); else 512 chunks in all, of 8 to 128 steps (8 units of
         // 125 steps: 10.6 us at 8, 24.8 at 64; 256 units of 938 steps: 325 us
