@@ -279,23 +279,46 @@ __device__ __forceinline__ float split_query(const Args &a, bool have, const QPi
     const bool fine = top < 0x7f800000u;
     // exponent of the row's largest value (zero and subnormal rows: 2^-126)
     const int e = fine ? max((int)(top >> 23), 1) - 127 : 0;
-    const int up = 12 - e;                   // in [-115, 138]: two factors
-    const float f0 = pow2i(up >> 1), f1 = pow2i(up - (up >> 1));
+    const int up = 12 - e;                   // in [-115, 138]
+    if constexpr (BF16) {
 #pragma unroll
-    for (int i = 0; i < KS; i++)
+        for (int i = 0; i < KS; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            float y[2];
-#pragma unroll
-            for (int n = 0; n < 2; n++) y[n] = !have ? 0.0f : fine ? x[i].at(j + n) * f0 * f1 : __uint_as_float(0x7fc00000u);
-            f16x2 hi, lo;
-            two_terms(y[0], y[1], hi, lo);
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                qf[0][i][j + n] = hi[n];
-                if (NB > 1) qf[NB - 1][i][j + n] = lo[n];
+            for (int j = 0; j < 8; j += 2) {
+                const f16x2 y = __builtin_convertvector((f32x2){__builtin_amdgcn_ldexpf(x[i].at(j), up),
+                                                                __builtin_amdgcn_ldexpf(x[i].at(j + 1), up)}, f16x2);
+                qf[0][i][j] = y[0];
+                qf[0][i][j + 1] = y[1];
             }
+        // lanes without a row, and rows that are not finite
+        if (__builtin_expect(__any(!have || !fine), 0)) {
+            const bool keep = have && fine;
+            const _Float16 other = have ? (_Float16)__builtin_nanf("") : (_Float16)0.0f;
+#pragma unroll
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) qf[0][i][j] = keep ? qf[0][i][j] : other;
         }
+    } else {
+        // two factors, and every value chosen as it is split: the form above took
+        // calls of 12 fp32 rows from 15.5 to 15.9 us
+        const float f0 = pow2i(up >> 1), f1 = pow2i(up - (up >> 1));
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                float y[2];
+#pragma unroll
+                for (int n = 0; n < 2; n++) y[n] = !have ? 0.0f : fine ? x[i].at(j + n) * f0 * f1 : __uint_as_float(0x7fc00000u);
+                f16x2 hi, lo;
+                two_terms(y[0], y[1], hi, lo);
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    qf[0][i][j + n] = hi[n];
+                    qf[NB - 1][i][j + n] = lo[n];
+                }
+            }
+    }
     return a.scale2 * pow2i((-up) >> 1) * pow2i(-up - ((-up) >> 1));
 }
 
@@ -380,6 +403,11 @@ __device__ __forceinline__ float settle(const f32x4 (&s)[U], float qs, const Hal
     return al;
 }
 
+// The score where the mask is all ones, -inf where it is 0.
+__device__ __forceinline__ float masked(uint32_t m, float s) {
+    return __uint_as_float((__float_as_uint(s) & m) | (0xff800000u & ~m));
+}
+
 // The keys the row at position pos of a sequence of len tokens sees: [0,
 // first) and [lo, lo + n).
 struct Sight {
@@ -392,17 +420,18 @@ struct Sight {
     }
     // all ones if the query sees the key, else 0: no comparison, whose results
     // for many keys at once would not fit the scalar registers
-    __device__ __forceinline__ uint32_t sees(const Args &a, int key) const {
+    __device__ __forceinline__ uint32_t sees(bool window, int key) const {
         const int before = (key - first) >> 31;
-        if (!a.window) return before;
+        if (!window) return before;
         return before | ~(((key - lo) | (lo + n - 1 - key)) >> 31);
     }
-    // the score, or -inf
-    __device__ __forceinline__ float masked(const Args &a, int key, float s) const {
-        const uint32_t m = sees(a, key);
-        return __uint_as_float((__float_as_uint(s) & m) | (0xff800000u & ~m));
+    // scores of keys key, key + 1, ...: -inf where they are not seen
+    __device__ __forceinline__ void mask(bool window, int key, f32x4 &s) const {
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[j] = masked(sees(window, key + j), s[j]);
     }
 };
+constexpr int NO_KEY = 1 << 30;                  // past every row's keys
 
 // The reference exponent follows the value scales (e1: the largest of this
 // step), but not more than 60 below the largest one met; returns the factor
@@ -454,7 +483,7 @@ __device__ __forceinline__ void spread_nan(const Args &a, const Tile &t, int h, 
             nan[j][x] = in ? nan_bytes(*reinterpret_cast<const uint32_t *>(a.v + base + 4 * x)) : 0;
 #pragma unroll
         for (int n = 0; n < NQ; n++)
-            one[n][j] = in && Sight(a, t.len, pos[n]).sees(a, kk) ? (_Float16)1.0f : (_Float16)0.0f;
+            one[n][j] = in && Sight(a, t.len, pos[n]).sees(a.window, kk) ? (_Float16)1.0f : (_Float16)0.0f;
     }
 #pragma unroll
     for (int i = 0; i < D / 16; i++) {
@@ -472,12 +501,15 @@ __device__ __forceinline__ void spread_nan(const Args &a, const Tile &t, int h, 
 }
 
 // w with its NaN codes as zeros.
-__device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~((nan_bytes(w) >> 7) * 0xffu); }
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) {
+    const uint32_t b = nan_bytes(w);
+    return w & ~(b | (b - (b >> 7)));
+}
 
 // Few rows of a sequence: W wavefronts share a tile's keys, step by step in
 // turn, each with two steps of codes in flight, and join their sums in LDS.
 // Bound by memory: 32 sequences of up to 30000 tokens, 32 heads over 8 of 128,
-// bf16 (1.35 GB of codes) take 240 us, 5.6 TB/s where a plain read reaches 6.3
+// bf16 (1.35 GB of codes) take 238 us, 5.7 TB/s where a plain read reaches 6.3
 // to 7.1 and a copy 4.8; 64 of up to 1000 tokens, 8 heads, fp32 (88 MB) 21.5 us;
 // one of 376 tokens 7.0 us, of which 4.7 are an empty call's.  fp32
 // rows take two terms each, so twice the products.
@@ -610,11 +642,16 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
             uint32_t bad = 0;
             const Sight see(a, t.len, pos[0]);
 #pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int k4 = (in[u] ? key + 16 * u : NO_KEY) + 4 * g;
+                if (a.window) see.mask(true, k4, s[u]);
+                else see.mask(false, k4, s[u]);
+            }
+#pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int kk = key + 16 * u + 4 * g + j;
-                    s[u][j] = in[u] ? see.masked(a, kk, s[u][j]) : -INFINITY;
                     // a token nobody sees may hold anything: 0 * NaN is NaN
                     const bool any = in[u] && kk < hard;
 #pragma unroll
@@ -724,7 +761,7 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
 // next keys' codes are in flight while this step's products run, and one
 // barrier a step keeps them apart.
 // Bound by instructions: 6 prompts of up to 2500 tokens, 32 heads over 8 of
-// 128, bf16 (163 GFLOP) take 228 us, 714 TFLOP/s; the matrix units are busy
+// 128, bf16 (163 GFLOP) take 224 us, 728 TFLOP/s; the matrix units are busy
 // 32% of the time, and vector instructions issue in 56% of it, with the two
 // wavefronts a SIMD that the registers allow.  Measured slower, when this form
 // took 259 us: 8 wavefronts with 128 keys an iteration (273), the two 32-key
@@ -977,12 +1014,13 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
                 for (int n = 0; n < NQ; n++) {
                     const Sight see(a, t.len, spos[WR * w + 16 * n + c]);
+                    // one form for both kinds of mask: two took fp32 prompts from 120 to 124 us
 #pragma unroll
                     for (int u = 0; u < 4; u++)
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const int kk = (u < 2 ? k0 : k1) + 16 * (u & 1) + 4 * g + j;
-                            s[n][u][j] = ev[u] == GONE ? -INFINITY : see.masked(a, kk, s[n][u][j]);
+                            s[n][u][j] = ev[u] == GONE ? -INFINITY : masked(see.sees(a.window, kk), s[n][u][j]);
                         }
                 }
             }
