@@ -276,6 +276,26 @@ def test_many_rows_scales_far_apart(hip):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_rows_queries_of_every_size(hip, D, bf16):
+    """Rows that are zero, subnormal, tiny or not finite beside ordinary ones of
+    the same tile: only those with an infinity or NaN are NaN, and no others."""
+    print(f"case: many rows, queries D={D} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(52)
+    d = filled(hip, rng, 32, 4, D, [200, 150], extra=1 << 24)
+    q = values(rng, 350, 32, D)
+    q[3, 5] = 0
+    q[4, 6] = ref.bf16_value(ref.bf16_bits(q[4, 6] * np.float32(1e-39)))
+    q[5] = ref.bf16_value(ref.bf16_bits(q[5] * np.float32(1e-30)))
+    q[6, :, 1:] = 0
+    q[20, 7, 1], q[21, 8, D - 1], q[349, 31, 0] = np.inf, -np.inf, np.nan
+    rows = starts([200, 150])
+    got = d.attn(0, q, 32, rows=rows, bf16=bf16)
+    check_rows(got, *d.model.attend(0, q, 32, D ** -0.5, True, 0, 0, rows, 350), bf16, D)
+    assert np.isnan(got).any(axis=2).sum() == 3
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 def test_sixteen_query_heads_of_128(hip, bf16):
     """A tile full of one token's heads, by four and by eight wavefronts (64 KB of joined sums)."""
     print(f"case: group 16 of 128 bf16={bf16}", flush=True)
