@@ -511,7 +511,7 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
 // Bound by memory: 32 sequences of up to 30000 tokens, 32 heads over 8 of 128,
 // bf16 (1.35 GB of codes) take 238 us, 5.7 TB/s where a plain read reaches 6.3
 // to 7.1 and a copy 4.8; 64 of up to 1000 tokens, 8 heads, fp32 (88 MB) 21.5 us;
-// one of 376 tokens 7.0 us, of which 4.7 are an empty call's.  fp32
+// one of 376 tokens 6.8 us, of which 4.7 are an empty call's.  fp32
 // rows take two terms each, so twice the products.
 // ONCE: a sequence's rows are one tile, so its codes are read once.
 template <int D, bool BF16, int W, bool ONCE>
