@@ -361,18 +361,18 @@ __device__ __forceinline__ void powers(const f32x4 (&s)[U], float qs, const Halv
                     pf[u >> 1][NB - 1][4 * (u & 1) + j + i] = lo[i];
                 }
             }
-            sum[u] = (p[0] + p[1]) + (p[2] + p[3]);
         } else {
-            // the sum is of the weights as the product takes them, two at a time
             const f16x2 a = __builtin_convertvector((f32x2){p[0], p[1]}, f16x2), b = __builtin_convertvector((f32x2){p[2], p[3]}, f16x2);
-            const f16x2 one = {1, 1};
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 pf[u >> 1][0][4 * (u & 1) + i] = a[i];
                 pf[u >> 1][0][4 * (u & 1) + 2 + i] = b[i];
             }
-            sum[u] = __builtin_amdgcn_fdot2(a, one, __builtin_amdgcn_fdot2(b, one, 0.0f, false), false);
         }
+        // of the fp32 weights, not of those the product takes: where a half's
+        // values are far smaller than others, f16 has none of its p' left, but
+        // its keys keep their share of the softmax
+        sum[u] = (p[0] + p[1]) + (p[2] + p[3]);
     }
 }
 

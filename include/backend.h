@@ -255,7 +255,9 @@ size_t backend_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a);
  * seen; what a masked token holds, NaN included, has no effect.  Rows of out
  * that belong to no sequence are left as they are.  Scores, softmax and sums
  * are fp32; fp32 rows keep fp32 accuracy relative to the largest value the
- * row sees, bf16 rows enter the products as they are. */
+ * row sees; bf16 rows enter the products as they are, and their weights
+ * rounded to f16 (by at most 2^-11 of themselves), the sum of the weights as
+ * fp32 leaves them. */
 void backend_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a);
 /* Sequences dst[i] become copies of src[i], all n (<= seqs) at once, from
  * what the cache held before the call (beam search: src = each beam's
