@@ -15,13 +15,16 @@
 //                 the way to f16.
 // e4m3 values are f16 values, so codes are converted exactly and the products
 // are those of the codes.  Scales are powers of two and never touch a code:
-// the key scale multiplies the score; the value scale is an offset of the
-// softmax exponent, relative to a running reference exponent (eref) of the
-// sums: p' = 2^(s - m + 6 + e - eref) <= 2^14 enters the product, O counts in
-// units of 2^(eref - 6).  Query rows are brought to a largest value in [2^12, 2^13)
-// by a power of two.  fp32 rows enter as the sum of two f16 (22 bits and
-// more), and so do their p; bf16 rows are one f16 each (exact down to 2^-26 of
-// the row's largest), and so p.
+// the key scale multiplies the score; the value scale 2^e is an offset of the
+// softmax exponent.  What enters the second product is p' = 2^(s + e - z), z a
+// whole number some 6 below the largest s + e among the keys that the row
+// sees, so p' <= 2^14 and the largest is never small, whatever scales the pages
+// of the other rows have; the denominator counts p' 2^-e, in fp32.  z is of the
+// row alone: with a reference exponent that the rows of a wavefront shared,
+// rows that saw none of the large values lost their own.  Query rows are
+// brought to a largest value in [2^12, 2^13) by a power of two.  fp32 rows
+// enter as the sum of two f16 (22 bits and more), and so do their p'; bf16 rows
+// are one f16 each (exact down to 2^-26 of the row's largest), and so p'.
 #include "ct_dev.h"
 #include "ct_kv8.h"
 #include "k_kv8.h"
@@ -36,7 +39,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int NT = 256, NW = NT / CT_WAVE;   // threads, wavefronts of a workgroup
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int P_EXP = 6;                     // p' is at most 2^(P_EXP + SLACK), within f16
-constexpr int SLACK = 8;                     // how far scores may pass the running maximum, in bits
+constexpr int SLACK = 8;                     // how far s + e may pass the running maximum, in bits
+constexpr float ONE_V = 1.0f / (1 << P_EXP); // what the sums of p' v have to be scaled by to count as l does
+constexpr int FAR = 90;                      // value scales 2^FAR apart: see add_far
+constexpr int MAX_EXP = 120;                 // exponent of the largest scale that an append gives
 
 struct Args {
     const uint8_t *k, *v;        // the layer's pools
@@ -322,21 +328,32 @@ __device__ __forceinline__ float split_query(const Args &a, bool have, const QPi
     return a.scale2 * pow2i((-up) >> 1) * pow2i(-up - ((-up) >> 1));
 }
 
+// Exponent of a value page's scale.
+__device__ __forceinline__ int exp_of(float scale) {
+    return min(max((int)(__float_as_uint(scale) >> 23 & 255) - 127, KV8_MIN_EXP), MAX_EXP);
+}
+
 // What the queries of a step's U 16-key halves share: the key scales, the
-// exponent offset of p' and what undoes it in l.  least: the smallest factor
-// of a score where some are masked, 0 elsewhere: -inf * 0 is NaN, and scores
-// that small are 0 to the softmax.
+// value scales' exponents and what makes a weight's share of l of p' (l counts
+// in units of 2^P_EXP, which keeps undo in fp32's range).  least: the smallest
+// factor of a score where some are masked, 0 elsewhere: -inf * 0 is NaN, and
+// scores that small are 0 to the softmax.
 template <int U>
 struct Halves {
-    float ks[U], adj[U], undo[U], least;
-    __device__ __forceinline__ void set(int u, int ev, int eref) {
-        const int x = max(P_EXP + ev - eref, -40);
-        adj[u] = (float)x;
-        undo[u] = pow2i(-x);
+    float ks[U], ev[U], undo[U], least;
+    __device__ __forceinline__ void set(int u, int e) {
+        ev[u] = (float)e;
+        undo[u] = pow2i(-e - P_EXP);
     }
 };
 
-// p' of one query over U halves, 2^(s qs ks - m + adj), as B operands, and
+// By how much the exponents of sums change (ldexp) whose maximum rises: x is the
+// old one less the new, whole; NaN (none yet on either side) counts as
+// -infinity.  No factor 2^x: it may be 0 where l, up to 2^100 over pages of
+// zeros, still counts.
+__device__ __forceinline__ int down(float x) { return (int)fmaxf(x, -400.0f); }
+
+// p' of one query over U halves, 2^(s qs ks + ev - m), as B operands, and
 // their sums.  The softmax is online, but its maximum is found only when it
 // has to be: p' are computed with the one so far, and again (settle) if that
 // was too_low for a lane of the wavefront.
@@ -346,7 +363,7 @@ __device__ __forceinline__ void powers(const f32x4 (&s)[U], float qs, const Halv
     const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const float ms = mu - hv.adj[u], f = fmaxf(qs * hv.ks[u], hv.least);
+        const float ms = mu - hv.ev[u], f = fmaxf(qs * hv.ks[u], hv.least);
         float p[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], f, -ms));
@@ -387,20 +404,40 @@ __device__ __forceinline__ bool too_low(float m, const float (&sum)[U]) {
 }
 
 // Moves a query's maximum to that of its scores s (-inf: not seen) and
-// computes its p' again; returns the factor of the sums so far.
+// computes its p' again; returns the factor of the sums so far.  A whole number:
+// factors are then exact, and so is m - ev.
 template <int U, int NB>
 __device__ __forceinline__ float settle(const f32x4 (&s)[U], float qs, const Halves<U> &hv, float &m, float &l,
                                         float (&sum)[U], f16x8 (&pf)[U / 2][NB]) {
     float mt = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; u++)
-        mt = fmaxf(mt, fmaxf(qs * hv.ks[u], hv.least) * fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])));
-    const float mn = fmaxf(m, fmax_q(mt));
-    const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        mt = fmaxf(mt, __builtin_fmaf(fmaxf(qs * hv.ks[u], hv.least), fmaxf(fmaxf(s[u][0], s[u][1]), fmaxf(s[u][2], s[u][3])), hv.ev[u]));
+    const float mn = fmaxf(m, __builtin_ceilf(fmax_q(mt)) - P_EXP);
+    const int by = down(m - mn);
     m = mn;
-    l *= al;
+    l = __builtin_amdgcn_ldexpf(l, by);
     powers<U, NB>(s, qs, hv, m, sum, pf);
-    return al;
+    return __builtin_amdgcn_ldexpf(1.0f, by);
+}
+
+// The weights' share of l of halves `far` (bits): those whose values are 2^-FAR
+// of the largest that the wavefront met and less, pages of zeros among them.
+// Their p' may be below fp32's range where the weights are not, so these come
+// without the value scale, straight from the scores.  Elsewhere p' of the row's
+// largest weight is 2^(5 - FAR) at least, so what fp32 loses is 2^-40 of it.
+template <int U>
+__device__ __forceinline__ void add_far(const f32x4 (&s)[U], float qs, const Halves<U> &hv, uint32_t far, float m,
+                                        float (&sum)[U], float &l) {
+    const float mu = (m == -INFINITY ? 0.0f : m) + P_EXP;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (far >> u & 1) {
+            const float f = fmaxf(qs * hv.ks[u], hv.least);
+#pragma unroll
+            for (int j = 0; j < 4; j++) l += __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], f, -mu));
+            sum[u] = 0.0f;
+        }
 }
 
 // The score where the mask is all ones, -inf where it is 0.
@@ -432,15 +469,6 @@ struct Sight {
     }
 };
 constexpr int NO_KEY = 1 << 30;                  // past every row's keys
-
-// The reference exponent follows the value scales (e1: the largest of this
-// step), but not more than 60 below the largest one met; returns the factor
-// that brings the sums to it.
-__device__ __forceinline__ float follow(int e1, int emax, int &eref) {
-    const int to = max(e1, emax - 60), by = max(min(eref - to, 126), -126);
-    eref = to;
-    return pow2i(by);
-}
 
 // V's A operands of four dims, code(j) their codes of the lane's key j: pairs
 // of keys side by side.
@@ -605,8 +633,8 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
     f32x4 o[1][DI];
 #pragma unroll
     for (int i = 0; i < DI; i++) o[0][i] = (f32x4){0, 0, 0, 0};
-    float m = have ? -INFINITY : 0.0f, l = 0.0f;         // lanes without a row never move the maximum
-    int eref = KV8_MIN_EXP, emax = KV8_MIN_EXP;
+    float m = have ? -INFINITY : INFINITY, l = 0.0f;     // lanes without a row: no weights, and never a new maximum
+    int emax = KV8_MIN_EXP;
     bool dirty = false;
 
     auto use = [&](int st, int i, Raw<D> &r) {
@@ -619,7 +647,7 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
         for (int u = 0; u < 2; u++) {
             in[u] = __builtin_amdgcn_readlane(pg, 2 * i + u) >= 0;
             hv.ks[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pks), 2 * i + u));
-            ev[u] = max((int)(__builtin_amdgcn_readlane(__float_as_uint(pvs), 2 * i + u) >> 23 & 255) - 127, KV8_MIN_EXP);
+            ev[u] = exp_of(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pvs), 2 * i + u)));
         }
         // a chain of products per half and query term, next to each other
         f32x4 sb[NB][2];
@@ -668,16 +696,14 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
                     for (int y = 0; y < D / 64; y++) r.v[j][y] = without_nan(r.v[j][y]);
             }
         }
-        const int e1 = max(ev[0], ev[1]);        // pages that are not there have the least
-        emax = max(emax, e1);
-        if (__builtin_expect(e1 > eref || e1 < eref - 8, 0)) {
-            const float by = follow(e1, emax, eref);
+        emax = max(emax, max(ev[0], ev[1]));     // pages that are not there have the least
+        uint32_t far = 0;
+        if (__builtin_expect(min(ev[0], ev[1]) < emax - FAR, 0))
 #pragma unroll
-            for (int y = 0; y < DI; y++) o[0][y] *= by;
-        }
+            for (int u = 0; u < 2; u++) far |= (uint32_t)(in[u] && ev[u] < emax - FAR) << u;
         hv.least = whole ? 0.0f : 0x1p-100f;
-        hv.set(0, ev[0], eref);
-        hv.set(1, ev[1], eref);
+        hv.set(0, ev[0]);
+        hv.set(1, ev[1]);
         f16x8 pf[1][NB];
         float sum[2];
         powers<2, NB>(s, qs, hv, m, sum, pf);
@@ -686,6 +712,7 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
 #pragma unroll
             for (int y = 0; y < DI; y++) o[0][y] *= al;
         }
+        if (__builtin_expect(far, 0)) add_far<2>(s, qs, hv, far, m, sum, l);
 #pragma unroll
         for (int u = 0; u < 2; u++) l = __builtin_fmaf(sum[u], hv.undo[u], l);
 #pragma unroll
@@ -715,13 +742,12 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
 
     // the wavefronts' sums joined, in their order
     l = sum_q(l);
-    const float unit = pow2i(eref - P_EXP);
     if (have) {
         if (g == 0) { sm[w][c] = m; sl[w][c] = l; }
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < DI; i++) so[(w * a.rpt + c) * D + (4 * g + j) * DI + i] = o[0][i][j] * unit;
+            for (int i = 0; i < DI; i++) so[(w * a.rpt + c) * D + (4 * g + j) * DI + i] = o[0][i][j];
     }
     __syncthreads();
     const int nr = min(16, t.n * a.group - t.row);
@@ -734,13 +760,13 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
         float num = 0.0f, den = 0.0f;
 #pragma unroll
         for (int i = 0; i < W; i++) {
-            const float f = __builtin_amdgcn_exp2f(sm[i][r] - Mu);
-            num += f * so[(i * a.rpt + r) * D + d];
-            den += f * sl[i][r];
+            const int by = down(sm[i][r] - Mu);
+            num += __builtin_amdgcn_ldexpf(so[(i * a.rpt + r) * D + d], by);
+            den += __builtin_amdgcn_ldexpf(sl[i][r], by);
         }
         if (chunks <= 1) {
             const int R2 = t.row + r, i = a.group > 1 ? R2 / a.group : R2;
-            const float y = den == 0.0f ? 0.0f : num / den;
+            const float y = den == 0.0f ? 0.0f : num * ONE_V / den;
             const long off = (long)(t.r0 + i) * a.ld_out + (long)(h * a.group + R2 - i * a.group) * D + d;
             if (BF16) reinterpret_cast<uint16_t *>(a.out)[off] = f2bf(y);
             else reinterpret_cast<float *>(a.out)[off] = y;
@@ -830,7 +856,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     auto put_scales = [&](int it0) {
         const int bt = it0 >> 5 & 1, i = lane >> 1, half = 2 * kb + (lane & 1);
         if (!isv) sscale[bt][i][half] = psc;
-        else sexp[bt][i][half] = pg < 0 ? GONE : max((int)(__float_as_uint(psc) >> 23 & 255) - 127, KV8_MIN_EXP);
+        else sexp[bt][i][half] = pg < 0 ? GONE : exp_of(psc);
     };
     const unsigned off = isv ? 4 * g * D + c * DI : c * D + 16 * g;
 
@@ -949,12 +975,12 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     float m[NQ], l[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
-        m[n] = t.row + WR * w + 16 * n + c < all ? -INFINITY : 0.0f;     // lanes without a row never move it
+        m[n] = t.row + WR * w + 16 * n + c < all ? -INFINITY : INFINITY;     // lanes without a row
         l[n] = 0.0f;
 #pragma unroll
         for (int i = 0; i < DI; i++) o[n][i] = (f32x4){0, 0, 0, 0};
     }
-    int eref = KV8_MIN_EXP, emax = KV8_MIN_EXP;
+    int emax = KV8_MIN_EXP;
 
     // iteration `it`: the unit asked for AHEAD iterations ago into the other
     // buffer, the next one asked for, and this one's products.  One barrier:
@@ -1009,7 +1035,8 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
                             to = mfma_f16(kf[i & 1][v], qf[n][y][i / (4 / KG)], to);
                         }
             }
-            const bool whole = min(min(ev[0], ev[1]), min(ev[2], ev[3])) > GONE && k0 >= full_lo && k0 + 32 <= full_hi && k1 >= full_lo && k1 + 32 <= full_hi;
+            const int least = min(min(ev[0], ev[1]), min(ev[2], ev[3]));
+            const bool whole = least > GONE && k0 >= full_lo && k0 + 32 <= full_hi && k1 >= full_lo && k1 + 32 <= full_hi;
             if (__builtin_expect(!whole, 0)) {
 #pragma unroll
                 for (int n = 0; n < NQ; n++) {
@@ -1024,18 +1051,14 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
                         }
                 }
             }
-            const int e1 = max(max(max(ev[0], ev[1]), max(ev[2], ev[3])), KV8_MIN_EXP);
-            emax = max(emax, e1);
-            if (__builtin_expect(e1 > eref || e1 < eref - 8, 0)) {
-                const float by = follow(e1, emax, eref);
+            emax = max(emax, max(max(ev[0], ev[1]), max(ev[2], ev[3])));
+            uint32_t far = 0;
+            if (__builtin_expect(least < emax - FAR, 0))
 #pragma unroll
-                for (int n = 0; n < NQ; n++)
-#pragma unroll
-                    for (int i = 0; i < DI; i++) o[n][i] *= by;
-            }
+                for (int u = 0; u < 4; u++) far |= (uint32_t)(ev[u] > GONE && ev[u] < emax - FAR) << u;
             hv.least = whole ? 0.0f : 0x1p-100f;
 #pragma unroll
-            for (int u = 0; u < 4; u++) hv.set(u, ev[u], eref);
+            for (int u = 0; u < 4; u++) hv.set(u, ev[u]);
             f16x8 pf[NQ][2][NB];
             float sum[NQ][4];
 #pragma unroll
@@ -1046,6 +1069,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
                     for (int i = 0; i < DI; i++) o[n][i] *= al;
                 }
+                if (__builtin_expect(far, 0)) add_far<4>(s[n], qs[n], hv, far, m[n], sum[n], l[n]);
 #pragma unroll
                 for (int u = 0; u < 4; u++) l[n] = __builtin_fmaf(sum[n][u], hv.undo[u], l[n]);
             }
@@ -1100,8 +1124,6 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     if (__builtin_expect(snan, 0))
         for (int st = s0; st < s1; st++) spread_nan<D, NQ>(z, t, h, step_key(t, st), c, g, pos, o);
 
-
-    const float unit = pow2i(eref - P_EXP);
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const float den = sum_q(l[n]);
@@ -1114,7 +1136,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int i = 0; i < DI; i++) {
-                    const float y = den == 0.0f ? 0.0f : o[n][i][j] * unit * f;
+                    const float y = den == 0.0f ? 0.0f : o[n][i][j] * ONE_V * f;
                     if (BF16) reinterpret_cast<uint16_t *>(z.out)[off + (4 * g + j) * DI + i] = f2bf(y);
                     else reinterpret_cast<float *>(z.out)[off + (4 * g + j) * DI + i] = y;
                 }
@@ -1123,7 +1145,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
-                for (int i = 0; i < DI; i++) z.part[at * D + (4 * g + j) * DI + i] = o[n][i][j] * unit;
+                for (int i = 0; i < DI; i++) z.part[at * D + (4 * g + j) * DI + i] = o[n][i][j];
             if (g == 0) z.stat[at] = make_float2(m[n], den);
         }
     }
@@ -1164,10 +1186,10 @@ __global__ __launch_bounds__(NT) void join_kernel(Args a) {
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             if (k0 + u * WPR >= chunks) break;
-            const float f = __builtin_amdgcn_exp2f(st[u].x - Mu);
-            den += f * st[u].y;
+            const int by = down(st[u].x - Mu);
+            den += __builtin_amdgcn_ldexpf(st[u].y, by);
 #pragma unroll
-            for (int j = 0; j < DL; j++) num[j] += f * x[u][j];
+            for (int j = 0; j < DL; j++) num[j] += __builtin_amdgcn_ldexpf(x[u][j], by);
         }
     }
     if (WPR > 1) {
@@ -1188,7 +1210,7 @@ __global__ __launch_bounds__(NT) void join_kernel(Args a) {
     const long off = (long)(t.r0 + R / a.group) * a.ld_out + (long)(h * a.group + R % a.group) * D + lane * DL;
 #pragma unroll
     for (int j = 0; j < DL; j++) {
-        const float y = den == 0.0f ? 0.0f : num[j] / den;
+        const float y = den == 0.0f ? 0.0f : num[j] * ONE_V / den;
         if (BF16) reinterpret_cast<uint16_t *>(a.out)[off + j] = f2bf(y);
         else reinterpret_cast<float *>(a.out)[off + j] = y;
     }

@@ -254,8 +254,9 @@ size_t backend_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a);
  * sees none gets zeros; tokens on a page that is not in the pool are not
  * seen; what a masked token holds, NaN included, has no effect.  Rows of out
  * that belong to no sequence are left as they are.  Scores, softmax and sums
- * are fp32; fp32 rows keep fp32 accuracy relative to the largest value the
- * row sees; bf16 rows enter the products as they are, and their weights
+ * are fp32; fp32 rows keep fp32 accuracy relative to the largest value that
+ * the pages of the tokens a row sees can hold (448 of their scales, which are
+ * powers of two from 2^-100 to 2^120), whatever other pages hold; bf16 rows enter the products as they are, and their weights
  * rounded to f16 (by at most 2^-11 of themselves), the sum of the weights as
  * fp32 leaves them. */
 void backend_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a);

@@ -12,12 +12,12 @@ pytestmark = pytest.mark.gpu
 ORDERS = {"after": lambda j, n: j >= (n + 1) // 2, "before": lambda j, n: j < n // 2, "among": lambda j, n: j % 2 == 1}
 
 
-def appended(hip, rng, P, kv, D, lens, small, order, extra=1 << 24):
-    """Sequences of lens tokens appended at once; the values of the pages that
-    `order` names are `small` times as large as the others'."""
+def appended(hip, rng, P, kv, D, lens, small, order, scale=1.0, extra=1 << 24):
+    """Sequences of lens tokens appended at once, with values of size `scale`;
+    those on the pages that `order` names are `small` times as large."""
     held = [-(-n // P) for n in lens]
     d = ref.Dev(hip, 1, sum(held) + 2, P, kv, D, len(lens), max(held) + 1, extra)
-    k, v = values(rng, sum(lens), kv, D) * np.float32(0.25), values(rng, sum(lens), kv, D)
+    k, v = values(rng, sum(lens), kv, D) * np.float32(0.25), values(rng, sum(lens), kv, D) * np.float32(scale)
     for s, r0 in enumerate(starts(lens)[:-1]):
         for j in range(held[s]):
             if ORDERS[order](j, held[s]):
@@ -76,3 +76,54 @@ def test_prompts_over_pages_of_zeros(hip, order, bf16):
         d = appended(hip, rng, P, 4, 64, [190, 170], 0.0, order)
         attends(d, rng, [190, 170], 32, bf16, ("many", P))
         attends(d, rng, [60, 0], 4, bf16, ("few", P))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("small", [2.0 ** -20, 2.0 ** -40, 2.0 ** -85])
+def test_rows_that_see_small_values_alone(hip, small, bf16):
+    """Rows whose tokens are all small, beside rows of the same tile, and masked
+    tokens of the same step, with large ones: as accurate, relative to what
+    they see, as without those."""
+    print(f"case: rows of small values {small} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(63)
+    for P in (16, 32, 64):
+        d = appended(hip, rng, P, 4, 64, [190, 170], small, "before")
+        attends(d, rng, [190, 170], 32, bf16, ("many", P))
+        attends(d, rng, [190, 170], 4, bf16, ("few", P))
+        d = appended(hip, rng, P, 4, 64, [190, 170, 6 * P + 3, 7 * P + 3], small, "among")
+        for kw in (dict(window=1), dict(window=7), dict(window=7, sinks=3), dict(window=P // 2, sinks=P + 2)):
+            attends(d, rng, [190, 170, 0, 0], 32, bf16, ("many", P, kw), **kw)
+            attends(d, rng, [190, 170, 1, 3], 4, bf16, ("few", P, kw), **kw)
+            attends(d, rng, [1, 1, 1, 1], 4, bf16, ("single", P, kw), **kw)
+    d = appended(hip, rng, 16, 1, 128, [330, 90], small, "before")
+    attends(d, rng, [330, 90], 64, bf16, "heads of 128")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("small,scale", [(0.0, 2.0 ** 20), (2.0 ** -110, 2.0 ** 60), (0.0, 2.0 ** 100)])
+@pytest.mark.parametrize("order", sorted(ORDERS))
+def test_the_whole_range_of_scales(hip, order, small, scale, bf16):
+    """Value scales up to 2^200 apart: weights that have no room beside their
+    page's scale still count."""
+    print(f"case: whole range {order} {small} {scale} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(64)
+    for P in (16, 64):
+        d = appended(hip, rng, P, 4, 64, [190, 700], small, order, scale=scale)
+        for causal in (True, False):
+            attends(d, rng, [170, 190], 32, bf16, ("many", P, causal), causal=causal)
+            attends(d, rng, [30, 60], 4, bf16, ("few", P, causal), causal=causal)
+        attends(d, rng, [1, 1], 4, bf16, ("single", P))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_scales_of_every_size_together(hip, bf16):
+    """Each page its own scale, up to 2^25 apart: prompts and single rows."""
+    print(f"case: mixed scales bf16={bf16}", flush=True)
+    rng = np.random.default_rng(65)
+    for P in (16, 32):
+        d = appended(hip, rng, P, 4, 64, [200, 150], 1.0, "among")
+        d.model.vs[:] *= 2.0 ** rng.integers(-20, 6, d.model.vs.shape)
+        d.push()
+        attends(d, rng, [200, 150], 32, bf16, ("many", P))
+        attends(d, rng, [33, 20], 4, bf16, ("few", P))
+        attends(d, rng, [1, 1], 4, bf16, ("single", P))
