@@ -127,3 +127,31 @@ def test_scales_of_every_size_together(hip, bf16):
         attends(d, rng, [200, 150], 32, bf16, ("many", P))
         attends(d, rng, [33, 20], 4, bf16, ("few", P))
         attends(d, rng, [1, 1], 4, bf16, ("single", P))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_values_near_the_largest_float(hip, bf16):
+    """Values up to 1e38: sums of several of them stay in range, whatever their
+    weights are relative to the largest score found so far."""
+    print(f"case: largest values bf16={bf16}", flush=True)
+    rng = np.random.default_rng(66)
+    P, kv, D, lens = 32, 4, 64, [190, 700]
+    d = ref.Dev(hip, 1, 40, P, kv, D, 2, 24, 1 << 24)
+    # keys of growing size along one direction, which the queries have too: scores rise by 5 bits over the text
+    k = values(rng, sum(lens), kv, D) * np.float32(0.05)
+    k[:, :, 0] = np.concatenate([np.linspace(0, 3.5, n) for n in lens])[:, None]
+    k = ref.bf16_value(ref.bf16_bits(k))
+    v = ref.bf16_value(ref.bf16_bits((rng.uniform(-1, 1, (sum(lens), kv, D)) * 1e38).astype(np.float32)))
+    d.reserve(lens)
+    d.append(0, k, v)
+    d.check()
+    for n, heads, kw in (([170, 190], 32, {}), ([170, 190], 32, dict(causal=False)), ([30, 60], 4, {}), ([1, 1], 4, {}),
+                         ([1, 1], 4, dict(max_len=700))):
+        rows = starts(n)
+        q = values(rng, int(rows[-1]), heads, D) * np.float32(0.05)
+        q[:, :, 0] = 8.0
+        q = ref.bf16_value(ref.bf16_bits(q))
+        got = d.attn(0, q, heads, bf16=bf16, rows=rows, **kw)
+        want = d.model.attend(0, q, heads, D ** -0.5, kw.get("causal", True), 0, 0, rows, len(q))
+        assert np.isfinite(got).all(), (n, kw)
+        check_rows(got, *want, bf16, (n, kw))
