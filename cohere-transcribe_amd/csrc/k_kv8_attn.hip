@@ -1302,12 +1302,12 @@ extern "C" size_t ctk_kv8_attn_need(const BackendKv8 *c, const BackendKv8Attn *a
 }
 
 // An upper bound of ctk_kv8_attn_need over all calls with at most these rows
-// and tokens: the chunks of all units are at most the number aimed at, or one
-// for every 128 steps where that is more, and one a unit for rounding up.
-extern "C" size_t ctk_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a) {
+// and tokens, of rows whose larger tiles hold `most_rows`: the chunks of all
+// units are at most the number aimed at, or one for every 128 steps where that is
+// more, and one a unit for rounding up.
+static size_t work_of(const BackendKv8 *c, const BackendKv8Attn *a, int most_rows) {
     const long group = a->heads / c->kv_heads, kv = c->kv_heads;
     const long rows = (long)(a->max_rows < a->n_rows ? a->max_rows : a->n_rows) * group;
-    const int most_rows = rows_of(a->bf16);
     const long steps = walk_of(c, a, most_rows), row = c->head_dim + 2;
     const long all16 = (long)a->n_rows * group / 16 + c->seqs;
     auto chunks = [&](long units, long aim) {
@@ -1328,6 +1328,12 @@ extern "C" size_t ctk_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a
     }
     // nothing is split where no tile walks further than one chunk's least
     return steps <= 8 ? 0 : (size_t)(most * row);
+}
+
+// Either type of rows: their tiles, and with them the split, differ.
+extern "C" size_t ctk_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a) {
+    const size_t f32 = work_of(c, a, rows_of(false)), bf16 = work_of(c, a, rows_of(true));
+    return f32 > bf16 ? f32 : bf16;
 }
 
 extern "C" void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *p, hipStream_t s) {

@@ -247,7 +247,7 @@ typedef struct {
 } BackendKv8Attn;
 /* Floats of work (0: none, work may be NULL) that are enough for this call
  * and for any with the same cache, heads, window and sinks and no more n_rows,
- * max_rows and max_len.  It depends on the sizes alone, not on the pointers. */
+ * max_rows and max_len, whichever type its rows have.  It depends on the sizes alone, not on the pointers. */
 size_t backend_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a);
 /* Softmax attention of the rows over a layer's pages: o = sum_j p_j v_j,
  * p = softmax_j(scale * q . k_j) over the tokens the row sees.  A row that

@@ -793,3 +793,28 @@ def test_captured_step(hip):
     assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
     assert all(np.array_equal(sa[k], sb[k]) for k in sa)
     assert np.isfinite(a).all()
+
+
+@pytest.mark.parametrize("sized", [False, True])
+def test_work_sized_with_the_other_row_type(hip, sized):
+    """Work sized with fp32 rows used by bf16 ones, and the other way round:
+    right, and nothing behind it written (most rows of the call belong to no
+    sequence)."""
+    print(f"case: work sized with bf16={sized}", flush=True)
+    rng = np.random.default_rng(53)
+    d = filled(hip, rng, 16, 1, 64, [2490], spare=1, extra=1 << 24)
+    n, heads, rows = 2110, 5, starts([268])
+    q = values(rng, n, heads, 64)
+    call = dict(ld_out=320, ld_q=320, heads=heads, scale=0.125, causal=1, rows=d.ints(rows), n_rows=n, max_rows=268)
+    for bf16 in (not sized, sized):
+        floats = hip.backend_kv8_attn_work(d.h, C.byref(cb.BackendKv8Attn(bf16=int(sized), **call)))
+        guard = 1 << 19
+        fl, work = q.reshape(-1), d.put(np.full(floats + guard, 7.0, np.float32))
+        old = np.full(fl.shape, 55.0, np.float32)
+        qp, op = d.put(ref.bf16_bits(fl) if bf16 else fl), d.put(ref.bf16_bits(old) if bf16 else old)
+        a = cb.BackendKv8Attn(out=op, q=qp, bf16=int(bf16), work=work, **call)
+        hip.backend_kv8_attn(d.h, 0, C.byref(a))
+        got = d.get(op, q.shape, np.uint16 if bf16 else np.float32)
+        got = ref.bf16_value(got) if bf16 else got
+        assert np.all(d.get(work + floats * 4, (guard,), np.float32) == 7.0), bf16
+        check_rows(got, *d.model.attend(0, q, heads, 0.125, True, 0, 0, rows, n), bf16, bf16)

@@ -145,6 +145,38 @@ def test_work_is_enough_for_smaller_calls():
     assert split > 1000
 
 
+def test_work_is_enough_for_either_row_type():
+    """Work sized with fp32 rows is enough for bf16 ones and the other way
+    round: the type is not among what has to stay the same."""
+    L = cb.hip()
+    L.ctk_kv8_attn_need.argtypes, L.ctk_kv8_attn_need.restype = [C.c_void_p, C.c_void_p], C.c_size_t
+    rng = np.random.default_rng(5)
+
+    def log(a, b):
+        return int(round(float(np.exp(rng.uniform(np.log(a), np.log(b))))))
+
+    def check(c, a, **smaller):
+        p = C.byref(c)
+        for sized in (0, 1):
+            work = L.backend_kv8_attn_work(p, C.byref(cb.BackendKv8Attn(bf16=sized, **a)))
+            for used in (0, 1):
+                need = L.ctk_kv8_attn_need(p, C.byref(cb.BackendKv8Attn(bf16=used, **{**a, **smaller})))
+                assert need <= work, (sized, used, need, work, a, smaller)
+
+    for kv, group, seqs, width, P, n, rows, D in ((1, 8, 46, 88, 32, 3358, 3358, 128), (27, 25, 9, 52, 64, 11, 5, 64)):
+        c = cb.BackendKv8(layers=1, pages=8, page_tokens=P, kv_heads=kv, head_dim=D, seqs=seqs, table_w=width)
+        check(c, dict(heads=kv * group, scale=1.0, causal=1, n_rows=n, max_rows=rows))
+    for _ in range(6000):
+        kv, group = int(rng.choice([1, 1, 2, 3, 8, 27, 256])), int(rng.choice([1, 2, 3, 5, 8, 16, 25, 32]))
+        c = cb.BackendKv8(layers=1, pages=8, page_tokens=int(rng.choice([16, 32, 64, 128])), kv_heads=kv,
+                          head_dim=int(rng.choice([64, 128])), seqs=log(1, 256), table_w=log(1, 2000))
+        n = log(1, min(1 << 14, (1 << 27) // (kv * group)))
+        rows, window = log(1, n), int(rng.integers(2)) * log(1, 20000)
+        a = dict(heads=kv * group, scale=1.0, causal=1, window=window, sinks=log(1, 300) if window else 0, n_rows=n, max_rows=rows)
+        check(c, a)
+        check(c, a, n_rows=log(1, n), max_rows=log(1, rows), max_len=log(1, 1 << 16))
+
+
 def test_model_rounding():
     """The model's rounding against the definition: every code is its own
     nearest, midpoints go to the even code, values past the largest are held."""
