@@ -126,7 +126,8 @@ static void check_attn(const BackendKv8 *c, const BackendKv8Attn *a) {
     if (a->max_len < 0) CT_FATAL("kv8_attn: max_len < 0");
     if (a->window < 0 || a->sinks < 0) CT_FATAL("kv8_attn: window or sinks < 0");
     if (a->window > 0 && !a->causal) CT_FATAL("kv8_attn: a window needs causal rows");
-    if (!(a->scale > 0.0f && a->scale <= 3.0e38f)) CT_FATAL("kv8_attn: scale is not positive and finite");
+    /* the kernels multiply it by log2(e), which must not overflow */
+    if (!(a->scale > 0.0f && a->scale <= 2.0e38f)) CT_FATAL("kv8_attn: scale is not positive and at most 2e38");
 }
 
 size_t backend_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a) {

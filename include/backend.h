@@ -231,7 +231,8 @@ typedef struct {
     int bf16;            /* q and out: 0 fp32, 1 bf16                         */
     int heads;           /* query heads, a multiple of kv_heads: head h reads
                             kv head h / (heads / kv_heads)                    */
-    float scale;         /* of the scores; 1 / sqrt(head_dim) for this model  */
+    float scale;         /* of the scores; 1 / sqrt(head_dim) for this model;
+                            positive, at most 2e38                            */
     int causal;          /* 1: a sequence's rows are its last tokens and see
                             the tokens up to their own; 0: they see all       */
     int window;          /* causal only: a row at position p sees p - window

@@ -818,3 +818,18 @@ def test_work_sized_with_the_other_row_type(hip, sized):
         got = ref.bf16_value(got) if bf16 else got
         assert np.all(d.get(work + floats * 4, (guard,), np.float32) == 7.0), bf16
         check_rows(got, *d.model.attend(0, q, heads, 0.125, True, 0, 0, rows, n), bf16, bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_the_largest_scale(hip, bf16):
+    """Scores of ordinary size, and zeros, from tiny queries and the largest scale allowed."""
+    print(f"case: largest scale bf16={bf16}", flush=True)
+    rng = np.random.default_rng(54)
+    scale = float(np.float32(2.0e38))
+    for n, heads in (([1, 1], 4), ([30, 60], 4), ([190, 170], 32)):
+        d = filled(hip, rng, 32, 4, 64, [200, 190], extra=1 << 24)
+        q = values(rng, sum(n), heads, 64) * np.float32(0.125 / scale * 2.0 ** 14) * np.float32(2.0 ** -14)
+        q = ref.bf16_value(ref.bf16_bits(q))
+        q[:, 1] = 0
+        got = d.attn(0, q, heads, bf16=bf16, rows=starts(n), scale=scale)
+        check_rows(got, *d.model.attend(0, q, heads, scale, True, 0, 0, starts(n), len(q)), bf16, n)

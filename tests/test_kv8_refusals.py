@@ -84,6 +84,10 @@ CASES = {
 }
 
 
+# a scale whose product with log2(e), by which the kernels multiply it, overflows: a score of 0 would be NaN
+CASES["attn_scale_large"] = (ATTN, {}, dict(scale=2.4e38), "scale is not positive and at most")
+
+
 @pytest.mark.parametrize("case", sorted(CASES))
 def test_refused_before_device_work(case):
     call, cache, attn, msg = CASES[case]
