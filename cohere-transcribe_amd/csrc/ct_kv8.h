@@ -19,8 +19,7 @@
 enum {
     CT_KV8_STATUS = 0, /* sticky flags                                       */
     CT_KV8_COUNT = 1,  /* pages to copy                                      */
-    CT_KV8_OK = 2,     /* the fork was admitted                              */
-    CT_KV8_LIVE = 3,   /* pages in use                                       */
+    CT_KV8_LIVE = 2,   /* pages in use                                       */
     CT_KV8_HEAD = 16
 };
 
