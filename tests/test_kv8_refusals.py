@@ -181,6 +181,30 @@ def test_work_is_enough_for_either_row_type():
         check(c, a, n_rows=log(1, n), max_rows=log(1, rows), max_len=log(1, 1 << 16))
 
 
+def test_more_rows_tokens_or_heads_never_take_less_work():
+    """And they do take more, where texts are split."""
+    L = cb.hip()
+    rng = np.random.default_rng(6)
+
+    def log(a, b):
+        return int(round(float(np.exp(rng.uniform(np.log(a), np.log(b))))))
+
+    more = {"n_rows": 0, "max_rows": 0, "max_len": 0, "heads": 0}
+    for _ in range(3000):
+        kv, group = int(rng.choice([1, 2, 8, 256])), int(rng.choice([1, 2, 5, 8, 16]))
+        c = cb.BackendKv8(layers=1, pages=8, page_tokens=64, kv_heads=kv, head_dim=128, seqs=log(1, 256), table_w=4000)
+        n, window = log(1, min(20000, (1 << 25) // (kv * (group + 8)))), int(rng.integers(2)) * log(1, 20000)
+        a = dict(heads=kv * group, scale=1.0, causal=1, bf16=int(rng.integers(2)), window=window,
+                 sinks=log(1, 300) if window else 0, n_rows=n, max_rows=log(1, n), max_len=log(1, 200000))
+        least = L.backend_kv8_attn_work(C.byref(c), C.byref(cb.BackendKv8Attn(**a)))
+        for name in more:
+            b = {**a, name: a[name] * 2 if name != "heads" else a[name] + kv * log(1, 8)}
+            work = L.backend_kv8_attn_work(C.byref(c), C.byref(cb.BackendKv8Attn(**b)))
+            assert work >= least, (name, a)
+            more[name] += work > least
+    assert min(more.values()) > 100, more
+
+
 def test_model_rounding():
     """The model's rounding against the definition: every code is its own
     nearest, midpoints go to the even code, values past the largest are held."""
