@@ -1259,7 +1259,8 @@ Shape shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
         // of 16 13.2); else 512 chunks in all, of 8 to 128 steps (8 units of
         // 125 steps: 10.6 us at 8, 24.8 at 64; 256 units of 938 steps: 325 us
         // at 8, 245 at 64 and 128).  seqs counts whether they have rows or not,
-        // so a row's bits do not depend on the other sequences.
+        // so with a tile a sequence (max_rows * group up to 16) a row's bits do
+        // not depend on the others.
         s.chunk = (int)steps;
         if (steps > 24 && (steps > 64 || units < 128)) {
             const long each = (units * steps + 511) / 512;

@@ -833,3 +833,25 @@ def test_the_largest_scale(hip, bf16):
         q[:, 1] = 0
         got = d.attn(0, q, heads, bf16=bf16, rows=starts(n), scale=scale)
         check_rows(got, *d.model.attend(0, q, heads, scale, True, 0, 0, starts(n), len(q)), bf16, n)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("group,n,kw", [(16, [1, 1, 1, 1], {}), (4, [4, 1, 2, 3], {}), (8, [1, 2, 0, 2], dict(window=300, sinks=5)),
+                                        (5, [3, 3, 3, 3], dict(max_len=700))])
+def test_one_tile_a_sequence_gives_the_same_bits(hip, group, n, kw, bf16):
+    """Up to 16 (row, query head) pairs a kv head: the same sequences in other
+    company, and behind rows of none."""
+    print(f"case: batch invariance group={group} n={n} {kw} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(55)
+    d = filled(hip, rng, 32, 2, 64, [700, 33, 1030, 5], extra=1 << 25)
+    rows, most = starts(n), 16 // group
+    q = values(rng, int(rows[-1]), 2 * group, 64)
+    both = d.attn(0, q, 2 * group, rows=rows, max_rows=most, bf16=bf16, **kw)
+    check_rows(both, *d.model.attend(0, q, 2 * group, 0.125, True, kw.get("window", 0), kw.get("sinks", 0), rows, len(q), kw.get("max_len")), bf16, n)
+    for s in range(4):
+        one = np.where(np.arange(5) > s, n[s], 0)
+        for behind in (0, 40):
+            x = np.concatenate([q[rows[s]:rows[s + 1]], np.zeros((behind, 2 * group, 64), np.float32)])
+            if len(x):
+                alone = d.attn(0, x, 2 * group, rows=one, max_rows=most, bf16=bf16, **kw)[:n[s]]
+                assert np.array_equal(alone.view(np.uint32), both[rows[s]:rows[s + 1]].view(np.uint32)), (s, behind)
