@@ -855,3 +855,51 @@ def test_one_tile_a_sequence_gives_the_same_bits(hip, group, n, kw, bf16):
             if len(x):
                 alone = d.attn(0, x, 2 * group, rows=one, max_rows=most, bf16=bf16, **kw)[:n[s]]
                 assert np.array_equal(alone.view(np.uint32), both[rows[s]:rows[s + 1]].view(np.uint32)), (s, behind)
+
+
+def test_reserve_and_fork_in_a_pool_of_many_pages(hip):
+    """More than 65536 pages, the free ones late in each planning thread's run:
+    taken lowest first, to the last one, and refused when there is one too few."""
+    print("case: pool of 150000 pages", flush=True)
+    pages, P = 150000, 16
+    c = cb.BackendKv8(layers=1, pages=pages, page_tokens=P, kv_heads=1, head_dim=64, seqs=4, table_w=300)
+    h = C.byref(c)
+    n = hip.backend_kv8_floats(h)
+    base = hip.backend_arena_alloc(n + (1 << 20))
+    hip.backend_kv8_bind(h, base)
+    d = ref.Dev.__new__(ref.Dev)
+    d.hip, d.c, d.h, d.at, d.end = hip, c, h, base + (n + 63) // 64 * 256, base + (n + (1 << 20)) * 4
+    rng = np.random.default_rng(56)
+    per = -(-pages // 1024)
+    free = np.sort(rng.choice([p for p in range(pages) if p % per >= 60], 500, replace=False))
+    refs = np.ones(pages, np.int32)
+    refs[free] = 0
+    d.write(c.refs, refs)
+
+    def table():
+        return d.get(c.table, (4, 300), np.int32)
+
+    hip.backend_kv8_reserve(h, d.ints([P * 200 + 3, 0, P * 150, 1]))             # 201 + 150 + 1 pages
+    got = table()
+    assert np.array_equal(got[0, :201], free[:201]) and np.array_equal(got[2, :150], free[201:351]) and got[3, 0] == free[351]
+    hip.backend_kv8_fork(h, d.ints([1]), d.ints([0]), 1)                         # copies one page
+    got = table()
+    assert np.array_equal(got[1, :200], free[:200]) and got[1, 200] == free[352]
+    hip.backend_kv8_reserve(h, d.ints([0, 0, P * 148, 0]))                       # one more than there are
+    assert hip.backend_kv8_status(h) == 1 and np.array_equal(table(), got)
+    hip.backend_kv8_reserve(h, d.ints([0, 0, P * 147, 0]))
+    assert hip.backend_kv8_status(h) == 0 and np.array_equal(table()[2, 150:297], free[353:])
+    refs[free] = 1
+    refs[free[:200]] = 2
+    assert np.array_equal(d.get(c.refs, (pages,), np.int32), refs)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("n,heads", [([1, 1, 1], 4), ([60, 30, 20], 4), ([190, 170, 20], 32)])
+def test_window_past_max_len(hip, n, heads, bf16):
+    """Rows behind max_len with a window: some see its end, some the first tokens alone, some nothing."""
+    print(f"case: window past max_len n={n} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(57)
+    for window, sinks, most in ((40, 3, 150), (10, 0, 333), (100, 40, 33)):
+        run_attn(hip, rng, 16, 4, heads // 4, 64, [340, 200, 150], n, (window, sinks, most), window=window, sinks=sinks,
+                 max_len=most, bf16=bf16)
