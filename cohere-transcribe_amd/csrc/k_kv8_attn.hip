@@ -379,6 +379,9 @@ __device__ __forceinline__ void powers(const f32x4 (&s)[U], float qs, const Halv
                 }
             }
         } else {
+            // the matrix instruction takes 16 bits: 11 of f16 are 8 times finer than
+            // the bf16 that the output is rounded to, and a second term would
+            // double the products
             const f16x2 a = __builtin_convertvector((f32x2){p[0], p[1]}, f16x2), b = __builtin_convertvector((f32x2){p[2], p[3]}, f16x2);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -538,8 +541,8 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
 // turn, each with two steps of codes in flight, and join their sums in LDS.
 // Bound by memory: 32 sequences of up to 30000 tokens, 32 heads over 8 of 128,
 // bf16 (1.35 GB of codes) take 238 us, 5.7 TB/s where a plain read reaches 6.3
-// to 7.1 and a copy 4.8; 64 of up to 1000 tokens, 8 heads, fp32 (88 MB) 21.5 us;
-// one of 376 tokens 6.8 us, of which 4.7 are an empty call's.  fp32
+// to 7.1 and a copy 4.8; 64 of up to 1000 tokens, 8 heads, fp32 (88 MB) 21.1 us;
+// one of 376 tokens 6.7 us, of which 4.7 are an empty call's.  fp32
 // rows take two terms each, so twice the products.
 // ONCE: a sequence's rows are one tile, so its codes are read once.
 template <int D, bool BF16, int W, bool ONCE>
@@ -787,8 +790,8 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
 // next keys' codes are in flight while this step's products run, and one
 // barrier a step keeps them apart.
 // Bound by instructions: 6 prompts of up to 2500 tokens, 32 heads over 8 of
-// 128, bf16 (163 GFLOP) take 224 us, 728 TFLOP/s; the matrix units are busy
-// 32% of the time, and vector instructions issue in 56% of it, with the two
+// 128, bf16 (163 GFLOP) take 218 us, 749 TFLOP/s; the matrix units are busy
+// 34% of the time, and vector instructions issue in 57% of it, with the two
 // wavefronts a SIMD that the registers allow.  Measured slower, when this form
 // took 259 us: 8 wavefronts with 128 keys an iteration (273), the two 32-key
 // halves a stage apart so that weights and products interleave (266).
