@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 ORDERS = {"after": lambda j, n: j >= (n + 1) // 2, "before": lambda j, n: j < n // 2, "among": lambda j, n: j % 2 == 1}
 
 
-def appended(hip, rng, P, kv, D, lens, small, order, scale=1.0, extra=1 << 24):
+def appended(hip, rng, P, kv, D, lens, small, order, scale=1.0, extra=1 << 26):
     """Sequences of lens tokens appended at once, with values of size `scale`;
     those on the pages that `order` names are `small` times as large."""
     held = [-(-n // P) for n in lens]
