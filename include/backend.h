@@ -248,18 +248,21 @@ typedef struct {
 } BackendKv8Attn;
 /* Floats of work (0: none, work may be NULL) that are enough for this call
  * and for any with the same cache, heads, window and sinks and no more n_rows,
- * max_rows and max_len, whichever type its rows have.  It depends on the sizes alone, not on the pointers. */
+ * max_rows and max_len, whichever type its rows have.  It depends on the sizes
+ * alone, not on the pointers. */
 size_t backend_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a);
 /* Softmax attention of the rows over a layer's pages: o = sum_j p_j v_j,
  * p = softmax_j(scale * q . k_j) over the tokens the row sees.  A row that
  * sees none gets zeros; tokens on a page that is not in the pool are not
  * seen; what a masked token holds, NaN included, has no effect.  Rows of out
  * that belong to no sequence are left as they are.  Scores, softmax and sums
- * are fp32; fp32 rows keep fp32 accuracy relative to the largest value that
+ * are fp32.  fp32 rows keep fp32 accuracy relative to the largest value that
  * the pages of the tokens a row sees can hold (448 of their scales, which are
- * powers of two from 2^-100 to 2^120), whatever other pages hold; bf16 rows enter the products as they are, and their weights
- * rounded to f16 (by at most 2^-11 of themselves), the sum of the weights as
- * fp32 leaves them. */
+ * powers of two from 2^-100 to 2^120), whatever other pages hold.  bf16 rows
+ * enter the products as they are, and their weights rounded to f16: by at most
+ * 2^-11 of themselves, or 2^-30 of the row's largest where they are smaller
+ * than 2^-20 of it (a weight counted with its page's scale).  The sum of the
+ * weights is of what they are in fp32. */
 void backend_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a);
 /* Sequences dst[i] become copies of src[i], all n (<= seqs) at once, from
  * what the cache held before the call (beam search: src = each beam's
