@@ -441,6 +441,7 @@ def _handle(st):
                              frequency=_at(st["frequency"]), presence=_at(st["presence"]), ngram=_at(st["ngram"]))
         if st["bias"] is not None:
             a.bias_start, a.bias_id, a.bias = _at(st["bias_start"]), _at(st["bias_id"]), _at(st["bias"])
+            a.biases = st["bias"].numel()
         if st["mask"] is not None:
             a.mask, a.ld_mask, a.masks, a.mask_of = _at(st["mask"]), st["mask"].shape[1], c["masks"], _at(st["mask_of"])
         st["work"] = torch.zeros(lib.backend_logits_work(C.byref(a)), device="cuda")
