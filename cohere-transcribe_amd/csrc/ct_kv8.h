@@ -40,6 +40,10 @@ size_t ctk_kv8_plan_ints(const BackendKv8 *c);
 size_t ctk_kv8_attn_need(const BackendKv8 *c, const BackendKv8Attn *a);
 size_t ctk_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a);
 void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a, hipStream_t s);
+void ctk_kv8_share(const BackendKv8 *c, int *share, hipStream_t s);
+size_t ctk_kv8_attn_shared_need(const BackendKv8 *c, const BackendKv8Attn *a);
+size_t ctk_kv8_attn_shared_work(const BackendKv8 *c, const BackendKv8Attn *a);
+void ctk_kv8_attn_shared(const BackendKv8 *c, int layer, const BackendKv8Attn *a, const int *share, hipStream_t s);
 
 #ifdef __cplusplus
 }

@@ -9,6 +9,7 @@
 #include "ct_dev.h"
 #include "ct_kv8.h"
 #include "k_kv8.h"
+#include <limits.h>
 
 namespace {
 
@@ -488,6 +489,49 @@ __global__ __launch_bounds__(NT) void trim_kernel(BackendKv8 c, int window, int 
     if (j >= lo && j < hi) give_back(c, s, j);
 }
 
+// Sequences that share their first pages: a group's leader is its lowest
+// sequence; a wavefront a sequence compares its table with the leader's.
+__global__ __launch_bounds__(PNT) void share_kernel(BackendKv8 c, int *share, int lp) {
+    __shared__ int first[CT_KV8_SEQS], lead[CT_KV8_SEQS], tokens[CT_KV8_SEQS], members[CT_KV8_SEQS];
+    const int s = threadIdx.x;
+    if (s < c.seqs) {
+        const int p = c.len[s] > 0 ? c.table[(long)s * c.table_w] : -1;
+        first[s] = (unsigned)p < (unsigned)c.pages ? p : -1;
+        tokens[s] = INT_MAX;
+        members[s] = 0;
+    }
+    __syncthreads();
+    if (s < c.seqs) {
+        int l = s;
+        if (first[s] >= 0)
+            for (l = 0; first[l] != first[s]; l++) {}
+        lead[s] = l;
+        atomicAdd(&members[l], 1);
+    }
+    __syncthreads();
+    const int lane = threadIdx.x % CT_WAVE;
+    for (int q = threadIdx.x / CT_WAVE; q < c.seqs; q += PNT / CT_WAVE) {
+        const int l = lead[q], len = max(c.len[q], 0);
+        const int *mine = c.table + (long)q * c.table_w, *other = c.table + (long)l * c.table_w;
+        const int n = min((int)(((long)len + (1 << lp) - 1) >> lp), c.table_w);    // entries it uses
+        int same = 0;
+        for (; same < n; same += CT_WAVE) {
+            const int j = same + lane;
+            const unsigned long long differ = __ballot(j >= n || mine[j] != other[j]);
+            if (differ) {
+                same += __builtin_ctzll(differ);
+                break;
+            }
+        }
+        if (lane == 0) atomicMin(&tokens[l], (int)min((long)min(same, n) << lp, (long)len));
+    }
+    __syncthreads();
+    if (s < c.seqs) {
+        share[s] = lead[s];
+        share[c.seqs + s] = members[lead[s]] > 1 ? tokens[lead[s]] : 0;
+    }
+}
+
 // Compact, first of two launches: pages in use at m and above (m pages are in
 // use) are paired, in ascending order, with the free ones below m.
 __global__ __launch_bounds__(PNT) void compact_plan_kernel(BackendKv8 c) {
@@ -610,6 +654,10 @@ extern "C" void ctk_kv8_trim(const BackendKv8 *c, int window, int sinks, hipStre
     const int cols = (c->table_w + NT - 1) / NT;
     hipLaunchKernelGGL(trim_kernel, dim3((unsigned)(c->seqs * cols)), dim3(NT), 0, s, *c, window, sinks, cols,
                        log2_of(c->page_tokens));
+}
+
+extern "C" void ctk_kv8_share(const BackendKv8 *c, int *share, hipStream_t s) {
+    hipLaunchKernelGGL(share_kernel, dim3(1), dim3(PNT), 0, s, *c, share, log2_of(c->page_tokens));
 }
 
 extern "C" void ctk_kv8_compact(const BackendKv8 *c, hipStream_t s) {

@@ -1388,3 +1388,12 @@ extern "C" void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Att
     else { if (p->bf16) ATTN(128, true); else ATTN(128, false); }
 #undef ATTN
 }
+
+extern "C" size_t ctk_kv8_attn_shared_need(const BackendKv8 *c, const BackendKv8Attn *a) { return ctk_kv8_attn_need(c, a); }
+
+extern "C" size_t ctk_kv8_attn_shared_work(const BackendKv8 *c, const BackendKv8Attn *a) { return ctk_kv8_attn_work(c, a); }
+
+extern "C" void ctk_kv8_attn_shared(const BackendKv8 *c, int layer, const BackendKv8Attn *a, const int *share, hipStream_t s) {
+    (void)share;                 // every sequence through its own table
+    ctk_kv8_attn(c, layer, a, s);
+}

@@ -136,21 +136,59 @@ size_t backend_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a) {
     return ctk_kv8_attn_work(c, a);
 }
 
-void backend_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a) {
+/* False if there is nothing to do. */
+static int check_call(const BackendKv8 *c, int layer, const BackendKv8Attn *a) {
     check_cache(c);
     check_layer(c, layer);
     check_attn(c, a);
     check_rows(a->rows, a->n_rows);
-    if (a->n_rows == 0) return;
+    if (a->n_rows == 0) return 0;
     const uintptr_t al = a->bf16 ? 1 : 3;
     if (!a->q || !a->out || ((uintptr_t)a->q & al) || ((uintptr_t)a->out & al))
         CT_FATAL("kv8_attn: q or out is NULL or not aligned");
     const long row = (long)a->heads * c->head_dim;
     if (a->ld_q < row || a->ld_out < row) CT_FATAL("kv8_attn: ld_q or ld_out below heads * head_dim");
-    if (ctk_kv8_attn_need(c, a) && (!a->work || ((uintptr_t)a->work & 15)))
+    return 1;
+}
+
+static void check_work(const BackendKv8Attn *a, size_t need) {
+    if (need && (!a->work || ((uintptr_t)a->work & 15)))
         CT_FATAL("kv8_attn: work is NULL or not 16-byte aligned");
+}
+
+void backend_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *a) {
+    if (!check_call(c, layer, a)) return;
+    check_work(a, ctk_kv8_attn_need(c, a));
     require_init();
     ctk_kv8_attn(c, layer, a, ct_t.stream);
+}
+
+void backend_kv8_share(const BackendKv8 *c, int *share) {
+    check_cache(c);
+    if (!share || ((uintptr_t)share & 3)) CT_FATAL("kv8_share: share is NULL or not aligned");
+    require_init();
+    ctk_kv8_share(c, share, ct_t.stream);
+}
+
+static void check_no_window(const BackendKv8Attn *a) {
+    if (a->window > 0) CT_FATAL("kv8_attn_shared: no window");
+}
+
+size_t backend_kv8_attn_shared_work(const BackendKv8 *c, const BackendKv8Attn *a) {
+    check_sizes(c);
+    check_attn(c, a);
+    check_no_window(a);
+    return ctk_kv8_attn_shared_work(c, a);
+}
+
+void backend_kv8_attn_shared(const BackendKv8 *c, int layer, const BackendKv8Attn *a, const int *share) {
+    const int any = check_call(c, layer, a);
+    check_no_window(a);
+    if (!share || ((uintptr_t)share & 3)) CT_FATAL("kv8_attn_shared: share is NULL or not aligned");
+    if (!any) return;
+    check_work(a, ctk_kv8_attn_shared_need(c, a));
+    require_init();
+    ctk_kv8_attn_shared(c, layer, a, share, ct_t.stream);
 }
 
 void backend_kv8_fork(const BackendKv8 *c, const int *dst, const int *src, int n) {

@@ -209,8 +209,20 @@ ABI_EXT_SIGS = {
     "backend_kv8_trim": ([_P, _I, _I], None),
     "backend_kv8_compact": ([_P], None),
     "backend_kv8_status": ([_P], _I),
+    "backend_kv8_share": ([_P, _P], None),
+    "backend_kv8_attn_shared_work": ([_P, _P], _Z),
+    "backend_kv8_attn_shared": ([_P, _I, _P, _P], None),
     "backend_stream": ([], _P),
+    "backend_w4_floats": ([_P], _Z),
+    "backend_w4_bind": ([_P, _P], None),
+    "backend_w4_load": ([_P, _P, _P, _P], None),
+    "backend_w4_quantize": ([_P, _P], None),
+    "backend_w4_unpack": ([_P, _P], None),
+    "backend_linear_w4": ([_P, _P], None),
+    "backend_logits_work": ([_P], _Z),
+    "backend_logits": ([_P], None),
 }
+W4_STORE, W4_SILU, W4_RELU, W4_ADD = 0, 1, 2, 3
 KV8_NO_PAGES, KV8_NO_ROOM, KV8_BAD_ARG = 1, 2, 4
 
 
@@ -225,6 +237,26 @@ class BackendKv8Attn(C.Structure):
     _fields_ = [("out", _P), ("q", _P), ("ld_out", _L), ("ld_q", _L), ("bf16", _I), ("heads", _I), ("scale", _F),
                 ("causal", _I), ("window", _I), ("sinks", _I), ("rows", _P), ("n_rows", _I), ("max_rows", _I),
                 ("max_len", _I), ("work", _P)]
+
+
+class BackendW4(C.Structure):
+    """A weight in 4 bits (include/backend.h); pass C.byref(weight)."""
+    _fields_ = [("in_d", _I), ("out_d", _I), ("group", _I), ("scale_f16", _I), ("codes", _P), ("scales", _P)]
+
+
+class BackendW4Linear(C.Structure):
+    """A product with such a weight; pass C.byref(call)."""
+    _fields_ = [("y", _P), ("x", _P), ("ld_y", _L), ("ld_x", _L), ("bf16", _I), ("rows", _I), ("bias", _P),
+                ("act", _I), ("scale", _F)]
+
+
+class BackendLogits(C.Structure):
+    """Penalties, biases and masks on logits; pass C.byref(call)."""
+    _fields_ = [("logits", _P), ("out", _P), ("ld", _L), ("ld_out", _L), ("rows", _I), ("vocab", _I), ("id", _P),
+                ("score", _P), ("hist", _P), ("ld_hist", _L), ("hist_len", _P), ("prompt_len", _P), ("repeat", _P),
+                ("frequency", _P), ("presence", _P), ("ngram", _P), ("bias_start", _P), ("bias_id", _P),
+                ("bias", _P), ("biases", _I), ("mask", _P), ("ld_mask", _L), ("masks", _I), ("mask_of", _P),
+                ("work", _P)]
 
 
 def bind_abi(lib):

@@ -290,8 +290,133 @@ void backend_kv8_compact(const BackendKv8 *c);
 #define KV8_NO_ROOM  2
 #define KV8_BAD_ARG  4
 int  backend_kv8_status(const BackendKv8 *c);
+/* Attention over sequences whose first tokens lie on the same pages (a clip's
+ * hypotheses, samples of one prompt, requests with one instruction): those are
+ * read once for all of them.
+ *
+ * backend_kv8_share finds them in the tables.  Sequences whose first table
+ * entries are the same page of the pool are a group; its lowest-numbered
+ * sequence leads it.  share[s] becomes s's leader and share[seqs + s] the tokens
+ * that its group has in common: those of the leading table entries that all its
+ * tables have alike, and no more than its shortest sequence holds; 0 where s is
+ * alone.  share is DEVICE memory, 2 * seqs ints. */
+void backend_kv8_share(const BackendKv8 *c, int *share);
+/* backend_kv8_attn where a group's common tokens are read once, through its
+ * leader's table, for the rows of all its sequences; the others as ever.  share
+ * is as backend_kv8_share writes it, or the caller's: share[seqs + l] tokens of
+ * leader l (share[l] == l) lie for all its sequences on the pages that l's table
+ * names, or on copies of them.  Of these as many are taken as every row of the
+ * group sees.  A leader that is out of range or does not lead itself stands for
+ * none.  No window.  Accuracy as of backend_kv8_attn, whose bits it does not
+ * give: they depend on the group.  work is backend_kv8_attn_shared_work floats,
+ * which are enough for smaller calls as backend_kv8_attn_work's are. */
+size_t backend_kv8_attn_shared_work(const BackendKv8 *c, const BackendKv8Attn *a);
+void backend_kv8_attn_shared(const BackendKv8 *c, int layer, const BackendKv8Attn *a, const int *share);
 /* The calling thread's stream (hipStream_t), to order other work with. */
 void *backend_stream(void);
+
+/* ---- Linear maps with 4-bit weights -------------------------------------- *
+ * backend_linear and its kin with weights of 4 bits, a quarter of the bytes a
+ * decode step reads.  No counterpart in the reference.  W[o][i] = scale[o][i /
+ * group] * (code[o][i] - zero[o][i / group]), codes and zeros 0..15.
+ * As for the 8-bit cache, every pointer is DEVICE memory (backend_device_ptr
+ * gives an uploaded tensor's), the calls run on the calling thread's stream,
+ * allocate nothing and can be captured in a graph. */
+typedef struct {
+    int in_d, out_d;     /* 1..2^20 each, in_d * out_d <= 2^31                */
+    int group;           /* inputs that share a scale: 32, 64 or 128          */
+    int scale_f16;       /* scales are f16 (1) or bf16 (0)                    */
+    /* laid out by the calls below, 16-byte aligned */
+    uint32_t *codes, *scales;
+} BackendW4;
+/* Floats both arrays take together. */
+size_t backend_w4_floats(const BackendW4 *w);
+/* Points the arrays into mem (16-byte aligned). */
+void backend_w4_bind(BackendW4 *w, float *mem);
+/* Lays out a weight given as codes, two a byte, the first in the low bits,
+ * [out_d][(in_d + 1) / 2]; scales [out_d][groups] of 16 bits; zeros
+ * [out_d][groups], of which the low 4 bits count, or NULL: 8.  groups = in_d /
+ * group, rounded up. */
+void backend_w4_load(const BackendW4 *w, const uint8_t *codes, const uint16_t *scales, const uint8_t *zeros);
+/* Rounds a bf16 weight [out_d][in_d] of finite values: with lo the least and hi
+ * the largest of a group's values and 0, scale = (hi - lo) / 15 in fp32, rounded
+ * to nearest (at most the type's largest value), zero = -lo / scale and code =
+ * value / scale + zero, each rounded to nearest even and held to 0..15 (scale 0:
+ * zero and codes 0). */
+void backend_w4_quantize(const BackendW4 *w, const uint16_t *W);
+/* The values a laid-out weight stands for, fp32 [out_d][in_d]. */
+void backend_w4_unpack(const BackendW4 *w, float *values);
+#define W4_STORE 0       /* y = W x + b                                       */
+#define W4_SILU  1       /* y = silu(W x + b)                                 */
+#define W4_RELU  2       /* y = max(W x + b, 0)                               */
+#define W4_ADD   3       /* y += scale * (W x + b)                            */
+typedef struct {
+    void *y;             /* [rows][out_d], ld_y values apart                  */
+    const void *x;       /* [rows][in_d], ld_x apart; not y                   */
+    long ld_y, ld_x;
+    int bf16;            /* x and y: 0 fp32, 1 bf16                           */
+    int rows;            /* 0..2^24                                           */
+    const uint16_t *bias;/* bf16 [out_d], or NULL                             */
+    int act;             /* W4_STORE ..                                       */
+    float scale;         /* of W4_ADD                                         */
+} BackendW4Linear;
+/* Products are summed in fp32; of a block of 128 inputs those far smaller than
+ * its largest are rounded at 2^-38 of it (fp32) or 2^-39 (bf16), the others to
+ * 22 bits (fp32) or not at all (bf16).  A row's bits depend neither on the
+ * other rows nor on their number.  A row with an input that is not finite has
+ * outputs that are not finite. */
+void backend_linear_w4(const BackendW4 *w, const BackendW4Linear *a);
+
+/* ---- Penalties, biases and masks on logits ------------------------------- *
+ * What a step does to its logits before a token is taken, and the token.  No
+ * counterpart in the reference (backend_argmax_batch takes logits as they are).
+ * Every pointer is DEVICE memory; NULL leaves a part out.  A row's logits go
+ * through, each result rounded to fp32:
+ *   1. tokens of its history:   l = l > 0 ? l / repeat : l * repeat
+ *   2. tokens of its history from prompt_len on, said n times:
+ *                               l = l - frequency * n, then l = l - presence
+ *   3. biased tokens:           l = l + bias; of entries with one token the
+ *                               last one holds
+ *   4. tokens that would complete a run of `ngram` tokens that the history
+ *      holds already:           l = -infinity (ngram 1: any token said)
+ *   5. tokens whose mask bit is 0: l = -infinity
+ * Token ids outside [0, vocab) in a history or bias list touch nothing. */
+typedef struct {
+    const float *logits; /* [rows][vocab], ld apart                           */
+    float *out;          /* the same after step 5, ld_out apart; may be logits
+                            themselves (with ld_out = ld); NULL: not wanted   */
+    long ld, ld_out;
+    int rows, vocab;     /* 0..65535 rows; 1..2^24                            */
+    int *id;             /* [rows] lowest id of the largest value above
+                            -infinity (a NaN is none); -1 if there is none    */
+    float *score;        /* [rows] that value; -infinity if there is none     */
+    const int *hist;     /* [rows] token ids, ld_hist apart, oldest first     */
+    long ld_hist;        /* at most 2^24                                      */
+    const int *hist_len; /* [rows] tokens of each; held to [0, ld_hist]       */
+    const int *prompt_len;  /* [rows] of them, the first ones are the prompt;
+                               NULL: none                                     */
+    const float *repeat, *frequency, *presence;  /* [rows]                    */
+    const int *ngram;    /* [rows]; below 1: no ban                           */
+    const int *bias_start;  /* [rows + 1]: row r has the entries bias_start[r]
+                               .. bias_start[r + 1] - 1 of the next two; starts
+                               below 0 or past biases: no bias                */
+    const int *bias_id;
+    const float *bias;
+    int biases;          /* entries of bias_id and bias                       */
+    const uint32_t *mask;/* [masks] bit rows, ld_mask words apart: token v is
+                            bit v % 32 of word v / 32                         */
+    long ld_mask;
+    int masks;
+    const int *mask_of;  /* [rows] which mask a row has; below 0: none; masks
+                            and above: all its tokens are masked.  NULL: row
+                            r has mask r                                      */
+    float *work;         /* backend_logits_work floats, zeroed once; a call
+                            leaves it zeroed                                  */
+} BackendLogits;
+/* Floats of work (0: none): enough for this call and any with no more rows and
+ * vocab. */
+size_t backend_logits_work(const BackendLogits *a);
+void backend_logits(const BackendLogits *a);
 
 #ifdef __cplusplus
 }

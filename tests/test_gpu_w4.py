@@ -1,0 +1,205 @@
+"""Linear maps with 4-bit weights on the device against their 64-bit model
+(w4_ref.py) — needs an MI355X."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import ctbind as cb
+import w4_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def weight(hip, rng, in_d, out_d, group, f16=False, zeros=True, floats=1 << 23):
+    mem = ref.Mem(hip, floats)
+    g = -(-in_d // group)
+    codes = rng.integers(0, 16, (out_d, in_d)).astype(np.uint8)
+    s = (np.exp(0.5 * rng.standard_normal((out_d, g))) / np.sqrt(in_d) / 4).astype(np.float32)
+    bits = s.astype(np.float16).view(np.uint16) if f16 else ref.bf16_bits(s)
+    z = rng.integers(0, 16, (out_d, g)).astype(np.uint8) if zeros else None
+    w = ref.Weight(hip, mem, in_d, out_d, group, f16)
+    w.load(codes, bits, z)
+    return w, ref.values(codes, bits, z, group, f16)
+
+
+def inputs(rng, rows, in_d, bf16):
+    x = (rng.standard_normal((rows, in_d)) * np.exp(rng.standard_normal((1, in_d)))).astype(np.float32)
+    return ref.bf16_value(ref.bf16_bits(x)) if bf16 else x
+
+
+def check(got, W, x, bf16, what, **kw):
+    v, size = ref.expected(W, x, **kw)
+    t = ref.tolerance(W, x, v, size, bf16)
+    bad = ~(np.abs(got - v) <= t)
+    assert not bad.any(), (what, float((np.abs(got - v) / t).max()), np.argwhere(bad)[:4])
+
+
+SHAPES = [  # in_d, out_d, group
+    (1024, 1024, 128), (128, 16, 128), (1, 1, 32), (7, 33, 64), (33, 16, 32), (127, 17, 32), (129, 15, 64),
+    (300, 130, 128), (1280, 100, 64), (2047, 65, 32), (4096, 48, 128), (1030, 257, 128)]
+
+
+@pytest.mark.parametrize("in_d,out_d,group", SHAPES)
+@pytest.mark.parametrize("f16,zeros", [(False, True), (True, False), (True, True)])
+def test_load_and_unpack(hip, in_d, out_d, group, f16, zeros):
+    """Every code, scale and zero point comes back as the value it stands for, exactly."""
+    print(f"case: load {in_d} {out_d} {group} f16={f16} zeros={zeros}", flush=True)
+    w, W = weight(hip, np.random.default_rng(in_d), in_d, out_d, group, f16, zeros)
+    assert np.array_equal(w.unpack().astype(np.float64), W)
+
+
+@pytest.mark.parametrize("in_d,out_d,group", SHAPES)
+@pytest.mark.parametrize("f16", [False, True])
+def test_quantize(hip, in_d, out_d, group, f16):
+    """The documented rule, bit for bit; values at the scale types' ends, groups
+    of zeros, of one sign and of one outlier."""
+    print(f"case: quantize {in_d} {out_d} {group} f16={f16}", flush=True)
+    rng = np.random.default_rng(out_d)
+    W = (rng.standard_normal((out_d, in_d)) * np.exp(2 * rng.standard_normal((out_d, 1)))).astype(np.float32)
+    W[0] = 0
+    if out_d > 8:
+        W[1], W[2], W[3], W[4] = np.abs(W[1]), -np.abs(W[2]), W[3] * 1e-30, W[4] * 1e30
+        W[5] = 0
+        W[5, in_d // 2] = 3.0
+        W[6] = 3.3e38 * np.sign(W[6])
+        W[7] *= 1e-6
+    W = ref.bf16_value(ref.bf16_bits(W))
+    mem = ref.Mem(hip, 1 << 23)
+    w = ref.Weight(hip, mem, in_d, out_d, group, f16)
+    hip.backend_w4_quantize(w.h, mem.put(ref.bf16_bits(W)))
+    assert np.array_equal(w.unpack().astype(np.float64), ref.values(*ref.quantize(W, group, f16), group, f16))
+
+
+ROWS = [1, 2, 5, 16, 17, 40, 64, 65, 130, 300]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("in_d,out_d,group", SHAPES)
+def test_linear(hip, in_d, out_d, group, bf16):
+    """Row counts around every tile, with a bias and each activation in turn."""
+    print(f"case: linear {in_d} {out_d} {group} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(in_d + out_d)
+    w, W = weight(hip, rng, in_d, out_d, group, f16=group == 64)
+    first = w.mem.at
+    for i, rows in enumerate(ROWS):
+        w.mem.at = first
+        x, act = inputs(rng, rows, in_d, bf16), i % 4
+        kw = dict(act=act, bias=ref.bf16_value(ref.bf16_bits(rng.standard_normal(out_d).astype(np.float32))) if i % 3 else None)
+        if act == cb.W4_ADD:
+            kw |= dict(scale=0.37, y=inputs(rng, rows, out_d, bf16))
+        got = w.linear(x, bf16=bf16, behind=2, **kw)
+        check(got, W, x, bf16, (rows, act), **kw)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("pad,off", [((0, 0), 1), ((1, 3), 0), ((8, 16), 8), ((3, 1), 5)])
+def test_strided_rows(hip, pad, off, bf16):
+    """Rows apart and off 16 bytes, inputs that end inside a piece of eight."""
+    print(f"case: strided {pad} {off} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(3)
+    for in_d, out_d, rows in ((260, 70, 3), (515, 40, 33), (1024, 64, 150)):
+        w, W = weight(hip, rng, in_d, out_d, 64)
+        x = inputs(rng, rows, in_d, bf16)
+        check(w.linear(x, bf16=bf16, pad=pad, off=off, behind=1), W, x, bf16, (in_d, rows))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_a_rows_bits_are_its_own(hip, bf16):
+    """A row gives the same bits alone, among others, in any place, at every row
+    count and over inputs of any length."""
+    print(f"case: own bits bf16={bf16}", flush=True)
+    rng = np.random.default_rng(8)
+    for in_d, out_d, group in ((1024, 528, 128), (2200, 96, 32), (100, 4096, 64)):
+        w, _ = weight(hip, rng, in_d, out_d, group, floats=1 << 24)
+        x = inputs(rng, 700, in_d, bf16)
+        first = w.mem.at
+        whole = w.linear(x, bf16=bf16)
+        for a, b in ((0, 1), (5, 6), (3, 7), (0, 16), (10, 43), (1, 65), (100, 228), (7, 400)):
+            w.mem.at = first
+            assert np.array_equal(w.linear(x[a:b], bf16=bf16).view(np.uint32), whole[a:b].view(np.uint32)), (in_d, a, b)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 200])
+def test_special_inputs(hip, rows):
+    """Zero rows, tiny and huge ones, blocks of very different sizes beside each
+    other; a row with an infinity or NaN touches no other row."""
+    print(f"case: special inputs rows={rows}", flush=True)
+    rng = np.random.default_rng(9)
+    for bf16 in (False, True):
+        w, W = weight(hip, rng, 640, 80, 64)
+        x = inputs(rng, rows, 640, bf16)
+        q = lambda v: ref.bf16_value(ref.bf16_bits(v.astype(np.float32)))  # noqa: E731
+        x[0, 128:256] = q(x[0, 128:256] * 1e12)
+        x[0, 256:384] = q(x[0, 256:384] * 1e-12)
+        if rows > 8:
+            x[1] = 0
+            x[2] = q(x[2] * 1e-30)
+            x[3] = q(x[3] * 1e-37)
+            x[4] = q(x[4] * 1e34)
+            x[5, 10:] = 0
+            x[6, 3], x[7, 639], x[8, 200] = np.inf, np.nan, -np.inf
+        got = w.linear(x, bf16=bf16)
+        fine = np.isfinite(x).all(1)
+        check(got[fine], W, x[fine], bf16, (rows, bf16))
+        assert not np.isfinite(got[~fine]).any()
+        if rows > 8:
+            assert np.all(got[1] == 0)
+            relu = w.linear(x, bf16=bf16, act=cb.W4_RELU)
+            assert np.isnan(relu[7]).all()
+
+
+def test_large_offsets(hip):
+    """A weight of 2^31 values, the most there may be: its last codes lie past 2^30 bytes."""
+    print("case: large", flush=True)
+    rng = np.random.default_rng(12)
+    in_d, out_d = 1 << 11, 1 << 20
+    mem = ref.Mem(hip, 600_000_000)
+    w = ref.Weight(hip, mem, in_d, out_d, 128, False)
+    part = 1 << 13                            # the rows of W repeat
+    codes = rng.integers(0, 16, (part, in_d)).astype(np.uint8)
+    bits = ref.bf16_bits(np.exp(rng.standard_normal((part, in_d // 128))).astype(np.float32))
+    z = rng.integers(0, 16, (part, in_d // 128)).astype(np.uint8)
+    cp, sp, zp = (mem.put(np.tile(v, (out_d // part, 1))) for v in (ref.pack(codes), bits, z))
+    hip.backend_w4_load(w.h, cp, sp, zp)
+    x = inputs(rng, 2, in_d, False)
+    got = w.linear(x)
+    v, size = ref.expected(ref.values(codes, bits, z, 128, False), x)
+    t = ref.tolerance(ref.values(codes, bits, z, 128, False), x, v, size, False)
+    for k in (0, 1, out_d // part - 1):
+        assert np.all(np.abs(got[:, k * part:(k + 1) * part] - v) <= t)
+    assert np.array_equal(got.reshape(2, -1, part), np.repeat(got[:, None, :part], out_d // part, 1))
+
+
+def test_nothing_to_do_and_captured(hip):
+    """No rows: y stays.  Captured once and replayed, with eager calls between:
+    the same bits, from the inputs of the moment."""
+    print("case: captured", flush=True)
+    rng = np.random.default_rng(13)
+    w, W = weight(hip, rng, 1024, 300, 128)
+    mem = w.mem
+    y = mem.put(np.full((40, 300), 55.0, np.float32))
+    xs = [inputs(rng, 40, 1024, False) for _ in range(3)]
+    xp = mem.put(xs[0])
+    a = cb.BackendW4Linear(y=y, x=xp, ld_y=300, ld_x=1024, rows=0)
+    hip.backend_linear_w4(w.h, C.byref(a))
+    assert np.all(mem.get(y, (40, 300), np.float32) == 55.0)
+    a.rows = 40
+    want = []
+    for x in xs:
+        mem.write(xp, x)
+        hip.backend_linear_w4(w.h, C.byref(a))
+        want.append(mem.get(y, (40, 300), np.float32))
+        check(want[-1], W, x, False, "eager")
+    tag = 1
+    assert hip.backend_graph_replay(tag, 7, 7, 7) == 0
+    hip.backend_graph_begin_capture(tag)
+    hip.backend_linear_w4(w.h, C.byref(a))
+    hip.backend_graph_end_capture(tag, 7, 7, 7)
+    for i in (1, 0, 2, 2, 1):
+        mem.write(xp, xs[i])
+        mem.write(y, np.zeros((40, 300), np.float32))
+        assert hip.backend_graph_replay(tag, 7, 7, 7) == 1
+        assert np.array_equal(mem.get(y, (40, 300), np.float32).view(np.uint32), want[i].view(np.uint32))
+        hip.backend_linear_w4(w.h, C.byref(a))
+        assert np.array_equal(mem.get(y, (40, 300), np.float32).view(np.uint32), want[i].view(np.uint32))
