@@ -28,6 +28,7 @@
 #include "ct_dev.h"
 #include "ct_kv8.h"
 #include "k_kv8.h"
+#include <limits.h>
 #include <type_traits>
 
 namespace {
@@ -61,6 +62,12 @@ struct Args {
     int rpt;                     // rows of a tile kept in the partial results
     float *part;                 // partial O [tile][kv][chunk][rpt][D], then (m, l) pairs
     float2 *stat;
+    // sequences with common tokens; partial results are [item][kv][row of the
+    // item's tile] there, first those of the items of common tokens, tile_rows each
+    const int *share;
+    int most;                    // rows of a sequence
+    int pitems;                  // items of common tokens in the grid
+    int want[2], least[2];       // chunks aimed at, least steps of one
 };
 
 // The kernel's arguments read again, past this point: what only its end
@@ -78,6 +85,7 @@ struct Tile {
     int len, pos0;               // tokens held; position of the sequence's first row
     int end, lo, sink_steps, steps;
     int full_lo, full_hi;        // steps at keys in [full_lo, full_hi) are seen whole by every row
+    int base;                    // keys below it are another tile's (shared launches)
 };
 
 // Inclusive prefix sum over the workgroup's W wavefronts.
@@ -90,6 +98,35 @@ __device__ __forceinline__ int block_sum(int v, int *part, int &total) {
         if (lane >= o) v += u;
     }
     if (lane == CT_WAVE - 1) part[w] = v;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        if (i < w) before += part[i];
+        total += part[i];
+    }
+    __syncthreads();
+    return v + before;
+}
+
+// Inclusive prefix sum over a wavefront, without LDS: shifts by 1, 2, 4 and 8
+// within rows of 16 lanes, then lane 15 into row 1 (and 47 into 3), lane 31 into
+// rows 2 and 3.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+}
+// The same over the workgroup's W wavefronts.
+template <int W>
+__device__ __forceinline__ int group_sum(int v, int *part, int &total) {
+    const int w = threadIdx.x / CT_WAVE;
+    v = wave_scan(v);
+    if (threadIdx.x % CT_WAVE == CT_WAVE - 1) part[w] = v;
     __syncthreads();
     int before = 0;
     total = 0;
@@ -156,6 +193,133 @@ __device__ __forceinline__ bool find_tile(const Args &a, int id, int rows_per_ti
     t.full_lo = a.window ? p1 - a.window + 1 : 0;
     t.full_hi = min(a.causal ? p0 + 1 : t.len, a.cap);
     return true;
+}
+
+// Sequences with common tokens.  A group's are E tokens: those that the caller
+// names, as far as every row of the group sees them (no row masks any of them),
+// if two sequences or more have rows.  All workgroups of the launches work
+// out the same groups and the same chunks: a part's steps (of tiles, over all
+// groups or sequences) are dealt in equal chunks to as many workgroups as are
+// meant for it, since only the device knows how many tokens are common.
+struct Groups {
+    int lead[CT_KV8_SEQS];                                             // as given
+    int least[CT_KV8_SEQS], rows[CT_KV8_SEQS], members[CT_KV8_SEQS];   // by leader
+    int part[8], info[8], steps[2];
+    __device__ __forceinline__ int common(int l) const { return members[l] > 1 ? least[l] : 0; }
+};
+struct Member {                  // thread s: sequence s, and what it leads
+    int r0, n, len, lead, base;  // base: its group's common tokens
+    int tiles[2], steps[2];      // tiles and steps of each: [0] over the common tokens of s's group, [1] over s's own
+    int chunk[2];                // of all
+    __device__ __forceinline__ int each(int part) const { return (steps[part] + chunk[part] - 1) / chunk[part]; }
+};
+
+// Every thread of a workgroup of at least CT_KV8_SEQS calls it.  What it reads
+// is asked for at once: three rounds of loads, as the leaders lead to them, took
+// 1.5 us more.
+__device__ __forceinline__ Member read_groups(const Args &a, Groups &g) {
+    const int s = threadIdx.x;
+    Member m = {0, 0, 0, s, 0, {0, 0}, {0, 0}, {0, 0}};
+    int l = -1;
+    if (s < a.seqs) {
+        m.r0 = a.rows[s];
+        const int end = a.rows[s + 1], len = a.len[s], want = a.share[a.seqs + s];
+        l = a.share[s];
+        m.n = end - m.r0;
+        m.len = max(len, 0);
+        if (m.r0 < 0 || m.n <= 0 || m.n > a.n_rows - m.r0 || m.n > a.most) m.n = 0;
+        g.least[s] = l == s ? max(want, 0) : 0;
+        g.lead[s] = l;
+        g.rows[s] = g.members[s] = 0;
+    }
+    if (s < 2) g.steps[s] = 0;
+    __syncthreads();
+    if ((unsigned)l < (unsigned)a.seqs && g.lead[l] == l) m.lead = l;
+    if (m.n > 0) {
+        const int sees = min(a.causal ? m.len - m.n + 1 : m.len, a.cap);
+        atomicMin(&g.least[m.lead], max(sees, 0));
+        atomicAdd(&g.rows[m.lead], m.n);
+        atomicAdd(&g.members[m.lead], 1);
+    }
+    __syncthreads();
+    if (s < a.seqs) {
+        m.steps[0] = (g.common(s) + 31) >> 5;
+        m.tiles[0] = m.steps[0] ? (g.rows[s] * a.group + a.tile_rows - 1) / a.tile_rows : 0;
+        m.base = g.common(m.lead);
+        m.tiles[1] = (m.n * a.group + 15) >> 4;
+        m.steps[1] = max(min(m.len, a.cap) - (m.base & ~31) + 31, 0) >> 5;
+        if (min(m.len, a.cap) <= m.base) m.tiles[1] = m.steps[1] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int all = wave_scan(m.tiles[i] * m.steps[i]);
+        if ((s & (CT_WAVE - 1)) == CT_WAVE - 1) atomicAdd(&g.steps[i], all);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; i++) m.chunk[i] = max((g.steps[i] + a.want[i] - 1) / a.want[i], a.least[i]);
+    m.chunk[0] += m.chunk[0] & 1;            // the rows kernel takes two steps at a time
+    return m;
+}
+
+// The keys that tile `tile` of a sequence's n rows has to itself: those past base.
+__device__ __forceinline__ void own_keys(const Args &a, int tile, Tile &t) {
+    t.row = tile * 16;
+    t.pos0 = t.len - t.n;
+    const int first = t.row / a.group, last = (min(t.row + 16, t.n * a.group) - 1) / a.group;
+    t.end = max(min(a.causal ? t.pos0 + last + 1 : t.len, a.cap), 0);
+    t.lo = t.base & ~31;
+    t.sink_steps = 0;
+    t.steps = t.end > t.base ? (t.end - t.lo + 31) >> 5 : 0;
+    t.full_lo = t.base;
+    t.full_hi = min(a.causal ? t.pos0 + first + 1 : t.len, a.cap);
+}
+
+// Where the sums of item `id` of the grid begin, of those with 16 rows at most a tile.
+__device__ __forceinline__ long own_at(const Args &a, int id, int h, int rows) {
+    if (id < a.pitems) return ((long)id * a.kv + h) * rows;
+    return (long)a.pitems * a.kv * a.tile_rows + ((long)(id - a.pitems) * a.kv + h) * rows;
+}
+
+// Finds item `id`, a chunk of a tile, of part 0 or 1 (then row[i] becomes the
+// i-th row of a tile of common tokens); returns its chunk, -1 if there is none.
+template <int W>
+__device__ __forceinline__ int find_item(const Args &a, int part, int id, Groups &g, int *row, Tile &t, int &chunk) {
+    const Member m = read_groups(a, g);
+    const int s = threadIdx.x;
+    chunk = part ? m.chunk[1] : m.chunk[0];
+    const int each = part ? m.each(1) : m.each(0), n = (part ? m.tiles[1] : m.tiles[0]) * each;
+    int total;
+    const int upto = group_sum<W>(n, g.part, total);
+    if (id >= total) return -1;
+    if (id >= upto - n && id < upto) {
+        g.info[0] = s; g.info[1] = (id - (upto - n)) / each; g.info[2] = (id - (upto - n)) % each;
+        if (part) {
+            g.info[3] = m.n; g.info[4] = m.len; g.info[5] = m.r0; g.info[6] = m.base;
+        } else {
+            g.info[3] = g.rows[s]; g.info[4] = g.common(s);
+        }
+    }
+    __syncthreads();
+    t.seq = __builtin_amdgcn_readfirstlane(g.info[0]);
+    const int tile = __builtin_amdgcn_readfirstlane(g.info[1]), ch = __builtin_amdgcn_readfirstlane(g.info[2]);
+    t.n = __builtin_amdgcn_readfirstlane(g.info[3]);
+    t.len = __builtin_amdgcn_readfirstlane(g.info[4]);
+    if (part) {
+        t.r0 = __builtin_amdgcn_readfirstlane(g.info[5]);
+        t.base = __builtin_amdgcn_readfirstlane(g.info[6]);
+        own_keys(a, tile, t);
+        return ch;
+    }
+    t.row = tile * a.tile_rows;
+    t.end = t.full_hi = t.len;
+    t.r0 = t.pos0 = t.lo = t.sink_steps = t.full_lo = t.base = 0;
+    t.steps = (t.end + 31) >> 5;
+    const int mine = m.lead == t.seq ? m.n : 0, to = group_sum<W>(mine, g.part, total), from = to - mine;
+    const int first = t.row / a.group, last = (min(t.row + a.tile_rows, t.n * a.group) - 1) / a.group;
+    for (int i = max(from, first); i < min(to, last + 1); i++) row[i - first] = m.r0 + i - from;
+    __syncthreads();
+    return ch;
 }
 
 __device__ __forceinline__ int step_key(const Tile &t, int step) {
@@ -452,6 +616,12 @@ __device__ __forceinline__ float masked(uint32_t m, float s) {
 // first) and [lo, lo + n).
 struct Sight {
     int first, n, lo;
+    // base: keys below it are another tile's
+    __device__ __forceinline__ Sight(const Args &a, int len, int pos, int base) {
+        first = 0;
+        lo = base;
+        n = max(min(a.causal ? pos + 1 : len, a.cap) - base, 0);
+    }
     __device__ __forceinline__ Sight(const Args &a, int len, int pos) {
         const int end = max(min(a.causal ? pos + 1 : len, a.cap), 0);
         lo = a.window ? pos - a.window + 1 : 0;
@@ -497,7 +667,7 @@ __device__ __forceinline__ void operand_v(Code code, f16x8 (&vf)[4]) {
 // reach the rows that see their token, and they alone (0 * NaN is NaN, so a
 // product over a masked one would spread it).  Rare, so it is done after all
 // steps, from the codes read again: in the loop it cost 40 registers.
-template <int D, int NQ>
+template <int D, int NQ, bool SHARED>
 __device__ __forceinline__ void spread_nan(const Args &a, const Tile &t, int h, int key, int c, int g,
                                            const int (&pos)[NQ], f32x4 (&o)[NQ][D / 16]) {
     f16x8 one[NQ];
@@ -514,7 +684,8 @@ __device__ __forceinline__ void spread_nan(const Args &a, const Tile &t, int h, 
             nan[j][x] = in ? nan_bytes(*reinterpret_cast<const uint32_t *>(a.v + base + 4 * x)) : 0;
 #pragma unroll
         for (int n = 0; n < NQ; n++)
-            one[n][j] = in && Sight(a, t.len, pos[n]).sees(a.window, kk) ? (_Float16)1.0f : (_Float16)0.0f;
+            one[n][j] = in && (SHARED ? Sight(a, t.len, pos[n], t.base).sees(true, kk)
+                                      : Sight(a, t.len, pos[n]).sees(a.window, kk)) ? (_Float16)1.0f : (_Float16)0.0f;
     }
 #pragma unroll
     for (int i = 0; i < D / 16; i++) {
@@ -545,33 +716,38 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
 // one of 376 tokens 6.7 us, of which 4.7 are an empty call's.  fp32
 // rows take two terms each, so twice the products.
 // ONCE: a sequence's rows are one tile, so its codes are read once.
-template <int D, bool BF16, int W, bool ONCE>
-__global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a) {
+// SHARED: a workgroup takes either rows of a group over its common tokens (the
+// first pitems items) or a sequence's rows over the others, and leaves its sums.
+template <int D, bool BF16, int W, bool ONCE, bool SHARED>
+__device__ __forceinline__ void attn_body(const Args &a, const int id, const int h, float *so) {
     constexpr int KS = D / 32;            // k steps of the score product
     constexpr int DI = D / 16;            // 16-dim tiles of O; dims of V a lane loads
     constexpr int NB = BF16 ? 1 : 2;      // f16 terms of a query value and of p
-    // the wavefronts' sums [W][rpt][D], maxima and l [W][16]: of the rows a tile
+    // the wavefronts' sums so [W][rpt][D], maxima and l [W][16]: of the rows a tile
     // has, mostly one
-    extern __shared__ float so[];
     __shared__ int sh[W + 5];
     __shared__ float sm[W][16], sl[W][16];
+    __shared__ std::conditional_t<SHARED, Groups, int> gr;
+    __shared__ int grow[SHARED ? 16 : 1];        // rows of a tile of common tokens
 
-    // heads vary fastest: workgroup i runs on XCD i % 8, so with 8 kv heads the
-    // tiles of one head share an L2
-    const int id = blockIdx.x / a.kv, h = blockIdx.x - id * a.kv, ch = blockIdx.y;
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
     // this wavefront's steps: first, first + W, ...; lane i keeps the page and
     // the scales of 16-key half i (-1: not in the pool).  Where a step's keys do
     // not depend on the lengths, its page is read along with them.
-    const int first = ch * a.chunk + w;
-    const bool ahead = a.one_tile && !a.window;
-    int key_i = 32 * (first + W * (lane >> 1)) + 16 * (lane & 1), pg = -1;
-    if (ahead && (lane >> 1) * W < a.chunk && key_i < a.cap) pg = a.table[(long)id * a.table_w + (key_i >> a.lp)];
+    const bool common = SHARED && id < a.pitems;
+    int ch = blockIdx.y, chunk = a.chunk;
     Tile t;
-    if (!find_tile<W>(a, id, 16, sh, t)) return;
-    const int chunks = a.nchunk > 1 ? (t.steps + a.chunk - 1) / a.chunk : 1;
-    if (ch >= max(chunks, 1)) return;
-    const int last = min(t.steps, (ch + 1) * a.chunk);
+    if constexpr (SHARED) ch = find_item<W>(a, !common, common ? id : id - a.pitems, gr, grow, t, chunk);
+    const int first = ch * chunk + w;
+    const bool ahead = !SHARED && a.one_tile && !a.window;
+    int key_i = 32 * (first + W * (lane >> 1)) + 16 * (lane & 1), pg = -1;
+    if (ahead && (lane >> 1) * W < chunk && key_i < a.cap) pg = a.table[(long)id * a.table_w + (key_i >> a.lp)];
+    if constexpr (!SHARED)
+        if (!find_tile<W>(a, id, 16, sh, t)) return;
+    const int chunks = !SHARED && a.nchunk > 1 ? (t.steps + chunk - 1) / chunk : 1;
+    // a tile of own tokens may end before the last of its sequence's chunks
+    if (SHARED ? ch < 0 || ch * chunk >= t.steps : ch >= max(chunks, 1)) return;
+    const int last = min(t.steps, (ch + 1) * chunk);
 
     // this lane's query row: asked for first, used after the keys are asked for
     const int R = t.row + c;
@@ -585,7 +761,8 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
         if (!mine || (unsigned)pg >= (unsigned)a.pages) pg = -1;
     }
     QPiece<BF16> x[KS];
-    fetch_query<D>(a, (long)(t.r0 + qi) * a.ld_q + (long)(h * a.group + qh) * D, g, x);
+    const int qrow = common ? grow[have ? qi - t.row / a.group : 0] : t.r0 + qi;
+    fetch_query<D>(a, (long)qrow * a.ld_q + (long)(h * a.group + qh) * D, g, x);
 
     const int P = 1 << a.lp;
     const unsigned koff = c * D + 16 * g, voff = 4 * g * D + c * DI;
@@ -630,7 +807,7 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
     if (first < last) load(first, 0, ra);
     f16x8 qf[NB][KS];
     const float qs = split_query<D, BF16>(a, have, x, qf);
-    const int pos[1] = {t.pos0 + qi};
+    const int pos[1] = {common ? t.end - 1 : t.pos0 + qi};      // all rows see all common tokens
     const int hard = min(t.len, a.cap);      // tokens at and past it hold anything
 
     f32x4 o[1][DI];
@@ -671,11 +848,11 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
         const bool whole = key >= t.full_lo && key + 32 <= t.full_hi && in[0] && in[1];   // sink steps lie below full_lo
         if (__builtin_expect(!whole, 0)) {
             uint32_t bad = 0;
-            const Sight see(a, t.len, pos[0]);
+            const Sight see = SHARED ? Sight(a, t.len, pos[0], t.base) : Sight(a, t.len, pos[0]);
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int k4 = (in[u] ? key + 16 * u : NO_KEY) + 4 * g;
-                if (a.window) see.mask(true, k4, s[u]);
+                if (SHARED || a.window) see.mask(true, k4, s[u]);
                 else see.mask(false, k4, s[u]);
             }
 #pragma unroll
@@ -741,16 +918,17 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
         use(st + W, i + 1, rb);
     }
     if (__builtin_expect(dirty, 0))
-        for (int st = first; st < last; st += W) spread_nan<D, 1>(a, t, h, step_key(t, st), c, g, pos, o);
+        for (int st = first; st < last; st += W) spread_nan<D, 1, SHARED>(a, t, h, step_key(t, st), c, g, pos, o);
 
     // the wavefronts' sums joined, in their order
+    const int so_rows = SHARED ? 16 : a.rpt;
     l = sum_q(l);
     if (have) {
         if (g == 0) { sm[w][c] = m; sl[w][c] = l; }
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int i = 0; i < DI; i++) so[(w * a.rpt + c) * D + (4 * g + j) * DI + i] = o[0][i][j];
+            for (int i = 0; i < DI; i++) so[(w * so_rows + c) * D + (4 * g + j) * DI + i] = o[0][i][j];
     }
     __syncthreads();
     const int nr = min(16, t.n * a.group - t.row);
@@ -764,10 +942,14 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
 #pragma unroll
         for (int i = 0; i < W; i++) {
             const int by = down(sm[i][r] - Mu);
-            num += __builtin_amdgcn_ldexpf(so[(i * a.rpt + r) * D + d], by);
+            num += __builtin_amdgcn_ldexpf(so[(i * so_rows + r) * D + d], by);
             den += __builtin_amdgcn_ldexpf(sl[i][r], by);
         }
-        if (chunks <= 1) {
+        if constexpr (SHARED) {
+            const long at = own_at(a, id, h, common ? 16 : a.rpt) + r;
+            a.part[at * D + d] = num;
+            if (d == 0) a.stat[at] = make_float2(M, den);
+        } else if (chunks <= 1) {
             const int R2 = t.row + r, i = a.group > 1 ? R2 / a.group : R2;
             const float y = den == 0.0f ? 0.0f : num * ONE_V / den;
             const long off = (long)(t.r0 + i) * a.ld_out + (long)(h * a.group + R2 - i * a.group) * D + d;
@@ -779,6 +961,15 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
             if (d == 0) a.stat[at] = make_float2(M, den);
         }
     }
+}
+
+template <int D, bool BF16, int W, bool ONCE>
+__global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a) {
+    extern __shared__ float so[];
+    // heads vary fastest: workgroup i runs on XCD i % 8, so with 8 kv heads the
+    // tiles of one head share an L2
+    const int id = blockIdx.x / a.kv, h = blockIdx.x - id * a.kv;
+    attn_body<D, BF16, W, ONCE, false>(a, id, h, so);
 }
 
 // Many rows of a sequence: a workgroup holds 128 packed rows, 32 a wavefront
@@ -797,14 +988,16 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
 // halves a stage apart so that weights and products interleave (266).
 constexpr int rows_of(bool bf16) { return bf16 ? 128 : 64; }
 
-template <int D, bool BF16>
-__global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
+// SHARED: the rows are a group's, the keys its common tokens; the sums are left.
+template <int D>
+using Operands = _Float16[2][4][D * 32];         // buffer; K, K, V, V of two 32-key steps
+
+template <int D, bool BF16, bool SHARED>
+__device__ __forceinline__ void rows_body(const Args &a, Operands<D> &lds) {
     constexpr int KS = D / 32, DI = D / 16, NB = BF16 ? 1 : 2;
     constexpr int ROWS = rows_of(BF16), WR = ROWS / NW, NQ = WR / 16;
-    constexpr int UNIT = D * 32;               // halves of a 32-key step's K or V
     static_assert(2 * KS == DI, "K and V take the same number of operands");
     __shared__ int sh[NW + 5];
-    __shared__ __align__(16) _Float16 lds[2][4][UNIT];   // buffer; K, K, V, V of the two steps
     // key scales and value scales' exponents (GONE: not in the pool) of each
     // iteration's four 16-key halves; two batches of 32 iterations in turn
     __shared__ __align__(16) float sscale[2][32][4];
@@ -813,24 +1006,33 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
     __shared__ int spos[ROWS];                 // the rows' positions, for the steps that not all see
     __shared__ int snan;                       // the V of some step holds a NaN
 
-    const int h = blockIdx.x % a.kv, id = gridDim.x / a.kv - 1 - blockIdx.x / a.kv, ch = blockIdx.y;
+    const int h = blockIdx.x % a.kv, id = gridDim.x / a.kv - 1 - blockIdx.x / a.kv;
+    __shared__ std::conditional_t<SHARED, Groups, int> gr;
+    __shared__ int grow[SHARED ? ROWS : 1];
+    int ch = blockIdx.y, chunk = a.chunk;
     Tile t;
-    if (!find_tile<NW>(a, id, ROWS, sh, t)) return;
-    const int chunks = a.nchunk > 1 ? (t.steps + a.chunk - 1) / a.chunk : 1;
-    if (ch >= max(chunks, 1)) return;
+    if constexpr (SHARED) {
+        ch = find_item<NW>(a, 0, blockIdx.x / a.kv, gr, grow, t, chunk);
+        if (ch < 0) return;
+    } else {
+        if (!find_tile<NW>(a, id, ROWS, sh, t)) return;
+    }
+    const int chunks = !SHARED && a.nchunk > 1 ? (t.steps + chunk - 1) / chunk : 1;
+    if (!SHARED && ch >= max(chunks, 1)) return;
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
     const int all = t.n * a.group, hard = min(t.len, a.cap);
 
     const int wr0 = min(t.row + WR * w, all - 1), wr1 = min(t.row + WR * w + WR, all) - 1;
     const bool idle = t.row + WR * w >= all;
     const int p0 = t.pos0 + wr0 / a.group, p1 = t.pos0 + wr1 / a.group;
-    const int full_lo = a.window ? p1 - a.window + 1 : 0, full_hi = min(a.causal ? p0 + 1 : t.len, a.cap);
-    const int wend = idle ? 0 : min(a.causal ? p1 + 1 : t.len, a.cap);
+    const int full_lo = !SHARED && a.window ? p1 - a.window + 1 : 0;
+    const int full_hi = SHARED ? t.full_hi : min(a.causal ? p0 + 1 : t.len, a.cap);
+    const int wend = idle ? 0 : SHARED ? t.end : min(a.causal ? p1 + 1 : t.len, a.cap);
 
     // the unit this wavefront fetches: K (isv 0) or V of step 2 it + kb; lane i
     // keeps the page and place of half i & 1 of the step of iteration base + i / 2
     const int kb = w & 1, isv = w >> 1;
-    const int s0 = ch * a.chunk, s1 = min(t.steps, s0 + a.chunk), iters = (s1 - s0 + 1) >> 1;
+    const int s0 = ch * chunk, s1 = min(t.steps, s0 + chunk), iters = (s1 - s0 + 1) >> 1;
     const int P = 1 << a.lp;
     auto key_of = [&](int it0) {                 // first key of this lane's half
         return step_key(t, min(s0 + 2 * (it0 + (lane >> 1)) + kb, s1 - 1)) + 16 * (lane & 1);
@@ -850,7 +1052,8 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const int R = min(t.row + WR * w + 16 * n + c, all - 1);
-        fetch_query<D>(a, (long)(t.r0 + R / a.group) * a.ld_q + (long)(h * a.group + R % a.group) * D, g, x[n]);
+        const int row = SHARED ? grow[R / a.group - t.row / a.group] : t.r0 + R / a.group;
+        fetch_query<D>(a, (long)row * a.ld_q + (long)(h * a.group + R % a.group) * D, g, x[n]);
     }
     float psc = fetch_scale(pg);
     long at64 = place_of(pg, 0);
@@ -970,7 +1173,7 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
         const int R = t.row + WR * w + 16 * n + c;
         const bool have = R < all;
         qs[n] = split_query<D, BF16>(a, have, x[n], qf[n]);
-        if (g == 0) spos[WR * w + 16 * n + c] = t.pos0 + (have ? R / a.group : 0);
+        if (g == 0) spos[WR * w + 16 * n + c] = SHARED ? t.end - 1 : t.pos0 + (have ? R / a.group : 0);
     }
     };
 
@@ -1043,14 +1246,15 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
             if (__builtin_expect(!whole, 0)) {
 #pragma unroll
                 for (int n = 0; n < NQ; n++) {
-                    const Sight see(a, t.len, spos[WR * w + 16 * n + c]);
+                    const int pos = spos[WR * w + 16 * n + c];
+                    const Sight see = SHARED ? Sight(a, t.len, pos, 0) : Sight(a, t.len, pos);
                     // one form for both kinds of mask: two took fp32 prompts from 120 to 124 us
 #pragma unroll
                     for (int u = 0; u < 4; u++)
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const int kk = (u < 2 ? k0 : k1) + 16 * (u & 1) + 4 * g + j;
-                            s[n][u][j] = ev[u] == GONE ? -INFINITY : masked(see.sees(a.window, kk), s[n][u][j]);
+                            s[n][u][j] = ev[u] == GONE ? -INFINITY : masked(see.sees(SHARED || a.window, kk), s[n][u][j]);
                         }
                 }
             }
@@ -1125,14 +1329,21 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 #pragma unroll
     for (int n = 0; n < NQ; n++) pos[n] = spos[WR * w + 16 * n + c];
     if (__builtin_expect(snan, 0))
-        for (int st = s0; st < s1; st++) spread_nan<D, NQ>(z, t, h, step_key(t, st), c, g, pos, o);
+        for (int st = s0; st < s1; st++) spread_nan<D, NQ, SHARED>(z, t, h, step_key(t, st), c, g, pos, o);
 
 #pragma unroll
     for (int n = 0; n < NQ; n++) {
         const float den = sum_q(l[n]);
         const int r = WR * w + 16 * n + c, R = t.row + r;
         if (R >= all) continue;
-        if (chunks <= 1) {
+        if constexpr (SHARED) {
+            const long at = ((long)(blockIdx.x / z.kv) * z.kv + h) * ROWS + r;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < DI; i++) z.part[at * D + (4 * g + j) * DI + i] = o[n][i][j];
+            if (g == 0) z.stat[at] = make_float2(m[n], den);
+        } else if (chunks <= 1) {
             const float f = den == 0.0f ? 0.0f : 1.0f / den;
             const long off = (long)(t.r0 + R / z.group) * z.ld_out + (long)(h * z.group + R % z.group) * D;
 #pragma unroll
@@ -1152,6 +1363,24 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
             if (g == 0) z.stat[at] = make_float2(m[n], den);
         }
     }
+}
+
+template <int D, bool BF16>
+__global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
+    __shared__ __align__(16) Operands<D> lds;
+    rows_body<D, BF16, false>(a, lds);
+}
+
+// Common and own tokens in one launch: the first pitems items' workgroups wait for
+// the matrix unit, the others for memory.  WIDE: common tokens in tiles of many
+// rows.
+template <int D, bool BF16, bool WIDE>
+__global__ __launch_bounds__(NT, WIDE || !BF16 ? 2 : 3) void shared_kernel(Args a) {
+    constexpr int SUMS = NW * 16 * D * sizeof(float), OPS = sizeof(Operands<D>);
+    __shared__ __align__(16) char mem[WIDE && OPS > SUMS ? OPS : SUMS];
+    const int id = blockIdx.x / a.kv, h = blockIdx.x - id * a.kv;
+    if (WIDE && id < a.pitems) rows_body<D, BF16, true>(a, reinterpret_cast<Operands<D> &>(mem));
+    else attn_body<D, BF16, NW, true, true>(a, id, h, reinterpret_cast<float *>(mem));
 }
 
 // Joins a tile's chunks, in an order that the lengths alone give (32 x 4 heads
@@ -1211,6 +1440,102 @@ __global__ __launch_bounds__(NT) void join_kernel(Args a) {
     if (!have) return;
     const int R = t.row + r;
     const long off = (long)(t.r0 + R / a.group) * a.ld_out + (long)(h * a.group + R % a.group) * D + lane * DL;
+#pragma unroll
+    for (int j = 0; j < DL; j++) {
+        const float y = den == 0.0f ? 0.0f : num[j] * ONE_V / den;
+        if (BF16) reinterpret_cast<uint16_t *>(a.out)[off + j] = f2bf(y);
+        else reinterpret_cast<float *>(a.out)[off + j] = y;
+    }
+}
+
+// Joins the chunks of common tokens and of a sequence's own, a wavefront a packed
+// row of a kv head, in that order.  A kv head's workgroups run on the XCD that
+// wrote its sums.
+template <int D, bool BF16>
+__global__ __launch_bounds__(NT) void join_shared_kernel(Args a) {
+    constexpr int DL = D / CT_WAVE;
+    __shared__ Groups g;
+    __shared__ int sr0[CT_KV8_SEQS], sn[CT_KV8_SEQS], slen[CT_KV8_SEQS], slead[CT_KV8_SEQS], sitem[2][CT_KV8_SEQS];
+    const int h = blockIdx.x % a.kv, s = threadIdx.x;
+    const Member m = read_groups(a, g);
+    static_assert(NT == CT_KV8_SEQS, "a thread a sequence");
+    sr0[s] = m.r0; sn[s] = m.n; slen[s] = m.len; slead[s] = m.lead;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        int total;
+        const int n = m.tiles[i] * m.each(i);
+        sitem[i][s] = group_sum<NW>(n, g.part, total) - n;       // ends with a barrier
+    }
+    __syncthreads();
+    const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE);
+    const long packed = (long)(blockIdx.x / a.kv) * NW + w;
+    const int r = (int)(packed / a.group), gq = (int)(packed % a.group), head = h * a.group + gq;
+    if (r >= a.n_rows) return;
+    int seq = -1;
+#pragma unroll
+    for (int i = 0; i < CT_KV8_SEQS / CT_WAVE; i++) {
+        const int q = i * CT_WAVE + lane;
+        const unsigned long long here = __ballot(sn[q] > 0 && r >= sr0[q] && r - sr0[q] < sn[q]);
+        if (seq < 0 && here) seq = i * CT_WAVE + __builtin_ctzll(here);
+    }
+    if (seq < 0) return;                     // no sequence's row
+    const int lead = __builtin_amdgcn_readfirstlane(slead[seq]);
+    Tile t;
+    t.n = sn[seq]; t.r0 = sr0[seq]; t.len = slen[seq];
+    t.base = g.common(lead);
+    const int row = (r - t.r0) * a.group + gq;
+    own_keys(a, row / 16, t);
+    // the row's place in its group
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < CT_KV8_SEQS / CT_WAVE; i++) {
+        const int q = i * CT_WAVE + lane;
+        before += q < seq && slead[q] == lead ? sn[q] : 0;
+    }
+    before = __builtin_amdgcn_readlane(wave_scan(before), CT_WAVE - 1);
+    const int grow = before * a.group + row;
+    const int first = (((t.base + 31) >> 5) + m.chunk[0] - 1) / m.chunk[0];
+    const int slots = __builtin_amdgcn_readfirstlane(first + (t.steps + m.chunk[1] - 1) / m.chunk[1]);
+    const int each = (max(min(t.len, a.cap) - (t.base & ~31) + 31, 0) / 32 + m.chunk[1] - 1) / m.chunk[1];
+    const long common = ((long)(sitem[0][lead] + grow / a.tile_rows * first) * a.kv + h) * a.tile_rows + grow % a.tile_rows;
+    const long own = own_at(a, a.pitems + sitem[1][seq] + row / 16 * each, h, a.rpt) + row % 16;
+    float M = -INFINITY, num[DL] = {}, den = 0.0f;
+    constexpr int AT = 8;                    // slots in flight
+    for (int k0 = 0; k0 < slots; k0 += AT) {
+        float2 st[AT];
+        float x[AT][DL];
+#pragma unroll
+        for (int u = 0; u < AT; u++) {
+            const int k = k0 + u;
+            st[u] = make_float2(-INFINITY, 0.0f);
+            if (k < slots) {
+                const long at = k < first ? common + (long)k * a.kv * a.tile_rows : own + (long)(k - first) * a.kv * a.rpt;
+                st[u] = a.stat[at];
+#pragma unroll
+                for (int j = 0; j < DL; j++) x[u][j] = a.part[at * D + lane * DL + j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < DL; j++) x[u][j] = 0.0f;
+            }
+        }
+        float mn = M;
+#pragma unroll
+        for (int u = 0; u < AT; u++) mn = fmaxf(mn, st[u].x);
+        const int was = down(M - mn);
+        M = mn;
+        const float Mu = M == -INFINITY ? 0.0f : M;
+        den = __builtin_amdgcn_ldexpf(den, was);
+#pragma unroll
+        for (int j = 0; j < DL; j++) num[j] = __builtin_amdgcn_ldexpf(num[j], was);
+#pragma unroll
+        for (int u = 0; u < AT; u++) {
+            const int by = down(st[u].x - Mu);
+            den += __builtin_amdgcn_ldexpf(st[u].y, by);
+#pragma unroll
+            for (int j = 0; j < DL; j++) num[j] += __builtin_amdgcn_ldexpf(x[u][j], by);
+        }
+    }
+    const long off = (long)r * a.ld_out + (long)head * D + lane * DL;
 #pragma unroll
     for (int j = 0; j < DL; j++) {
         const float y = den == 0.0f ? 0.0f : num[j] * ONE_V / den;
@@ -1341,10 +1666,10 @@ extern "C" size_t ctk_kv8_attn_work(const BackendKv8 *c, const BackendKv8Attn *a
     return f32 > bf16 ? f32 : bf16;
 }
 
-extern "C" void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *p, hipStream_t s) {
-    const Shape sh = shape_of(c, p);
+// The arguments that a launch's shape does not change.
+static Args args_of(const BackendKv8 *c, int layer, const BackendKv8Attn *p) {
     const long heads = (long)layer * c->pages * c->kv_heads;
-    Args a;
+    Args a = {};
     a.lp = 31 - __builtin_clz((unsigned)c->page_tokens);
     a.k = c->k + (heads << a.lp) * c->head_dim;
     a.v = c->v + (heads << a.lp) * c->head_dim;
@@ -1361,6 +1686,12 @@ extern "C" void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Att
     a.cap = (int)(p->max_len > 0 && p->max_len < cap ? p->max_len : cap);
     a.scale2 = p->scale * LOG2E;
     a.vec = ((uintptr_t)p->q & 15) == 0 && p->ld_q % (p->bf16 ? 8 : 4) == 0;
+    return a;
+}
+
+extern "C" void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Attn *p, hipStream_t s) {
+    const Shape sh = shape_of(c, p);
+    Args a = args_of(c, layer, p);
     a.tile_rows = sh.tile_rows; a.one_tile = sh.one_tile; a.chunk = sh.chunk; a.nchunk = sh.nchunk; a.rpt = sh.rpt;
     const size_t n = (size_t)sh.tiles * c->kv_heads * sh.nchunk * sh.rpt;
     a.part = p->work;
@@ -1389,11 +1720,101 @@ extern "C" void ctk_kv8_attn(const BackendKv8 *c, int layer, const BackendKv8Att
 #undef ATTN
 }
 
-extern "C" size_t ctk_kv8_attn_shared_need(const BackendKv8 *c, const BackendKv8Attn *a) { return ctk_kv8_attn_need(c, a); }
+// ---- Sequences with common tokens ----
 
-extern "C" size_t ctk_kv8_attn_shared_work(const BackendKv8 *c, const BackendKv8Attn *a) { return ctk_kv8_attn_work(c, a); }
+namespace {
 
-extern "C" void ctk_kv8_attn_shared(const BackendKv8 *c, int layer, const BackendKv8Attn *a, const int *share, hipStream_t s) {
-    (void)share;                 // every sequence through its own table
-    ctk_kv8_attn(c, layer, a, s);
+constexpr int ITEMS = 512, WIDE_ITEMS = 128;     // items aimed at
+constexpr double APART_BYTES = 192.0 * (1 << 20);
+constexpr int OWN_ROWS = 64;     // packed rows of a sequence up to which common tokens are taken apart
+
+struct SharedShape {
+    int apart;                   // 0: every sequence through its own table
+    int wide;                    // common tokens by the rows kernel
+    int tile_rows, rpt, one_tile, want[2], least[2], items[2];
+};
+
+SharedShape shared_shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
+    SharedShape s = {};
+    const int group = a->heads / c->kv_heads, kv = c->kv_heads;
+    const long each = (long)(a->max_rows < a->n_rows ? a->max_rows : a->n_rows) * group;
+    const long all = (long)a->n_rows * group, steps = walk_of(c, a, 16);
+    // Two launches and what finding the groups takes are 13 us at least, and codes
+    // that several sequences read come from the caches: every sequence by itself
+    // up to 192 MB of codes in all (120 sequences of up to 376 tokens, 92 MB:
+    // 17.4 us against 19.0; 64 of 1100, 144 MB: 18.6, 22.1; 240 of up to 376,
+    // 184 MB: 28.9, 27.2; 64 of 2200, four heads a group, 288 MB: 31.2, 28.6;
+    // 64 of 9000, 1.2 GB: 116, 43.5).
+    const double codes = (double)(c->seqs < a->n_rows ? c->seqs : a->n_rows) * steps * 32 * kv * 2 * c->head_dim;
+    s.apart = each <= OWN_ROWS && c->seqs > 1 && codes > APART_BYTES;
+    if (!s.apart) return s;
+    s.wide = all > 64;
+    s.tile_rows = s.wide ? rows_of(a->bf16) : 16;
+    s.one_tile = each <= 16;
+    s.want[0] = ((s.wide ? WIDE_ITEMS : ITEMS) + kv - 1) / kv;
+    s.want[1] = (ITEMS + kv - 1) / kv;
+    s.least[0] = s.wide ? 16 : 8;
+    s.least[1] = 8;
+    // chunks of equal steps: those aimed at, and one a tile for rounding up
+    s.items[0] = s.want[0] + (int)(all / s.tile_rows) + c->seqs / 2;
+    s.items[1] = s.want[1] + (int)(all / 16) + c->seqs;
+    s.rpt = each < 16 ? (int)each : 16;
+    return s;
+}
+
+// Rows of partial results.
+size_t rows_apart(const BackendKv8 *c, const SharedShape &s) {
+    return ((size_t)s.items[0] * s.tile_rows + (size_t)s.items[1] * s.rpt) * c->kv_heads;
+}
+
+}  // namespace
+
+extern "C" size_t ctk_kv8_attn_shared_need(const BackendKv8 *c, const BackendKv8Attn *a) {
+    const SharedShape s = shared_shape_of(c, a);
+    if (!s.apart) return ctk_kv8_attn_need(c, a);
+    return rows_apart(c, s) * (c->head_dim + 2);
+}
+
+// Whatever a smaller call's shape: more rows or heads make no part of any smaller.
+extern "C" size_t ctk_kv8_attn_shared_work(const BackendKv8 *c, const BackendKv8Attn *a) {
+    size_t most = ctk_kv8_attn_work(c, a);
+    const long kv = c->kv_heads, all = (long)a->n_rows * (a->heads / kv);
+    const int rows[3] = {16, rows_of(false), rows_of(true)};
+    for (int i = 0; i < 3; i++) {
+        SharedShape s = {};
+        s.tile_rows = rows[i];
+        s.rpt = 16;
+        s.items[0] = (int)(((i ? WIDE_ITEMS : ITEMS) + kv - 1) / kv + all / rows[i] + c->seqs / 2);
+        s.items[1] = (int)((ITEMS + kv - 1) / kv + all / 16 + c->seqs);
+        const size_t n = rows_apart(c, s) * (c->head_dim + 2);
+        most = n > most ? n : most;
+    }
+    return most;
+}
+
+extern "C" void ctk_kv8_attn_shared(const BackendKv8 *c, int layer, const BackendKv8Attn *p, const int *share, hipStream_t s) {
+    const SharedShape sh = shared_shape_of(c, p);
+    if (!sh.apart) {
+        ctk_kv8_attn(c, layer, p, s);
+        return;
+    }
+    Args a = args_of(c, layer, p);
+    a.share = share;
+    a.most = p->max_rows < p->n_rows ? p->max_rows : p->n_rows;
+    a.tile_rows = sh.tile_rows; a.one_tile = sh.one_tile; a.rpt = sh.rpt;
+    for (int i = 0; i < 2; i++) { a.want[i] = sh.want[i]; a.least[i] = sh.least[i]; }
+    a.pitems = sh.items[0];
+    a.part = p->work;
+    a.stat = reinterpret_cast<float2 *>(p->work + rows_apart(c, sh) * c->head_dim);
+    const dim3 grid((unsigned)(c->kv_heads * (sh.items[0] + sh.items[1])));
+    const dim3 join((unsigned)(c->kv_heads * (((long)p->n_rows * a.group + NW - 1) / NW)));
+#define SHARED(D, B)                                                                              \
+    do {                                                                                          \
+        if (sh.wide) hipLaunchKernelGGL((shared_kernel<D, B, true>), grid, dim3(NT), 0, s, a);    \
+        else hipLaunchKernelGGL((shared_kernel<D, B, false>), grid, dim3(NT), 0, s, a);           \
+        hipLaunchKernelGGL((join_shared_kernel<D, B>), join, dim3(NT), 0, s, a);                  \
+    } while (0)
+    if (c->head_dim == 64) { if (p->bf16) SHARED(64, true); else SHARED(64, false); }
+    else { if (p->bf16) SHARED(128, true); else SHARED(128, false); }
+#undef SHARED
 }

@@ -16,14 +16,28 @@ from test_gpu_kv8 import check_rows, starts, values
 pytestmark = pytest.mark.gpu
 
 
-def family(hip, rng, P, kv, D, groups, layers=1, extra=1 << 24, junk=True):
+def entries(P, kv, D, seqs):
+    """Table entries with which a call without max_len could read so many codes
+    that common tokens are taken apart (the launch goes by the sizes alone)."""
+    return int(1.05 * 192 * 2 ** 20 / (seqs * kv * 2 * D * P)) + 2
+
+
+def is_apart(d, a):
+    for name in ("ctk_kv8_attn_shared_need", "ctk_kv8_attn_need"):
+        f = getattr(d.hip, name)
+        f.argtypes, f.restype = [C.c_void_p, C.c_void_p], C.c_size_t
+    return d.hip.ctk_kv8_attn_shared_need(d.h, C.byref(a)) != d.hip.ctk_kv8_attn_need(d.h, C.byref(a))
+
+
+def family(hip, rng, P, kv, D, groups, layers=1, extra=1 << 25, junk=True, rows=0):
     """A cache of `groups`, each (common tokens, [a sequence's tokens in all]),
     whose sequences take turns; the pages of the common tokens are shared, the
     last one of them too where no sequence goes on past it.  What is behind the
-    last tokens is NaN codes and large values."""
+    last tokens is NaN codes and large values.  rows: those of a call, if fewer
+    than the sequences."""
     turn = [(g, i) for i in range(max(len(m) for _, m in groups)) for g, (_, m) in enumerate(groups) if i < len(m)]
     lens = [groups[g][1][i] for g, i in turn]
-    width = max(max(-(-n // P) for n in lens), 1) + 1
+    width = max(max(-(-n // P) for n in lens) + 1, entries(P, kv, D, min(len(lens), rows or len(lens))))
     common = [(c // P if any(n > c for n in m) else -(-c // P)) for c, m in groups]
     used = sum(common) + sum(max(0, -(-n // P) - common[g]) for n, (g, _) in zip(lens, turn))
     d = ref.Dev(hip, layers, used + 3, P, kv, D, len(lens), width, extra)
@@ -81,8 +95,8 @@ def found(d):
     return p, want
 
 
-def attend(d, layer, q, heads, share, rows, causal=True, bf16=False, pad=0, off=0, max_rows=None, max_len=0, scale=None, spare=0):
-    n, D = q.shape[0], q.shape[2]
+def attend(d, layer, q, heads, share, rows, causal=True, bf16=False, pad=0, off=0, max_rows=None, max_len=0, scale=None, apart=True):
+    n, D, at = q.shape[0], q.shape[2], d.at
     ld, size = heads * D + pad, 2 if bf16 else 4
     flat = np.full(off + n * ld + 8, 77.0, np.float32)
     flat[off:off + n * ld].reshape(n, ld)[:, :heads * D] = q.reshape(n, -1)
@@ -91,6 +105,7 @@ def attend(d, layer, q, heads, share, rows, causal=True, bf16=False, pad=0, off=
     a = cb.BackendKv8Attn(out=op + off * size, q=qp + off * size, ld_out=ld, ld_q=ld, bf16=int(bf16), heads=heads,
                           scale=scale or D ** -0.5, causal=int(causal), rows=d.ints(rows), n_rows=n,
                           max_rows=max_rows or max(1, int(np.diff(rows).max())), max_len=max_len)
+    assert apart is None or is_apart(d, a) == apart
     w = d.hip.backend_kv8_attn_shared_work(d.h, C.byref(a))
     work = d.put(np.full(w + 64, np.nan, np.float32))
     a.work = work
@@ -98,21 +113,28 @@ def attend(d, layer, q, heads, share, rows, causal=True, bf16=False, pad=0, off=
     got = d.get(op, flat.shape, np.uint16 if bf16 else np.float32)
     got = ref.bf16_value(got) if bf16 else got
     assert np.isnan(d.get(work + 4 * w, (64,), np.float32)).all(), "past the work"
+    d.at = at
     body = got[off:off + n * ld].reshape(n, ld)
     assert np.all(got[:off] == 55.0) and np.all(got[off + n * ld:] == 55.0) and np.all(body[:, heads * D:] == 55.0)
     return body[:, :heads * D].reshape(n, heads, D).copy()
 
 
-def run(hip, rng, P, kv, group, D, groups, n, what, layer=0, layers=1, causal=True, bf16=False, behind=0, share=None, **kw):
-    d, lens, of = family(hip, rng, P, kv, D, groups, layers)
+def run(hip, rng, P, kv, group, D, groups, n, what, layer=0, layers=1, causal=True, bf16=False, behind=0, share=None, apart=True,
+        **kw):
+    total = sum(len(m) for _, m in groups)
+    rows = total if isinstance(n, int) else sum(min(x, y) for x, y in zip(n, [max(m) for _, m in groups for _ in m]))
+    d, lens, of = family(hip, rng, P, kv, D, groups, layers, rows=rows)
     n = [n] * len(lens) if isinstance(n, int) else n
     n = [min(x, y) for x, y in zip(n, lens)]
     rows = starts(n)
     q = values(rng, int(rows[-1]) + behind, kv * group, D)
     p = found(d)[0] if share is None else d.ints(share(d, lens, of))
-    got = attend(d, layer, q, kv * group, p, rows, causal, bf16, **kw)
     want = d.model.attend(layer, q, kv * group, kw.get("scale") or D ** -0.5, causal, 0, 0, rows, len(q), kw.get("max_len"))
+    got = attend(d, layer, q, kv * group, p, rows, causal, bf16, apart=apart, **kw)
     check_rows(got, *want, bf16, what)
+    if "max_len" not in kw:                   # and where so few tokens are not taken apart
+        got = attend(d, layer, q, kv * group, p, rows, causal, bf16, apart=None, max_len=max(lens), **kw)
+        check_rows(got, *want, bf16, (what, "short"))
     return d, q, got
 
 
@@ -147,8 +169,11 @@ def test_several_rows(hip, P, kv, group, D, bf16):
     print(f"case: shared rows P={P} kv={kv} group={group} D={D} bf16={bf16}", flush=True)
     rng = np.random.default_rng(P + kv + group + 2)
     run(hip, rng, P, kv, group, D, [(256, [300, 290, 270, 330]), (384, [450, 400, 390]), (0, [20, 40])],
-        [7, 3, 1, 4, 0, 40, 2, 6, 9], "rows", bf16=bf16, behind=3)
-    run(hip, rng, P, kv, group, D, [(256, [300, 290, 270])], [40, 30, 14], "pieces", bf16=bf16)
+        [7, 3, 1, 4, 0, 40, 2, 6, 9], "rows", bf16=bf16, behind=3, apart=group == 1)
+    few = 64 // group                         # rows of a sequence that still count as few
+    run(hip, rng, P, kv, group, D, [(256, [300, 290, 270, 330]), (384, [450, 400, 390]), (0, [20, 40])],
+        [min(few, x) for x in (7, 3, 1, 4, 0, 40, 2, 6, 9)], "fewer rows", bf16=bf16, behind=3)
+    run(hip, rng, P, kv, group, D, [(256, [300, 290, 270])], [40, 30, 14], "pieces", bf16=bf16, apart=group == 1)
 
 
 @pytest.mark.parametrize("bf16", [False, True])
@@ -157,7 +182,7 @@ def test_many_sequences(hip, P, kv, group, D, bf16):
     """A group whose rows fill many tiles, over a text that is split."""
     print(f"case: shared, many P={P} kv={kv} group={group} D={D} bf16={bf16}", flush=True)
     rng = np.random.default_rng(P + 3)
-    run(hip, rng, P, kv, group, D, [(1500, [1501 + 7 * i for i in range(61)]), (640, [700] * 3)], 1, "many", bf16=bf16, max_len=2000)
+    run(hip, rng, P, kv, group, D, [(1500, [1501 + 7 * i for i in range(37)]), (640, [700] * 3)], 1, "many", bf16=bf16)
     run(hip, rng, P, kv, group, D, [(1024, [1024 + 5 + i % 9 for i in range(40)])], [1 + i % 5 for i in range(40)], "drafts", bf16=bf16)
 
 
@@ -172,12 +197,21 @@ def test_all_sequences_of_a_cache(hip, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
-@pytest.mark.parametrize("kw", [dict(max_len=200), dict(max_len=33), dict(pad=3, off=5), dict(pad=8, off=8), dict(scale=3.0)])
+@pytest.mark.parametrize("kw", [dict(max_len=200, apart=False), dict(max_len=33, apart=False), dict(pad=3, off=5), dict(pad=8, off=8),
+                                dict(scale=3.0), dict(max_len=10 ** 9)])
 def test_options(hip, kw, bf16):
     print(f"case: shared {kw} bf16={bf16}", flush=True)
     rng = np.random.default_rng(5)
     for causal in (True, False):
         run(hip, rng, 32, 2, 2, 64, [(256, [300, 290, 270, 260]), (96, [100, 130])], 1, "options", causal=causal, bf16=bf16, **kw)
+
+
+@pytest.mark.parametrize("bf16,common,causal", [(False, 1100, True), (True, 700, False)])
+def test_tokens_past_max_len(hip, bf16, common, causal):
+    """Sequences that hold more than max_len tokens: the common ones pass it, or the others."""
+    print(f"case: shared, max_len bf16={bf16}", flush=True)
+    run(hip, np.random.default_rng(11), 32, 8, 1, 128, [(common, [1101 + i % 7 for i in range(112)])], 1, common, causal=causal,
+        bf16=bf16, max_len=970)
 
 
 @pytest.mark.parametrize("bf16", [False, True])
@@ -203,7 +237,8 @@ def test_a_callers_own_groups(hip, bf16):
     for lead in ({1: -1}, {2: 7}, {2: 2 ** 31 - 1}, {2: 3}, {0: 1, 1: 0}, {0: -2 ** 31}):
         run(hip, rng, 16, 2, 4, 64, groups, 1, lead, bf16=bf16, share=given(150, lead))
     # rows inside the common tokens: they see a part of them
-    run(hip, rng, 32, 2, 2, 64, [(256, [256] * 5)], [1, 30, 2, 100, 256], "rows within", bf16=bf16)
+    run(hip, rng, 32, 2, 2, 64, [(256, [256] * 5)], [1, 30, 2, 32, 31], "rows within", bf16=bf16)
+    run(hip, rng, 32, 2, 2, 64, [(256, [256] * 5)], [1, 30, 2, 100, 256], "rows within", bf16=bf16, apart=False)
     run(hip, rng, 32, 2, 2, 64, [(256, [256] * 5)], 1, "last tokens", bf16=bf16)
 
 
@@ -313,10 +348,11 @@ def test_the_same_call_gives_the_same_bits(hip, bf16):
     qs = [values(rng, n, 8, 64) for _ in range(2)]
     put = lambda x: ref.bf16_bits(x) if bf16 else x.astype(np.float32)  # noqa: E731
     qp, op, rows = d.put(put(qs[0])), d.put(put(qs[0])), d.ints(starts([1] * n))
-    big = cb.BackendKv8Attn(heads=8, scale=0.125, causal=1, n_rows=200, max_rows=9, max_len=1500)
+    big = cb.BackendKv8Attn(heads=8, scale=0.125, causal=1, n_rows=200, max_rows=9)
     work = d.put(np.full(hip.backend_kv8_attn_shared_work(d.h, C.byref(big)) + 64, np.nan, np.float32))
     a = cb.BackendKv8Attn(out=op, q=qp, ld_out=512, ld_q=512, bf16=int(bf16), heads=8, scale=0.125, causal=1, rows=rows,
-                          n_rows=n, max_rows=1, max_len=1300, work=work)
+                          n_rows=n, max_rows=1, work=work)
+    assert is_apart(d, a)
 
     def result():
         return d.get(op, qs[0].shape, np.uint16 if bf16 else np.uint32)
