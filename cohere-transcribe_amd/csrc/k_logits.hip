@@ -1,20 +1,26 @@
 // k_logits.hip — penalties for tokens that were said, biases, n-gram bans and
 // grammar masks on a step's logits, and the largest logit that is left.
 //
-// A workgroup holds CHUNK tokens of one row: it reads the row's history and bias
-// list once, leaves in LDS for each of its tokens how often it was said, whether
-// it is banned and which bias it has (whole numbers, so the order of the atomics
-// changes nothing), and then passes over its logits once: 4 bytes read and, where
-// wanted, 4 written.  The row's workgroups meet in one 64-bit maximum of (value,
-// lowest id) in memory; the last of them writes the token and leaves the
-// memory as it was.
+// A thread holds 16 of a row's logits, a workgroup 16 x NT of them, asked for
+// before anything else.  Meanwhile the workgroup goes through the row's history
+// and counts in LDS how often each of its tokens was said and whether it is
+// banned (whole numbers, so the order of the atomics changes nothing); then
+// through the bias list, which leaves each token's last entry in the same
+// word.  4 bytes a logit are read and, where wanted, 4 written: bound by memory
+// where there are many, else by the chain history, LDS, largest.  A row's
+// workgroups meet in one 64-bit maximum of (value, lowest id) in memory; the
+// last of them writes the token and leaves the memory as it was.
 #include "ct_dev.h"
 #include "ct_w4.h"
+#include <limits.h>
 
 namespace {
 
-constexpr int CHUNK = 4096, NT = 256;
-constexpr uint32_t SEEN = 1u << 30, BAN = 1u << 31;     // above the counts: a history holds at most 2^24
+constexpr int EACH = 16;                                 // logits of a thread
+constexpr int SMALL = 256, LARGE = 512;                 // threads of a workgroup
+// a token's word: a count in the low bits (a history holds at most 2^24), or
+// ENTRY and the number of its last bias entry
+constexpr uint32_t BAN = 1u << 29, SEEN = 1u << 30, ENTRY = 1u << 31;
 
 struct Row {                     // of work: zero between calls
     unsigned long long best;     // order_key(value) << 32 | ~id; 0: none
@@ -35,117 +41,238 @@ __device__ __forceinline__ float sub_rn(float a, float b) {
     return a - b;
 }
 
-__global__ __launch_bounds__(NT) void logits_kernel(BackendLogits a) {
-    __shared__ uint32_t state[CHUNK];
-    __shared__ int entry[CHUNK];             // the token's last bias entry, from 1
-    __shared__ unsigned long long part[NT / CT_WAVE];
-    const int r = blockIdx.y, v0 = blockIdx.x * CHUNK, n = min(CHUNK, a.vocab - v0);
-    const int tid = threadIdx.x;
+// four floats that need not lie on 16 bytes
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-    const int len = a.hist ? (int)min((long)max(a.hist_len[r], 0), a.ld_hist) : 0;
+__device__ __forceinline__ float max_dpp(float v) {      // over a wavefront, in lane 63
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x111, 0xF, 0xF, false)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x112, 0xF, 0xF, false)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x114, 0xF, 0xF, false)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x118, 0xF, 0xF, false)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x142, 0xA, 0xF, false)));
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x143, 0xC, 0xF, false)));
+}
+__device__ __forceinline__ int min_dpp(int v) {
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x111, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x112, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x114, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x118, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));
+    return min(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xC, 0xF, false));
+}
+// The largest of a wavefront's values and the lowest place of it, for all lanes.
+__device__ __forceinline__ void wave_best(float &v, int &at) {
+    const float top = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(max_dpp(v)), CT_WAVE - 1));
+    at = __builtin_amdgcn_readlane(min_dpp(v == top ? at : INT_MAX), CT_WAVE - 1);
+    v = top;
+}
+
+template <int NT>
+__global__ __launch_bounds__(NT, 6) void logits_kernel(BackendLogits a) {
+    constexpr int CHUNK = EACH * NT, STEP = 4 * NT;
+    __shared__ __align__(16) uint32_t state[CHUNK];
+    __shared__ float stop[NT / CT_WAVE];
+    __shared__ int splace[NT / CT_WAVE], slast;
+    const int r = blockIdx.y, v0 = blockIdx.x * CHUNK, n = min(CHUNK, a.vocab - v0), tid = threadIdx.x;
+
+    // asked for first: the logits and the first of the history
+    const float *x = a.logits + (long)r * a.ld + v0;
+    float l[EACH];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int i = j * STEP + 4 * tid;
+        f32x4u y = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (i + 4 <= n) {
+            y = *reinterpret_cast<const f32x4u *>(x + i);
+        } else {
+            if (i < n) y[0] = x[i];
+            if (i + 1 < n) y[1] = x[i + 1];
+            if (i + 2 < n) y[2] = x[i + 2];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) l[4 * j + e] = y[e];
+    }
+    const int *h = a.hist ? a.hist + (long)r * a.ld_hist : nullptr;
+    int said[4], prev[4];                    // the token at i and the one before it
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        const int i = u * NT + tid;
+        said[u] = h && i < a.ld_hist ? h[i] : -1;
+        prev[u] = a.ngram && i > 0 && i - 1 < a.ld_hist ? h[i - 1] : -1;
+    }
+
+    const int len = h ? (int)min((long)max(a.hist_len[r], 0), a.ld_hist) : 0;
     int b0 = 0, b1 = 0;
     if (a.bias_start) {
         b0 = a.bias_start[r];
         b1 = a.bias_start[r + 1];
         if (b0 < 0 || b1 > a.biases) b1 = b0;
     }
-    const bool listed = len > 0 || b1 > b0;
-    if (listed) {
-        for (int i = tid; i < CHUNK; i += NT) {
-            state[i] = 0;
-            entry[i] = 0;
-        }
-        __syncthreads();
-        const int *h = a.hist + (long)r * a.ld_hist;
-        const int from = a.prompt_len ? a.prompt_len[r] : 0;
-        for (int i = tid; i < len; i += NT) {
-            const unsigned t = (unsigned)h[i] - (unsigned)v0;
-            if (t < (unsigned)n) {
-                if (i >= from) atomicAdd(&state[t], 1u);
-                else atomicOr(&state[t], SEEN);
-            }
-        }
-        const int k = a.ngram ? a.ngram[r] : 0;
-        if (k >= 1 && k <= len) {
-            const int *end = h + len - (k - 1);
-            for (int i = tid; i <= len - k; i += NT) {
-                const unsigned t = (unsigned)h[i + k - 1] - (unsigned)v0;
-                if (t >= (unsigned)n) continue;
-                int j = 0;
-                while (j < k - 1 && h[i + j] == end[j]) j++;
-                if (j == k - 1) atomicOr(&state[t], BAN);
-            }
-        }
-        for (int i = b0 + tid; i < b1; i += NT) {
-            const unsigned t = (unsigned)a.bias_id[i] - (unsigned)v0;
-            if (t < (unsigned)n) atomicMax(&entry[t], i - b0 + 1);
-        }
-        __syncthreads();
+    const int from = a.prompt_len ? a.prompt_len[r] : 0, k = a.ngram ? a.ngram[r] : 0;
+    // the first of the bias list; its values are near when they are looked up
+    int biased = -1;
+    if (b0 + tid < b1) {
+        biased = a.bias_id[b0 + tid];
+        __builtin_prefetch(a.bias + b0 + tid);
     }
-
     const float repeat = a.repeat ? a.repeat[r] : 1.0f, frequency = a.frequency ? a.frequency[r] : 0.0f,
                 presence = a.presence ? a.presence[r] : 0.0f;
     const int which = !a.mask ? -1 : a.mask_of ? a.mask_of[r] : r;
-    const uint32_t *mask = which >= 0 && which < a.masks ? a.mask + (long)which * a.ld_mask : nullptr;
-    const bool none = which >= a.masks && a.mask;           // a mask that is not there allows nothing
-    const float *x = a.logits + (long)r * a.ld + v0;
-    float *y = a.out ? a.out + (long)r * a.ld_out + v0 : nullptr;
+    uint32_t allowed[4];                     // bits 0..3: this thread's tokens of group j
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int v = v0 + j * STEP + 4 * tid;
+        allowed[j] = 15;
+        if (which >= a.masks && a.mask) allowed[j] = 0;      // a mask that is not there allows nothing
+        else if (which >= 0 && v < a.vocab) allowed[j] = a.mask[(long)which * a.ld_mask + (v >> 5)] >> (v & 31) & 15;
+    }
 
-    float top = -INFINITY;
-    int at = 0;
-    for (int i = tid; i < n; i += NT) {
-        float l = x[i];
-        if (listed) {
-            const uint32_t st = state[i];
-            if (st) {
-                const uint32_t said = st & (SEEN - 1);
-                if (a.repeat && (st & ~BAN)) l = l > 0.0f ? l / repeat : mul_rn(l, repeat);
-                if (said) {
-                    if (a.frequency) l = sub_rn(l, mul_rn(frequency, (float)said));
-                    if (a.presence) l = sub_rn(l, presence);
+    if (len > 0 || b1 > b0) {
+        u32x4 *mine = reinterpret_cast<u32x4 *>(state) + tid;
+#pragma unroll
+        for (int j = 0; j < 4; j++) mine[j * NT] = (u32x4){0, 0, 0, 0};
+        if (len <= 4 * NT) {
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (u * NT + tid == len - 1) slast = said[u];
+        } else if (tid == 0) {
+            slast = h[len - 1];
+        }
+        __syncthreads();
+    }
+    uint32_t banned = 0;                     // a bit for each of the 16
+    if (len > 0) {
+        for (int i0 = 0;;) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int i = i0 + u * NT + tid;
+                const unsigned t = (unsigned)said[u] - (unsigned)v0;
+                if (i < len && t < (unsigned)n) {
+                    if (i >= from) atomicAdd(&state[t], 1u);
+                    else atomicOr(&state[t], SEEN);
                 }
             }
-            if (entry[i]) l += a.bias[b0 + entry[i] - 1];
-            if (st & BAN) l = -INFINITY;
+            // the token at i is banned if the k - 1 before it are the last ones
+            if (k >= 1 && k <= len) {
+                const int last = slast;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int i = i0 + u * NT + tid;
+                    const unsigned t = (unsigned)said[u] - (unsigned)v0;
+                    if (i >= k - 1 && i < len && t < (unsigned)n) {
+                        bool same = k == 1 || prev[u] == last;
+                        for (int j = 2; same && j < k; j++) same = h[i - j] == h[len - j];
+                        if (same) atomicOr(&state[t], BAN);
+                    }
+                }
+            }
+            i0 += 4 * NT;
+            if (i0 >= len) break;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int i = i0 + u * NT + tid;
+                said[u] = i < len ? h[i] : -1;
+                prev[u] = a.ngram && i - 1 < len ? h[i - 1] : -1;
+            }
         }
-        if (none || (mask && !(mask[(v0 + i) >> 5] >> ((v0 + i) & 31) & 1))) l = -INFINITY;
-        if (y) y[i] = l;
-        if (l > top) { top = l; at = i; }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const u32x4 st = reinterpret_cast<const u32x4 *>(state)[j * NT + tid];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t w = st[e], times = w & (BAN - 1);
+                banned |= (w & BAN ? 1u : 0u) << (4 * j + e);
+                if (w) {
+                    float y = l[4 * j + e];
+                    if (a.repeat && (w & ~BAN)) y = y > 0.0f ? y / repeat : mul_rn(y, repeat);
+                    const float less = a.frequency ? sub_rn(y, mul_rn(frequency, (float)times)) : y;
+                    l[4 * j + e] = times ? (a.presence ? sub_rn(less, presence) : less) : y;
+                }
+            }
+        }
+    }
+    if (b1 > b0) {
+        // over the counts, which all have read
+        __syncthreads();
+        for (int i = b0 + tid; i < b1; i += NT) {
+            const unsigned t = (unsigned)biased - (unsigned)v0;
+            if (t < (unsigned)n) atomicMax(&state[t], ENTRY | (uint32_t)(i - b0));
+            if (i + NT < b1) biased = a.bias_id[i + NT];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const u32x4 st = reinterpret_cast<const u32x4 *>(state)[j * NT + tid];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (st[e] & ENTRY) l[4 * j + e] += a.bias[b0 + (int)(st[e] & ~ENTRY)];
+        }
+    }
+
+    float top = -INFINITY;
+    int at = INT_MAX;
+    float *y = a.out ? a.out + (long)r * a.ld_out + v0 : nullptr;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int i = j * STEP + 4 * tid;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float &z = l[4 * j + e];
+            z = (banned >> (4 * j + e) & 1) || !(allowed[j] >> e & 1) ? -INFINITY : z;
+            at = z > top ? v0 + i + e : at;
+            top = z > top ? z : top;
+        }
+        if (y && i + 4 <= n) {
+            *reinterpret_cast<f32x4u *>(y + i) = (f32x4u){l[4 * j], l[4 * j + 1], l[4 * j + 2], l[4 * j + 3]};
+        } else if (y) {
+            if (i < n) y[i] = l[4 * j];
+            if (i + 1 < n) y[i + 1] = l[4 * j + 1];
+            if (i + 2 < n) y[i + 2] = l[4 * j + 2];
+        }
     }
     if (!a.id && !a.score) return;
 
-    // + 0: a negative zero counts as zero
-    unsigned long long best = top == -INFINITY ? 0 : (unsigned long long)order_key(top + 0.0f) << 32 | (uint32_t)~(v0 + at);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor(best, o, CT_WAVE);
-        best = other > best ? other : best;
-    }
-    if ((tid & (CT_WAVE - 1)) == 0) part[tid / CT_WAVE] = best;
+    wave_best(top, at);
+    if ((tid & (CT_WAVE - 1)) == 0) { stop[tid / CT_WAVE] = top; splace[tid / CT_WAVE] = at; }
     __syncthreads();
+    if (tid >= CT_WAVE) return;
+    top = tid < NT / CT_WAVE ? stop[tid] : -INFINITY;
+    at = tid < NT / CT_WAVE ? splace[tid] : INT_MAX;
+    wave_best(top, at);
     if (tid) return;
-#pragma unroll
-    for (int i = 1; i < NT / CT_WAVE; i++) best = part[i] > best ? part[i] : best;
     if (gridDim.x > 1) {
+        // + 0: a negative zero counts as zero
+        unsigned long long best = top == -INFINITY ? 0 : (unsigned long long)order_key(top + 0.0f) << 32 | (uint32_t)~at;
         Row *row = reinterpret_cast<Row *>(a.work) + r;
+        // Only these words pass between workgroups, and device-wide atomics meet in
+        // one place, so the maximum has to be done before the count and nothing
+        // else has to be visible: a wait.  A fence writes the XCD's whole L2 back,
+        // once a workgroup (200 x 100003 logits: 142 us with it).
         if (best) atomicMax(&row->best, best);
-        __threadfence();
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (atomicAdd(&row->done, 1u) != gridDim.x - 1) return;
-        __threadfence();
         best = atomicExch(&row->best, 0ull);
         atomicExch(&row->done, 0u);
+        top = best ? from_key((uint32_t)(best >> 32)) : -INFINITY;
+        at = (int)~(uint32_t)best;
     }
-    if (a.id) a.id[r] = best ? (int)~(uint32_t)best : -1;
-    if (a.score) a.score[r] = best ? from_key((uint32_t)(best >> 32)) : -INFINITY;
+    if (a.id) a.id[r] = top == -INFINITY ? -1 : at;
+    if (a.score) a.score[r] = top;
 }
+
+int threads_of(const BackendLogits *a) { return a->vocab > EACH * SMALL ? LARGE : SMALL; }
 
 }  // namespace
 
 extern "C" size_t ctk_logits_work(const BackendLogits *a) {
-    return a->vocab > CHUNK ? (size_t)a->rows * (sizeof(Row) / sizeof(float)) : 0;
+    return a->vocab > EACH * LARGE ? (size_t)a->rows * (sizeof(Row) / sizeof(float)) : 0;
 }
 
 extern "C" void ctk_logits(const BackendLogits *a, hipStream_t s) {
-    const dim3 grid((unsigned)((a->vocab + CHUNK - 1) / CHUNK), (unsigned)a->rows);
-    hipLaunchKernelGGL(logits_kernel, grid, dim3(NT), 0, s, *a);
+    const int nt = threads_of(a);
+    const dim3 grid((unsigned)((a->vocab + EACH * nt - 1) / (EACH * nt)), (unsigned)a->rows);
+    if (nt == SMALL) hipLaunchKernelGGL((logits_kernel<SMALL>), grid, dim3(SMALL), 0, s, *a);
+    else hipLaunchKernelGGL((logits_kernel<LARGE>), grid, dim3(LARGE), 0, s, *a);
 }

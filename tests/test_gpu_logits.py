@@ -185,6 +185,38 @@ def test_many_rows(hip):
     run(hip, x, "rows", **everything(rng, 700, 4500, 90, 5, 700))
 
 
+def test_rows_of_many_workgroups(hip):
+    """Rows of several workgroups' tokens, many at once and again and again over
+    one work: each gives its own largest, wherever it lies."""
+    print("case: many workgroups", flush=True)
+    rng = np.random.default_rng(10)
+    rows, vocab = 150, 70000
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    mem = Mem(hip, 1 << 25)
+    c = Call(hip, mem, x, out=False)
+    for i in range(20):
+        at = rng.integers(0, vocab, rows)
+        x[np.arange(rows), at] = 10 + i
+        mem.write(c.x, x)
+        for _ in range(3):
+            c.launch()
+        c.check((None, at.astype(np.int32), np.full(rows, 10 + i, np.float32)), i)
+
+
+@pytest.mark.parametrize("hist", [4095, 4096, 4097, 9000])
+def test_long_histories(hip, hist):
+    """Histories around what a workgroup's threads hold at once, and past it; n-grams over the edges."""
+    print(f"case: history {hist}", flush=True)
+    rng = np.random.default_rng(hist)
+    for vocab in (30, 3000, 20000):
+        x = (3 * rng.standard_normal((4, vocab))).astype(np.float32)
+        h = rng.integers(0, min(vocab, 40), (4, hist))
+        h[1, 1020:1030] = h[1, hist - 10:]
+        h[2, 4090:4100] = h[2, hist - 10:][:len(h[2, 4090:4100])]
+        run(hip, x, vocab, hist=h, hist_len=np.array([hist, hist, hist, hist - 1]), ngram=np.array([2, 8, 6, 3]),
+            prompt_len=np.array([0, 1024, 4096, 5]), frequency=np.full(4, 0.01, np.float32))
+
+
 def test_captured_and_replayed(hip):
     """Replays of a captured call give what an eager one gives, with the inputs
     of the moment; a call without rows leaves all as it is."""
