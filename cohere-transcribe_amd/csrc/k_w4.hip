@@ -30,30 +30,29 @@ constexpr int SEGS = 8;          // runs of tiles that a row's inputs are summed
 struct Args {
     const uint32_t *codes, *scales;
     int in_d, out_d, itiles, otiles, per;    // per: tiles of a segment
-    int scale_f16;
+    uint32_t scale_f16;
     void *y;
     const void *x;
     long ld_y, ld_x;
-    int rows, act, vec;
+    int rows, act;
     float scale;
     const uint16_t *bias;
 };
 
-__device__ __forceinline__ float scale_of(uint32_t word, int f16) {
-    if (f16) return (float)__builtin_bit_cast(f16x2, word)[1];
-    return __uint_as_float(word & 0xffff0000u);
+// f16: all ones for f16 scales, 0 for bf16.  A choice, not a branch: branches
+// among the products took twice the registers.
+__device__ __forceinline__ float scale_of(uint32_t word, uint32_t f16) {
+    const uint32_t h = __float_as_uint((float)__builtin_bit_cast(f16x2, word)[1]);
+    return __uint_as_float((h & f16) | (word & 0xffff0000u & ~f16));
 }
 
 // Eight codes less their zero point (both halves of `less`: -(1024 + z)).
 __device__ __forceinline__ f16x8 weights8(uint32_t q, f16x2 less) {
-    f16x8 w;
+    u32x4 w;                     // whole registers: halves set one by one took twice as many
 #pragma unroll
-    for (int p = 0; p < 4; p++) {
-        const f16x2 c = __builtin_bit_cast(f16x2, (q >> (4 * p) & 0x000f000fu) | 0x64006400u) + less;
-        w[2 * p] = c[0];
-        w[2 * p + 1] = c[1];
-    }
-    return w;
+    for (int p = 0; p < 4; p++)
+        w[p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, (q >> (4 * p) & 0x000f000fu) | 0x64006400u) + less);
+    return __builtin_bit_cast(f16x8, w);
 }
 
 __device__ __forceinline__ f16x2 less_of(uint32_t word) {
@@ -76,30 +75,59 @@ __device__ __forceinline__ uint32_t max16(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xF, 0xF, false));
 }
 
-// Values k .. k + 7 of row t; zeros past in_d.
+// pieces of a row, which need not lie on 16 bytes
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+
+// Input k of row t.
 template <bool BF16>
-__device__ __forceinline__ void fetch8(const Args &a, long t, int k, float (&v)[8]) {
+__device__ __forceinline__ const char *input_at(const Args &a, long t, int k) {
+    return reinterpret_cast<const char *>(a.x) + (t * a.ld_x + k) * (BF16 ? 2 : 4);
+}
+
+typedef float f32a __attribute__((may_alias));
+typedef uint16_t u16a __attribute__((may_alias));
+
+// Eight inputs from p on, of a tile that ends before in_d.
+template <bool BF16>
+__device__ __forceinline__ void fetch8(const char *x, float (&v)[8]) {
     if constexpr (BF16) {
-        const uint16_t *p = reinterpret_cast<const uint16_t *>(a.x) + t * a.ld_x + k;
-        if (a.vec && k + 8 <= a.in_d) {
-            const u16x8 u = *reinterpret_cast<const u16x8 *>(p);
+        const u16x8u u = *reinterpret_cast<const u16x8u *>(x);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = bf2f(u[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = k + i < a.in_d ? bf2f(p[i]) : 0.0f;
-        }
+        for (int i = 0; i < 8; i++) v[i] = bf2f(u[i]);
     } else {
-        const float *p = reinterpret_cast<const float *>(a.x) + t * a.ld_x + k;
-        if (a.vec && k + 8 <= a.in_d) {
-            const f32x4 u = *reinterpret_cast<const f32x4 *>(p), w = *reinterpret_cast<const f32x4 *>(p + 4);
+        const float *p = reinterpret_cast<const float *>(x);
+        const f32x4u u = *reinterpret_cast<const f32x4u *>(p), w = *reinterpret_cast<const f32x4u *>(p + 4);
 #pragma unroll
-            for (int i = 0; i < 4; i++) { v[i] = u[i]; v[4 + i] = w[i]; }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = k + i < a.in_d ? p[i] : 0.0f;
-        }
+        for (int i = 0; i < 4; i++) { v[i] = u[i]; v[4 + i] = w[i]; }
     }
+}
+
+// The same of a row's last tile, zeros after the first `n`: one by one through the
+// LDS pieces that the split values go to, so that it takes few registers.
+template <bool BF16>
+__device__ __forceinline__ void fetch_last8(const char *x, int n, f16x8 *hi, f16x8 *lo, float (&v)[8]) {
+    if constexpr (BF16) {
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(x);
+        u16a *h = reinterpret_cast<u16a *>(hi);
+#pragma unroll 1
+        for (int i = 0; i < 8; i++) h[i] = i < n ? p[i] : 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = bf2f(h[i]);
+    } else {
+        const float *p = reinterpret_cast<const float *>(x);
+        f32a *h = reinterpret_cast<f32a *>(hi), *l = reinterpret_cast<f32a *>(lo);
+#pragma unroll 1
+        for (int i = 0; i < 4; i++) {
+            h[i] = i < n ? p[i] : 0.0f;
+            l[i] = 4 + i < n ? p[4 + i] : 0.0f;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[i] = h[i]; v[4 + i] = l[i]; }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // A row's 128 inputs, eight in each of its 16 lanes, as f16 terms; returns the
@@ -112,31 +140,32 @@ __device__ __forceinline__ float split8(const float (&v)[8], f16x8 (&h)[NB]) {
     // exponent of the largest, at least 15 - 127 so that the factor is in range
     const int e = max((int)(max16(top) >> 23), 15);
     const float up = __uint_as_float((uint32_t)(127 + 14 - (e - 127)) << 23);
+    u32x4 t[NB];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const float a = v[i] * up, b = v[i + 1] * up;
-        f16x2 hi, lo;
+    for (int i = 0; i < 4; i++) {
+        const float a = v[2 * i] * up, b = v[2 * i + 1] * up;
+        f16x2 hi, lo = {0, 0};
         if (NB > 1) two_terms(a, b, hi, lo);
         else hi = __builtin_convertvector((f32x2){a, b}, f16x2);
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-            h[0][i + n] = hi[n];
-            if (NB > 1) h[NB - 1][i + n] = lo[n];
-        }
+        t[0][i] = __builtin_bit_cast(uint32_t, hi);
+        if (NB > 1) t[NB - 1][i] = __builtin_bit_cast(uint32_t, lo);
     }
+#pragma unroll
+    for (int n = 0; n < NB; n++) h[n] = __builtin_bit_cast(f16x8, t[n]);
     return __uint_as_float((uint32_t)(127 - 14 + (e - 127)) << 23);
 }
 
-// Where a row's eight inputs 8 k8 .. + 7 lie among a tile's 256 pieces of 16
-// bytes: piece k8 * 16 + row, rows changed so that neither the stores of a row
-// nor the loads of a product meet in a bank.
-__device__ __forceinline__ int piece(int k8, int row) { return k8 * 16 + (row ^ k8); }
+// Where a row's eight inputs 8 k8 .. + 7 lie among a tile's pieces of 16 bytes:
+// piece k8 * RR + row, rows changed so that neither the stores of a row nor the
+// loads of a product meet in a bank.
+template <int RR>
+__device__ __forceinline__ int piece(int k8, int row) { return k8 * RR + ((row ^ k8) & (RR - 1)); }
 
 // One tile of 16 outputs times 16 rows: the groups' products into the rows' sums.
 // A operand x (row = lane % 16), B operand the weights (output = lane % 16);
 // lane (o, q) gets rows 4 q + i of output o.
 template <int NB, int GS>
-__device__ __forceinline__ void tile_product(const u32x4 &code, const uint32_t (&word)[4 / GS], int scale_f16,
+__device__ __forceinline__ void tile_product(const u32x4 &code, const uint32_t (&word)[4 / GS], uint32_t scale_f16,
                                              const f16x8 (&xf)[NB][4], const f32x4 &undo, f32x4 &sum) {
 #pragma unroll
     for (int g = 0; g < 4 / GS; g++) {
@@ -152,12 +181,6 @@ __device__ __forceinline__ void tile_product(const u32x4 &code, const uint32_t (
 #pragma unroll
         for (int i = 0; i < 4; i++) sum[i] = __builtin_fmaf(mul_rn(acc[i], s), undo[i], sum[i]);
     }
-}
-
-template <int GS>
-__device__ __forceinline__ void fetch_words(const uint32_t *p, uint32_t (&word)[4 / GS]) {
-#pragma unroll
-    for (int g = 0; g < 4 / GS; g++) word[g] = p[g];
 }
 
 template <bool BF16>
@@ -176,42 +199,59 @@ __device__ __forceinline__ void finish(const Args &a, long t, int o, float v) {
     }
 }
 
-// NT tiles of outputs a workgroup, 16 rows at a time; its eight wavefronts each
-// take one segment of the inputs and join their sums in LDS, in order.
-template <bool BF16, int GS, int NT>
-__global__ __launch_bounds__(SEGS * CT_WAVE) void linear_kernel(Args a) {
-    constexpr int NB = BF16 ? 1 : 2;
+// Few rows of many inputs: NT tiles of outputs a workgroup, RR rows at a time; its
+// eight wavefronts each take one segment of the inputs and join their sums in
+// LDS, in order.  A wavefront has AHEAD tiles of codes and inputs in flight.
+template <bool BF16, int GS, int NT, int RR>
+__global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
+    constexpr int NB = BF16 ? 1 : 2, RI = RR / 4, AHEAD = RR == 4 ? 4 : 2;
     __shared__ __align__(16) union {
-        f16x8 x[SEGS][NB][256];
+        f16x8 x[SEGS][NB][16 * RR];
         float sum[SEGS][NT][16][TO];
     } sh;
-    __shared__ __align__(16) float sundo[SEGS][16];
+    __shared__ __align__(16) float sundo[SEGS][RR];
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE);
     const int c = lane & 15, q = lane >> 4;
     const int ot0 = blockIdx.x * NT;
     const int k0 = w * a.per, k1 = min(k0 + a.per, a.itiles);
-    for (long r0 = 16L * blockIdx.y; r0 < a.rows; r0 += 16L * gridDim.y) {
-        const int nr = (int)min(16L, a.rows - r0);
+    struct Ahead {
+        u32x4 code[NT];
+        uint32_t word[NT][4 / GS];
+        float v[RI][8];
+    };
+    for (long r0 = (long)RR * blockIdx.y; r0 < a.rows; r0 += (long)RR * gridDim.y) {
+        const int nr = (int)min((long)RR, a.rows - r0);
         f32x4 sum[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) sum[n] = (f32x4){0, 0, 0, 0};
-        for (int kt = k0; kt < k1; kt++) {
-            u32x4 code[NT];
-            uint32_t word[NT][4 / GS];
+        Ahead t[AHEAD];
+        auto fetch = [&](int kt, Ahead &f) __attribute__((always_inline)) {
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const long tile = (long)min(ot0 + n, a.otiles - 1) * a.itiles + kt;
-                code[n] = reinterpret_cast<const u32x4 *>(a.codes)[tile * CT_WAVE + lane];
-                fetch_words<GS>(a.scales + (tile * 16 + c) * (4 / GS), word[n]);
-            }
-            for (int r = q; r < nr; r += 4) {
-                float v[8];
-                f16x8 h[NB];
-                fetch8<BF16>(a, r0 + r, kt * TI + 8 * c, v);
-                const float undo = split8<NB>(v, h);
+                f.code[n] = reinterpret_cast<const u32x4 *>(a.codes)[tile * CT_WAVE + lane];
 #pragma unroll
-                for (int n = 0; n < NB; n++) sh.x[w][n][piece(c, r)] = h[n];
-                if (c == 0) sundo[w][r] = undo;
+                for (int g = 0; g < 4 / GS; g++) f.word[n][g] = a.scales[(tile * 16 + c) * (4 / GS) + g];
+            }
+            if (kt * TI + TI <= a.in_d)
+#pragma unroll
+                for (int i = 0; i < RI; i++)
+                    if (q + 4 * i < nr) fetch8<BF16>(input_at<BF16>(a, r0 + q + 4 * i, kt * TI + 8 * c), f.v[i]);
+        };
+        auto use = [&](int kt, Ahead &f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < RI; i++) {
+                const int r = q + 4 * i;
+                if (r < nr) {
+                    f16x8 h[NB];
+                    if (kt * TI + TI > a.in_d)
+                        fetch_last8<BF16>(input_at<BF16>(a, r0 + r, kt * TI + 8 * c), a.in_d - kt * TI - 8 * c, &sh.x[w][0][piece<RR>(c, r)],
+                                          &sh.x[w][NB - 1][piece<RR>(c, r)], f.v[i]);
+                    const float undo = split8<NB>(f.v[i], h);
+#pragma unroll
+                    for (int n = 0; n < NB; n++) sh.x[w][n][piece<RR>(c, r)] = h[n];
+                    if (c == 0) sundo[w][r] = undo;
+                }
             }
             // the wavefront's own part of LDS: its accesses are in order
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -220,30 +260,305 @@ __global__ __launch_bounds__(SEGS * CT_WAVE) void linear_kernel(Args a) {
 #pragma unroll
             for (int n = 0; n < NB; n++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) xf[n][j] = sh.x[w][n][piece(4 * j + q, c)];
-            const f32x4 undo = *reinterpret_cast<const f32x4 *>(&sundo[w][4 * q]);
+                for (int j = 0; j < 4; j++) xf[n][j] = sh.x[w][n][piece<RR>(4 * j + q, c)];
+            const f32x4 undo = *reinterpret_cast<const f32x4 *>(&sundo[w][RR == 4 ? 0 : 4 * q]);
 #pragma unroll
-            for (int n = 0; n < NT; n++) tile_product<NB, GS>(code[n], word[n], a.scale_f16, xf, undo, sum[n]);
+            for (int n = 0; n < NT; n++) tile_product<NB, GS>(f.code[n], f.word[n], a.scale_f16, xf, undo, sum[n]);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (k0 + i < k1) fetch(k0 + i, t[i]);
+        for (int kt = k0; kt < k1; kt += AHEAD)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                if (kt + i < k1) {
+                    use(kt + i, t[i]);
+                    if (kt + i + AHEAD < k1) fetch(kt + i + AHEAD, t[i]);
+                }
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) sh.sum[w][n][4 * q + i][c] = sum[n][i];
+            for (int i = 0; i < 4; i++)
+                if (RR == 16 || q == 0) sh.sum[w][n][4 * q + i][c] = sum[n][i];
         __syncthreads();
-        for (int i = threadIdx.x; i < NT * 256; i += SEGS * CT_WAVE) {
-            const int n = i >> 8, r = i >> 4 & 15, o = (ot0 + n) * TO + (i & 15);
+        for (int i = threadIdx.x; i < NT * RR * 16; i += SEGS * CT_WAVE) {
+            const int n = i / (RR * 16), r = i >> 4 & (RR - 1), o = (ot0 + n) * TO + (i & 15);
             if (r < nr && o < a.out_d) {
-                float v = sh.sum[0][n][r][i & 15];
+                float v = 0.0f;
 #pragma unroll
-                for (int s = 1; s < SEGS; s++) v += sh.sum[s][n][r][i & 15];
+                for (int s = 0; s < SEGS; s++) v += sh.sum[s][n][r][i & 15];
                 finish<BF16>(a, r0 + r, o, v);
             }
         }
         __syncthreads();
     }
+}
+
+// Few rows whose inputs fit LDS: a workgroup splits all of them once, RR rows (a
+// power of two up to 16), and then goes from outputs to outputs, NT tiles at a
+// time; its eight wavefronts each take one segment of the inputs and join
+// their sums in LDS, in order.  A wavefront has AHEAD tiles of codes in flight,
+// those of the next outputs among them, from before the inputs are split.
+constexpr int FEW_LDS = 136 << 10;           // of inputs, beside 16 KB of sums, within a CU's 160
+
+template <bool BF16, int GS, int NT>
+__global__ __launch_bounds__(SEGS * CT_WAVE, 4) void linear_few_kernel(Args a, int lr, int groups) {
+    constexpr int NB = BF16 ? 1 : 2, AHEAD = 4 / NT;
+    extern __shared__ __align__(16) f16x8 sx[];          // [NB][itiles][16][RR], then undo [itiles][RR]
+    __shared__ float ssum[2][SEGS][NT][16][TO];
+    const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE);
+    const int c = lane & 15, q = lane >> 4, RR = 1 << lr;
+    const int k0 = w * a.per, mine = max(min(a.per, a.itiles - k0), 0);
+    const int pieces = (a.itiles * 16) << lr;
+    float *sundo = reinterpret_cast<float *>(sx + NB * pieces);
+    const long r0 = (long)RR * blockIdx.y;
+    const int nr = (int)min((long)RR, a.rows - r0);
+
+    u32x4 code[AHEAD][NT];
+    uint32_t word[AHEAD][NT][4 / GS];
+    auto fetch = [&](int grp, int t, u32x4 (&cd)[NT], uint32_t (&wd)[NT][4 / GS]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const long tile = (long)min(grp * NT + n, a.otiles - 1) * a.itiles + k0 + t;
+            cd[n] = reinterpret_cast<const u32x4 *>(a.codes)[tile * CT_WAVE + lane];
+#pragma unroll
+            for (int g = 0; g < 4 / GS; g++) wd[n][g] = a.scales[(tile * 16 + c) * (4 / GS) + g];
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+        if (i < mine) fetch(blockIdx.x, i, code[i], word[i]);
+
+    // 16 lanes a row's tile
+    auto at = [&](int kt, int k8, int row) { return ((kt * 16 + k8) << lr) + ((row ^ k8) & (RR - 1)); };
+    for (int i = threadIdx.x >> 4; i < a.itiles * nr; i += SEGS * CT_WAVE / 16) {
+        const int kt = nr == 1 ? i : i / nr, row = i - kt * nr;
+        f16x8 h[NB];
+        float v[8];
+        f16x8 *hi = &sx[at(kt, c, row)], *lo = &sx[(NB - 1) * pieces + at(kt, c, row)];
+        const char *x = input_at<BF16>(a, r0 + row, kt * TI + 8 * c);
+        if (kt * TI + TI <= a.in_d) fetch8<BF16>(x, v);
+        else fetch_last8<BF16>(x, a.in_d - kt * TI - 8 * c, hi, lo, v);
+        const float undo = split8<NB>(v, h);
+        *hi = h[0];
+        if (NB > 1) *lo = h[NB - 1];
+        if (c == 0) sundo[(kt << lr) + row] = undo;
+    }
+    __syncthreads();
+
+    const int row = c & (RR - 1);
+    int px[4];                               // this lane's pieces of a tile
+#pragma unroll
+    for (int j = 0; j < 4; j++) px[j] = at(k0, 4 * j + q, row);
+    for (int grp = blockIdx.x, turn = 0; grp < groups; grp += gridDim.x, turn ^= 1) {
+        f32x4 sum[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) sum[n] = (f32x4){0, 0, 0, 0};
+        for (int t = 0; t < mine; t += AHEAD)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                if (t + i >= mine) break;
+                f16x8 xf[NB][4];
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) xf[n][j] = sx[n * pieces + px[j] + ((t + i) << (4 + lr))];
+                // rows 4 q + i of the products; past RR they repeat and are not used
+                f32x4 undo;
+                const float *u = sundo + ((k0 + t + i) << lr);
+                if (lr < 2) undo = (f32x4){u[0], u[RR - 1], u[0], u[0]};
+                else undo = *reinterpret_cast<const f32x4 *>(u + (4 * q & (RR - 1)));
+#pragma unroll
+                for (int n = 0; n < NT; n++) tile_product<NB, GS>(code[i][n], word[i][n], a.scale_f16, xf, undo, sum[n]);
+                if (t + i + AHEAD < mine) fetch(grp, t + i + AHEAD, code[i], word[i]);
+                else if (grp + (int)gridDim.x < groups) fetch(grp + gridDim.x, i, code[i], word[i]);
+            }
+        // two buffers: the one written here was read before the last barrier
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (4 * q + i < RR) ssum[turn][w][n][4 * q + i][c] = sum[n][i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < (NT * 16) << lr; i += SEGS * CT_WAVE) {
+            const int n = i >> (4 + lr), r = i >> 4 & (RR - 1), o = (grp * NT + n) * TO + (i & 15);
+            if (r < nr && o < a.out_d) {
+                float v = 0.0f;
+#pragma unroll
+                for (int s = 0; s < SEGS; s++) v += ssum[turn][s][n][r][i & 15];
+                finish<BF16>(a, r0 + r, o, v);
+            }
+        }
+    }
+}
+
+// Many rows: a workgroup of eight wavefronts takes 64 rows and 128 outputs, a
+// wavefront 32 and 32 of them.  Its inputs are split once and left in LDS as the
+// products' A operands, in two buffers, while the tile before is multiplied;
+// codes and inputs are asked for a tile ahead.  The sums are those of
+// linear_kernel, segment by segment.
+constexpr int BR = 64, BO = 128, BT = 512;   // rows, outputs, threads of a workgroup
+
+template <bool BF16, int GS>
+__global__ __launch_bounds__(BT, 4) void linear_rows_kernel(Args a) {
+    constexpr int NB = BF16 ? 1 : 2, MT = 2, NT = 2, SI = BR * 16 / BT;
+    __shared__ __align__(16) f16x8 sx[2][NB][BR / 16][256];
+    __shared__ __align__(16) float sundo[2][BR];
+    const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE);
+    const int c = lane & 15, q = lane >> 4, wr = w >> 2;         // rows 32 wr ..
+    const int ot0 = (blockIdx.y * 4 + (w & 3)) * NT;
+    const int k8 = threadIdx.x & 15, sr = threadIdx.x >> 4;      // staged: rows sr + 32 i, piece k8
+    const u32x4 *codes[NT];
+    // a thread a word: of tile threadIdx.x / WT of the workgroup's eight
+    constexpr int WT = 16 * (4 / GS);
+    __shared__ uint32_t sword[2][BO / 16 * WT];
+    const uint32_t words = (min((int)(blockIdx.y * (BO / 16) + threadIdx.x / WT), a.otiles - 1) * a.itiles * WT + threadIdx.x % WT) * 4u;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        codes[n] = reinterpret_cast<const u32x4 *>(a.codes) + (long)min(ot0 + n, a.otiles - 1) * a.itiles * CT_WAVE;
+    }
+    const long r0 = (long)BR * blockIdx.x;
+    const int nr = (int)min((long)BR, a.rows - r0);
+    float total[MT][NT][4], sum[MT][NT][4];
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) total[m][n][i] = sum[m][n][i] = 0.0f;
+    // 32-bit offsets beside scalar bases, here and of the words: 64-bit addresses
+    // do not fit the registers
+    uint32_t xat[SI];
+#pragma unroll
+    for (int i = 0; i < SI; i++)                 // rows that are not there repeat the last one
+        xat[i] = ((uint32_t)min(sr + 32 * i, nr - 1) * (uint32_t)a.ld_x + 8 * k8) * (BF16 ? 2 : 4);
+    const char *xbase = input_at<BF16>(a, r0, 0);
+    float v[SI][8];
+    auto fetch_x = [&](int kt) __attribute__((always_inline)) {
+        if (kt * TI + TI <= a.in_d)
+#pragma unroll
+            for (int i = 0; i < SI; i++) fetch8<BF16>(xbase + kt * (TI * (BF16 ? 2 : 4)) + xat[i], v[i]);
+    };
+    auto place_x = [&](int kt) __attribute__((always_inline)) {
+        const int b = kt & 1;
+#pragma unroll
+        for (int i = 0; i < SI; i++) {
+            const int row = sr + 32 * i, m = row >> 4, at = piece<16>(k8, row & 15);
+            f16x8 h[NB];
+            if (kt * TI + TI > a.in_d)
+                fetch_last8<BF16>(xbase + kt * (TI * (BF16 ? 2 : 4)) + xat[i], a.in_d - kt * TI - 8 * k8, &sx[b][0][m][at],
+                                  &sx[b][NB - 1][m][at], v[i]);
+            const float undo = split8<NB>(v[i], h);
+#pragma unroll
+            for (int n = 0; n < NB; n++) sx[b][n][m][at] = h[n];
+            if (k8 == 0) sundo[b][row] = undo;
+        }
+    };
+    u32x4 code[NT];
+    uint32_t word = 0;
+    auto fetch_w = [&](int kt) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) code[n] = codes[n][kt * CT_WAVE + lane];
+        if (threadIdx.x < BO / 16 * WT) word = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const char *>(a.scales) + (words + kt * WT * 4u));
+    };
+    auto place_w = [&](int kt) __attribute__((always_inline)) {
+        if (threadIdx.x < BO / 16 * WT) sword[kt & 1][threadIdx.x] = word;
+    };
+    fetch_x(0);
+    fetch_w(0);
+    place_x(0);
+    place_w(0);
+    if (a.itiles > 1) fetch_x(1);
+    int left = a.per;                    // tiles of this segment
+    for (int kt = 0; kt < a.itiles; kt++) {
+        __syncthreads();
+        const int b = kt & 1;
+        u32x4 now[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) now[n] = code[n];
+        uint32_t nw[NT];
+        if (kt + 1 < a.itiles) fetch_w(kt + 1);
+        f32x4 acc[MT][NT];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j % GS == 0) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) nw[n] = sword[b][((w & 3) * NT + n) * WT + c * (4 / GS) + j / GS];
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) acc[m][n] = (f32x4){0, 0, 0, 0};
+            }
+            f16x8 wf[NT], xf[NB][MT];
+#pragma unroll
+            for (int x = 0; x < NB; x++)
+#pragma unroll
+                for (int m = 0; m < MT; m++) xf[x][m] = sx[b][x][MT * wr + m][piece<16>(4 * j + q, c)];
+#pragma unroll
+            for (int n = 0; n < NT; n++) wf[n] = weights8(now[n][j], less_of(nw[n]));
+#pragma unroll
+            for (int x = 0; x < NB; x++)
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[x][m], wf[n], acc[m][n], 0, 0, 0);
+            if (j % GS == GS - 1)
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    const f32x4 undo = *reinterpret_cast<const f32x4 *>(&sundo[b][16 * (MT * wr + m) + 4 * q]);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const float s = scale_of(nw[n], a.scale_f16);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sum[m][n][i] = __builtin_fmaf(mul_rn(acc[m][n][i], s), undo[i], sum[m][n][i]);
+                    }
+                }
+            // nothing of a later step is read yet, and a group's sums come before the
+            // next one's products: side by side they do not fit the registers
+            asm volatile("" ::: "memory");
+            if (GS < 4 && j % GS == GS - 1) {
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+                        asm volatile("" : "+v"(sum[m][n][0]), "+v"(sum[m][n][1]), "+v"(sum[m][n][2]), "+v"(sum[m][n][3]) : : "memory");
+            }
+        }
+        if (kt + 1 < a.itiles) {
+            place_x(kt + 1);
+            place_w(kt + 1);
+            if (kt + 2 < a.itiles) fetch_x(kt + 2);
+        }
+        if (--left == 0 || kt + 1 == a.itiles) {
+            left = a.per;
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        total[m][n][i] += sum[m][n][i];
+                        sum[m][n][i] = 0.0f;
+                    }
+        }
+    }
+    __syncthreads();
+    float *out = reinterpret_cast<float *>(sx) + w * (16 * MT * 16 * NT);     // this wavefront's [32][32]
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) out[(16 * m + 4 * q + i) * (16 * NT) + 16 * n + c] = total[m][n][i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int o = ot0 * TO + (lane & 31), n_rows = min(nr - 16 * MT * wr, 16 * MT);
+#pragma unroll 2
+    for (int r = lane >> 5; r < n_rows; r += 2)
+        if (o < a.out_d) finish<BF16>(a, r0 + 16 * MT * wr + r, o, out[r * (16 * NT) + (lane & 31)]);
 }
 
 // ---- Laying out ----------------------------------------------------------
@@ -335,7 +650,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(BackendW4 w, float *values,
         const int i = threadIdx.x, j = i & 3, row = (i >> 2) & 15, q = i >> 6;
         const int o = (int)(tile / itiles) * TO + row, k = (int)(tile % itiles) * TI + 32 * j + 8 * q;
         const uint32_t v = w.codes[tile * 256 + i], word = w.scales[(tile * TO + row) * per + (32 * j + 8 * q) / w.group];
-        const float s = scale_of(word, w.scale_f16), less = (float)less_of(word)[0] + 1024.0f;
+        const float s = scale_of(word, w.scale_f16 ? ~0u : 0u), less = (float)less_of(word)[0] + 1024.0f;
         if (o < w.out_d)
 #pragma unroll
             for (int e = 0; e < 8; e++)
@@ -372,13 +687,55 @@ extern "C" void ctk_w4_linear(const BackendW4 *w, const BackendW4Linear *p, hipS
     a.in_d = w->in_d; a.out_d = w->out_d;
     a.itiles = itiles_of(w); a.otiles = otiles_of(w);
     a.per = (a.itiles + SEGS - 1) / SEGS;
-    a.scale_f16 = w->scale_f16;
+    a.scale_f16 = w->scale_f16 ? ~0u : 0u;
     a.y = p->y; a.x = p->x; a.ld_y = p->ld_y; a.ld_x = p->ld_x;
     a.rows = p->rows; a.act = p->act; a.scale = p->scale; a.bias = p->bias;
-    a.vec = ((uintptr_t)p->x & 15) == 0 && p->ld_x % (p->bf16 ? 8 : 4) == 0;
-    const long rt = ((long)p->rows + 15) / 16;
+    const long rows = p->rows;
+    if (((rows + BR - 1) / BR) * ((w->out_d + BO - 1) / BO) >= 96 && rows > 32 && p->ld_x < 1 << 24) {
+        const long rt = (rows + BR - 1) / BR;
+        const dim3 grid((unsigned)rt, (unsigned)((w->out_d + BO - 1) / BO));
+#define ROWS(B, GS) hipLaunchKernelGGL((linear_rows_kernel<B, GS>), grid, dim3(BT), 0, s, a)
+        if (p->bf16) {
+            if (w->group == 32) ROWS(true, 1);
+            else if (w->group == 64) ROWS(true, 2);
+            else ROWS(true, 4);
+        } else {
+            if (w->group == 32) ROWS(false, 1);
+            else if (w->group == 64) ROWS(false, 2);
+            else ROWS(false, 4);
+        }
+#undef ROWS
+        return;
+    }
+    const int lr = rows == 1 ? 0 : rows <= 4 ? 2 : rows <= 8 ? 3 : 4;
+    const size_t inputs = (size_t)a.itiles * ((256 * (p->bf16 ? 1 : 2) + 4) << lr);
+    if (inputs <= FEW_LDS) {
+        const long rt = (rows + (1 << lr) - 1) >> lr;
+        const int two = w->group > 32 && inputs <= 120 << 10 && (long)a.otiles * rt >= 1024;     // a word for each 32 does not fit twice
+        const int groups = (a.otiles + two) / (1 + two);
+        // as many workgroups as the CUs hold at once
+        const long fit = inputs + (two ? 32768 : 16384) <= 80 << 10 ? 512 : 256;
+        const dim3 grid((unsigned)(groups * rt > fit ? (fit + rt - 1) / rt : groups), (unsigned)rt);
+#define FEW(B, GS)                                                                                                              \
+    do {                                                                                                                        \
+        if (two) hipLaunchKernelGGL((linear_few_kernel<B, GS, (GS > 1 ? 2 : 1)>), grid, dim3(SEGS * CT_WAVE), inputs, s, a, lr, groups); \
+        else hipLaunchKernelGGL((linear_few_kernel<B, GS, 1>), grid, dim3(SEGS * CT_WAVE), inputs, s, a, lr, groups);           \
+    } while (0)
+        if (p->bf16) {
+            if (w->group == 32) FEW(true, 1);
+            else if (w->group == 64) FEW(true, 2);
+            else FEW(true, 4);
+        } else {
+            if (w->group == 32) FEW(false, 1);
+            else if (w->group == 64) FEW(false, 2);
+            else FEW(false, 4);
+        }
+#undef FEW
+        return;
+    }
+    const long rt = (rows + 15) / 16;
     const dim3 grid((unsigned)a.otiles, (unsigned)(rt < 4096 ? rt : 4096));
-#define LINEAR(B, GS) hipLaunchKernelGGL((linear_kernel<B, GS, 1>), grid, dim3(SEGS * CT_WAVE), 0, s, a)
+#define LINEAR(B, GS) hipLaunchKernelGGL((linear_kernel<B, GS, 1, 16>), grid, dim3(SEGS * CT_WAVE), 0, s, a)
     if (p->bf16) {
         if (w->group == 32) LINEAR(true, 1);
         else if (w->group == 64) LINEAR(true, 2);
