@@ -10,10 +10,19 @@
 // bits of two f16.  Each (output, group) has one word: the scale's 16 bits above
 // the f16 bits of -(1024 + z).
 // Products.  c | 0x6400 is the f16 1024 + c, and adding -(1024 + z) gives c - z
-// exactly: two instructions for a pair of weights.  Activations are brought, 128 inputs
+// exactly: 9 instructions for 8 weights.  Activations are brought, 128 inputs
 // of a row at a time, to a largest value in [2^14, 2^15) by a power of two and
-// split into two f16 (bf16 rows are one f16).  A group's products are summed by
-// the matrix unit in fp32 and enter the row's sum times the scale.
+// split into two f16 (bf16 rows are one f16): 22 bits of each fp32 input stay.
+// A group's products are summed by the matrix unit in fp32 and enter the row's
+// sum times the scale.  A row's inputs are summed in SEGS runs of tiles that are
+// joined in order, in every kernel here, so that a row's answer does not depend
+// on how many rows the call has.
+//
+// What bounds them, at the listed times of one MI355X.  One row: the launch and one
+// pass of loads (1024 -> 4096, 2.2 MB: 4.0 us).  Few rows of large maps: the codes'
+// bytes (1 x 8192 -> 24576, 106 MB: 22.4 us, 4.7 TB/s).  Many rows: vector
+// instructions that prepare both operands, which do not overlap the products (752 x
+// 1280 -> 5120: 32 us, 308 Tflop/s of them, twice that of f16 terms).
 #include "ct_dev.h"
 #include "ct_w4.h"
 
@@ -46,17 +55,30 @@ __device__ __forceinline__ float scale_of(uint32_t word, uint32_t f16) {
     return __uint_as_float((h & f16) | (word & 0xffff0000u & ~f16));
 }
 
-// Eight codes less their zero point (both halves of `less`: -(1024 + z)).
-__device__ __forceinline__ f16x8 weights8(uint32_t q, f16x2 less) {
-    u32x4 w;                     // whole registers: halves set one by one took twice as many
-#pragma unroll
-    for (int p = 0; p < 4; p++)
-        w[p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, (q >> (4 * p) & 0x000f000fu) | 0x64006400u) + less);
-    return __builtin_bit_cast(f16x8, w);
+// A zero point as it is taken off: -(1024 + z) and -(64 + z), in both halves.
+struct Less {
+    f16x2 low, high;
+};
+__device__ __forceinline__ Less less_of(uint32_t word) {
+    const f16x2 low = __builtin_bit_cast(f16x2, (word & 0xffffu) | word << 16);
+    return {low, low + (f16x2){960, 960}};
 }
 
-__device__ __forceinline__ f16x2 less_of(uint32_t word) {
-    return __builtin_bit_cast(f16x2, (word & 0xffffu) | word << 16);
+// Eight codes less their zero point.  A code in the low four bits of a f16 1024.0
+// makes it 1024 + c, in the next four of a 64.0 64 + c: one shift and four masks a
+// dword (a shift a pair took 15 instructions where this takes 9).
+__device__ __forceinline__ f16x8 weights8(uint32_t q, const Less &less) {
+    // constants in registers: one instruction takes a mask and a constant only so
+    uint32_t m0 = 0x000f000fu, m1 = 0x00f000f0u, one = 0x64006400u, two = 0x54005400u;
+    asm("" : "+s"(m0), "+s"(m1), "+v"(one), "+v"(two));
+    u32x4 w;                     // whole registers: halves set one by one took twice as many
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        const uint32_t x = p ? q >> 8 : q;
+        w[2 * p] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, (x & m0) | one) + less.low);
+        w[2 * p + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, (x & m1) | two) + less.high);
+    }
+    return __builtin_bit_cast(f16x8, w);
 }
 
 // Two values as f16 terms: rounded, and what the rounding left, rounded.
@@ -134,9 +156,11 @@ __device__ __forceinline__ void fetch_last8(const char *x, int n, f16x8 *hi, f16
 // power of two that undoes theirs.
 template <int NB>
 __device__ __forceinline__ float split8(const float (&v)[8], f16x8 (&h)[NB]) {
-    uint32_t top = 0;
+    // a NaN is no largest value: it stays one without
+    float big = fmaxf(fabsf(v[0]), fabsf(v[1]));
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int i = 2; i < 8; i++) big = fmaxf(big, fabsf(v[i]));
+    const uint32_t top = __float_as_uint(big);
     // exponent of the largest, at least 15 - 127 so that the factor is in range
     const int e = max((int)(max16(top) >> 23), 15);
     const float up = __uint_as_float((uint32_t)(127 + 14 - (e - 127)) << 23);
@@ -156,10 +180,9 @@ __device__ __forceinline__ float split8(const float (&v)[8], f16x8 (&h)[NB]) {
 }
 
 // Where a row's eight inputs 8 k8 .. + 7 lie among a tile's pieces of 16 bytes:
-// piece k8 * RR + row, rows changed so that neither the stores of a row nor the
+// piece k8 * 16 + row, rows changed so that neither the stores of a row nor the
 // loads of a product meet in a bank.
-template <int RR>
-__device__ __forceinline__ int piece(int k8, int row) { return k8 * RR + ((row ^ k8) & (RR - 1)); }
+__device__ __forceinline__ int piece(int k8, int row) { return k8 * 16 + (row ^ k8); }
 
 // One tile of 16 outputs times 16 rows: the groups' products into the rows' sums.
 // A operand x (row = lane % 16), B operand the weights (output = lane % 16);
@@ -169,7 +192,7 @@ __device__ __forceinline__ void tile_product(const u32x4 &code, const uint32_t (
                                              const f16x8 (&xf)[NB][4], const f32x4 &undo, f32x4 &sum) {
 #pragma unroll
     for (int g = 0; g < 4 / GS; g++) {
-        const f16x2 less = less_of(word[g]);
+        const Less less = less_of(word[g]);
         f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
         for (int j = g * GS; j < (g + 1) * GS; j++) {
@@ -199,40 +222,35 @@ __device__ __forceinline__ void finish(const Args &a, long t, int o, float v) {
     }
 }
 
-// Few rows of many inputs: NT tiles of outputs a workgroup, RR rows at a time; its
-// eight wavefronts each take one segment of the inputs and join their sums in
-// LDS, in order.  A wavefront has AHEAD tiles of codes and inputs in flight.
-template <bool BF16, int GS, int NT, int RR>
+// Rows whose inputs do not fit LDS: one tile of outputs a workgroup, 16 rows at a
+// time; its eight wavefronts each take one segment of the inputs, split them a tile
+// at a time and join their sums in LDS, in order.  A wavefront has AHEAD tiles of
+// codes and inputs in flight.  64 x 4096 -> 1024: 9.5 us.
+template <bool BF16, int GS>
 __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
-    constexpr int NB = BF16 ? 1 : 2, RI = RR / 4, AHEAD = RR == 4 ? 4 : 2;
+    constexpr int NB = BF16 ? 1 : 2, RR = 16, RI = RR / 4, AHEAD = 2;
     __shared__ __align__(16) union {
         f16x8 x[SEGS][NB][16 * RR];
-        float sum[SEGS][NT][16][TO];
+        float sum[SEGS][RR][TO];
     } sh;
     __shared__ __align__(16) float sundo[SEGS][RR];
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE);
     const int c = lane & 15, q = lane >> 4;
-    const int ot0 = blockIdx.x * NT;
-    const int k0 = w * a.per, k1 = min(k0 + a.per, a.itiles);
+        const int k0 = w * a.per, k1 = min(k0 + a.per, a.itiles);
     struct Ahead {
-        u32x4 code[NT];
-        uint32_t word[NT][4 / GS];
+        u32x4 code;
+        uint32_t word[4 / GS];
         float v[RI][8];
     };
     for (long r0 = (long)RR * blockIdx.y; r0 < a.rows; r0 += (long)RR * gridDim.y) {
         const int nr = (int)min((long)RR, a.rows - r0);
-        f32x4 sum[NT];
-#pragma unroll
-        for (int n = 0; n < NT; n++) sum[n] = (f32x4){0, 0, 0, 0};
+        f32x4 sum = {0, 0, 0, 0};
         Ahead t[AHEAD];
         auto fetch = [&](int kt, Ahead &f) __attribute__((always_inline)) {
+            const long tile = (long)blockIdx.x * a.itiles + kt;
+            f.code = reinterpret_cast<const u32x4 *>(a.codes)[tile * CT_WAVE + lane];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const long tile = (long)min(ot0 + n, a.otiles - 1) * a.itiles + kt;
-                f.code[n] = reinterpret_cast<const u32x4 *>(a.codes)[tile * CT_WAVE + lane];
-#pragma unroll
-                for (int g = 0; g < 4 / GS; g++) f.word[n][g] = a.scales[(tile * 16 + c) * (4 / GS) + g];
-            }
+            for (int g = 0; g < 4 / GS; g++) f.word[g] = a.scales[(tile * 16 + c) * (4 / GS) + g];
             if (kt * TI + TI <= a.in_d)
 #pragma unroll
                 for (int i = 0; i < RI; i++)
@@ -245,11 +263,11 @@ __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
                 if (r < nr) {
                     f16x8 h[NB];
                     if (kt * TI + TI > a.in_d)
-                        fetch_last8<BF16>(input_at<BF16>(a, r0 + r, kt * TI + 8 * c), a.in_d - kt * TI - 8 * c, &sh.x[w][0][piece<RR>(c, r)],
-                                          &sh.x[w][NB - 1][piece<RR>(c, r)], f.v[i]);
+                        fetch_last8<BF16>(input_at<BF16>(a, r0 + r, kt * TI + 8 * c), a.in_d - kt * TI - 8 * c, &sh.x[w][0][piece(c, r)],
+                                          &sh.x[w][NB - 1][piece(c, r)], f.v[i]);
                     const float undo = split8<NB>(f.v[i], h);
 #pragma unroll
-                    for (int n = 0; n < NB; n++) sh.x[w][n][piece<RR>(c, r)] = h[n];
+                    for (int n = 0; n < NB; n++) sh.x[w][n][piece(c, r)] = h[n];
                     if (c == 0) sundo[w][r] = undo;
                 }
             }
@@ -260,10 +278,9 @@ __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
 #pragma unroll
             for (int n = 0; n < NB; n++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) xf[n][j] = sh.x[w][n][piece<RR>(4 * j + q, c)];
-            const f32x4 undo = *reinterpret_cast<const f32x4 *>(&sundo[w][RR == 4 ? 0 : 4 * q]);
-#pragma unroll
-            for (int n = 0; n < NT; n++) tile_product<NB, GS>(f.code[n], f.word[n], a.scale_f16, xf, undo, sum[n]);
+                for (int j = 0; j < 4; j++) xf[n][j] = sh.x[w][n][piece(4 * j + q, c)];
+            const f32x4 undo = *reinterpret_cast<const f32x4 *>(&sundo[w][4 * q]);
+            tile_product<NB, GS>(f.code, f.word, a.scale_f16, xf, undo, sum);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         };
@@ -279,19 +296,14 @@ __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
                 }
         __syncthreads();
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (RR == 16 || q == 0) sh.sum[w][n][4 * q + i][c] = sum[n][i];
+        for (int i = 0; i < 4; i++) sh.sum[w][4 * q + i][c] = sum[i];
         __syncthreads();
-        for (int i = threadIdx.x; i < NT * RR * 16; i += SEGS * CT_WAVE) {
-            const int n = i / (RR * 16), r = i >> 4 & (RR - 1), o = (ot0 + n) * TO + (i & 15);
-            if (r < nr && o < a.out_d) {
-                float v = 0.0f;
+        const int r = threadIdx.x >> 4, o = blockIdx.x * TO + c;
+        if (r < nr && o < a.out_d) {
+            float v = 0.0f;
 #pragma unroll
-                for (int s = 0; s < SEGS; s++) v += sh.sum[s][n][r][i & 15];
-                finish<BF16>(a, r0 + r, o, v);
-            }
+            for (int s = 0; s < SEGS; s++) v += sh.sum[s][r][c];
+            finish<BF16>(a, r0 + r, o, v);
         }
         __syncthreads();
     }
@@ -302,6 +314,7 @@ __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
 // time; its eight wavefronts each take one segment of the inputs and join
 // their sums in LDS, in order.  A wavefront has AHEAD tiles of codes in flight,
 // those of the next outputs among them, from before the inputs are split.
+// 64 x 1024 -> 4096: 7.2 us, of which about 3 are the split and one pass of loads.
 constexpr int FEW_LDS = 136 << 10;           // of inputs, beside 16 KB of sums, within a CU's 160
 
 template <bool BF16, int GS, int NT>
@@ -395,27 +408,35 @@ __global__ __launch_bounds__(SEGS * CT_WAVE, 4) void linear_few_kernel(Args a, i
     }
 }
 
-// Many rows: a workgroup of eight wavefronts takes 64 rows and 128 outputs, a
-// wavefront 32 and 32 of them.  Its inputs are split once and left in LDS as the
-// products' A operands, in two buffers, while the tile before is multiplied;
-// codes and inputs are asked for a tile ahead.  The sums are those of
-// linear_kernel, segment by segment.
-constexpr int BR = 64, BO = 128, BT = 512;   // rows, outputs, threads of a workgroup
+// Many rows: a workgroup takes 64 rows and 32 outputs a wavefront.  Its inputs are
+// split once and left in LDS as the products' A operands, in two buffers: while
+// one tile is multiplied the next is split, between the products, and the one
+// after it is asked for.  No branches among them: they cost registers for operands
+// that are read a step ahead.  The sums are those of linear_few_kernel, segment by
+// segment.  in_d >= 128.  W = 8 splits the inputs half as often for an output as
+// W = 4: 752 x 1280 -> 5120 in 32 us instead of 38, 4000 x 4096 -> 4096 of bf16 in
+// 212 instead of 263.
+constexpr int BR = 64;
 
-template <bool BF16, int GS>
-__global__ __launch_bounds__(BT, 4) void linear_rows_kernel(Args a) {
-    constexpr int NB = BF16 ? 1 : 2, MT = 2, NT = 2, SI = BR * 16 / BT;
+template <bool BF16, int GS, int W>
+__global__ __launch_bounds__(W * CT_WAVE, 2) void linear_rows_kernel(Args a) {
+    constexpr int NB = BF16 ? 1 : 2, MT = BR / 16, NT = 2, BO = W * 16 * NT, BT = W * CT_WAVE, SI = BR * 16 / BT, RS = BT / 16;
     __shared__ __align__(16) f16x8 sx[2][NB][BR / 16][256];
     __shared__ __align__(16) float sundo[2][BR];
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE);
-    const int c = lane & 15, q = lane >> 4, wr = w >> 2;         // rows 32 wr ..
-    const int ot0 = (blockIdx.y * 4 + (w & 3)) * NT;
-    const int k8 = threadIdx.x & 15, sr = threadIdx.x >> 4;      // staged: rows sr + 32 i, piece k8
+    const int c = lane & 15, q = lane >> 4;
+    const int ot0 = (blockIdx.y * W + w) * NT;
+    const int k8 = threadIdx.x & 15, sr = threadIdx.x >> 4;      // staged: rows sr + SR i, piece k8
     const u32x4 *codes[NT];
-    // a thread a word: of tile threadIdx.x / WT of the workgroup's eight
-    constexpr int WT = 16 * (4 / GS);
-    __shared__ uint32_t sword[2][BO / 16 * WT];
-    const uint32_t words = (min((int)(blockIdx.y * (BO / 16) + threadIdx.x / WT), a.otiles - 1) * a.itiles * WT + threadIdx.x % WT) * 4u;
+    // scale words: WT a tile, tile after tile; threads past the last repeat it
+    constexpr int WT = 16 * (4 / GS), WORDS = BO / 16 * WT, SW = (WORDS + BT - 1) / BT;
+    __shared__ uint32_t sword[2][SW * BT];
+    uint32_t words[SW];
+#pragma unroll
+    for (int i = 0; i < SW; i++) {
+        const int t = min((int)threadIdx.x + i * BT, WORDS - 1);
+        words[i] = (min((int)blockIdx.y * (BO / 16) + t / WT, a.otiles - 1) * a.itiles * WT + t % WT) * 4u;
+    }
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         codes[n] = reinterpret_cast<const u32x4 *>(a.codes) + (long)min(ot0 + n, a.otiles - 1) * a.itiles * CT_WAVE;
@@ -434,103 +455,114 @@ __global__ __launch_bounds__(BT, 4) void linear_rows_kernel(Args a) {
     uint32_t xat[SI];
 #pragma unroll
     for (int i = 0; i < SI; i++)                 // rows that are not there repeat the last one
-        xat[i] = ((uint32_t)min(sr + 32 * i, nr - 1) * (uint32_t)a.ld_x + 8 * k8) * (BF16 ? 2 : 4);
+        xat[i] = ((uint32_t)min(sr + RS * i, nr - 1) * (uint32_t)a.ld_x + 8 * k8) * (BF16 ? 2 : 4);
     const char *xbase = input_at<BF16>(a, r0, 0);
     float v[SI][8];
-    auto fetch_x = [&](int kt) __attribute__((always_inline)) {
-        if (kt * TI + TI <= a.in_d)
-#pragma unroll
-            for (int i = 0; i < SI; i++) fetch8<BF16>(xbase + kt * (TI * (BF16 ? 2 : 4)) + xat[i], v[i]);
+    const int whole = a.in_d / TI;               // tiles that end before in_d
+    auto fetch_x = [&](int kt, int i) __attribute__((always_inline)) {
+        fetch8<BF16>(xbase + min(kt, whole - 1) * (TI * (BF16 ? 2 : 4)) + xat[i], v[i]);
     };
-    auto place_x = [&](int kt) __attribute__((always_inline)) {
-        const int b = kt & 1;
+    auto place_x = [&](int b, int i) __attribute__((always_inline)) {
+        const int row = sr + RS * i, m = row >> 4, at = piece(k8, row & 15);
+        f16x8 h[NB];
+        const float undo = split8<NB>(v[i], h);
+#pragma unroll
+        for (int n = 0; n < NB; n++) sx[b][n][m][at] = h[n];
+        sundo[b][row] = undo;                    // the same of all 16 lanes
+    };
+    auto last_x = [&](int kt) __attribute__((always_inline)) {           // a tile past the whole ones, into v
 #pragma unroll
         for (int i = 0; i < SI; i++) {
-            const int row = sr + 32 * i, m = row >> 4, at = piece<16>(k8, row & 15);
-            f16x8 h[NB];
-            if (kt * TI + TI > a.in_d)
-                fetch_last8<BF16>(xbase + kt * (TI * (BF16 ? 2 : 4)) + xat[i], a.in_d - kt * TI - 8 * k8, &sx[b][0][m][at],
-                                  &sx[b][NB - 1][m][at], v[i]);
-            const float undo = split8<NB>(v[i], h);
-#pragma unroll
-            for (int n = 0; n < NB; n++) sx[b][n][m][at] = h[n];
-            if (k8 == 0) sundo[b][row] = undo;
+            const int row = sr + RS * i, m = row >> 4, at = piece(k8, row & 15);
+            fetch_last8<BF16>(xbase + kt * (TI * (BF16 ? 2 : 4)) + xat[i], a.in_d - kt * TI - 8 * k8, &sx[kt & 1][0][m][at],
+                              &sx[kt & 1][NB - 1][m][at], v[i]);
         }
     };
     u32x4 code[NT];
-    uint32_t word = 0;
+    uint32_t word[SW];
     auto fetch_w = [&](int kt) __attribute__((always_inline)) {
+        kt = min(kt, a.itiles - 1);
 #pragma unroll
         for (int n = 0; n < NT; n++) code[n] = codes[n][kt * CT_WAVE + lane];
-        if (threadIdx.x < BO / 16 * WT) word = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const char *>(a.scales) + (words + kt * WT * 4u));
+#pragma unroll
+        for (int i = 0; i < SW; i++)
+            word[i] = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const char *>(a.scales) + (words[i] + kt * WT * 4u));
     };
-    auto place_w = [&](int kt) __attribute__((always_inline)) {
-        if (threadIdx.x < BO / 16 * WT) sword[kt & 1][threadIdx.x] = word;
+    auto place_w = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < SW; i++) sword[b][threadIdx.x + i * BT] = word[i];
     };
-    fetch_x(0);
+#pragma unroll
+    for (int i = 0; i < SI; i++) fetch_x(0, i);
     fetch_w(0);
-    place_x(0);
+#pragma unroll
+    for (int i = 0; i < SI; i++) place_x(0, i);
     place_w(0);
-    if (a.itiles > 1) fetch_x(1);
-    int left = a.per;                    // tiles of this segment
+#pragma unroll
+    for (int i = 0; i < SI; i++) fetch_x(1, i);
+    int left = a.per;                            // tiles of this segment
     for (int kt = 0; kt < a.itiles; kt++) {
         __syncthreads();
         const int b = kt & 1;
-        u32x4 now[NT];
+        // the buffer that the tile before last leaves is free
+        if (kt + 1 == whole && whole < a.itiles) last_x(kt + 1);
+        // operands are read a step (a term of 32 inputs) ahead of their products
+        f16x8 wf[2][NT], xf[2][MT];
+        auto read_x = [&](int step) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) now[n] = code[n];
-        uint32_t nw[NT];
-        if (kt + 1 < a.itiles) fetch_w(kt + 1);
+            for (int m = 0; m < MT; m++) xf[step & 1][m] = sx[b][step % NB][m][piece(4 * (step / NB) + q, c)];
+        };
+        uint32_t nw[2][NT];
+        auto read_w = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                if (j % GS == 0) nw[j / GS & 1][n] = sword[b][(w * NT + n) * WT + c * (4 / GS) + j / GS];
+                wf[j & 1][n] = weights8(code[n][j], less_of(nw[j / GS & 1][n]));
+            }
+        };
         f32x4 acc[MT][NT];
+        read_x(0);
+        read_w(0);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j % GS == 0) {
-#pragma unroll
-                for (int n = 0; n < NT; n++) nw[n] = sword[b][((w & 3) * NT + n) * WT + c * (4 / GS) + j / GS];
+        for (int step = 0; step < 4 * NB; step++) {
+            const int j = step / NB;
+            if (step + 1 < 4 * NB) read_x(step + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (step % NB == 0 && j % GS == 0)
 #pragma unroll
                 for (int m = 0; m < MT; m++)
 #pragma unroll
                     for (int n = 0; n < NT; n++) acc[m][n] = (f32x4){0, 0, 0, 0};
-            }
-            f16x8 wf[NT], xf[NB][MT];
 #pragma unroll
-            for (int x = 0; x < NB; x++)
+            for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int m = 0; m < MT; m++) xf[x][m] = sx[b][x][MT * wr + m][piece<16>(4 * j + q, c)];
+                for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[step & 1][m], wf[j & 1][n], acc[m][n], 0, 0, 0);
+            if (step % NB == NB - 1 && j < 3) read_w(j + 1);
+            if (step % NB == NB - 1 && j == 2) fetch_w(kt + 1);
+            // the next tile's inputs, and the one after it
+            constexpr int EVERY = 4 * NB / SI ? 4 * NB / SI : 1, AT = SI > 4 * NB ? SI / (4 * NB) : 1;
+            if (step % EVERY == 0)
 #pragma unroll
-            for (int n = 0; n < NT; n++) wf[n] = weights8(now[n][j], less_of(nw[n]));
-#pragma unroll
-            for (int x = 0; x < NB; x++)
-#pragma unroll
-                for (int m = 0; m < MT; m++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xf[x][m], wf[n], acc[m][n], 0, 0, 0);
-            if (j % GS == GS - 1)
+                for (int i = step / EVERY * AT; i < (step / EVERY + 1) * AT; i++) {
+                    place_x(b ^ 1, i);
+                    fetch_x(kt + 2, i);
+                }
+            if (step == 4 * NB - 1) place_w(b ^ 1);
+            if (step % NB == NB - 1 && j % GS == GS - 1) {
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
-                    const f32x4 undo = *reinterpret_cast<const f32x4 *>(&sundo[b][16 * (MT * wr + m) + 4 * q]);
+                    const f32x4 undo = *reinterpret_cast<const f32x4 *>(&sundo[b][16 * m + 4 * q]);
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        const float s = scale_of(nw[n], a.scale_f16);
+                        const float s = scale_of(nw[j / GS & 1][n], a.scale_f16);
 #pragma unroll
                         for (int i = 0; i < 4; i++) sum[m][n][i] = __builtin_fmaf(mul_rn(acc[m][n][i], s), undo[i], sum[m][n][i]);
+                        // a group's sums before the next one's products: side by side
+                        // they do not fit the registers
+                        if (GS < 4) asm volatile("" : "+v"(sum[m][n][0]), "+v"(sum[m][n][1]), "+v"(sum[m][n][2]), "+v"(sum[m][n][3]));
                     }
                 }
-            // nothing of a later step is read yet, and a group's sums come before the
-            // next one's products: side by side they do not fit the registers
-            asm volatile("" ::: "memory");
-            if (GS < 4 && j % GS == GS - 1) {
-#pragma unroll
-                for (int m = 0; m < MT; m++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-                        asm volatile("" : "+v"(sum[m][n][0]), "+v"(sum[m][n][1]), "+v"(sum[m][n][2]), "+v"(sum[m][n][3]) : : "memory");
             }
-        }
-        if (kt + 1 < a.itiles) {
-            place_x(kt + 1);
-            place_w(kt + 1);
-            if (kt + 2 < a.itiles) fetch_x(kt + 2);
         }
         if (--left == 0 || kt + 1 == a.itiles) {
             left = a.per;
@@ -546,19 +578,27 @@ __global__ __launch_bounds__(BT, 4) void linear_rows_kernel(Args a) {
         }
     }
     __syncthreads();
-    float *out = reinterpret_cast<float *>(sx) + w * (16 * MT * 16 * NT);     // this wavefront's [32][32]
+    // through LDS, in as many turns as a part of each wavefront's [64][32] needs
+    constexpr int TURN = BF16 ? 2 : 1, ROWS = BR / TURN;
+    float *out = reinterpret_cast<float *>(sx) + w * (ROWS * 16 * NT);
+    static_assert(sizeof(float) * W * ROWS * 16 * NT <= sizeof(sx), "the sums take the inputs' place");
+    const int o = ot0 * TO + (lane & 31);
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int h = 0; h < TURN; h++) {
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int m = 0; m < MT / TURN; m++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) out[(16 * m + 4 * q + i) * (16 * NT) + 16 * n + c] = total[m][n][i];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int o = ot0 * TO + (lane & 31), n_rows = min(nr - 16 * MT * wr, 16 * MT);
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[(16 * m + 4 * q + i) * (16 * NT) + 16 * n + c] = total[h * (MT / TURN) + m][n][i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll 2
-    for (int r = lane >> 5; r < n_rows; r += 2)
-        if (o < a.out_d) finish<BF16>(a, r0 + 16 * MT * wr + r, o, out[r * (16 * NT) + (lane & 31)]);
+        for (int r = lane >> 5; r < min(nr - ROWS * h, ROWS); r += 2)
+            if (o < a.out_d) finish<BF16>(a, r0 + ROWS * h + r, o, out[r * (16 * NT) + (lane & 31)]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 // ---- Laying out ----------------------------------------------------------
@@ -650,7 +690,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(BackendW4 w, float *values,
         const int i = threadIdx.x, j = i & 3, row = (i >> 2) & 15, q = i >> 6;
         const int o = (int)(tile / itiles) * TO + row, k = (int)(tile % itiles) * TI + 32 * j + 8 * q;
         const uint32_t v = w.codes[tile * 256 + i], word = w.scales[(tile * TO + row) * per + (32 * j + 8 * q) / w.group];
-        const float s = scale_of(word, w.scale_f16 ? ~0u : 0u), less = (float)less_of(word)[0] + 1024.0f;
+        const float s = scale_of(word, w.scale_f16 ? ~0u : 0u), less = (float)less_of(word).low[0] + 1024.0f;
         if (o < w.out_d)
 #pragma unroll
             for (int e = 0; e < 8; e++)
@@ -691,10 +731,27 @@ extern "C" void ctk_w4_linear(const BackendW4 *w, const BackendW4Linear *p, hipS
     a.y = p->y; a.x = p->x; a.ld_y = p->ld_y; a.ld_x = p->ld_x;
     a.rows = p->rows; a.act = p->act; a.scale = p->scale; a.bias = p->bias;
     const long rows = p->rows;
-    if (((rows + BR - 1) / BR) * ((w->out_d + BO - 1) / BO) >= 96 && rows > 32 && p->ld_x < 1 << 24) {
-        const long rt = (rows + BR - 1) / BR;
-        const dim3 grid((unsigned)rt, (unsigned)((w->out_d + BO - 1) / BO));
-#define ROWS(B, GS) hipLaunchKernelGGL((linear_rows_kernel<B, GS>), grid, dim3(BT), 0, s, a)
+    const long rt64 = (rows + BR - 1) / BR;
+    const int lr = rows == 1 ? 0 : rows <= 4 ? 2 : rows <= 8 ? 3 : 4;
+    const size_t inputs = (size_t)a.itiles * ((256 * (p->bf16 ? 1 : 2) + 4) << lr);
+    const long rt = (rows + (1 << lr) - 1) >> lr;
+    const bool few = inputs <= FEW_LDS && rt <= 65535;
+    // Many rows in tiles of 64 once these fill the card.  With the inputs in LDS in us, few /
+    // rows, in 128 workgroups of 64 rows: 64 x 1024 -> 16384 19.3 / 24.1; in 160: 300 x 1024
+    // -> 4096 23.6 / 24.5; in 176: 700 x 1024 -> 2048 28.8 / 24.8; in 256: 128 x 1024 ->
+    // 16384 35 / 25.  Inputs that do not fit LDS are split again for each tile of
+    // outputs otherwise, in 64: 64 x 4096 -> 8192 59 / 66 (bf16 64 x 8192 -> 8192 129 /
+    // 108); in 80: 480 x 5120 -> 1280 87 / 81; in 120: 752 x 5120 -> 1280 129 / 81.
+    if (rt64 * ((w->out_d + 127) / 128) >= (few ? 176 : 72) && rows > 32 && w->in_d >= TI && p->ld_x < 1 << 24) {
+        // 256 outputs a workgroup where that leaves enough of them: 752 x 5120 -> 1280, 60
+        // of them, 104 us instead of 84; 752 x 1280 -> 5120, 240, 32 instead of 38
+        const int wide = rt64 * ((w->out_d + 255) / 256) >= 200;
+        const dim3 grid((unsigned)rt64, (unsigned)(wide ? (w->out_d + 255) / 256 : (w->out_d + 127) / 128));
+#define ROWS(B, GS)                                                                                                 \
+    do {                                                                                                            \
+        if (wide) hipLaunchKernelGGL((linear_rows_kernel<B, GS, 8>), grid, dim3(8 * CT_WAVE), 0, s, a);             \
+        else hipLaunchKernelGGL((linear_rows_kernel<B, GS, 4>), grid, dim3(4 * CT_WAVE), 0, s, a);                  \
+    } while (0)
         if (p->bf16) {
             if (w->group == 32) ROWS(true, 1);
             else if (w->group == 64) ROWS(true, 2);
@@ -707,15 +764,12 @@ extern "C" void ctk_w4_linear(const BackendW4 *w, const BackendW4Linear *p, hipS
 #undef ROWS
         return;
     }
-    const int lr = rows == 1 ? 0 : rows <= 4 ? 2 : rows <= 8 ? 3 : 4;
-    const size_t inputs = (size_t)a.itiles * ((256 * (p->bf16 ? 1 : 2) + 4) << lr);
-    if (inputs <= FEW_LDS) {
-        const long rt = (rows + (1 << lr) - 1) >> lr;
+    if (few) {
         const int two = w->group > 32 && inputs <= 120 << 10 && (long)a.otiles * rt >= 1024;     // a word for each 32 does not fit twice
         const int groups = (a.otiles + two) / (1 + two);
         // as many workgroups as the CUs hold at once
         const long fit = inputs + (two ? 32768 : 16384) <= 80 << 10 ? 512 : 256;
-        const dim3 grid((unsigned)(groups * rt > fit ? (fit + rt - 1) / rt : groups), (unsigned)rt);
+        const dim3 grid((unsigned)(groups * rt <= fit ? groups : rt < fit ? fit / rt : 1), (unsigned)rt);
 #define FEW(B, GS)                                                                                                              \
     do {                                                                                                                        \
         if (two) hipLaunchKernelGGL((linear_few_kernel<B, GS, (GS > 1 ? 2 : 1)>), grid, dim3(SEGS * CT_WAVE), inputs, s, a, lr, groups); \
@@ -733,9 +787,9 @@ extern "C" void ctk_w4_linear(const BackendW4 *w, const BackendW4Linear *p, hipS
 #undef FEW
         return;
     }
-    const long rt = (rows + 15) / 16;
-    const dim3 grid((unsigned)a.otiles, (unsigned)(rt < 4096 ? rt : 4096));
-#define LINEAR(B, GS) hipLaunchKernelGGL((linear_kernel<B, GS, 1, 16>), grid, dim3(SEGS * CT_WAVE), 0, s, a)
+    const long rt16 = (rows + 15) / 16;
+    const dim3 grid((unsigned)a.otiles, (unsigned)(rt16 < 4096 ? rt16 : 4096));
+#define LINEAR(B, GS) hipLaunchKernelGGL((linear_kernel<B, GS>), grid, dim3(SEGS * CT_WAVE), 0, s, a)
     if (p->bf16) {
         if (w->group == 32) LINEAR(true, 1);
         else if (w->group == 64) LINEAR(true, 2);
