@@ -241,3 +241,12 @@ def test_captured_and_replayed(hip):
         c.check(ref.process(xs[i], **kw), i)
         c.launch()
         c.check(ref.process(xs[i], **kw), i)
+
+
+def test_the_most_rows(hip):
+    print("case: most rows", flush=True)
+    rng = np.random.default_rng(11)
+    x = rng.standard_normal((65535, 33)).astype(np.float32)
+    h = rng.integers(0, 33, (65535, 4))
+    run(hip, x, "rows", hist=h, hist_len=rng.integers(0, 5, 65535), repeat=np.full(65535, 1.5, np.float32),
+        mask=rng.integers(0, 2 ** 32, (65535, 2), dtype=np.uint32))

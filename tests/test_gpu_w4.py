@@ -171,6 +171,65 @@ def test_large_offsets(hip):
     assert np.array_equal(got.reshape(2, -1, part), np.repeat(got[:, None, :part], out_d // part, 1))
 
 
+MANY = [  # in_d, out_d, group, rows: tiles of 64 rows, by 128 outputs or, the last three of them, by 256
+    (1024, 528, 128, 2300), (129, 20, 64, 11300), (128, 130, 32, 5700), (300, 1030, 64, 1300), (2200, 1030, 32, 1345),
+    (129, 4100, 32, 1000), (1030, 2600, 64, 1290), (640, 25700, 128, 100)]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("in_d,out_d,group,rows", MANY)
+def test_many_rows(hip, in_d, out_d, group, rows, bf16):
+    """Enough rows and outputs for the kernel of 64 rows; the last rows, outputs
+    and inputs end inside its tiles.  The same bits as of few rows."""
+    print(f"case: many rows {in_d} {out_d} {group} {rows} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(rows)
+    w, W = weight(hip, rng, in_d, out_d, group, f16=group == 32, floats=1 << 25)
+    x = inputs(rng, rows, in_d, bf16)
+    first = w.mem.at
+    whole = w.linear(x, bf16=bf16, pad=(1, 3), off=1, behind=2)
+    some = np.unique(np.concatenate([np.arange(70), rng.integers(0, rows, 100), np.arange(rows - 70, rows)]) % rows)
+    check(whole[some], W, x[some], bf16, rows)
+    for a, b in ((0, 5), (61, 77), (rows - 30, rows)):
+        w.mem.at = first
+        assert np.array_equal(w.linear(x[a:b], bf16=bf16).view(np.uint32), whole[a:b].view(np.uint32)), (a, b)
+    for act in (cb.W4_SILU, cb.W4_ADD):
+        w.mem.at = first
+        kw = dict(act=act, bias=ref.bf16_value(ref.bf16_bits(rng.standard_normal(out_d).astype(np.float32))), scale=-1.5)
+        if act == cb.W4_ADD:
+            kw["y"] = inputs(rng, rows, out_d, bf16)
+        got = w.linear(x, bf16=bf16, **kw)
+        if act == cb.W4_ADD:
+            kw["y"] = kw["y"][some]
+        check(got[some], W, x[some], bf16, (rows, act), **kw)
+
+
+@pytest.mark.parametrize("ld", [(1 << 24) - 1, (1 << 24) + 4])
+def test_rows_far_apart(hip, ld):
+    """Inputs whose offsets pass 32 bits, and nearly do."""
+    print(f"case: far apart {ld}", flush=True)
+    rng = np.random.default_rng(14)
+    for in_d, out_d in ((200, 22600), (200, 100)):
+        w, W = weight(hip, rng, in_d, out_d, 64, floats=66 * ld + (1 << 25))
+        x, at = inputs(rng, 66, in_d, False), w.mem.take(4 * 66 * ld)
+        for i, row in enumerate(x):
+            w.mem.write(at + 4 * i * ld, row)
+        y = w.mem.take(4 * 66 * out_d)
+        a = cb.BackendW4Linear(y=y, x=at, ld_y=out_d, ld_x=ld, rows=66)
+        hip.backend_linear_w4(w.h, C.byref(a))
+        check(w.mem.get(y, (66, out_d), np.float32), W, x, False, ld)
+
+
+@pytest.mark.parametrize("rows", [1 << 24, 70000])
+def test_the_most_rows(hip, rows):
+    """Inputs shorter than a tile and so many rows that they take more than 65535 workgroups."""
+    print(f"case: most rows {rows}", flush=True)
+    rng = np.random.default_rng(15)
+    w, W = weight(hip, rng, 3, 2, 32, floats=1 << 27)
+    x = inputs(rng, rows, 3, False)
+    got = w.linear(x)
+    check(got, W, x, False, rows)
+
+
 def test_nothing_to_do_and_captured(hip):
     """No rows: y stays.  Captured once and replayed, with eager calls between:
     the same bits, from the inputs of the moment."""
