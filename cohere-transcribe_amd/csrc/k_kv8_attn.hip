@@ -322,6 +322,49 @@ __device__ __forceinline__ int find_item(const Args &a, int part, int id, Groups
     return ch;
 }
 
+// Sequence `id`'s tile where no row masks a token: if all tokens of all its group
+// are common and the group's rows fit one tile, they are the tile of its first
+// sequence that has rows (then row[i] is the i-th), and there is none for the
+// others; else the sequence's own rows, as find_tile finds them.
+template <int W>
+__device__ __forceinline__ bool find_group(const Args &a, int id, int *sh, int *row, Tile &t, bool &common) {
+    const int s = threadIdx.x;
+    int r0 = 0, n = 0, len = 0, l = -1;
+    if (s < a.seqs) {
+        r0 = a.rows[s];
+        n = a.rows[s + 1] - r0;
+        len = a.len[s];
+        l = a.share[s];
+        if (r0 < 0 || n <= 0 || n > a.n_rows - r0 || n > a.most) n = 0;
+    }
+    t.r0 = a.rows[id];
+    t.n = a.rows[id + 1] - t.r0;
+    t.len = max(a.len[id], 0);
+    if (t.r0 < 0 || t.n <= 0 || t.n > a.n_rows - t.r0 || t.n > a.most) return false;
+    t.end = min(t.len, a.cap);
+    const int lead = a.share[id];
+    const bool led = (unsigned)lead < (unsigned)a.seqs && a.share[lead] == lead && a.share[a.seqs + lead] >= t.end;
+    // a sequence that holds other tokens, or too many rows, counts as 4096
+    const int mine = led && l == lead ? (min(max(len, 0), a.cap) == t.end ? min(n, 4096) : n ? 4096 : 0) : 0;
+    int total;
+    const int to = group_sum<W>(mine, sh, total), from = to - mine;
+    common = total > t.n && total * a.group <= 16;
+    t.seq = id;
+    if (common) {
+        if (s == id) sh[W] = from;
+        for (int i = from; i < to; i++) row[i] = r0 + i - from;
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(sh[W]) != 0) return false;
+        t.seq = lead;
+        t.n = total;
+    }
+    t.row = t.lo = t.sink_steps = t.full_lo = t.base = 0;
+    t.pos0 = t.len - t.n;
+    t.steps = (t.end + 31) >> 5;
+    t.full_hi = t.end;
+    return true;
+}
+
 __device__ __forceinline__ int step_key(const Tile &t, int step) {
     return step < t.sink_steps ? step << 5 : t.lo + ((step - t.sink_steps) << 5);
 }
@@ -716,34 +759,40 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
 // one of 376 tokens 6.7 us, of which 4.7 are an empty call's.  fp32
 // rows take two terms each, so twice the products.
 // ONCE: a sequence's rows are one tile, so its codes are read once.
-// SHARED: a workgroup takes either rows of a group over its common tokens (the
-// first pitems items) or a sequence's rows over the others, and leaves its sums.
-template <int D, bool BF16, int W, bool ONCE, bool SHARED>
+// HOW: ALONE, a sequence's rows.  APART, a workgroup takes either rows of a group
+// over its common tokens (the first pitems items) or a sequence's rows over the
+// others, and leaves its sums.  GROUPS, rows of a group that has all tokens in
+// common, or else a sequence's.
+enum How { ALONE, APART, GROUPS };
+template <int D, bool BF16, int W, bool ONCE, How HOW>
 __device__ __forceinline__ void attn_body(const Args &a, const int id, const int h, float *so) {
     constexpr int KS = D / 32;            // k steps of the score product
     constexpr int DI = D / 16;            // 16-dim tiles of O; dims of V a lane loads
     constexpr int NB = BF16 ? 1 : 2;      // f16 terms of a query value and of p
+    constexpr bool SHARED = HOW == APART;
     // the wavefronts' sums so [W][rpt][D], maxima and l [W][16]: of the rows a tile
     // has, mostly one
     __shared__ int sh[W + 5];
     __shared__ float sm[W][16], sl[W][16];
     __shared__ std::conditional_t<SHARED, Groups, int> gr;
-    __shared__ int grow[SHARED ? 16 : 1];        // rows of a tile of common tokens
+    __shared__ int grow[HOW != ALONE ? 16 : 1];  // rows of a tile of common tokens
 
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE), c = lane & 15, g = lane >> 4;
     // this wavefront's steps: first, first + W, ...; lane i keeps the page and
     // the scales of 16-key half i (-1: not in the pool).  Where a step's keys do
     // not depend on the lengths, its page is read along with them.
-    const bool common = SHARED && id < a.pitems;
+    bool common = SHARED && id < a.pitems;
     int ch = blockIdx.y, chunk = a.chunk;
     Tile t;
     if constexpr (SHARED) ch = find_item<W>(a, !common, common ? id : id - a.pitems, gr, grow, t, chunk);
     const int first = ch * chunk + w;
-    const bool ahead = !SHARED && a.one_tile && !a.window;
+    const bool ahead = HOW == ALONE && a.one_tile && !a.window;
     int key_i = 32 * (first + W * (lane >> 1)) + 16 * (lane & 1), pg = -1;
     if (ahead && (lane >> 1) * W < chunk && key_i < a.cap) pg = a.table[(long)id * a.table_w + (key_i >> a.lp)];
-    if constexpr (!SHARED)
+    if constexpr (HOW == ALONE)
         if (!find_tile<W>(a, id, 16, sh, t)) return;
+    if constexpr (HOW == GROUPS)
+        if (!find_group<W>(a, id, sh, grow, t, common)) return;
     const int chunks = !SHARED && a.nchunk > 1 ? (t.steps + chunk - 1) / chunk : 1;
     // a tile of own tokens may end before the last of its sequence's chunks
     if (SHARED ? ch < 0 || ch * chunk >= t.steps : ch >= max(chunks, 1)) return;
@@ -921,7 +970,7 @@ __device__ __forceinline__ void attn_body(const Args &a, const int id, const int
         for (int st = first; st < last; st += W) spread_nan<D, 1, SHARED>(a, t, h, step_key(t, st), c, g, pos, o);
 
     // the wavefronts' sums joined, in their order
-    const int so_rows = SHARED ? 16 : a.rpt;
+    const int so_rows = HOW != ALONE ? 16 : a.rpt;
     l = sum_q(l);
     if (have) {
         if (g == 0) { sm[w][c] = m; sl[w][c] = l; }
@@ -952,7 +1001,7 @@ __device__ __forceinline__ void attn_body(const Args &a, const int id, const int
         } else if (chunks <= 1) {
             const int R2 = t.row + r, i = a.group > 1 ? R2 / a.group : R2;
             const float y = den == 0.0f ? 0.0f : num * ONE_V / den;
-            const long off = (long)(t.r0 + i) * a.ld_out + (long)(h * a.group + R2 - i * a.group) * D + d;
+            const long off = (long)(common ? grow[i] : t.r0 + i) * a.ld_out + (long)(h * a.group + R2 - i * a.group) * D + d;
             if (BF16) reinterpret_cast<uint16_t *>(a.out)[off] = f2bf(y);
             else reinterpret_cast<float *>(a.out)[off] = y;
         } else {
@@ -969,7 +1018,7 @@ __global__ __launch_bounds__(W * CT_WAVE, BF16 ? 3 : 2) void attn_kernel(Args a)
     // heads vary fastest: workgroup i runs on XCD i % 8, so with 8 kv heads the
     // tiles of one head share an L2
     const int id = blockIdx.x / a.kv, h = blockIdx.x - id * a.kv;
-    attn_body<D, BF16, W, ONCE, false>(a, id, h, so);
+    attn_body<D, BF16, W, ONCE, ALONE>(a, id, h, so);
 }
 
 // Many rows of a sequence: a workgroup holds 128 packed rows, 32 a wavefront
@@ -1380,7 +1429,18 @@ __global__ __launch_bounds__(NT, WIDE || !BF16 ? 2 : 3) void shared_kernel(Args 
     __shared__ __align__(16) char mem[WIDE && OPS > SUMS ? OPS : SUMS];
     const int id = blockIdx.x / a.kv, h = blockIdx.x - id * a.kv;
     if (WIDE && id < a.pitems) rows_body<D, BF16, true>(a, reinterpret_cast<Operands<D> &>(mem));
-    else attn_body<D, BF16, NW, true, true>(a, id, h, reinterpret_cast<float *>(mem));
+    else attn_body<D, BF16, NW, true, APART>(a, id, h, reinterpret_cast<float *>(mem));
+}
+
+// Sequences whose tokens are all common, as a clip's hypotheses have them, in one
+// launch: a workgroup for each of them, of which those that do not begin a group
+// leave.  24 clips of up to 376 tokens, 5 hypotheses each, 8 heads, fp32 (18 MB of
+// codes): 13.1 us, of which an empty call's are 4.7, finding the group some 2.
+template <int D, bool BF16>
+__global__ __launch_bounds__(NT, 2) void groups_kernel(Args a) {
+    __shared__ __align__(16) float so[NW * 16 * D];
+    const int id = blockIdx.x / a.kv, h = blockIdx.x - id * a.kv;
+    attn_body<D, BF16, NW, true, GROUPS>(a, id, h, so);
 }
 
 // Joins a tile's chunks, in an order that the lengths alone give (32 x 4 heads
@@ -1794,12 +1854,31 @@ extern "C" size_t ctk_kv8_attn_shared_work(const BackendKv8 *c, const BackendKv8
 
 extern "C" void ctk_kv8_attn_shared(const BackendKv8 *c, int layer, const BackendKv8Attn *p, const int *share, hipStream_t s) {
     const SharedShape sh = shared_shape_of(c, p);
-    if (!sh.apart) {
+    const Shape plain = shape_of(c, p);
+    // A group's rows in one workgroup, where all tokens may be common and there
+    // are so many sequences that those that leave free CUs for it (fp32, 376
+    // tokens, 8 heads, groups of sequences; us by groups / each alone: 13 of 5, 520
+    // units 9.5 / 12.5; 24 of 5 13.1 / 17.3; 48 of 5 17.7 / 29.2; 40 of 3 with 60
+    // tokens 9.0 / 11.2; but 1 of 64, 512 units 10.6 / 9.7; 24 of 2 11.4 / 10.4; bf16 8
+    // of 8 with 700 tokens 16.9 / 12.4).  8 wavefronts each: 24 of 5 16.1.
+    const bool groups = !sh.apart && !p->causal && plain.one_tile && plain.tile_rows == 16 && plain.nchunk == 1 &&
+                        plain.tiles * c->kv_heads > 512;
+    if (!sh.apart && !groups) {
         ctk_kv8_attn(c, layer, p, s);
         return;
     }
     Args a = args_of(c, layer, p);
     a.share = share;
+    if (groups) {
+        a.most = p->max_rows < p->n_rows ? p->max_rows : p->n_rows;
+        a.one_tile = 1; a.chunk = plain.chunk; a.nchunk = 1;
+        const dim3 grid((unsigned)(c->kv_heads * plain.tiles));
+#define GROUPS(D, B) hipLaunchKernelGGL((groups_kernel<D, B>), grid, dim3(NT), 0, s, a)
+        if (c->head_dim == 64) { if (p->bf16) GROUPS(64, true); else GROUPS(64, false); }
+        else { if (p->bf16) GROUPS(128, true); else GROUPS(128, false); }
+#undef GROUPS
+        return;
+    }
     a.most = p->max_rows < p->n_rows ? p->max_rows : p->n_rows;
     a.tile_rows = sh.tile_rows; a.one_tile = sh.one_tile; a.rpt = sh.rpt;
     for (int i = 0; i < 2; i++) { a.want[i] = sh.want[i]; a.least[i] = sh.least[i]; }

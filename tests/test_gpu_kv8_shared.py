@@ -196,6 +196,100 @@ def test_all_sequences_of_a_cache(hip, bf16):
     run(hip, rng, 16, 1, 1, 64, [(0, [20 + i]) for i in range(256)], 1, "alone", bf16=bf16)
 
 
+def short(hip, rng, P, kv, group, D, groups, n, what, bf16, max_len=None, share=None, zero=()):
+    """A call that is small enough for one workgroup a group, every row seeing all tokens."""
+    d, lens, of = family(hip, rng, P, kv, D, groups, rows=1)
+    assert len(lens) * kv > 512
+    for s in zero:
+        d.model.len[s] = 0
+    d.push()
+    n = [min(x, max(y, 1)) for x, y in zip([n] * len(lens) if isinstance(n, int) else n, lens)]
+    rows = starts(n)
+    q = values(rng, int(rows[-1]) + 2, kv * group, D)
+    p = found(d)[0] if share is None else d.ints(share(d))
+    max_len = max_len or max(lens)
+    want = d.model.attend(0, q, kv * group, D ** -0.5, False, 0, 0, rows, len(q), max_len)
+    for pad, off in ((0, 0), (5, 3)):
+        got = attend(d, 0, q, kv * group, p, rows, False, bf16, max_len=max_len, apart=False, pad=pad, off=off)
+        check_rows(got, *want, bf16, what)
+    return d, rows, q, p, max_len
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("P,kv,group,D", [(16, 8, 1, 128), (64, 8, 1, 64), (32, 4, 4, 128), (16, 3, 2, 64), (128, 16, 16, 64)])
+def test_whole_groups(hip, P, kv, group, D, bf16):
+    """Many clips' hypotheses in one launch; beside them groups with tokens of
+    their own, of too many rows for a tile, and sequences alone, empty or without rows."""
+    print(f"case: whole groups P={P} kv={kv} group={group} D={D} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(P + kv + 7)
+    each = max(1, 16 // group)
+    groups = [(c, [c] * k) for c, k in ((376, 5), (1, 3), (33, 2), (129, 4), (31, 1), (300, each), (64, each + 1), (200, 2))]
+    groups += [(128, [130, 129, 140]), (256, [256, 256, 300]), (0, [77])] + [(40 + i, [40 + i] * (1 + i % 4)) for i in range(12)]
+    groups += [(50, [50, 50])] * max(0, (514 // kv - sum(len(m) for _, m in groups) + 3) // 2)
+    seqs = sum(len(m) for _, m in groups)
+    short(hip, rng, P, kv, group, D, groups, 1, "tokens", bf16)
+    short(hip, rng, P, kv, group, D, groups, 1, "capped", bf16, max_len=100)
+    short(hip, rng, P, kv, group, D, groups, 1, "empty", bf16, zero=range(0, seqs, 3))
+    most = [int(x) for x in rng.integers(0, 16 // group + 1, seqs)]
+    short(hip, rng, P, kv, group, D, groups, most, "rows", bf16)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_whole_groups_of_a_caller(hip, bf16):
+    """Fewer common tokens than there are, leaders out of range or without tokens."""
+    print(f"case: whole groups, given bf16={bf16}", flush=True)
+    groups = [(96, [96] * 4)] * 20
+
+    def given(change):
+        def make(d):
+            s = model_share(d.model)
+            change(s)
+            return s
+        return make
+
+    def tokens(t):
+        def change(s):
+            s[1, ::2] = t
+        return change
+
+    def leaders(l):
+        def change(s):
+            s[0, 3::4] = l
+        return change
+    for change in (tokens(95), tokens(0), tokens(-1), tokens(2 ** 31 - 1), leaders(-1), leaders(40), leaders(2 ** 31 - 1), leaders(13),
+                   leaders(-2 ** 31)):
+        short(hip, np.random.default_rng(12), 32, 8, 2, 64, groups, 1, "given", bf16, share=given(change))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_whole_groups_bad_pages(hip, bf16):
+    """Missing pages, NaN in K, V and q; rows out of range and more than max_rows."""
+    print(f"case: whole groups, bad pages bf16={bf16}", flush=True)
+    rng = np.random.default_rng(13)
+    d, rows, q, p, max_len = short(hip, rng, 16, 16, 1, 64, [(200, [200] * 5), (90, [90] * 3)] * 6, 1, "fine", bf16)
+    m, seqs = d.model, len(rows) - 1
+    first = m.table[:, 0].copy()
+    for lead in range(seqs):
+        mine = np.flatnonzero(first == first[lead])
+        if mine[0] == lead and lead % 2:
+            m.table[mine, 2] = 10 ** 6
+        if mine[0] == lead and lead % 3 == 0:
+            m.v[0, m.table[lead, 1], 2, 7, 9] = 0x7F
+            m.k[0, m.table[lead, 3], 5, 3, 1] = 0xFF
+    d.push()
+    q[1, 3, 5], q[4, 0, 0] = np.inf, np.nan
+    odd = rows.copy()
+    odd[5:8] = [9, 4, 60]
+    for r in (rows, odd):
+        want = m.attend(0, q, 16, 0.125, False, 0, 0, r, len(q), max_len)
+        got = attend(d, 0, q, 16, found(d)[0], r, False, bf16, max_rows=16, max_len=max_len, apart=False)
+        # odd: row 8 is both the fifth row of sequence 4 (rows 4 .. 8) and sequence 8's
+        # own (8 .. 8), so either's result may stand there
+        one = np.array([sum(a <= i < b for a, b in zip(r, r[1:]) if 0 <= a and b <= len(q)) < 2 for i in range(len(q))])
+        assert list(np.flatnonzero(~one)) == ([8] if r is odd else [])
+        check_rows(got[one], *(x[one] for x in want), bf16, r.tolist())
+
+
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("kw", [dict(max_len=200, apart=False), dict(max_len=33, apart=False), dict(pad=3, off=5), dict(pad=8, off=8),
                                 dict(scale=3.0), dict(max_len=10 ** 9)])
