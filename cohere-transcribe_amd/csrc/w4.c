@@ -74,6 +74,7 @@ void backend_linear_w4(const BackendW4 *w, const BackendW4Linear *a) {
     const uintptr_t al = a->bf16 ? 1 : 3;
     if (!a->x || !a->y || ((uintptr_t)a->x & al) || ((uintptr_t)a->y & al))
         CT_FATAL("linear_w4: x or y is NULL or not aligned");
+    if (a->x == a->y) CT_FATAL("linear_w4: y is x");
     if (a->ld_x < w->in_d || a->ld_y < w->out_d) CT_FATAL("linear_w4: ld_x below in_d or ld_y below out_d");
     if ((uintptr_t)a->bias & 1) CT_FATAL("linear_w4: bias is not aligned");
     require_init();

@@ -58,6 +58,7 @@ CASES = {
     "linear_ld_y": (LIN, dict(ld_y=63), "ld_y below"),
     "linear_bias": (LIN, dict(bias=4097), "bias is not aligned"),
     "linear_before_init": (LIN, {}, "has not called backend_init"),
+    "linear_in_place": (LIN, dict(y=4096, x=4096), "y is x"),
     "load_before_init": ("L.backend_w4_load(r(w), 4096, 4096, None)", {}, "has not called backend_init"),
     "logits_null": ("L.backend_logits(None)", {}, "no arguments"),
     "logits_rows": (LOG, dict(rows=65536), "rows outside"),
@@ -130,6 +131,34 @@ def test_logits_work():
         assert a == sorted(a)
     for a, b in zip(work, work[1:]):
         assert all(x <= y for x, y in zip(a, b))
+
+
+def test_shared_work_covers_smaller_calls():
+    """Work sized once is enough for every smaller call, of either type, and
+    never less for a larger one; what a call needs is within what it is told."""
+    L = cb.hip()
+    for f in (L.ctk_kv8_attn_shared_need, L.backend_kv8_attn_shared_work):
+        f.argtypes, f.restype = [C.c_void_p, C.c_void_p], C.c_size_t
+    rng = np.random.default_rng(0)
+    apart = 0
+    for _ in range(300):
+        kv, group = int(rng.choice([1, 2, 8, 16])), int(rng.choice([1, 2, 4, 8]))
+        c = cb.BackendKv8(layers=1, pages=50, page_tokens=int(rng.choice([16, 64, 128])), kv_heads=kv, head_dim=int(rng.choice([64, 128])),
+                          seqs=int(rng.choice([1, 2, 7, 64, 256])), table_w=int(np.exp(rng.uniform(0, 9))))
+
+        def call(n_rows, max_rows, max_len, bf16, causal):
+            return cb.BackendKv8Attn(out=4096, q=4096, ld_out=kv * group * 128, ld_q=kv * group * 128, heads=kv * group, scale=1.0,
+                                     rows=4096, n_rows=n_rows, max_rows=max_rows, max_len=max_len, bf16=bf16, causal=causal)
+        n, m, ml = (int(np.exp(rng.uniform(0, x))) for x in (8, 6, 11))
+        whole = L.backend_kv8_attn_shared_work(C.byref(c), C.byref(call(n, m, ml, 0, 1)))
+        assert whole == L.backend_kv8_attn_shared_work(C.byref(c), C.byref(call(n, m, ml, 1, 0)))
+        for _ in range(10):
+            a = call(int(rng.integers(1, n + 1)), int(rng.integers(1, m + 1)), int(rng.integers(1, ml + 1)), int(rng.integers(2)),
+                     int(rng.integers(2)))
+            need, work = (f(C.byref(c), C.byref(a)) for f in (L.ctk_kv8_attn_shared_need, L.backend_kv8_attn_shared_work))
+            assert need <= work <= whole
+            apart += need > 0
+    assert apart > 300
 
 
 def test_struct_mirrors(tmp_path):

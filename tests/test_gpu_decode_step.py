@@ -213,3 +213,24 @@ def test_steps(hip, wide):
         got = decode(hip, wide, mode)
         for i, (a, b) in enumerate(zip(want, got)):
             assert a[0] == b[0] and np.array_equal(a[1], b[1]), (mode, i)
+
+
+def test_two_threads(hip):
+    """Two threads with a stream and memory each, at once: what each gets alone."""
+    print("case: decode steps, two threads", flush=True)
+    import threading
+    alone, both = [decode(hip, wide, "eager") for wide in (True, False)], [None, None]
+
+    def run(i):
+        hip.backend_init(0)
+        both[i] = [decode(hip, i == 0, "eager") for _ in range(3)]
+        hip.backend_thread_cleanup()
+
+    ts = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join(60)
+    for one, three in zip(alone, both):
+        for got in three:
+            assert all(a[0] == b[0] and np.array_equal(a[1], b[1]) for a, b in zip(one, got))
