@@ -7,7 +7,9 @@
 // banned (whole numbers, so the order of the atomics changes nothing); then
 // through the bias list, which leaves each token's last entry in the same
 // word.  4 bytes a logit are read and, where wanted, 4 written: bound by memory
-// where there are many, else by the chain history, LDS, largest.  A row's
+// where there are many (200 x 100003, 165 MB: 46 to 49 us, of which a copy of as much
+// takes 34.5), else by the chain history, LDS, largest (5 x 16384: 7.7 us, 64 x
+// 16384 with histories of 1000: 8.9; a call of one workgroup is 3.6).  A row's
 // workgroups meet in one 64-bit maximum of (value, lowest id) in memory; the
 // last of them writes the token and leaves the memory as it was.
 #include "ct_dev.h"
@@ -262,6 +264,9 @@ __global__ __launch_bounds__(NT, 6) void logits_kernel(BackendLogits a) {
     if (a.score) a.score[r] = top;
 }
 
+// 512 threads go through a row's history half as often as 256 (200 x 100003: 46 us,
+// with 1024 48); a row that 256 hold has no use for more (300 x 4000: 8.2 us, 512
+// 8.8; 1 x 4000: 6.2, 6.7).
 int threads_of(const BackendLogits *a) { return a->vocab > EACH * SMALL ? LARGE : SMALL; }
 
 }  // namespace

@@ -18,9 +18,9 @@
 // joined in order, in every kernel here, so that a row's answer does not depend
 // on how many rows the call has.
 //
-// What bounds them, at the listed times of one MI355X.  One row: the launch and one
-// pass of loads (1024 -> 4096, 2.2 MB: 4.0 us).  Few rows of large maps: the codes'
-// bytes (1 x 8192 -> 24576, 106 MB: 22.4 us, 4.7 TB/s).  Many rows: vector
+// What bounds them.  One row of a small map: the launch and one pass of loads
+// (1024 -> 1024, 0.55 MB: 3.8 us, where a call of one workgroup takes 3.6).  Few rows of large maps: the codes'
+// bytes (1 x 8192 -> 24576, 106 MB: 22.5 us, 4.7 TB/s).  Many rows: vector
 // instructions that prepare both operands, which do not overlap the products (752 x
 // 1280 -> 5120: 32 us, 308 Tflop/s of them, twice that of f16 terms).
 #include "ct_dev.h"
@@ -765,9 +765,15 @@ extern "C" void ctk_w4_linear(const BackendW4 *w, const BackendW4Linear *p, hipS
         return;
     }
     if (few) {
-        const int two = w->group > 32 && inputs <= 120 << 10 && (long)a.otiles * rt >= 1024;     // a word for each 32 does not fit twice
+        // two tiles of outputs at a time share the inputs' loads from LDS (64 x 1024 ->
+        // 4096: 7.1 us, one at a time 8.3; 256 x 1024 -> 4096: 17.9, 24.2; 1 x 8192 ->
+        // 24576: 22.5, 24.8), but for few tiles, which it leaves to fewer workgroups (1 x
+        // 1024 -> 1024: 4.1, 3.8; 64 x 1024 -> 1024: 5.4, 5.1); words for each 32 inputs do
+        // not fit the registers twice
+        const int two = w->group > 32 && inputs <= 120 << 10 && (long)a.otiles * rt >= 1024;
         const int groups = (a.otiles + two) / (1 + two);
-        // as many workgroups as the CUs hold at once
+        // as many workgroups as the CUs hold at once: one more than that is a second round
+        // for all (48 x 1024 -> 16384 in 513 of them 28 us, in 510 18.5)
         const long fit = inputs + (two ? 32768 : 16384) <= 80 << 10 ? 512 : 256;
         const dim3 grid((unsigned)(groups * rt <= fit ? groups : rt < fit ? fit / rt : 1), (unsigned)rt);
 #define FEW(B, GS)                                                                                                              \
