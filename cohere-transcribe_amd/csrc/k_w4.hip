@@ -222,40 +222,47 @@ __device__ __forceinline__ void finish(const Args &a, long t, int o, float v) {
     }
 }
 
-// Rows whose inputs do not fit LDS: one tile of outputs a workgroup, 16 rows at a
-// time; its eight wavefronts each take one segment of the inputs, split them a tile
+// Work of a round or few: NT tiles of outputs a workgroup, 16 rows at a time; its eight wavefronts each take one segment of the inputs, split them a tile
 // at a time and join their sums in LDS, in order.  A wavefront has AHEAD tiles of
-// codes and inputs in flight.  64 x 4096 -> 1024: 9.5 us.
-template <bool BF16, int GS>
+// codes and inputs in flight, or, of four tiles together, asks for each operand of
+// the next one as this one leaves its registers (two whole sets spill).  64 x 1024 -> 4096:
+// 6.1 us, bound by the chain of loads, split, products and join; 64 x 4096 -> 4096
+// 13.6, by the vector instructions that make operands of codes and inputs.
+template <bool BF16, int GS, int NT>
 __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
-    constexpr int NB = BF16 ? 1 : 2, RR = 16, RI = RR / 4, AHEAD = 2;
+    constexpr int NB = BF16 ? 1 : 2, RR = 16, RI = RR / 4, AHEAD = NT == 4 ? 1 : 2;
     __shared__ __align__(16) union {
         f16x8 x[SEGS][NB][16 * RR];
-        float sum[SEGS][RR][TO];
+        float sum[SEGS][NT][RR][TO];
     } sh;
     __shared__ __align__(16) float sundo[SEGS][RR];
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE);
     const int c = lane & 15, q = lane >> 4;
         const int k0 = w * a.per, k1 = min(k0 + a.per, a.itiles);
     struct Ahead {
-        u32x4 code;
-        uint32_t word[4 / GS];
+        u32x4 code[NT];
+        uint32_t word[NT][4 / GS];
         float v[RI][8];
     };
     for (long r0 = (long)RR * blockIdx.y; r0 < a.rows; r0 += (long)RR * gridDim.y) {
         const int nr = (int)min((long)RR, a.rows - r0);
-        f32x4 sum = {0, 0, 0, 0};
-        Ahead t[AHEAD];
-        auto fetch = [&](int kt, Ahead &f) __attribute__((always_inline)) {
-            const long tile = (long)blockIdx.x * a.itiles + kt;
-            f.code = reinterpret_cast<const u32x4 *>(a.codes)[tile * CT_WAVE + lane];
+        f32x4 sum[NT];
 #pragma unroll
-            for (int g = 0; g < 4 / GS; g++) f.word[g] = a.scales[(tile * 16 + c) * (4 / GS) + g];
+        for (int n = 0; n < NT; n++) sum[n] = (f32x4){0, 0, 0, 0};
+        Ahead t[AHEAD];
+        auto fetch_w = [&](int kt, int n, Ahead &f) __attribute__((always_inline)) {
+            const long tile = (long)min((int)blockIdx.x * NT + n, a.otiles - 1) * a.itiles + kt;
+            f.code[n] = reinterpret_cast<const u32x4 *>(a.codes)[tile * CT_WAVE + lane];
+#pragma unroll
+            for (int g = 0; g < 4 / GS; g++) f.word[n][g] = a.scales[(tile * 16 + c) * (4 / GS) + g];
+        };
+        auto fetch_x = [&](int kt, Ahead &f) __attribute__((always_inline)) {
             if (kt * TI + TI <= a.in_d)
 #pragma unroll
                 for (int i = 0; i < RI; i++)
                     if (q + 4 * i < nr) fetch8<BF16>(input_at<BF16>(a, r0 + q + 4 * i, kt * TI + 8 * c), f.v[i]);
         };
+        // what the tile leaves takes the one AHEAD of it at once (past the last one: that again)
         auto use = [&](int kt, Ahead &f) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < RI; i++) {
@@ -271,6 +278,8 @@ __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
                     if (c == 0) sundo[w][r] = undo;
                 }
             }
+            const int next = min(kt + AHEAD, k1 - 1);
+            fetch_x(next, f);
             // the wavefront's own part of LDS: its accesses are in order
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -280,30 +289,39 @@ __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) xf[n][j] = sh.x[w][n][piece(4 * j + q, c)];
             const f32x4 undo = *reinterpret_cast<const f32x4 *>(&sundo[w][4 * q]);
-            tile_product<NB, GS>(f.code, f.word, a.scale_f16, xf, undo, sum);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                tile_product<NB, GS>(f.code[n], f.word[n], a.scale_f16, xf, undo, sum[n]);
+                fetch_w(next, n, f);
+            }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         };
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
-            if (k0 + i < k1) fetch(k0 + i, t[i]);
+            if (k0 + i < k1) {
+                fetch_x(k0 + i, t[i]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) fetch_w(k0 + i, n, t[i]);
+            }
         for (int kt = k0; kt < k1; kt += AHEAD)
 #pragma unroll
             for (int i = 0; i < AHEAD; i++)
-                if (kt + i < k1) {
-                    use(kt + i, t[i]);
-                    if (kt + i + AHEAD < k1) fetch(kt + i + AHEAD, t[i]);
-                }
+                if (kt + i < k1) use(kt + i, t[i]);
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; i++) sh.sum[w][4 * q + i][c] = sum[i];
-        __syncthreads();
-        const int r = threadIdx.x >> 4, o = blockIdx.x * TO + c;
-        if (r < nr && o < a.out_d) {
-            float v = 0.0f;
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int s = 0; s < SEGS; s++) v += sh.sum[s][r][c];
-            finish<BF16>(a, r0 + r, o, v);
+            for (int i = 0; i < 4; i++) sh.sum[w][n][4 * q + i][c] = sum[n][i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < NT * RR * TO; i += SEGS * CT_WAVE) {
+            const int n = i / (RR * TO), r = i >> 4 & (RR - 1), o = (blockIdx.x * NT + n) * TO + c;
+            if (r < nr && o < a.out_d) {
+                float v = 0.0f;
+#pragma unroll
+                for (int s = 0; s < SEGS; s++) v += sh.sum[s][n][r][c];
+                finish<BF16>(a, r0 + r, o, v);
+            }
         }
         __syncthreads();
     }
@@ -314,7 +332,8 @@ __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
 // time; its eight wavefronts each take one segment of the inputs and join
 // their sums in LDS, in order.  A wavefront has AHEAD tiles of codes in flight,
 // those of the next outputs among them, from before the inputs are split.
-// 64 x 1024 -> 4096: 7.2 us, of which about 3 are the split and one pass of loads.
+// Where linear_kernel would take many rounds, splitting inputs in each: 1 x 8192 -> 24576
+// 22.5 us, there 36.
 constexpr int FEW_LDS = 136 << 10;           // of inputs, beside 16 KB of sums, within a CU's 160
 
 template <bool BF16, int GS, int NT>
@@ -735,14 +754,28 @@ extern "C" void ctk_w4_linear(const BackendW4 *w, const BackendW4Linear *p, hipS
     const int lr = rows == 1 ? 0 : rows <= 4 ? 2 : rows <= 8 ? 3 : 4;
     const size_t inputs = (size_t)a.itiles * ((256 * (p->bf16 ? 1 : 2) + 4) << lr);
     const long rt = (rows + (1 << lr) - 1) >> lr;
-    const bool few = inputs <= FEW_LDS && rt <= 65535;
+    const bool fits = inputs <= FEW_LDS && rt <= 65535;
+    // linear_kernel's tiles of outputs together.  A CU holds one of its workgroups: as few
+    // rounds of them as there can be.  Two cost 1.2 times one, four 1.4 (one / two / four in
+    // us: 64 x 4096 -> 1024, 256 tiles 9.6 / 10.5 / 12.6; 64 x 5120 -> 1280, 320 tiles 19 /
+    // 12.7 / 15.6; 64 x 4096 -> 4096, 1024 tiles 31 / 20.8 / 13.6; bf16 16 x 8192 -> 8192,
+    // 512 tiles 34 / 23 / 26; 64 x 8192 -> 8192, 2048 tiles 129 / 85 / 49).
+    const long rt16 = (rows + 15) / 16;
+    auto rounds = [&](int n) { return ((a.otiles + n - 1) / n * rt16 + 255) / 256; };
+    const int nt = rounds(4) * 14 < rounds(2) * 12 && rounds(4) * 14 < rounds(1) * 10 ? 4 : rounds(2) * 12 < rounds(1) * 10 ? 2 : 1;
+    // It takes inputs that fit LDS too where it is done in one round, or in three for fp32
+    // rows that fill its tiles (it / linear_few_kernel: 64 x 1024 -> 4096 6.2 / 7.0 us; 5 x
+    // 1024 -> 16384 5.8 / 6.9; 3 x 8192 -> 8192 14.2 / 19.6; three rounds: 48 x 1024 -> 16384
+    // 15.9 / 18.5; four: 64 x 1024 -> 16384 20.7 / 19.2; bf16, two: 1 x 8192 -> 24576 36 /
+    // 22.5; four: 256 x 1024 -> 4096 19.3 / 12.7).
+    const bool few = fits && rounds(nt) > (rows > 16 && !p->bf16 ? 3 : 1);
     // Many rows in tiles of 64 once these fill the card.  With the inputs in LDS in us, few /
     // rows, in 128 workgroups of 64 rows: 64 x 1024 -> 16384 19.3 / 24.1; in 160: 300 x 1024
     // -> 4096 23.6 / 24.5; in 176: 700 x 1024 -> 2048 28.8 / 24.8; in 256: 128 x 1024 ->
-    // 16384 35 / 25.  Inputs that do not fit LDS are split again for each tile of
-    // outputs otherwise, in 64: 64 x 4096 -> 8192 59 / 66 (bf16 64 x 8192 -> 8192 129 /
-    // 108); in 80: 480 x 5120 -> 1280 87 / 81; in 120: 752 x 5120 -> 1280 129 / 81.
-    if (rt64 * ((w->out_d + 127) / 128) >= (few ? 176 : 72) && rows > 32 && w->in_d >= TI && p->ld_x < 1 << 24) {
+    // 16384 35 / 25.  Inputs that do not fit LDS, linear_kernel / rows: in 120: 752 x 5120
+    // -> 1280 58 / 81; in 128: bf16 256 x 8192 -> 4096 95 / 108; in 150: 900 x 5120 -> 1280
+    // 73 / 81, some 11 us for each of its rounds.
+    if (rt64 * ((w->out_d + 127) / 128) >= (fits ? 176 : p->bf16 ? 144 : 200) && rows > 32 && w->in_d >= TI && p->ld_x < 1 << 24) {
         // 256 outputs a workgroup where that leaves enough of them: 752 x 5120 -> 1280, 60
         // of them, 104 us instead of 84; 752 x 1280 -> 5120, 240, 32 instead of 38
         const int wide = rt64 * ((w->out_d + 255) / 256) >= 200;
@@ -765,12 +798,10 @@ extern "C" void ctk_w4_linear(const BackendW4 *w, const BackendW4Linear *p, hipS
         return;
     }
     if (few) {
-        // two tiles of outputs at a time share the inputs' loads from LDS (64 x 1024 ->
-        // 4096: 7.1 us, one at a time 8.3; 256 x 1024 -> 4096: 17.9, 24.2; 1 x 8192 ->
-        // 24576: 22.5, 24.8), but for few tiles, which it leaves to fewer workgroups (1 x
-        // 1024 -> 1024: 4.1, 3.8; 64 x 1024 -> 1024: 5.4, 5.1); words for each 32 inputs do
-        // not fit the registers twice
-        const int two = w->group > 32 && inputs <= 120 << 10 && (long)a.otiles * rt >= 1024;
+        // two tiles of outputs at a time share the inputs' loads from LDS (256 x 1024 ->
+        // 4096: 17.9 us, one at a time 24.2; 1 x 8192 -> 24576: 22.5, 24.8); words for
+        // each 32 inputs do not fit the registers twice
+        const int two = w->group > 32 && inputs <= 120 << 10;
         const int groups = (a.otiles + two) / (1 + two);
         // as many workgroups as the CUs hold at once: one more than that is a second round
         // for all (48 x 1024 -> 16384 in 513 of them 28 us, in 510 18.5)
@@ -793,9 +824,13 @@ extern "C" void ctk_w4_linear(const BackendW4 *w, const BackendW4Linear *p, hipS
 #undef FEW
         return;
     }
-    const long rt16 = (rows + 15) / 16;
-    const dim3 grid((unsigned)a.otiles, (unsigned)(rt16 < 4096 ? rt16 : 4096));
-#define LINEAR(B, GS) hipLaunchKernelGGL((linear_kernel<B, GS>), grid, dim3(SEGS * CT_WAVE), 0, s, a)
+    const dim3 grid((unsigned)((a.otiles + nt - 1) / nt), (unsigned)(rt16 < 4096 ? rt16 : 4096));
+#define LINEAR(B, GS)                                                                                               \
+    do {                                                                                                            \
+        if (nt == 4) hipLaunchKernelGGL((linear_kernel<B, GS, 4>), grid, dim3(SEGS * CT_WAVE), 0, s, a);            \
+        else if (nt == 2) hipLaunchKernelGGL((linear_kernel<B, GS, 2>), grid, dim3(SEGS * CT_WAVE), 0, s, a);       \
+        else hipLaunchKernelGGL((linear_kernel<B, GS, 1>), grid, dim3(SEGS * CT_WAVE), 0, s, a);                    \
+    } while (0)
     if (p->bf16) {
         if (w->group == 32) LINEAR(true, 1);
         else if (w->group == 64) LINEAR(true, 2);

@@ -203,6 +203,48 @@ def test_many_rows(hip, in_d, out_d, group, rows, bf16):
         check(got[some], W, x[some], bf16, (rows, act), **kw)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("in_d,out_d,group,rows", [
+    (260, 17000, 32, 1), (260, 17000, 64, 3), (520, 17000, 128, 7), (260, 17000, 64, 13), (2048, 16500, 64, 13), (2300, 16450, 128, 6),
+    (7, 17000, 128, 2), (130, 4200, 64, 200), (130, 4200, 32, 190), (1100, 4200, 128, 65), (96, 4100, 32, 260)])
+def test_many_outputs(hip, in_d, out_d, group, rows, bf16):
+    """Inputs kept in LDS while a workgroup goes from outputs to outputs, one tile and two at a time."""
+    print(f"case: many outputs {in_d} {out_d} {group} {rows} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(in_d + rows)
+    w, W = weight(hip, rng, in_d, out_d, group, f16=group == 64, floats=1 << 25)
+    x, first = inputs(rng, rows, in_d, bf16), w.mem.at
+    whole = w.linear(x, bf16=bf16, pad=(1, 3), off=3, behind=2)
+    check(whole, W, x, bf16, rows)
+    w.mem.at = first
+    last = w.linear(x[-1:], bf16=bf16)
+    assert np.array_equal(last.view(np.uint32), whole[-1:].view(np.uint32))
+    kw = dict(act=cb.W4_ADD, bias=ref.bf16_value(ref.bf16_bits(rng.standard_normal(out_d).astype(np.float32))), scale=0.3,
+              y=inputs(rng, rows, out_d, bf16))
+    check(w.linear(x, bf16=bf16, **kw), W, x, bf16, (rows, "add"), **kw)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_long_inputs(hip, group, bf16):
+    """Inputs that do not fit LDS, one, two and four tiles of outputs together, the last ones fewer."""
+    print(f"case: long inputs {group} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(group)
+    in_d, out_d = 4300, 1030
+    w, W = weight(hip, rng, in_d, out_d, group, f16=group == 64, floats=1 << 25)
+    x = inputs(rng, 700, in_d, bf16)
+    first, one = w.mem.at, None
+    for i, rows in enumerate((700, 300, 70, 33, 17, 4)):
+        w.mem.at = first
+        kw = dict(act=i % 4, bias=ref.bf16_value(ref.bf16_bits(rng.standard_normal(out_d).astype(np.float32))))
+        if kw["act"] == cb.W4_ADD:
+            kw |= dict(scale=0.7, y=inputs(rng, rows, out_d, bf16))
+        got = w.linear(x[:rows], bf16=bf16, pad=(3, 1), off=i, behind=1, **kw)
+        check(got, W, x[:rows], bf16, (rows, kw["act"]), **kw)
+        plain = w.linear(x[:rows], bf16=bf16)
+        one = plain if one is None else one
+        assert np.array_equal(plain.view(np.uint32), one[:rows].view(np.uint32)), rows
+
+
 @pytest.mark.parametrize("ld", [(1 << 24) - 1, (1 << 24) + 4])
 def test_rows_far_apart(hip, ld):
     """Inputs whose offsets pass 32 bits, and nearly do."""
