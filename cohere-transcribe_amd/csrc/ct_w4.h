@@ -1,6 +1,6 @@
 /* ct_w4.h — launchers of the linear maps with 4-bit weights (k_w4.hip) and of
  * the logits' penalties and masks (k_logits.hip).  Arguments are checked by
- * w4.c and logits.c. */
+ * w4.c. */
 #ifndef CT_W4_H
 #define CT_W4_H
 

@@ -490,7 +490,9 @@ __global__ __launch_bounds__(NT) void trim_kernel(BackendKv8 c, int window, int 
 }
 
 // Sequences that share their first pages: a group's leader is its lowest
-// sequence; a wavefront a sequence compares its table with the leader's.
+// sequence; a wavefront a sequence compares its table with the leader's.  One
+// workgroup, since a step has one call of it for all its layers: 64 sequences with
+// 125 pages in common 4.5 us, 256 with 24 9.1, 5 with 6 3.0 (the launch).
 __global__ __launch_bounds__(PNT) void share_kernel(BackendKv8 c, int *share, int lp) {
     __shared__ int first[CT_KV8_SEQS], lead[CT_KV8_SEQS], tokens[CT_KV8_SEQS], members[CT_KV8_SEQS];
     const int s = threadIdx.x;

@@ -66,7 +66,7 @@ struct Args {
     // item's tile] there, first those of the items of common tokens, tile_rows each
     const int *share;
     int most;                    // rows of a sequence
-    int pitems;                  // items of common tokens in the grid
+    int pitems, oitems;          // items of common and of own tokens in the grid
     int want[2], least[2];       // chunks aimed at, least steps of one
 };
 
@@ -1422,7 +1422,10 @@ __global__ __launch_bounds__(NT, 2) void rows_kernel(Args a) {
 
 // Common and own tokens in one launch: the first pitems items' workgroups wait for
 // the matrix unit, the others for memory.  WIDE: common tokens in tiles of many
-// rows.
+// rows.  64 rows, 32 heads over 8, 8000 common tokens and up to 1000 more, bf16 (105
+// MB): 37 us and a join of 7, each sequence by itself 116; in a launch each 62 in all.
+// An item of common tokens is 16 iterations of 64 keys, 27 us, one wavefront a SIMD;
+// one of own tokens 12 us, of which finding the groups is 2 and the keys 5.
 template <int D, bool BF16, bool WIDE>
 __global__ __launch_bounds__(NT, WIDE || !BF16 ? 2 : 3) void shared_kernel(Args a) {
     constexpr int SUMS = NW * 16 * D * sizeof(float), OPS = sizeof(Operands<D>);
@@ -1435,7 +1438,7 @@ __global__ __launch_bounds__(NT, WIDE || !BF16 ? 2 : 3) void shared_kernel(Args 
 // Sequences whose tokens are all common, as a clip's hypotheses have them, in one
 // launch: a workgroup for each of them, of which those that do not begin a group
 // leave.  24 clips of up to 376 tokens, 5 hypotheses each, 8 heads, fp32 (18 MB of
-// codes): 13.1 us, of which an empty call's are 4.7, finding the group some 2.
+// codes): 12.9 us, where a call of one workgroup takes 3.6; finding the group is some 2.
 template <int D, bool BF16>
 __global__ __launch_bounds__(NT, 2) void groups_kernel(Args a) {
     __shared__ __align__(16) float so[NW * 16 * D];
@@ -1557,8 +1560,11 @@ __global__ __launch_bounds__(NT) void join_shared_kernel(Args a) {
     const int first = (((t.base + 31) >> 5) + m.chunk[0] - 1) / m.chunk[0];
     const int slots = __builtin_amdgcn_readfirstlane(first + (t.steps + m.chunk[1] - 1) / m.chunk[1]);
     const int each = (max(min(t.len, a.cap) - (t.base & ~31) + 31, 0) / 32 + m.chunk[1] - 1) / m.chunk[1];
-    const long common = ((long)(sitem[0][lead] + grow / a.tile_rows * first) * a.kv + h) * a.tile_rows + grow % a.tile_rows;
-    const long own = own_at(a, a.pitems + sitem[1][seq] + row / 16 * each, h, a.rpt) + row % 16;
+    // sequences that name the same rows may have more items than the grid: no sums of them
+    const int item0 = sitem[0][lead] + grow / a.tile_rows * first, item1 = sitem[1][seq] + row / 16 * each;
+    if (item0 + first > a.pitems || item1 + slots - first > a.oitems) return;
+    const long common = ((long)item0 * a.kv + h) * a.tile_rows + grow % a.tile_rows;
+    const long own = own_at(a, a.pitems + item1, h, a.rpt) + row % 16;
     float M = -INFINITY, num[DL] = {}, den = 0.0f;
     constexpr int AT = 8;                    // slots in flight
     for (int k0 = 0; k0 < slots; k0 += AT) {
@@ -1883,6 +1889,7 @@ extern "C" void ctk_kv8_attn_shared(const BackendKv8 *c, int layer, const Backen
     a.tile_rows = sh.tile_rows; a.one_tile = sh.one_tile; a.rpt = sh.rpt;
     for (int i = 0; i < 2; i++) { a.want[i] = sh.want[i]; a.least[i] = sh.least[i]; }
     a.pitems = sh.items[0];
+    a.oitems = sh.items[1];
     a.part = p->work;
     a.stat = reinterpret_cast<float2 *>(p->work + rows_apart(c, sh) * c->head_dim);
     const dim3 grid((unsigned)(c->kv_heads * (sh.items[0] + sh.items[1])));

@@ -363,6 +363,24 @@ def test_bad_pages_lengths_and_rows(hip, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+def test_sequences_that_name_the_same_rows(hip, bf16):
+    """Row ranges that go back, so that the sequences' rows are many more than
+    there are: a row is its first sequence's, or stays where that finds no room."""
+    print(f"case: shared, the same rows bf16={bf16}", flush=True)
+    rng = np.random.default_rng(14)
+    d, lens, of = family(hip, rng, 16, 2, 64, [(256, [300 + i for i in range(120)]), (96, [130 + i for i in range(120)])], rows=4)
+    for n, heads in ((8, 2), (4, 8)):
+        rows = np.array([0, n] * (len(lens) // 2) + [0], np.int32)
+        q = values(rng, n, heads, 64)
+        first = np.array([0, n] + [n] * (len(lens) - 1), np.int32)
+        want = d.model.attend(0, q, heads, 0.125, True, 0, 0, first, n)
+        got = attend(d, 0, q, heads, found(d)[0], rows, True, bf16, max_rows=n)
+        left = (got == 55.0).all(axis=2)
+        ok = ~left.any(axis=1)
+        check_rows(got[ok], *(x[ok] for x in want), bf16, n)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 def test_scales_far_apart(hip, bf16):
     """Value pages of very different sizes in the common text and past it."""
     print(f"case: shared, scales bf16={bf16}", flush=True)
