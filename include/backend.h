@@ -410,8 +410,9 @@ typedef struct {
     const int *mask_of;  /* [rows] which mask a row has; below 0: none; masks
                             and above: all its tokens are masked.  NULL: row
                             r has mask r                                      */
-    float *work;         /* backend_logits_work floats, zeroed once; a call
-                            leaves it zeroed                                  */
+    float *work;         /* backend_logits_work floats, 16-byte aligned, zeroed
+                            once; a call leaves it zeroed.  One call's at a
+                            time                                              */
 } BackendLogits;
 /* Floats of work (0: none): enough for this call and any with no more rows and
  * vocab. */
