@@ -489,3 +489,76 @@ def test_the_same_call_gives_the_same_bits(hip, bf16):
         assert replayed, i
         again = np.array_equal(eager(1 - i), want[1 - i])
         assert again, i
+
+
+def long_texts(hip, rng, P, kv, D, lens, common, extra):
+    """A cache of sequences whose tables name 211 pages again and again in an order of
+    their own, after `common` tokens that all have; sequence 0 misses a page far behind."""
+    pages, width = 211, -(-max(lens) // P) + 1
+    d = ref.Dev(hip, 1, pages, P, kv, D, len(lens), width, extra)
+    m = d.model
+    m.k[:], m.v[:] = (ref.to_codes(64 * rng.standard_normal(m.k.shape).astype(np.float32)) for _ in range(2))
+    m.ks[:], m.vs[:] = (2.0 ** rng.integers(-9, -5, m.ks.shape) for _ in range(2))
+    m.table[:] = rng.integers(0, pages - 1, m.table.shape)
+    m.table[:, :common // P] = m.table[0, :common // P]
+    m.table[:, common // P] = rng.permutation(pages - 1)[:len(lens)]      # another one each
+    m.table[0, (lens[0] - 100) // P] = -1
+    m.len[:] = lens
+    m.refs[:] = 1
+    m.v[0, pages - 1, 1, 3, 5] = 0x7F
+    d.push()
+    return d
+
+
+def attend_last(m, q, scale):
+    """Cache.attend of a row a sequence, its last token, a page and a kv head at a time: for long texts."""
+    _, pages, P, kv, D, seqs, _ = m.dims
+    K, V = (ref.E4M3[x[0]] * s[0][..., None, None].astype(np.float64) for x, s in ((m.k, m.ks), (m.v, m.vs)))
+    n, heads, _ = q.shape
+    out, vmax, smax = np.zeros((n, heads, D)), np.zeros((n, heads, 1)), np.zeros((n, heads, 1))
+    for s in range(seqs):
+        page = m.table[s, :-(-int(m.len[s]) // P)]
+        see = np.repeat((page >= 0) & (page < pages), P)[:int(m.len[s])]
+        pg = np.where((page >= 0) & (page < pages), page, 0)
+        for h in range(kv):
+            k, v = (x[pg, h].reshape(-1, D)[:len(see)][see] for x in (K, V))
+            at = slice(h * heads // kv, (h + 1) * heads // kv)
+            qh = q[s, at].astype(np.float64)
+            sc = qh @ k.T * scale
+            smax[s, at, 0] = (np.abs(qh) @ np.abs(k).T).max(1) * scale
+            w = np.exp(sc - sc.max(1, keepdims=True))
+            out[s, at] = (w / w.sum(1, keepdims=True)) @ v
+            vmax[s, at] = np.nanmax(np.abs(v))
+    return out, vmax, smax
+
+
+@pytest.mark.parametrize("P,kv,group,D,lens,common,least", [
+    (64, 8, 1, 64, [15000 + 37 * i for i in range(20)], 0, 130),
+    (128, 16, 2, 64, [9000 - 11 * i for i in range(24)], 384, 190),
+    (16, 64, 1, 64, [36000, 35000, 36100, 35517], 0, 500),
+    (32, 8, 4, 128, [15001 + 64 * i for i in range(20)], 96, 130),
+    (64, 8, 8, 64, [70000 + 31 * i for i in range(8)], 69952, 130),
+    (128, 8, 16, 64, [140001 + 50 * i for i in range(4)], 139904, 260)])
+def test_chunks_of_many_pages(hip, P, kv, group, D, lens, common, least):
+    """So many own or common tokens that a workgroup walks more than 128 steps of
+    32, one that ends inside the last ones, with a page that is not there and a
+    NaN behind the first of them."""
+    print(f"case: shared, long chunks P={P} kv={kv} group={group} D={D} {lens[0]} x {len(lens)} {common}", flush=True)
+    rng = np.random.default_rng(lens[0])
+    n, heads = len(lens), kv * group
+    d = long_texts(hip, rng, P, kv, D, lens, common, 1 << 24)
+    m = d.model
+    tiles = -(-n * group // 16) * (common // 32) if n * group <= 64 and common > 5000 else 0
+    own = sum(-(-(x - common) // 32) for x in lens) if common < 5000 else 0
+    assert max(tiles, own) / -(-512 // kv) > least        # steps of a chunk
+    far = (min(lens) if not tiles else common) - 3 * P
+    m.table[:2 if own else None, far // P] = m.dims[1] - 1
+    d.push()
+    q = values(rng, n, heads, D)
+    p = found(d)[0]
+    rows = starts([1] * n)
+    want = attend_last(m, q, D ** -0.5)
+    assert np.isnan(want[0]).any()
+    for bf16 in (False, True):
+        got = attend(d, 0, q, heads, p, rows, True, bf16)
+        check_rows(got, *want, bf16, bf16)
