@@ -8,15 +8,19 @@
 // o, which is the B operand of one 16x16x32 product: value e of the eight in
 // bits 4 (e / 2) + 16 (e % 2), so that a mask leaves a pair of them in the low
 // bits of two f16.  Each (output, group) has one word: the scale's 16 bits above
-// the f16 bits of -(1024 + z).
-// Products.  c | 0x6400 is the f16 1024 + c, and adding -(1024 + z) gives c - z
-// exactly: 9 instructions for 8 weights.  Activations are brought, 128 inputs
-// of a row at a time, to a largest value in [2^14, 2^15) by a power of two and
-// split into two f16 (bf16 rows are one f16): 22 bits of each fp32 input stay.
-// A group's products are summed by the matrix unit in fp32 and enter the row's
-// sum times the scale.  A row's inputs are summed in SEGS runs of tiles that are
-// joined in order, in every kernel here, so that a row's answer does not depend
-// on how many rows the call has.
+// the f16 bits of -(2^-1 + z 2^-11).
+// Products.  c | 0x3800 is the f16 2^-1 + c 2^-11, and adding -(2^-1 + z 2^-11)
+// gives (c - z) 2^-11 exactly: 9 instructions for 8 weights.  Activations are
+// brought, 128 inputs of a row at a time, to a largest value in [2^14, 2^15) by a
+// power of two and split into two f16 (bf16 rows are one f16): 22 bits of each
+// fp32 input stay.  A group's products are summed by the matrix unit in fp32,
+// brought back by the power of two and enter the row's sum times the scale, in
+// that order: with the weights' 2^-11, 128 times 15 times the largest float is
+// within fp32's range, so nothing is infinite before the result is, whatever the
+// sizes of inputs and scales.  The sums are brought back from the 2^-11 at the end.
+// A row's inputs are summed in SEGS runs of tiles that are joined in order, in
+// every kernel here, so that a row's answer does not depend on how many rows the
+// call has.
 //
 // What bounds them.  One row of a small map: the launch and one pass of loads
 // (1024 -> 1024, 0.55 MB: 3.8 us, where a call of one workgroup takes 3.6).  Few rows of large maps: the codes'
@@ -55,21 +59,21 @@ __device__ __forceinline__ float scale_of(uint32_t word, uint32_t f16) {
     return __uint_as_float((h & f16) | (word & 0xffff0000u & ~f16));
 }
 
-// A zero point as it is taken off: -(1024 + z) and -(64 + z), in both halves.
+// A zero point as it is taken off: -(2^-1 + z 2^-11) and -(2^-5 + z 2^-11), in both halves.
 struct Less {
     f16x2 low, high;
 };
 __device__ __forceinline__ Less less_of(uint32_t word) {
     const f16x2 low = __builtin_bit_cast(f16x2, (word & 0xffffu) | word << 16);
-    return {low, low + (f16x2){960, 960}};
+    return {low, low + (f16x2){0.46875, 0.46875}};
 }
 
-// Eight codes less their zero point.  A code in the low four bits of a f16 1024.0
-// makes it 1024 + c, in the next four of a 64.0 64 + c: one shift and four masks a
-// dword (a shift a pair took 15 instructions where this takes 9).
+// Eight codes less their zero point, times 2^-11.  A code in the low four bits of a
+// f16 2^-1 makes it 2^-1 + c 2^-11, in the next four of a 2^-5 2^-5 + c 2^-11: one
+// shift and four masks a dword (a shift a pair took 15 instructions where this takes 9).
 __device__ __forceinline__ f16x8 weights8(uint32_t q, const Less &less) {
     // constants in registers: one instruction takes a mask and a constant only so
-    uint32_t m0 = 0x000f000fu, m1 = 0x00f000f0u, one = 0x64006400u, two = 0x54005400u;
+    uint32_t m0 = 0x000f000fu, m1 = 0x00f000f0u, one = 0x38003800u, two = 0x28002800u;
     asm("" : "+s"(m0), "+s"(m1), "+v"(one), "+v"(two));
     u32x4 w;                     // whole registers: halves set one by one took twice as many
 #pragma unroll
@@ -187,12 +191,13 @@ __device__ __forceinline__ void tile_product(const u32x4 &code, const uint32_t (
         }
         const float s = scale_of(word[g], scale_f16);
 #pragma unroll
-        for (int i = 0; i < 4; i++) sum[i] = __builtin_fmaf(mul_rn(acc[i], s), undo[i], sum[i]);
+        for (int i = 0; i < 4; i++) sum[i] = __builtin_fmaf(acc[i] * undo[i], s, sum[i]);
     }
 }
 
 template <bool BF16>
 __device__ __forceinline__ void finish(const Args &a, long t, int o, float v) {
+    v *= 0x1p11f;                            // the weights' 2^-11
     if (a.bias) v += bf2f(a.bias[o]);
     if (a.act == W4_SILU) v = v * sigmoid_hw(v);
     else if (a.act == W4_RELU) v = v < 0.0f ? 0.0f : v;      // a NaN stays
@@ -557,7 +562,7 @@ __global__ __launch_bounds__(W * CT_WAVE, 2) void linear_rows_kernel(Args a) {
                     for (int n = 0; n < NT; n++) {
                         const float s = scale_of(nw[j / GS & 1][n], a.scale_f16);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) sum[m][n][i] = __builtin_fmaf(mul_rn(acc[m][n][i], s), undo[i], sum[m][n][i]);
+                        for (int i = 0; i < 4; i++) sum[m][n][i] = __builtin_fmaf(acc[m][n][i] * undo[i], s, sum[m][n][i]);
                         // a group's sums before the next one's products: side by side
                         // they do not fit the registers
                         if (GS < 4) asm volatile("" : "+v"(sum[m][n][0]), "+v"(sum[m][n][1]), "+v"(sum[m][n][2]), "+v"(sum[m][n][3]));
@@ -605,7 +610,7 @@ __global__ __launch_bounds__(W * CT_WAVE, 2) void linear_rows_kernel(Args a) {
 // ---- Laying out ----------------------------------------------------------
 
 __device__ __forceinline__ uint32_t word_of(uint16_t scale, int zero) {
-    return (uint32_t)scale << 16 | __builtin_bit_cast(uint16_t, (_Float16)(float)(-1024 - zero));
+    return (uint32_t)scale << 16 | __builtin_bit_cast(uint16_t, (_Float16)(-0.5f - (float)zero * 0x1p-11f));
 }
 
 // Codes of one tile, a byte each [16][128] in LDS, as its 64 lanes' dwords.
@@ -691,7 +696,7 @@ __global__ __launch_bounds__(256) void unpack_kernel(BackendW4 w, float *values,
         const int i = threadIdx.x, j = i & 3, row = (i >> 2) & 15, q = i >> 6;
         const int o = (int)(tile / itiles) * TO + row, k = (int)(tile % itiles) * TI + 32 * j + 8 * q;
         const uint32_t v = w.codes[tile * 256 + i], word = w.scales[(tile * TO + row) * per + (32 * j + 8 * q) / w.group];
-        const float s = scale_of(word, w.scale_f16 ? ~0u : 0u), less = (float)less_of(word).low[0] + 1024.0f;
+        const float s = scale_of(word, w.scale_f16 ? ~0u : 0u), less = ((float)less_of(word).low[0] + 0.5f) * 0x1p11f;
         if (o < w.out_d)
 #pragma unroll
             for (int e = 0; e < 8; e++)

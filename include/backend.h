@@ -362,7 +362,9 @@ typedef struct {
 } BackendW4Linear;
 /* Products are summed in fp32; of a block of 128 inputs those far smaller than
  * its largest are rounded at 2^-38 of it (fp32) or 2^-39 (bf16), the others to
- * 22 bits (fp32) or not at all (bf16).  A row's bits depend neither on the
+ * 22 bits (fp32) or not at all (bf16); a group's sum of codes times inputs and the
+ * result's sum, where they are below 2^-115, at 2^-139.  Scales and inputs of any
+ * size: nothing overflows but sums that do.  A row's bits depend neither on the
  * other rows nor on their number.  A row with an input that is not finite has
  * outputs that are not finite. */
 void backend_linear_w4(const BackendW4 *w, const BackendW4Linear *a);

@@ -304,3 +304,43 @@ def test_nothing_to_do_and_captured(hip):
         assert np.array_equal(mem.get(y, (40, 300), np.float32).view(np.uint32), want[i].view(np.uint32))
         hip.backend_linear_w4(w.h, C.byref(a))
         assert np.array_equal(mem.get(y, (40, 300), np.float32).view(np.uint32), want[i].view(np.uint32))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("in_d,out_d,group,rows", [
+    (1024, 48, 128, 1), (640, 80, 32, 20), (4300, 1030, 64, 33), (260, 17000, 64, 3), (300, 1030, 64, 1300), (640, 4100, 128, 700)])
+def test_scales_and_inputs_of_any_size(hip, in_d, out_d, group, rows, bf16):
+    """Scales up to the type's largest value over inputs so small that the result
+    is finite, the smallest ones over large inputs, and both beside scales of 1."""
+    print(f"case: scales of any size {in_d} {out_d} {group} {rows} bf16={bf16}", flush=True)
+    rng = np.random.default_rng(rows)
+    mem = ref.Mem(hip, 1 << 25)
+    w = ref.Weight(hip, mem, in_d, out_d, group, False)
+    g, first = -(-in_d // group), mem.at
+    for top, low in ((127.99, -60), (127.99, -100), (-133, 100), (-110, 80), (0, 106), (0, -80)):
+        mem.at = first
+        codes, z = rng.integers(0, 16, (out_d, in_d)).astype(np.uint8), rng.integers(0, 16, (out_d, g)).astype(np.uint8)
+        bits = ref.bf16_bits((2.0 ** (top - 3 * rng.random((out_d, g)) * (top > 0))).astype(np.float32))
+        if top in (127.99, -110):
+            some = rng.random((out_d, g)) < 0.5
+            bits[some] = ref.bf16_bits(np.ones(some.sum(), np.float32))
+        w.load(codes, bits, z)
+        W = ref.values(codes, bits, z, group, False)
+        x = (inputs(rng, rows, in_d, bf16).astype(np.float64) * 2.0 ** low).astype(np.float32)
+        some = np.unique(np.concatenate([np.arange(min(rows, 40)), np.arange(max(rows - 40, 0), rows)]))
+        got = w.linear(x, bf16=bf16)
+        assert np.isfinite(got).all(), (top, low)
+        check(got[some], W, x[some], bf16, (top, low))
+
+
+def test_quantized_weights_of_any_size(hip):
+    """Weights up to the largest finite one through quantising and a product."""
+    print("case: quantized, any size", flush=True)
+    rng = np.random.default_rng(16)
+    for size, low in ((3.3e38, 1e-12), (1e34, 1e-20), (1e-34, 1e20)):
+        W = np.clip(rng.standard_normal((48, 512)) * size, -3.38e38, 3.38e38).astype(np.float32)
+        mem = ref.Mem(hip, 1 << 22)
+        w = ref.Weight(hip, mem, 512, 48, 64, False)
+        hip.backend_w4_quantize(w.h, mem.put(ref.bf16_bits(W)))
+        x = (inputs(rng, 5, 512, False) * np.float32(low)).astype(np.float32)
+        check(w.linear(x), w.unpack().astype(np.float64), x, False, size)
