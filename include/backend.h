@@ -365,8 +365,9 @@ typedef struct {
  * 22 bits (fp32) or not at all (bf16); a group's sum of codes times inputs and the
  * result's sum, where they are below 2^-115, at 2^-139.  Scales and inputs of any
  * size: nothing overflows but sums that do.  A row's bits depend neither on the
- * other rows nor on their number.  A row with an input that is not finite has
- * outputs that are not finite. */
+ * other rows nor on their number.  Where a row has an input that is not
+ * finite, no output's W x is: NaN, or of bf16 rows an infinity too, of which relu
+ * makes 0 if it is negative. */
 void backend_linear_w4(const BackendW4 *w, const BackendW4Linear *a);
 
 /* ---- Penalties, biases and masks on logits ------------------------------- *

@@ -344,3 +344,19 @@ def test_quantized_weights_of_any_size(hip):
         hip.backend_w4_quantize(w.h, mem.put(ref.bf16_bits(W)))
         x = (inputs(rng, 5, 512, False) * np.float32(low)).astype(np.float32)
         check(w.linear(x), w.unpack().astype(np.float64), x, False, size)
+
+
+@pytest.mark.parametrize("rows", [9, 200])
+def test_what_relu_leaves_of_infinite_inputs(hip, rows):
+    """A row with an infinity: a finite output is the zero of a product of
+    -infinity, of bf16 rows; everything else is not finite."""
+    print(f"case: relu of infinities rows={rows}", flush=True)
+    rng = np.random.default_rng(17)
+    for bf16 in (False, True):
+        w, W = weight(hip, rng, 640, 80, 64)
+        x = inputs(rng, rows, 640, bf16)
+        x[6, 3], x[7, 639], x[8, 200] = np.inf, np.nan, -np.inf
+        plain, relu, silu = (w.linear(x, bf16=bf16, act=a)[6:9] for a in (cb.W4_STORE, cb.W4_RELU, cb.W4_SILU))
+        assert not np.isfinite(plain).any() and np.isnan(plain[1]).all()
+        assert np.array_equal(relu == 0, plain == -np.inf) and not np.isfinite(relu[relu != 0]).any()
+        assert (bf16 or np.isnan(relu).all()) and not np.isfinite(silu).any()
