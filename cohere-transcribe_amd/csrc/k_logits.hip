@@ -105,18 +105,25 @@ __global__ __launch_bounds__(NT, 6) void logits_kernel(BackendLogits a) {
     }
 
     const int len = h ? (int)min((long)max(a.hist_len[r], 0), a.ld_hist) : 0;
-    int b0 = 0, b1 = 0;
+    // the row's entries: nb from b0 on.  Counted from there: a start near 2^31 plus a
+    // thread's number would be below any end
+    int b0 = 0;
+    uint32_t nb = 0;
     if (a.bias_start) {
-        b0 = a.bias_start[r];
-        b1 = a.bias_start[r + 1];
-        if (b0 < 0 || b1 > a.biases) b1 = b0;
+        const int start = a.bias_start[r], end = a.bias_start[r + 1];
+        if (start >= 0 && end <= a.biases && start < end) {
+            b0 = start;
+            nb = (uint32_t)(end - start);
+        }
     }
+    const int *bias_id = a.bias_id + b0;
+    const float *bias = a.bias + b0;
     const int from = a.prompt_len ? a.prompt_len[r] : 0, k = a.ngram ? a.ngram[r] : 0;
     // the first of the bias list; its values are near when they are looked up
     int biased = -1;
-    if (b0 + tid < b1) {
-        biased = a.bias_id[b0 + tid];
-        __builtin_prefetch(a.bias + b0 + tid);
+    if ((uint32_t)tid < nb) {
+        biased = bias_id[tid];
+        __builtin_prefetch(bias + tid);
     }
     const float repeat = a.repeat ? a.repeat[r] : 1.0f, frequency = a.frequency ? a.frequency[r] : 0.0f,
                 presence = a.presence ? a.presence[r] : 0.0f;
@@ -130,7 +137,7 @@ __global__ __launch_bounds__(NT, 6) void logits_kernel(BackendLogits a) {
         else if (which >= 0 && v < a.vocab) allowed[j] = a.mask[(long)which * a.ld_mask + (v >> 5)] >> (v & 31) & 15;
     }
 
-    if (len > 0 || b1 > b0) {
+    if (len > 0 || nb) {
         u32x4 *mine = reinterpret_cast<u32x4 *>(state) + tid;
 #pragma unroll
         for (int j = 0; j < 4; j++) mine[j * NT] = (u32x4){0, 0, 0, 0};
@@ -195,13 +202,13 @@ __global__ __launch_bounds__(NT, 6) void logits_kernel(BackendLogits a) {
             }
         }
     }
-    if (b1 > b0) {
+    if (nb) {
         // over the counts, which all have read
         __syncthreads();
-        for (int i = b0 + tid; i < b1; i += NT) {
+        for (uint32_t i = tid; i < nb; i += NT) {
             const unsigned t = (unsigned)biased - (unsigned)v0;
-            if (t < (unsigned)n) atomicMax(&state[t], ENTRY | (uint32_t)(i - b0));
-            if (i + NT < b1) biased = a.bias_id[i + NT];
+            if (t < (unsigned)n) atomicMax(&state[t], ENTRY | i);
+            if (i + NT < nb) biased = bias_id[i + NT];
         }
         __syncthreads();
 #pragma unroll
@@ -209,7 +216,7 @@ __global__ __launch_bounds__(NT, 6) void logits_kernel(BackendLogits a) {
             const u32x4 st = reinterpret_cast<const u32x4 *>(state)[j * NT + tid];
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (st[e] & ENTRY) l[4 * j + e] += a.bias[b0 + (int)(st[e] & ~ENTRY)];
+                if (st[e] & ENTRY) l[4 * j + e] += bias[st[e] & ~ENTRY];
         }
     }
 

@@ -250,3 +250,16 @@ def test_the_most_rows(hip):
     h = rng.integers(0, 33, (65535, 4))
     run(hip, x, "rows", hist=h, hist_len=rng.integers(0, 5, 65535), repeat=np.full(65535, 1.5, np.float32),
         mask=rng.integers(0, 2 ** 32, (65535, 2), dtype=np.uint32))
+
+
+def test_bias_starts_far_out_of_range(hip):
+    """Starts whose sum with a thread's number passes 2^31, ends before them, the
+    whole list, and lists longer than a workgroup has threads: as the header says,
+    starts below 0 or past the list, and those that run backwards, give no bias."""
+    print("case: bias starts, far", flush=True)
+    rng = np.random.default_rng(12)
+    top = 2 ** 31 - 1
+    for vocab, n in ((50, 6), (9000, 1500)):
+        start = np.array([top, 0, top - 5, 2, top - 254, 1, top - 510, n, top, top - 511, -2 ** 31, 3, 0, n, top, n - 1, n])
+        x = rng.standard_normal((len(start) - 1, vocab)).astype(np.float32)
+        run(hip, x, ("starts", vocab), bias_start=start, bias_id=rng.integers(-3, vocab + 3, n), bias=rng.standard_normal(n).astype(np.float32))
