@@ -96,15 +96,16 @@ __global__ __launch_bounds__(NT, 6) void logits_kernel(BackendLogits a) {
         for (int e = 0; e < 4; e++) l[4 * j + e] = y[e];
     }
     const int *h = a.hist ? a.hist + (long)r * a.ld_hist : nullptr;
+    // no more than the row's tokens: behind the last row's there need be no memory
+    const int len = h ? (int)min((long)max(a.hist_len[r], 0), a.ld_hist) : 0;
     int said[4], prev[4];                    // the token at i and the one before it
 #pragma unroll
     for (int u = 0; u < 4; u++) {
         const int i = u * NT + tid;
-        said[u] = h && i < a.ld_hist ? h[i] : -1;
-        prev[u] = a.ngram && i > 0 && i - 1 < a.ld_hist ? h[i - 1] : -1;
+        said[u] = i < len ? h[i] : -1;
+        prev[u] = a.ngram && i > 0 && i - 1 < len ? h[i - 1] : -1;
     }
 
-    const int len = h ? (int)min((long)max(a.hist_len[r], 0), a.ld_hist) : 0;
     // the row's entries: nb from b0 on.  Counted from there: a start near 2^31 plus a
     // thread's number would be below any end
     int b0 = 0;

@@ -263,3 +263,25 @@ def test_bias_starts_far_out_of_range(hip):
         start = np.array([top, 0, top - 5, 2, top - 254, 1, top - 510, n, top, top - 511, -2 ** 31, 3, 0, n, top, n - 1, n])
         x = rng.standard_normal((len(start) - 1, vocab)).astype(np.float32)
         run(hip, x, ("starts", vocab), bias_start=start, bias_id=rng.integers(-3, vocab + 3, n), bias=rng.standard_normal(n).astype(np.float32))
+
+
+@pytest.mark.parametrize("vocab", [300, 9000])
+def test_history_that_ends_with_its_last_token(hip, vocab):
+    """Histories that start inside their rows, the last row's last token at the end of
+    the memory: only what hist_len counts is read, so the results are the tokens' alone."""
+    print(f"case: history at the end {vocab}", flush=True)
+    rng = np.random.default_rng(13)
+    rows, ld, off = 5, 2500, 1700
+    mem = Mem(hip, 1 << 22)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    full = rng.integers(0, vocab, (rows, ld)).astype(np.int32)
+    full[:, off + 300:off + 310] = full[:, -10:]
+    kw = dict(hist=full[:, off:], hist_len=np.full(rows, ld - off), repeat=np.full(rows, 1.3, np.float32),
+              frequency=np.full(rows, 0.25, np.float32), ngram=np.full(rows, 3))
+    at = mem.end - full.nbytes
+    mem.write(at, full)
+    c = Call(hip, mem, x, **kw)
+    c.a.hist, c.a.ld_hist = at + 4 * off, ld
+    want = ref.process(x, **kw)
+    c.launch()
+    c.check(want, vocab)
