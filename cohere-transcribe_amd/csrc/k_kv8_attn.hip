@@ -1813,6 +1813,7 @@ namespace {
 
 constexpr int ITEMS = 512, WIDE_ITEMS = 128;     // items aimed at
 constexpr double APART_BYTES = 192.0 * (1 << 20);
+constexpr long JOIN_ROWS = 1L << 25;             // rows * query heads of a call
 constexpr int OWN_ROWS = 64;     // packed rows of a sequence up to which common tokens are taken apart
 
 struct SharedShape {
@@ -1833,7 +1834,9 @@ SharedShape shared_shape_of(const BackendKv8 *c, const BackendKv8Attn *a) {
     // 184 MB: 28.9, 27.2; 64 of 2200, four heads a group, 288 MB: 31.2, 28.6;
     // 64 of 9000, 1.2 GB: 116, 43.5).
     const double codes = (double)(c->seqs < a->n_rows ? c->seqs : a->n_rows) * steps * 32 * kv * 2 * c->head_dim;
-    s.apart = each <= OWN_ROWS && c->seqs > 1 && codes > APART_BYTES;
+    // The join has a wavefront for each row and head, whether a sequence has the row
+    // or not: up to 2^25 of them, so that its grid stays below 2^32 threads too.
+    s.apart = each <= OWN_ROWS && c->seqs > 1 && codes > APART_BYTES && (long)a->n_rows * a->heads <= JOIN_ROWS;
     if (!s.apart) return s;
     s.wide = all > 64;
     s.tile_rows = s.wide ? rows_of(a->bf16) : 16;

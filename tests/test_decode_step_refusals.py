@@ -206,3 +206,24 @@ def test_logits_model():
     y, i, s = logits_ref.process(x, mask=np.array([[0b000010]], np.uint32), mask_of=[0])
     assert i[0] == 1 and s[0] == -2.0 and np.isneginf(y[0, [0, 2, 3, 4, 5]]).all()
     assert logits_ref.process(x, mask=np.zeros((1, 1), np.uint32))[1][0] == -1
+
+
+def test_shared_join_fits_a_grid():
+    """Rows that no sequence has count too: a call whose join would be a wavefront for
+    each of 2^26 rows and heads or more (2^32 threads) goes through every sequence's own table."""
+    L = cb.hip()
+    for f in (L.ctk_kv8_attn_shared_need, L.ctk_kv8_attn_need):
+        f.argtypes, f.restype = [C.c_void_p, C.c_void_p], C.c_size_t
+    c = cb.BackendKv8(layers=1, pages=50, page_tokens=64, kv_heads=2, head_dim=64, seqs=64, table_w=4096)
+    for heads in (2, 8, 32):
+        for rows in (64, 1 << 10, 1 << 19, 1 << 20, 1 << 21, 1 << 22, 1 << 24):
+            if rows * heads > 1 << 27:
+                continue
+            a = cb.BackendKv8Attn(out=4096, q=4096, ld_out=heads * 64, ld_q=heads * 64, heads=heads, scale=1.0, rows=4096,
+                                  n_rows=rows, max_rows=1, causal=1)
+            shared, own = (f(C.byref(c), C.byref(a)) for f in (L.ctk_kv8_attn_shared_need, L.ctk_kv8_attn_need))
+            apart = shared != own
+            threads = 2 * -(-rows * (heads // 2) // 4) * 256
+            assert not apart or threads < 1 << 32, (heads, rows)
+            assert apart or rows * heads > 1 << 20, (heads, rows)
+            assert shared <= L.backend_kv8_attn_shared_work(C.byref(c), C.byref(a))
