@@ -20,6 +20,8 @@ void ctk_w4_quantize(const BackendW4 *w, const uint16_t *W, hipStream_t s);
 void ctk_w4_unpack(const BackendW4 *w, float *values, hipStream_t s);
 void ctk_w4_linear(const BackendW4 *w, const BackendW4Linear *a, hipStream_t s);
 
+int ct_rows_meet(const void *a, size_t lda, size_t wa, const void *b, size_t ldb, size_t wb, long rows);
+
 size_t ctk_logits_work(const BackendLogits *a);
 void ctk_logits(const BackendLogits *a, hipStream_t s);
 

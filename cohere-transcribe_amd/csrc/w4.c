@@ -10,6 +10,28 @@ static void require_init(void) {
     if (ct_t.dev < 0) CT_FATAL("backend used on a thread that has not called backend_init");
 }
 
+/* Whether any of `rows` pieces of wa bytes, lda bytes apart from a on, shares a
+ * byte with one of wb bytes, ldb apart from b on (wa <= lda, wb <= ldb). */
+int ct_rows_meet(const void *a, size_t lda, size_t wa, const void *b, size_t ldb, size_t wb, long rows) {
+    const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+    const size_t last = (size_t)rows - 1;
+    if (pa + last * lda + wa <= pb || pb + last * ldb + wb <= pa) return 0;
+    /* one within the other's pitch, as columns of one array are: all pairs of rows
+     * at once, else row by row */
+    const size_t n = lda == ldb ? 1 : (size_t)rows;
+    for (size_t i = 0; i < n; i++) {
+        const uintptr_t lo = pa + i * lda, hi = lo + wa;
+        /* the first piece of b that ends past lo */
+        size_t j = pb + wb > lo ? 0 : (lo - pb - wb) / ldb + 1;
+        if (j <= last && pb + j * ldb < hi) return 1;
+        if (lda != ldb) continue;
+        /* and a's pieces over b's first */
+        j = pa + wa > pb ? 0 : (pb - pa - wa) / lda + 1;
+        if (j <= last && pa + j * lda < pb + wb) return 1;
+    }
+    return 0;
+}
+
 /* ---- Linear maps with 4-bit weights ---- */
 static void check_sizes(const BackendW4 *w) {
     if (!w) CT_FATAL("w4: no weight");
@@ -76,6 +98,9 @@ void backend_linear_w4(const BackendW4 *w, const BackendW4Linear *a) {
         CT_FATAL("linear_w4: x or y is NULL or not aligned");
     if (a->x == a->y) CT_FATAL("linear_w4: y is x");
     if (a->ld_x < w->in_d || a->ld_y < w->out_d) CT_FATAL("linear_w4: ld_x below in_d or ld_y below out_d");
+    const size_t size = a->bf16 ? 2 : 4;
+    if (ct_rows_meet(a->x, a->ld_x * size, w->in_d * size, a->y, a->ld_y * size, w->out_d * size, a->rows))
+        CT_FATAL("linear_w4: y and x overlap");
     if ((uintptr_t)a->bias & 1) CT_FATAL("linear_w4: bias is not aligned");
     require_init();
     ctk_w4_linear(w, a, ct_t.stream);
@@ -124,5 +149,8 @@ void backend_logits(const BackendLogits *a) {
     if (ctk_logits_work(a) && (!a->work || ((uintptr_t)a->work & 15)))
         CT_FATAL("logits: work is NULL or not 16-byte aligned");
     require_init();
+    if (a->out && a->out != a->logits &&
+        ct_rows_meet(a->logits, 4 * a->ld, 4 * (size_t)a->vocab, a->out, 4 * a->ld_out, 4 * (size_t)a->vocab, a->rows))
+        CT_FATAL("logits: out overlaps the logits without being them");
     ctk_logits(a, ct_t.stream);
 }

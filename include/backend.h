@@ -352,7 +352,7 @@ void backend_w4_unpack(const BackendW4 *w, float *values);
 #define W4_ADD   3       /* y += scale * (W x + b)                            */
 typedef struct {
     void *y;             /* [rows][out_d], ld_y values apart                  */
-    const void *x;       /* [rows][in_d], ld_x apart; not y                   */
+    const void *x;       /* [rows][in_d], ld_x apart; no memory of y's        */
     long ld_y, ld_x;
     int bf16;            /* x and y: 0 fp32, 1 bf16                           */
     int rows;            /* 0..2^24                                           */
@@ -387,7 +387,8 @@ void backend_linear_w4(const BackendW4 *w, const BackendW4Linear *a);
 typedef struct {
     const float *logits; /* [rows][vocab], ld apart                           */
     float *out;          /* the same after step 5, ld_out apart; may be logits
-                            themselves (with ld_out = ld); NULL: not wanted   */
+                            themselves (with ld_out = ld), else shares no
+                            memory with them; NULL: not wanted                */
     long ld, ld_out;
     int rows, vocab;     /* 0..65535 rows; 1..2^24                            */
     int *id;             /* [rows] lowest id of the largest value above

@@ -227,3 +227,38 @@ def test_shared_join_fits_a_grid():
             assert not apart or threads < 1 << 32, (heads, rows)
             assert apart or rows * heads > 1 << 20, (heads, rows)
             assert shared <= L.backend_kv8_attn_shared_work(C.byref(c), C.byref(a))
+
+
+@pytest.mark.parametrize("change", [dict(y=8196), dict(y=8192 + 1024 - 4), dict(y=8192 - 3 * 256 + 4), dict(y=8192 + 2 * 1024 + 1020),
+                                    dict(y=8192 + 2 * 600, bf16=1, ld_y=300, ld_x=300), dict(y=8194, bf16=1, rows=1)])
+def test_overlapping_rows_are_refused(change):
+    """Outputs among the inputs, from their first to their last value."""
+    r = subprocess.run([sys.executable, "-c", program(LIN, **change)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 1 and "y and x overlap" in r.stderr, r.stderr
+
+
+@pytest.mark.parametrize("change", [dict(y=8192 + 1024, ld_x=320, ld_y=320), dict(x=8192 + 256, y=8192, ld_x=320, ld_y=320),
+                                    dict(y=8192 + 3 * 1024), dict(y=8192 - 3 * 256), dict(y=8192 + 512, bf16=1, ld_x=288 + 32, ld_y=320)])
+def test_columns_of_one_array_are_not(change):
+    """Inputs and outputs side by side in one array, or right behind each other."""
+    r = subprocess.run([sys.executable, "-c", program(LIN, **change)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 1 and "has not called backend_init" in r.stderr, r.stderr
+
+
+def test_rows_that_meet():
+    """The check of two sets of rows against every pair of bytes."""
+    L = cb.hip()
+    L.ct_rows_meet.argtypes, L.ct_rows_meet.restype = [C.c_void_p, C.c_size_t, C.c_size_t] * 2 + [C.c_long], C.c_int
+    rng = np.random.default_rng(5)
+    seen = [0, 0]
+    for _ in range(4000):
+        wa, wb, rows = (int(v) for v in rng.integers(1, 9, 3))
+        lda, ldb = wa + int(rng.integers(0, 12)), wb + int(rng.integers(0, 12))
+        if rng.random() < 0.5:
+            lda = ldb = max(lda, ldb)
+        a, b = 1000, 1000 + int(rng.integers(-100, 100))
+        at = [{p + i * ld + k for i in range(rows) for k in range(w)} for p, ld, w in ((a, lda, wa), (b, ldb, wb))]
+        want = bool(at[0] & at[1])
+        assert bool(L.ct_rows_meet(a, lda, wa, b, ldb, wb, rows)) == want, (a, lda, wa, b, ldb, wb, rows)
+        seen[want] += 1
+    assert min(seen) > 500

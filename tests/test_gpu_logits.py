@@ -285,3 +285,23 @@ def test_history_that_ends_with_its_last_token(hip, vocab):
     want = ref.process(x, **kw)
     c.launch()
     c.check(want, vocab)
+
+
+def test_overlapping_result_is_refused(hip):
+    """out among the logits' rows without being them; beside them in one array it is fine."""
+    print("case: overlap", flush=True)
+    import subprocess
+    import sys
+    prog = (f"import sys; sys.path.insert(0, {cb.PKG_DIR!r}); import ctypes as C, ctbind as cb; L = cb.hip(); L.backend_init(0); "
+            "l = cb.BackendLogits(logits=1 << 20, out=(1 << 20) + 400, ld=101, ld_out=150, rows=3, vocab=101); "
+            "L.backend_logits(C.byref(l)); print('returned')")
+    r = subprocess.run([sys.executable, "-c", prog], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 1 and "out overlaps the logits" in r.stderr and "returned" not in r.stdout, r.stderr
+    rng = np.random.default_rng(14)
+    x = rng.standard_normal((3, 202)).astype(np.float32)
+    mem = Mem(hip, 1 << 20)
+    at, ids = mem.put(x), mem.put(np.zeros(3, np.int32))
+    a = cb.BackendLogits(logits=at, out=at + 404, ld=202, ld_out=202, rows=3, vocab=101, id=ids)
+    hip.backend_logits(C.byref(a))
+    assert np.array_equal(mem.get(at, (3, 202), np.float32), np.concatenate([x[:, :101]] * 2, 1))
+    assert np.array_equal(mem.get(ids, (3,), np.int32), x[:, :101].argmax(1))
