@@ -562,3 +562,25 @@ def test_chunks_of_many_pages(hip, P, kv, group, D, lens, common, least):
     for bf16 in (False, True):
         got = attend(d, 0, q, heads, p, rows, True, bf16)
         check_rows(got, *want, bf16, bf16)
+
+
+@pytest.mark.parametrize("P,kv,group,D,lens,common", [
+    (128, 8, 16, 64, [70001 + 50 * i for i in range(8)], 69888), (64, 8, 10, 128, [45000 + 7 * i for i in range(7)], 44992)])
+def test_long_common_text_of_many_rows(hip, P, kv, group, D, lens, common):
+    """The many-row kernel over common tokens whose chunks are longer than what it
+    keeps places of at a time (32 iterations of 64), a page missing and a NaN near their end."""
+    print(f"case: shared, long common text P={P} kv={kv} group={group} D={D} {lens[0]} x {len(lens)}", flush=True)
+    rng = np.random.default_rng(lens[0])
+    n, heads = len(lens), kv * group
+    d = long_texts(hip, rng, P, kv, D, lens, common, 1 << 24)
+    m = d.model
+    assert n * group > 64 and (common // 32) / -(-128 // kv) > 64
+    m.table[:, common // P - 3] = m.dims[1] - 1
+    m.table[:, common // P - 9] = -1
+    d.push()
+    q, rows = values(rng, n, heads, D), starts([1] * n)
+    p = found(d)[0]
+    want = attend_last(m, q, D ** -0.5)
+    assert np.isnan(want[0]).any()
+    for bf16 in (False, True):
+        check_rows(attend(d, 0, q, heads, p, rows, True, bf16), *want, bf16, bf16)
