@@ -1458,8 +1458,8 @@ __global__ __launch_bounds__(NT, WIDE || !BF16 ? 2 : 3) void shared_kernel(Args 
 
 // Sequences whose tokens are all common, as a clip's hypotheses have them, in one
 // launch: a workgroup for each of them, of which those that do not begin a group
-// leave.  24 clips of up to 376 tokens, 5 hypotheses each, 8 heads, fp32 (18 MB of
-// codes): 12.9 us, where a call of one workgroup takes 3.6; finding the group is some 2.
+// leave.  24 clips of up to 376 tokens, 5 hypotheses each, 8 heads, fp32 (13.6
+// MB): 12.9 us, where a call of one workgroup takes 3.6; finding the group is some 2.
 template <int D, bool BF16>
 __global__ __launch_bounds__(NT, 2) void groups_kernel(Args a) {
     __shared__ __align__(16) float so[NW * 16 * D];

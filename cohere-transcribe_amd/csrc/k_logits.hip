@@ -2,14 +2,16 @@
 // grammar masks on a step's logits, and the largest logit that is left.
 //
 // A thread holds 16 of a row's logits, a workgroup 16 x NT of them, asked for
-// before anything else.  Meanwhile the workgroup goes through the row's history
-// and counts in LDS how often each of its tokens was said and whether it is
-// banned (whole numbers, so the order of the atomics changes nothing); then
-// through the bias list, which leaves each token's last entry in the same
-// word.  4 bytes a logit are read and, where wanted, 4 written: bound by memory
-// where there are many (200 x 100003, 165 MB: 46 to 49 us, of which a copy of as much
-// takes 34.5), else by the chain history, LDS, largest (5 x 16384: 7.7 us, 64 x
-// 16384 with histories of 1000: 8.9; a call of one workgroup is 3.6).  A row's
+// first and the first of the history and bias list behind them; the four words of
+// the mask are each waited for, and all that was asked for before with them.  The
+// workgroup then goes through the row's history and counts in LDS how often each
+// of its tokens was said and whether it is banned (whole numbers, so the order of
+// the atomics changes nothing); then through the bias list, which leaves each
+// token's last entry in the same word.  4 bytes a logit are read and, where wanted,
+// 4 written: bound by memory where there are many (200 x 100003, 165 MB: 48.4 us, of
+// which a copy of as much takes 34.5), else by the chain arguments, logits and masks,
+// history, LDS, largest (5 x 16384: 7.6 us, 64 x 16384 with histories of 1000: 8.7; a
+// call of one workgroup is 3.6).  A row's
 // workgroups meet in one 64-bit maximum of (value, lowest id) in memory; the
 // last of them writes the token and leaves the memory as it was.
 #include "ct_dev.h"
@@ -78,7 +80,7 @@ __global__ __launch_bounds__(NT, 6) void logits_kernel(BackendLogits a) {
     __shared__ int splace[NT / CT_WAVE], slast;
     const int r = blockIdx.y, v0 = blockIdx.x * CHUNK, n = min(CHUNK, a.vocab - v0), tid = threadIdx.x;
 
-    // asked for first: the logits and the first of the history
+    // asked for first: the logits
     const float *x = a.logits + (long)r * a.ld + v0;
     float l[EACH];
 #pragma unroll
@@ -272,8 +274,8 @@ __global__ __launch_bounds__(NT, 6) void logits_kernel(BackendLogits a) {
     if (a.score) a.score[r] = top;
 }
 
-// 512 threads go through a row's history half as often as 256 (200 x 100003: 46 us,
-// with 1024 48); a row that 256 hold has no use for more (300 x 4000: 8.2 us, 512
+// 512 threads go through a row's history half as often as 256 (200 x 100003 on one card:
+// 46 us, with 1024 48); a row that 256 hold has no use for more (300 x 4000: 8.2 us, 512
 // 8.8; 1 x 4000: 6.2, 6.7).
 int threads_of(const BackendLogits *a) { return a->vocab > EACH * SMALL ? LARGE : SMALL; }
 

@@ -23,10 +23,11 @@
 // call has.
 //
 // What bounds them.  One row of a small map: the launch and one pass of loads
-// (1024 -> 1024, 0.55 MB: 3.8 us, where a call of one workgroup takes 3.6).  Few rows of large maps: the codes'
-// bytes (1 x 8192 -> 24576, 106 MB: 22.5 us, 4.7 TB/s).  Many rows: vector
-// instructions that prepare both operands, which do not overlap the products (752 x
-// 1280 -> 5120: 32 us, 308 Tflop/s of them, twice that of f16 terms).
+// (1024 -> 1024, 0.55 MB: 3.8 us, where a call of one workgroup takes 3.6).  Few rows
+// of large maps: the codes' bytes (1 x 8192 -> 24576, 106 MB: 22.5 us, 4.7 TB/s).
+// Many rows: vector instructions that prepare both operands and the products, which
+// take turns (752 x 1280 -> 5120: 32 us, 308 Tflop/s of them, twice that of f16 terms;
+// 48% and 29% of the SIMDs' time).
 #include "ct_dev.h"
 #include "ct_w4.h"
 
@@ -212,12 +213,14 @@ __device__ __forceinline__ void finish(const Args &a, long t, int o, float v) {
     }
 }
 
-// Work of a round or few: NT tiles of outputs a workgroup, 16 rows at a time; its eight wavefronts each take one segment of the inputs, split them a tile
-// at a time and join their sums in LDS, in order.  A wavefront has AHEAD tiles of
-// codes and inputs in flight, or, of four tiles together, asks for each operand of
-// the next one as this one leaves its registers (two whole sets spill).  64 x 1024 -> 4096:
+// Work of a round or few: NT tiles of outputs a workgroup, 16 rows at a time; its
+// eight wavefronts each take one segment of the inputs, split them a tile at a time
+// and join their sums in LDS, in order.  A wavefront has AHEAD tiles of codes and
+// inputs in flight, or, of four tiles together, asks for each operand of the next
+// one as this one leaves its registers (two whole sets spill).  64 x 1024 -> 4096:
 // 6.1 us, bound by the chain of loads, split, products and join; 64 x 4096 -> 4096
-// 13.6, by the vector instructions that make operands of codes and inputs.
+// 13.6: vector instructions, most of which make operands of codes and inputs, take
+// 55% of the SIMDs' time and products 13%, and wavefronts wait 41% of theirs.
 template <bool BF16, int GS, int NT>
 __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
     constexpr int NB = BF16 ? 1 : 2, RR = 16, RI = RR / 4, AHEAD = NT == 4 ? 1 : 2;
@@ -228,7 +231,7 @@ __global__ __launch_bounds__(SEGS * CT_WAVE, 2) void linear_kernel(Args a) {
     __shared__ __align__(16) float sundo[SEGS][RR];
     const int lane = threadIdx.x % CT_WAVE, w = __builtin_amdgcn_readfirstlane(threadIdx.x / CT_WAVE);
     const int c = lane & 15, q = lane >> 4;
-        const int k0 = w * a.per, k1 = min(k0 + a.per, a.itiles);
+    const int k0 = w * a.per, k1 = min(k0 + a.per, a.itiles);
     struct Ahead {
         u32x4 code[NT];
         uint32_t word[NT][4 / GS];

@@ -292,7 +292,7 @@ void backend_kv8_compact(const BackendKv8 *c);
 int  backend_kv8_status(const BackendKv8 *c);
 /* Attention over sequences whose first tokens lie on the same pages (a clip's
  * hypotheses, samples of one prompt, requests with one instruction): those are
- * read once for all of them.
+ * read once for all of them where that is faster.
  *
  * backend_kv8_share finds them in the tables.  Sequences whose first table
  * entries are the same page of the pool are a group; its lowest-numbered
@@ -302,9 +302,17 @@ int  backend_kv8_status(const BackendKv8 *c);
  * alone.  share is DEVICE memory, 2 * seqs ints. */
 void backend_kv8_share(const BackendKv8 *c, int *share);
 /* backend_kv8_attn where a group's common tokens are read once, through its
- * leader's table, for the rows of all its sequences; the others as ever.  share
- * is as backend_kv8_share writes it, or the caller's: share[seqs + l] tokens of
- * leader l (share[l] == l) lie for all its sequences on the pages that l's table
+ * leader's table, for the rows of all its sequences; the others as ever.  So they
+ * are, by the sizes of the call alone,
+ *   - where a sequence has up to 64 query rows of a kv head (max_rows * heads /
+ *     kv_heads) and all sequences may read more than 192 MB of codes together (by
+ *     max_len or the tables' width);
+ *   - below that, in calls that are not causal, of up to 16 such rows a sequence, up
+ *     to 4096 tokens and more than 512 sequences times kv heads: in groups that have
+ *     all tokens in common and up to 16 such rows together.
+ * Elsewhere each sequence goes through its own table, as in backend_kv8_attn.
+ * share is as backend_kv8_share writes it, or the caller's: share[seqs + l] tokens
+ * of leader l (share[l] == l) lie for all its sequences on the pages that l's table
  * names, or on copies of them.  Of these as many are taken as every row of the
  * group sees.  A leader that is out of range or does not lead itself stands for
  * none.  No window.  Accuracy as of backend_kv8_attn, whose bits it does not
@@ -383,7 +391,8 @@ void backend_linear_w4(const BackendW4 *w, const BackendW4Linear *a);
  *   4. tokens that would complete a run of `ngram` tokens that the history
  *      holds already:           l = -infinity (ngram 1: any token said)
  *   5. tokens whose mask bit is 0: l = -infinity
- * Token ids outside [0, vocab) in a history or bias list touch nothing. */
+ * Token ids outside [0, vocab) in a history or bias list touch nothing.  Step 4
+ * compares a place of the history until a token differs, up to ngram of them. */
 typedef struct {
     const float *logits; /* [rows][vocab], ld apart                           */
     float *out;          /* the same after step 5, ld_out apart; may be logits
