@@ -405,7 +405,8 @@ typedef struct {
     float *score;        /* [rows] that value; -infinity if there is none     */
     const int *hist;     /* [rows] token ids, ld_hist apart, oldest first     */
     long ld_hist;        /* at most 2^24                                      */
-    const int *hist_len; /* [rows] tokens of each; held to [0, ld_hist]       */
+    const int *hist_len; /* [rows] tokens of each; held to [0, ld_hist]; none
+                            past them are read                                */
     const int *prompt_len;  /* [rows] of them, the first ones are the prompt;
                                NULL: none                                     */
     const float *repeat, *frequency, *presence;  /* [rows]                    */
